@@ -376,8 +376,8 @@ int32_t objeta_hip_moe_layer_shared_device(objeta_hip_context* ctx, int32_t form
                                            uint32_t* d_ids_out, float* d_weights_out, uint64_t hidden,
                                            uint64_t intermediate, uint64_t out_dim, float swiglu_limit);
 
-/* Reads and clears the context's device error word. Bit 0: a kernel met an expert
- * id outside its table. Bit 1 (a report, not a failure): a router call's selecting
+/* Reads and clears the context's device error word. Bits 2 and 3: see the attention
+ * section. Bit 0: a kernel met an expert id outside its table. Bit 1 (a report, not a failure): a router call's selecting
  * workgroup found other workgroups' logits still missing after its spin limit (the
  * device kept them from running, about a second by default) and computed every
  * logit itself in the reference's order, so its result is exact. The spin limit is
@@ -803,6 +803,177 @@ int32_t objeta_hip_st_deepseek_shared_expert(const objeta_hip_st_model* model, u
  * name; read it with objeta_hip_st_get_f32. */
 int32_t objeta_hip_st_deepseek_router(const objeta_hip_st_model* model, uint64_t layer, int32_t mtp,
                                       char* name_buf, uint64_t cap, objeta_hip_st_info* info);
+
+/* ------------------------------------------------ attention and its cache */
+/* The attention half of a decoder layer: rotary positions, attention over packed
+ * prompts, a paged key/value cache with the attention that reads it, and that cache's
+ * page operations. The reference's AttentionBackend names this place and answers
+ * Unsupported to every call (crates/objeta-cuda/src/attention.rs:1-21); none of these
+ * has a counterpart in it.
+ *
+ * Element types are OBJETA_HIP_DT_F32 / _F16 / _BF16. head_dim is a multiple of 8 up to
+ * 256. Strides count elements from one token to the next; a token's heads lie behind one
+ * another. Attention reads rows of 16-byte aligned addresses (base and stride). Query
+ * head h reads key/value head h / (n_q_heads / n_kv_heads).
+ *
+ * Indices on the device (cu_seqlens, sequences, lengths, page tables) are checked by the
+ * kernels before any access they lead to: an index outside its table sets bit 2 of the
+ * device error word (objeta_hip_device_error), page allocation without free pages bit 3.
+ * The entry point says what becomes of the work concerned. Calls allocate nothing once
+ * a call as large has run on their stream, and may be captured after it. Graphs
+ * captured on one stream share that stream's workspace: their replays are ordered one
+ * after the other, as calls on the stream are. */
+
+/* Pairs of a rotated head: (2i, 2i + 1), or (i, i + rotary_dim / 2). */
+enum { OBJETA_HIP_ROPE_INTERLEAVED = 0, OBJETA_HIP_ROPE_HALF = 1 };
+/* Scaling for contexts longer than the trained one, with f_i = theta^(-2i / rotary_dim):
+ * LINEAR f_i / factor; NTK theta' = theta * factor^(rotary_dim / (rotary_dim - 2)); YARN
+ * f_i / factor for the pairs that turn less than beta_slow times over original_context,
+ * f_i for those that turn more than beta_fast times, a linear ramp over the pair's index
+ * between (floor and ceil of the two indices), and cosines and sines times
+ * 0.1 ln(factor) + 1. */
+enum { OBJETA_HIP_ROPE_NONE = 0, OBJETA_HIP_ROPE_LINEAR = 1, OBJETA_HIP_ROPE_NTK = 2, OBJETA_HIP_ROPE_YARN = 3 };
+
+typedef struct {
+    double theta;
+    uint32_t rotary_dim; /* even, 2 .. 256: the head's first dimensions; the others are copied */
+    int32_t layout;
+    int32_t scaling;
+    int32_t reserved;
+    double factor;           /* LINEAR, NTK, YARN: > 0 (YARN: >= 1) */
+    double original_context; /* YARN */
+    double beta_fast;        /* YARN, usually 32 */
+    double beta_slow;        /* YARN, usually 1 */
+    double amplitude;        /* factor of cosines and sines; 0: the scaling's own */
+} objeta_hip_rope_params;
+
+/* What the calls take: each pair's turn per position as a 64-bit fraction of a full
+ * turn (a position times it, modulo 2^64, is the exact place on the circle however far
+ * the position), the layout and the amplitude. Plain data; made once by rope_init. */
+typedef struct {
+    uint64_t turn[128];
+    uint32_t rotary_dim;
+    int32_t layout;
+    float amplitude;
+    uint32_t reserved;
+} objeta_hip_rope;
+
+/* Fills *out on the host; needs no device. */
+int32_t objeta_hip_rope_init(const objeta_hip_rope_params* params, objeta_hip_rope* out);
+
+/* Rotary positions for the queries and, unless n_k_heads is 0, the keys of n_tokens
+ * tokens in one launch: q [n_tokens][n_q_heads][head_dim] (token stride q_stride) by the
+ * angles of d_positions[t] (int32, any value), written to q_out; k likewise. Types:
+ * `dtype` in, `out_dtype` out; computed in float, angles exact to 2^-32 of a turn. An
+ * output may be its own input (same address, stride and type); otherwise outputs may not
+ * overlap inputs or one another. Pointers aligned to their element type. */
+int32_t objeta_hip_rope_device(objeta_hip_context* ctx, objeta_hip_stream stream, const objeta_hip_rope* rope,
+                               const int32_t* d_positions, uint64_t n_tokens, uint64_t head_dim, int32_t dtype,
+                               int32_t out_dtype, const void* d_q, uint64_t q_stride, void* d_q_out,
+                               uint64_t q_out_stride, uint64_t n_q_heads, const void* d_k, uint64_t k_stride,
+                               void* d_k_out, uint64_t k_out_stride, uint64_t n_k_heads);
+
+/* Attention over packed sequences: token t of n_tokens belongs to sequence b when
+ * d_cu_seqlens[b] <= t < d_cu_seqlens[b + 1] (int32 [n_seqs + 1], ascending, within
+ * [0, n_tokens]) and sees that sequence's tokens, with causal != 0 only those up to
+ * itself:
+ *   out_t = sum_j p_j v_j,  p = softmax_j(scale q_t . k_j),  lse_t = ln sum_j exp(scale q_t . k_j)
+ * q, out [n_tokens][n_q_heads][head_dim], k, v [n_tokens][n_kv_heads][head_dim], all of
+ * `dtype`; d_lse [n_tokens][n_q_heads] float, nullable. Rows of no sequence (behind the
+ * last one, or under indices out of order) are left as they were. What lies in places a
+ * row does not see, infinities and NaN included, does not reach it. scale > 0. Sums and
+ * softmax are held in float; 16-bit types round the probabilities to their type before the
+ * product with v (float: not). out may not overlap q, k or v. n_tokens * n_q_heads < 2^31. */
+int32_t objeta_hip_attn_prompt_device(objeta_hip_context* ctx, objeta_hip_stream stream, int32_t dtype,
+                                      const void* d_q, uint64_t q_stride, uint64_t n_q_heads, const void* d_k,
+                                      uint64_t k_stride, const void* d_v, uint64_t v_stride, uint64_t n_kv_heads,
+                                      uint64_t head_dim, uint64_t n_tokens, const int32_t* d_cu_seqlens,
+                                      uint64_t n_seqs, int32_t causal, float scale, void* d_out, uint64_t out_stride,
+                                      float* d_lse);
+
+/* A paged key/value cache of a stack of layers in the caller's device buffers. Token
+ * `slot` of sequence s lies in page page_table[s][slot / page_size], row slot % page_size
+ * of every layer. A sequence of seq_lens[s] tokens holds ceil(len / page_size) pages, its
+ * other table entries are -1; a page's ref_counts entry counts the sequences that hold
+ * it, 0 is free. The calls keep it so. */
+typedef struct {
+    void* k;             /* [n_layers][n_pages][n_kv_heads][page_size][head_dim], 16-byte aligned */
+    void* v;             /* the same */
+    int32_t* page_table; /* [n_seqs][max_pages] */
+    int32_t* seq_lens;   /* [n_seqs] */
+    int32_t* ref_counts; /* [n_pages] */
+    int32_t dtype;
+    uint32_t n_layers;
+    uint32_t n_pages;
+    uint32_t n_kv_heads;
+    uint32_t page_size; /* a power of two, 8 .. 256 */
+    uint32_t head_dim;
+    uint32_t n_seqs;
+    uint32_t max_pages; /* of one sequence */
+} objeta_hip_kv_cache;
+
+/* Writes the keys and values of new tokens to layer `layer` of the cache. The batch:
+ * entry b < n_batch is sequence d_seqs[b] with the rows d_cu_rows[b] .. d_cu_rows[b + 1]
+ * of k and v [n_rows][n_kv_heads][head_dim] (`dtype`; rounded to the cache's type), which
+ * become the last slots of the sequence: objeta_hip_kv_extend_device has made room for
+ * them. With `rope`, keys are rotated by d_positions[row] first (a draft's position need
+ * not be its slot); with d_q also queries, q [n_rows][n_q_heads][head_dim] to q_out
+ * (q_out_dtype; in place as for objeta_hip_rope_device), in the same launch. A sequence
+ * that the batch names twice takes its last entry's rows. Keys and values of no entry, or
+ * whose slot has no page (bit 2), are not written; queries of every row are. Sources may
+ * not overlap the cache. */
+int32_t objeta_hip_kv_append_device(objeta_hip_context* ctx, objeta_hip_stream stream, const objeta_hip_kv_cache* cache,
+                                    uint64_t layer, const int32_t* d_seqs, const int32_t* d_cu_rows, uint64_t n_batch,
+                                    uint64_t n_rows, int32_t dtype, const void* d_k, uint64_t k_stride, const void* d_v,
+                                    uint64_t v_stride, const objeta_hip_rope* rope, const int32_t* d_positions,
+                                    const void* d_q, uint64_t q_stride, uint64_t n_q_heads, int32_t q_out_dtype,
+                                    void* d_q_out, uint64_t q_out_stride);
+
+/* Attention of new tokens over the cache: decode (one row an entry), trees of drafted
+ * tokens, chunks of a prompt. The batch is that of objeta_hip_kv_append_device, q and out
+ * [n_rows][n_q_heads][head_dim] of `dtype`; the cache is of the same type, or q is float
+ * and the cache f16 or bf16. Row i of an entry with n rows over a sequence of len tokens
+ * sees the slots before len - n, and
+ *   without d_tree, the slots up to its own (len - n + i);
+ *   with d_tree (uint64 [n_rows], n <= 64), slot len - n + j where bit j of its mask is set.
+ * A row that sees nothing gets out 0 and lse -inf. d_lse as for prompts. max_rows and
+ * max_len: the most rows of an entry and the longest sequence as the host knows them; they
+ * only decide how the work is cut, larger ones are computed too. Entries whose sequence,
+ * length or pages are out of range, or that have more rows than the sequence tokens, get
+ * NaN (bit 2). n_rows * n_q_heads < 2^31; n_batch and n_kv_heads <= 65535. */
+int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream stream,
+                                      const objeta_hip_kv_cache* cache, uint64_t layer, const int32_t* d_seqs,
+                                      const int32_t* d_cu_rows, uint64_t n_batch, uint64_t n_rows, uint64_t max_rows,
+                                      uint64_t max_len, int32_t dtype, const void* d_q, uint64_t q_stride,
+                                      uint64_t n_q_heads, const uint64_t* d_tree, float scale, void* d_out,
+                                      uint64_t out_stride, float* d_lse);
+
+/* Page operations over up to 1024 entries a call. An entry whose indices are out of
+ * range, or whose sequence (fork: destination) an earlier entry of the call names too,
+ * changes nothing and sets bit 2.
+ *
+ * extend: room for d_counts[i] >= 0 more tokens of sequence d_seqs[i]; their slots' contents
+ * are undefined until written. New pages are the free ones of lowest index, in entry order;
+ * a last page that is partly filled and held by another sequence too is replaced by a copy
+ * of its filled rows in every layer. Where the free pages do not last, that entry and all
+ * behind it change nothing (bit 3). */
+int32_t objeta_hip_kv_extend_device(objeta_hip_context* ctx, objeta_hip_stream stream, const objeta_hip_kv_cache* cache,
+                                    const int32_t* d_seqs, const int32_t* d_counts, uint64_t n);
+/* fork: sequence d_dst[i] becomes d_src[i] as it was before the call, on shared pages; what
+ * it held is released. A destination may be another entry's source (beams in a new order). */
+int32_t objeta_hip_kv_fork_device(objeta_hip_context* ctx, objeta_hip_stream stream, const objeta_hip_kv_cache* cache,
+                                  const int32_t* d_src, const int32_t* d_dst, uint64_t n);
+/* compact: of the last d_drafts[i] tokens of sequence d_seqs[i], the d_kept[i] ones with the
+ * strictly ascending indices d_keep[i][0 .. kept) among them move together in every layer,
+ * the rest is dropped and pages past the new end are released. kept 0 takes the drafts back.
+ * d_keep int32 [n][max_keep], max_keep <= 64 (0: d_keep may be NULL). An entry that would
+ * move rows within a page held by another sequence too changes nothing (bit 2). */
+int32_t objeta_hip_kv_compact_device(objeta_hip_context* ctx, objeta_hip_stream stream, const objeta_hip_kv_cache* cache,
+                                     const int32_t* d_seqs, const int32_t* d_drafts, const int32_t* d_keep,
+                                     const int32_t* d_kept, uint64_t n, uint64_t max_keep);
+/* free: sequence d_seqs[i] releases its pages and is empty. */
+int32_t objeta_hip_kv_free_device(objeta_hip_context* ctx, objeta_hip_stream stream, const objeta_hip_kv_cache* cache,
+                                  const int32_t* d_seqs, uint64_t n);
 
 #ifdef __cplusplus
 }

@@ -7,7 +7,8 @@ benchmark.
 from .api import (DeviceBuffer, ExpertCache, ExpertCacheKey, ExpertTable, ExpertTensorKind, HipBackend,
                   HipBackendBuilder, HipError, HostExpertSet, MoeExecutor, PinnedHostBuffer, QGemvShape, QuantBackend, QuantFormat, check,
                   discover_devices)
+from .attention import AttentionBackend, KvCache, Rope
 
-__all__ = ["DeviceBuffer", "ExpertCache", "ExpertCacheKey", "ExpertTable", "ExpertTensorKind", "HipBackend",
-           "HipBackendBuilder", "HipError", "HostExpertSet", "MoeExecutor", "PinnedHostBuffer", "QGemvShape", "QuantBackend", "QuantFormat", "check",
+__all__ = ["AttentionBackend", "DeviceBuffer", "ExpertCache", "ExpertCacheKey", "ExpertTable", "ExpertTensorKind", "HipBackend",
+           "HipBackendBuilder", "HipError", "HostExpertSet", "KvCache", "MoeExecutor", "PinnedHostBuffer", "QGemvShape", "QuantBackend", "QuantFormat", "Rope", "check",
            "discover_devices"]

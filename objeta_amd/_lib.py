@@ -22,6 +22,7 @@ U32 = C.c_uint32
 U64 = C.c_uint64
 I64 = C.c_int64
 F32 = C.c_float
+F64 = C.c_double
 
 
 class Error(C.Structure):
@@ -102,6 +103,21 @@ class StackTelemetry(C.Structure):
 class QGemvTelemetry(C.Structure):
     _fields_ = [("h2d_ms", F32), ("kernel_ms", F32), ("d2h_ms", F32), ("unaccounted_ms", F32),
                 ("total_ms", F32), ("effective_gbps", F32), ("bytes_read", U64)]
+
+
+class RopeParams(C.Structure):
+    _fields_ = [("theta", F64), ("rotary_dim", U32), ("layout", I32), ("scaling", I32), ("reserved", I32),
+                ("factor", F64), ("original_context", F64), ("beta_fast", F64), ("beta_slow", F64), ("amplitude", F64)]
+
+
+class RopePlan(C.Structure):
+    _fields_ = [("turn", U64 * 128), ("rotary_dim", U32), ("layout", I32), ("amplitude", F32), ("reserved", U32)]
+
+
+class KvCacheDesc(C.Structure):
+    _fields_ = [("k", P), ("v", P), ("page_table", P), ("seq_lens", P), ("ref_counts", P), ("dtype", I32),
+                ("n_layers", U32), ("n_pages", U32), ("n_kv_heads", U32), ("page_size", U32), ("head_dim", U32),
+                ("n_seqs", U32), ("max_pages", U32)]
 
 
 # name -> (restype, argtypes)
@@ -196,6 +212,18 @@ SIGNATURES = {
     "objeta_hip_st_deepseek_expert": (I32, [P, U64, U64, I32, P, P, P, P]),
     "objeta_hip_st_deepseek_shared_expert": (I32, [P, U64, I32, P, P, P, P]),
     "objeta_hip_st_deepseek_router": (I32, [P, U64, I32, P, U64, P]),
+    "objeta_hip_rope_init": (I32, [P, P]),
+    "objeta_hip_rope_device": (I32, [P, P, P, P, U64, U64, I32, I32, P, U64, P, U64, U64, P, U64, P, U64, U64]),
+    "objeta_hip_attn_prompt_device": (I32, [P, P, I32, P, U64, U64, P, U64, P, U64, U64, U64, U64, P, U64, I32, F32, P,
+                                            U64, P]),
+    "objeta_hip_kv_append_device": (I32, [P, P, P, U64, P, P, U64, U64, I32, P, U64, P, U64, P, P, P, U64, U64, I32, P,
+                                          U64]),
+    "objeta_hip_attn_cached_device": (I32, [P, P, P, U64, P, P, U64, U64, U64, U64, I32, P, U64, U64, P, F32, P, U64,
+                                            P]),
+    "objeta_hip_kv_extend_device": (I32, [P, P, P, P, P, U64]),
+    "objeta_hip_kv_fork_device": (I32, [P, P, P, P, P, U64]),
+    "objeta_hip_kv_compact_device": (I32, [P, P, P, P, P, P, P, U64, U64]),
+    "objeta_hip_kv_free_device": (I32, [P, P, P, P, U64]),
 }
 
 

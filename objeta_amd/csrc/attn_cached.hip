@@ -1,0 +1,155 @@
+// attn_cached.hip — attention over the paged key/value cache (objeta_hip_attn_cached_device):
+// which kernel takes a call, how its keys are cut over workgroups, and the join of the parts.
+#include "attn_cached.hpp"
+#include "kernels.hpp"
+
+namespace objeta {
+namespace dev {
+
+// Joins the parts of one (row, head), a wave each: with M the largest m, l = sum l_s 2^(m_s - M),
+// o = sum o_s 2^(m_s - M) / l.
+template <int QT>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+    typedef typename ElemOf<QT>::type elem;
+    const uint32_t lane = threadIdx.x & 63;
+    const uint64_t rh = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    if (rh >= static_cast<uint64_t>(a.n_rows) * a.n_heads) return;
+    const uint32_t row = static_cast<uint32_t>(rh / a.n_heads), head = static_cast<uint32_t>(rh % a.n_heads);
+    const uint32_t le = count_le(a.cu, a.n_batch + 1, row);
+    if (le == 0 || le > a.n_batch) return;
+    const uint32_t b = le - 1;
+    const int32_t lo = a.cu[b], hi = a.cu[b + 1];
+    if (lo < 0 || lo > static_cast<int32_t>(row) || static_cast<int32_t>(row) >= hi ||
+        static_cast<uint32_t>(hi) > a.n_rows)
+        return;
+    const int32_t seq = a.seqs[b];
+    int32_t len = seq_ok(a.kv, seq) ? a.kv.lens[seq] : 0;
+    if (!len_ok(a.kv, len) || hi - lo > len || (a.tree && hi - lo > 64)) len = 0;
+    uint32_t n = (static_cast<uint32_t>(len) + a.chunk - 1) / a.chunk;
+    n = n < 1 ? 1 : (n > a.n_splits ? a.n_splits : n);
+    const uint64_t step = static_cast<uint64_t>(a.n_rows) * a.n_heads;
+    float top = -kInf;
+    for (uint32_t s = lane; s < n; s += 64) top = __builtin_fmaxf(top, a.part_ml[2 * (s * step + rh)]);
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x, 64));
+    const float ref = top == -kInf ? 0.0f : top;
+    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (uint32_t s = 0; s < n; ++s) {
+        const uint64_t at = s * step + rh;
+        const float f = exp2_hw(a.part_ml[2 * at] - ref);
+        l = __builtin_fmaf(a.part_ml[2 * at + 1], f, l);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            if (lane + 64 * x < a.dim) o[x] = __builtin_fmaf(a.part[at * a.dim + lane + 64 * x], f, o[x]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    elem* p = static_cast<elem*>(a.out) + row * a.out_stride + static_cast<uint64_t>(head) * a.dim;
+#pragma unroll
+    for (int x = 0; x < 4; ++x)
+        if (lane + 64 * x < a.dim) p[lane + 64 * x] = static_cast<elem>(o[x] * inv);
+    if (a.lse && lane == 0) a.lse[rh] = l == 0.0f ? -kInf : (top + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+}  // namespace dev
+
+using namespace dev;
+
+namespace {
+
+template <int QT>
+int32_t launch_join(hipStream_t s, const AttnArgs& a, const char* action) {
+    const uint64_t rows = static_cast<uint64_t>(a.n_rows) * a.n_heads;
+    hipLaunchKernelGGL(attn_join_kernel<QT>, dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, s, a);
+    OBJ_HIP(hipGetLastError(), action);
+    return 0;
+}
+
+}  // namespace
+
+}  // namespace objeta
+
+using namespace objeta;
+
+extern "C" {
+
+int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream stream,
+                                      const objeta_hip_kv_cache* cache, uint64_t layer, const int32_t* d_seqs,
+                                      const int32_t* d_cu_rows, uint64_t n_batch, uint64_t n_rows, uint64_t max_rows,
+                                      uint64_t max_len, int32_t dtype, const void* d_q, uint64_t q_stride,
+                                      uint64_t n_q_heads, const uint64_t* d_tree, float scale, void* d_out,
+                                      uint64_t out_stride, float* d_lse) {
+    OBJ_GUARD_BEGIN
+    const char* action = "attn_cached_device";
+    OBJ_TRY(check_ctx(ctx, action));
+    OBJ_TRY(check_kv(cache, action));
+    const objeta_hip_kv_cache& c = *cache;
+    if (layer >= c.n_layers)
+        OBJ_FAIL(kInvalidInput, action, strf("layer %llu out of bounds (len=%u)", (unsigned long long)layer, c.n_layers));
+    if (!dtype_ok(dtype)) OBJ_FAIL(kInvalidInput, action, "dtype must be F32, F16 or BF16");
+    if (dtype != c.dtype && dtype != kDtF32)
+        OBJ_FAIL(kUnsupported, action, "q must be float or of the cache's type");
+    OBJ_TRY(check_heads(action, n_q_heads, c.n_kv_heads, n_rows, scale));
+    if (n_batch > 65535) OBJ_FAIL(kInvalidInput, action, "at most 65535 entries a call");
+    if (n_batch == 0 || n_rows == 0) return 0;
+    if (!d_seqs || !d_cu_rows) OBJ_FAIL(kInvalidInput, action, "sequences or cu_rows are NULL");
+    if (max_rows == 0 || max_len == 0) OBJ_FAIL(kInvalidInput, action, "max_rows and max_len must be positive");
+    const uint64_t es = dtype_size(dtype), dim = c.head_dim;
+    OBJ_TRY(check_attn_rows(action, "q", d_q, n_rows, q_stride, n_q_heads, dim, es));
+    OBJ_TRY(check_attn_rows(action, "out", d_out, n_rows, out_stride, n_q_heads, dim, es));
+    if (reinterpret_cast<uintptr_t>(d_lse) % 4 || reinterpret_cast<uintptr_t>(d_tree) % 8)
+        OBJ_FAIL(kInvalidInput, action, "lse or tree masks are not aligned");
+    const uint64_t pool = static_cast<uint64_t>(c.n_layers) * c.n_pages * c.n_kv_heads * c.page_size * dim * dtype_size(c.dtype);
+    const RowSet out{d_out, out_stride * es, n_q_heads * dim * es, n_rows};
+    const RowSet lse{d_lse, n_q_heads * 4, n_q_heads * 4, n_rows};
+    const RowSet in[] = {{d_q, q_stride * es, n_q_heads * dim * es, n_rows}, {c.k, pool, pool, 1}, {c.v, pool, pool, 1}};
+    for (const RowSet& r : in)
+        if (rows_overlap(out, r) || rows_overlap(lse, r)) OBJ_FAIL(kInvalidInput, action, "an output overlaps q or the cache");
+    if (rows_overlap(out, lse)) OBJ_FAIL(kInvalidInput, action, "out overlaps lse");
+    OBJ_HIP(hipSetDevice(ctx->device), "hipSetDevice");
+
+    AttnArgs a{};
+    a.q = d_q, a.k = c.k, a.v = c.v, a.out = d_out, a.lse = d_lse;
+    a.q_stride = q_stride, a.out_stride = out_stride;
+    a.cu = d_cu_rows, a.seqs = d_seqs, a.tree = d_tree;
+    a.n_batch = static_cast<uint32_t>(n_batch), a.n_rows = static_cast<uint32_t>(n_rows);
+    a.n_heads = static_cast<uint32_t>(n_q_heads), a.n_kv = c.n_kv_heads;
+    a.group = a.n_heads / a.n_kv;
+    a.dim = c.head_dim;
+    a.scale = scale, a.scale_log2 = scale * kLog2e;
+    a.kv = kv_view(c);
+    a.layer_off = layer * c.n_pages * c.n_kv_heads * c.page_size * dim;
+    a.err = ctx->err_word;
+    const hipStream_t s = resolve_stream(ctx, stream);
+
+    // rows of an entry and head; the host's bounds, no more than can be
+    const uint64_t rows = (max_rows < n_rows ? max_rows : n_rows) * a.group;
+    const uint64_t most = static_cast<uint64_t>(c.max_pages) * c.page_size;
+    const uint64_t len = max_len < most ? max_len : most;
+    // one wave's 32 rows: each wave reads keys of its own; more: 128 rows share the tiles
+    const bool stream_form = rows <= 32;
+    a.n_tiles = static_cast<uint32_t>(stream_form ? (rows + 31) / 32 : (rows + 127) / 128);
+    // Keys are cut so that there are about 2048 workgroups if every sequence were the
+    // longest, in chunks of whole 256 keys.
+    const uint64_t units = n_batch * a.n_kv * a.n_tiles;
+    uint64_t splits = (2048 + units - 1) / units;
+    uint64_t chunk = ((len + splits - 1) / splits + 255) / 256 * 256;
+    splits = (len + chunk - 1) / chunk;
+    a.chunk = static_cast<uint32_t>(chunk);
+    a.n_splits = static_cast<uint32_t>(splits);
+    if (splits > 1) {
+        const size_t parts = static_cast<size_t>(splits) * n_rows * n_q_heads;
+        void* ws = nullptr;
+        OBJ_TRY(ensure_workspace(ctx, s, kWsAttn, parts * (dim + 2) * sizeof(float), &ws));
+        a.part = static_cast<float*>(ws);
+        a.part_ml = a.part + parts * dim;
+    }
+    OBJ_TRY(stream_form ? launch_attn_stream(s, dtype, c.dtype, a, action) : launch_attn_cached_block(s, dtype, c.dtype, a, action));
+    if (splits == 1) return 0;
+    if (dtype == kDtF32) return launch_join<kDtF32>(s, a, action);
+    if (dtype == kDtF16) return launch_join<kDtF16>(s, a, action);
+    return launch_join<kDtBF16>(s, a, action);
+    OBJ_GUARD_END
+}
+
+}  // extern "C"

@@ -1,0 +1,37 @@
+// attn_cached_block.hip — the instances of attn_block.hpp for the paged cache, by types and head size.
+#include "attn_cached.hpp"
+#include "attn_block.hpp"
+
+namespace objeta {
+
+using namespace dev;
+
+namespace {
+
+template <int Q, int K, int DT>
+int32_t launch(hipStream_t s, const AttnArgs& a, const char* action) {
+    const uint64_t x = static_cast<uint64_t>(a.n_splits) * a.n_tiles;
+    if (x > 0x7FFFFFFFull) OBJ_FAIL(kInvalidInput, action, "too many workgroups for one launch");
+    hipLaunchKernelGGL((attn_block_kernel<Q, K, DT, true>), dim3(static_cast<uint32_t>(x), a.n_kv, a.n_batch), dim3(256), 0, s, a);
+    OBJ_HIP(hipGetLastError(), action);
+    return 0;
+}
+
+template <int Q, int K>
+int32_t launch_dim(hipStream_t s, const AttnArgs& a, const char* action) {
+    if (a.dim <= 64) return launch<Q, K, 64>(s, a, action);
+    if (a.dim <= 128) return launch<Q, K, 128>(s, a, action);
+    return launch<Q, K, 256>(s, a, action);
+}
+
+}  // namespace
+
+int32_t launch_attn_cached_block(hipStream_t s, int32_t q_type, int32_t kv_type, const AttnArgs& a, const char* action) {
+    if (q_type == kDtF16) return launch_dim<kDtF16, kDtF16>(s, a, action);
+    if (q_type == kDtBF16) return launch_dim<kDtBF16, kDtBF16>(s, a, action);
+    if (kv_type == kDtF32) return launch_dim<kDtF32, kDtF32>(s, a, action);
+    if (kv_type == kDtF16) return launch_dim<kDtF32, kDtF16>(s, a, action);
+    return launch_dim<kDtF32, kDtBF16>(s, a, action);
+}
+
+}  // namespace objeta

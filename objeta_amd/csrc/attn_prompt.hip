@@ -1,0 +1,112 @@
+// attn_prompt.hip — attention over packed prompts (objeta_hip_attn_prompt_device).
+#include "attn_block.hpp"
+#include "kernels.hpp"
+
+#include <cmath>
+
+namespace objeta {
+
+using namespace dev;
+
+namespace {
+
+template <int T, int DT>
+int32_t launch_prompt(hipStream_t s, const AttnArgs& a, const char* action) {
+    hipLaunchKernelGGL((attn_block_kernel<T, T, DT, false>), dim3(a.n_tiles * a.n_kv), dim3(256), 0, s, a);
+    OBJ_HIP(hipGetLastError(), action);
+    return 0;
+}
+
+template <int T>
+int32_t launch_prompt_dim(hipStream_t s, const AttnArgs& a, const char* action) {
+    if (a.dim <= 64) return launch_prompt<T, 64>(s, a, action);
+    if (a.dim <= 128) return launch_prompt<T, 128>(s, a, action);
+    return launch_prompt<T, 256>(s, a, action);
+}
+
+}  // namespace
+
+int32_t check_attn_rows(const char* action, const char* what, const void* p, uint64_t n, uint64_t stride, uint64_t heads,
+                        uint64_t dim, uint64_t size) {
+    if (!p) OBJ_FAIL(kInvalidInput, action, strf("%s is NULL", what));
+    if (!extent_ok(n, stride, heads * dim, size)) OBJ_FAIL(kInvalidInput, action, strf("%s is too large", what));
+    if (n > 1 && stride < heads * dim)
+        OBJ_FAIL(kInvalidInput, action,
+                 strf("%s stride %llu is less than its %llu elements", what, (unsigned long long)stride,
+                      (unsigned long long)(heads * dim)));
+    if (reinterpret_cast<uintptr_t>(p) % 16 || (n > 1 && stride * size % 16))
+        OBJ_FAIL(kInvalidInput, action, strf("%s rows must be 16-byte aligned", what));
+    return 0;
+}
+
+int32_t check_heads(const char* action, uint64_t n_q_heads, uint64_t n_kv_heads, uint64_t n_rows, float scale) {
+    if (n_q_heads == 0 || n_kv_heads == 0 || n_q_heads > 65535 || n_q_heads % n_kv_heads)
+        OBJ_FAIL(kInvalidInput, action,
+                 strf("n_q_heads %llu must be a multiple of n_kv_heads %llu, at most 65535",
+                      (unsigned long long)n_q_heads, (unsigned long long)n_kv_heads));
+    if (n_rows >= (uint64_t(1) << 31) || n_rows * n_q_heads >= (uint64_t(1) << 31))
+        OBJ_FAIL(kInvalidInput, action, "rows times heads must be below 2^31");
+    if (!(std::isfinite(scale) && scale > 0.0f)) OBJ_FAIL(kInvalidInput, action, "scale must be positive and finite");
+    return 0;
+}
+
+}  // namespace objeta
+
+using namespace objeta;
+
+extern "C" {
+
+int32_t objeta_hip_attn_prompt_device(objeta_hip_context* ctx, objeta_hip_stream stream, int32_t dtype,
+                                      const void* d_q, uint64_t q_stride, uint64_t n_q_heads, const void* d_k,
+                                      uint64_t k_stride, const void* d_v, uint64_t v_stride, uint64_t n_kv_heads,
+                                      uint64_t head_dim, uint64_t n_tokens, const int32_t* d_cu_seqlens,
+                                      uint64_t n_seqs, int32_t causal, float scale, void* d_out, uint64_t out_stride,
+                                      float* d_lse) {
+    OBJ_GUARD_BEGIN
+    const char* action = "attn_prompt_device";
+    OBJ_TRY(check_ctx(ctx, action));
+    if (!dtype_ok(dtype)) OBJ_FAIL(kInvalidInput, action, "dtype must be F32, F16 or BF16");
+    if (!head_dim_ok(head_dim))
+        OBJ_FAIL(kInvalidInput, action, strf("head_dim %llu must be a multiple of 8 up to 256", (unsigned long long)head_dim));
+    OBJ_TRY(check_heads(action, n_q_heads, n_kv_heads, n_tokens, scale));
+    if (n_seqs >= (uint64_t(1) << 31)) OBJ_FAIL(kInvalidInput, action, "too many sequences");
+    if (n_tokens == 0 || n_seqs == 0) return 0;
+    if (!d_cu_seqlens) OBJ_FAIL(kInvalidInput, action, "cu_seqlens are NULL");
+    const uint64_t es = dtype_size(dtype);
+    OBJ_TRY(check_attn_rows(action, "q", d_q, n_tokens, q_stride, n_q_heads, head_dim, es));
+    OBJ_TRY(check_attn_rows(action, "k", d_k, n_tokens, k_stride, n_kv_heads, head_dim, es));
+    OBJ_TRY(check_attn_rows(action, "v", d_v, n_tokens, v_stride, n_kv_heads, head_dim, es));
+    OBJ_TRY(check_attn_rows(action, "out", d_out, n_tokens, out_stride, n_q_heads, head_dim, es));
+    const RowSet out{d_out, out_stride * es, n_q_heads * head_dim * es, n_tokens};
+    const RowSet in[] = {{d_q, q_stride * es, n_q_heads * head_dim * es, n_tokens},
+                         {d_k, k_stride * es, n_kv_heads * head_dim * es, n_tokens},
+                         {d_v, v_stride * es, n_kv_heads * head_dim * es, n_tokens},
+                         {d_lse, n_q_heads * 4, n_q_heads * 4, n_tokens}};
+    for (const RowSet& r : in)
+        if (rows_overlap(out, r)) OBJ_FAIL(kInvalidInput, action, "out overlaps q, k, v or lse");
+    for (int i = 0; i < 3; ++i)
+        if (rows_overlap(in[3], in[i])) OBJ_FAIL(kInvalidInput, action, "lse overlaps q, k or v");
+    if (reinterpret_cast<uintptr_t>(d_lse) % 4) OBJ_FAIL(kInvalidInput, action, "lse is not aligned");
+    OBJ_HIP(hipSetDevice(ctx->device), "hipSetDevice");
+    AttnArgs a{};
+    a.q = d_q, a.k = d_k, a.v = d_v, a.out = d_out, a.lse = d_lse;
+    a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride, a.out_stride = out_stride;
+    a.cu = d_cu_seqlens;
+    a.n_batch = static_cast<uint32_t>(n_seqs);
+    a.n_rows = static_cast<uint32_t>(n_tokens);
+    a.n_heads = static_cast<uint32_t>(n_q_heads), a.n_kv = static_cast<uint32_t>(n_kv_heads);
+    a.group = a.n_heads / a.n_kv;
+    a.dim = static_cast<uint32_t>(head_dim);
+    a.scale = scale, a.scale_log2 = scale * kLog2e;
+    a.causal = causal;
+    a.n_splits = 1;
+    a.n_tiles = static_cast<uint32_t>((n_tokens * a.group + 127) / 128);
+    a.err = ctx->err_word;
+    const hipStream_t s = resolve_stream(ctx, stream);
+    if (dtype == kDtF32) return launch_prompt_dim<kDtF32>(s, a, action);
+    if (dtype == kDtF16) return launch_prompt_dim<kDtF16>(s, a, action);
+    return launch_prompt_dim<kDtBF16>(s, a, action);
+    OBJ_GUARD_END
+}
+
+}  // extern "C"

@@ -80,7 +80,9 @@ enum WsSlot : int {
     kWsOfficial = 5,  // dequantized FP8 activations of the official path
     kWsGemv = 6,      // split activations and partial sums of the batched MFMA GEMV
     kWsStack = 7,     // routing results and expert tables of the cached decode stack
-    kWsSlots = 8
+    kWsPages = 8,     // free pages, copies and staged tables of the cache's page operations
+    kWsAttn = 9,      // partial sums of attention over a cache cut along its length
+    kWsSlots = 10
 };
 
 // The scratch of one stream. Calls on different streams of a context may be in

@@ -1,0 +1,89 @@
+// kv_common.hpp — what the rotary, paged-cache and attention translation units share:
+// element types, host checks of a cache descriptor and of overlapping rows, and the
+// device view of a cache with its bounds checks.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "host_common.hpp"
+
+namespace objeta {
+
+enum : int { kDtF32 = OBJETA_HIP_DT_F32, kDtF16 = OBJETA_HIP_DT_F16, kDtBF16 = OBJETA_HIP_DT_BF16 };
+constexpr uint32_t kErrIndex = 4u;    // device error word, bit 2: an index outside its table
+constexpr uint32_t kErrNoPages = 8u;  // bit 3: not enough free pages
+constexpr uint64_t kMaxHeadDim = 256;
+constexpr uint64_t kMaxPageOps = 1024;  // entries of one page operation
+
+inline bool dtype_ok(int32_t t) { return t == kDtF32 || t == kDtF16 || t == kDtBF16; }
+inline uint64_t dtype_size(int32_t t) { return t == kDtF32 ? 4 : 2; }
+inline bool head_dim_ok(uint64_t d) { return d >= 8 && d <= kMaxHeadDim && d % 8 == 0; }
+
+// n rows of `width` bytes, `stride` bytes apart.
+struct RowSet {
+    const void* p;
+    uint64_t stride, width, n;
+};
+// Whether two row sets share a byte. Sets of one stride are compared row by row (columns of
+// one packed buffer do not overlap), others by their whole extents.
+inline bool rows_overlap(const RowSet& a, const RowSet& b) {
+    if (!a.p || !b.p || !a.n || !b.n || !a.width || !b.width) return false;
+    const uint64_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
+    const uint64_t ea = pa + (a.n - 1) * a.stride + a.width, eb = pb + (b.n - 1) * b.stride + b.width;
+    if (ea <= pb || eb <= pa) return false;
+    if (a.n > 1 && b.n > 1 && a.stride == b.stride && a.stride >= a.width && a.stride >= b.width) {
+        const uint64_t d = (pb >= pa ? pb - pa : a.stride - (pa - pb) % a.stride) % a.stride;  // b's column in a's rows
+        return d < a.width || d + b.width > a.stride;
+    }
+    return true;
+}
+// (n - 1) * stride + width elements of `size` bytes without a 64-bit overflow.
+inline bool extent_ok(uint64_t n, uint64_t stride, uint64_t width, uint64_t size) {
+    return n < (uint64_t(1) << 31) && stride < (uint64_t(1) << 31) && width < (uint64_t(1) << 31) && size <= 8;
+}
+
+// Checks a cache descriptor (sizes, pointers, alignment).
+int32_t check_kv(const objeta_hip_kv_cache* c, const char* action);
+int32_t check_rope(const objeta_hip_rope* r, uint64_t head_dim, const char* action);
+
+#if defined(__HIPCC__)
+namespace dev {
+
+// The cache's tables as kernels read them. Every index is checked here before use.
+struct KvView {
+    int32_t* table;
+    int32_t* lens;
+    int32_t* refs;
+    uint32_t n_seqs, max_pages, n_pages, shift;  // page size 1 << shift
+};
+
+__device__ __forceinline__ bool seq_ok(const KvView& kv, int32_t s) {
+    return static_cast<uint32_t>(s) < kv.n_seqs;
+}
+__device__ __forceinline__ bool page_ok(const KvView& kv, int32_t p) {
+    return static_cast<uint32_t>(p) < kv.n_pages;
+}
+__device__ __forceinline__ bool len_ok(const KvView& kv, int32_t len) {
+    return len >= 0 && static_cast<uint64_t>(len) <= (static_cast<uint64_t>(kv.max_pages) << kv.shift);
+}
+
+// How many of cu[0 .. n) are <= r, by one wave; with ascending cu the batch entry that
+// holds row r is this less one.
+__device__ __forceinline__ uint32_t count_le(const int32_t* __restrict__ cu, uint32_t n, int64_t r) {
+    uint32_t c = 0;
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint32_t i = 0; i < n; i += 64) c += __popcll(__ballot(i + lane < n && cu[i + lane] <= r));
+    return c;
+}
+
+}  // namespace dev
+
+inline dev::KvView kv_view(const objeta_hip_kv_cache& c) {
+    uint32_t shift = 0;
+    while ((1u << shift) < c.page_size) ++shift;
+    return dev::KvView{c.page_table, c.seq_lens, c.ref_counts, c.n_seqs, c.max_pages, c.n_pages, shift};
+}
+#endif
+
+}  // namespace objeta
