@@ -16,7 +16,7 @@ namespace dev {
 
 template <int KT, int DT>
 struct Block {
-    typedef Rows<KT, DT> R;
+    typedef Rows<KT, DT, 32> R;
     static constexpr int kKeys = R::kBytes <= 512 ? 64 : 32;
     static constexpr int kSub = kKeys / 32;
     static constexpr int kLoads = kKeys * R::kUnits / 256;  // 16-byte units of K (and of V) a thread stages
@@ -29,8 +29,8 @@ struct Block {
 
 template <int QT, int KT, int DT, bool PAGED>
 __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) void attn_block_kernel(AttnArgs a) {
-    typedef Math<QT, KT, DT> M;
-    typedef Rows<KT, DT> R;
+    typedef Math<QT, KT, DT, 32> M;
+    typedef Rows<KT, DT, 32> R;
     typedef Block<KT, DT> B;
     constexpr int kKeys = B::kKeys;
     __shared__ alignas(16) char lds[2][2][B::kTile];
@@ -44,10 +44,10 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
     KvRows<PAGED, KT> kv;
     bool usable = true;
     if constexpr (PAGED) {
-        split = blockIdx.x % a.n_splits;
-        tile = blockIdx.x / a.n_splits;
-        head = blockIdx.y;
-        const uint32_t b = blockIdx.z;
+        const CachedItem item(a, blockIdx.x);
+        if (!item.any) return;
+        split = item.split, tile = item.tile, head = item.head;
+        const uint32_t b = item.b;
         row0 = a.cu[b];
         const int32_t end = a.cu[b + 1];
         n_q = end - row0;
@@ -109,14 +109,10 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
                 if (real) view.lo = s, view.hi = a.causal ? static_cast<int32_t>(i) : e - 1;
             }
         }
-        typename M::frag q[DT / 16];
-        const typename M::qelem* qp =
-            static_cast<const typename M::qelem*>(a.q) + row * a.q_stride + static_cast<uint64_t>(q_head) * a.dim;
-#pragma unroll
-        for (int s = 0; s < DT / 16; ++s) {
-            const uint32_t d = 16 * s + 8 * h;
-            q[s] = (real && d < a.dim) ? M::load_q(qp + d) : M::zero();
-        }
+        typename M::Query q;
+        float scale = a.scale_log2;
+        M::load_q(q, static_cast<const typename M::qelem*>(a.q) + row * a.q_stride + static_cast<uint64_t>(q_head) * a.dim, real,
+                  a.dim, lane, scale);
         // ---- what the wave and the workgroup see
         const bool sees_any = view.lo <= view.hi;
         int32_t w_lo = sees_any ? view.lo : 0x7FFFFFFF, w_hi = sees_any ? view.hi : -1;
@@ -144,7 +140,7 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
             if (k_lo < c0) k_lo = static_cast<int32_t>(c0);
             if (split + 1 < a.n_splits && k_end > c1) k_end = static_cast<int32_t>(c1);
         }
-        RowState<DT> st;
+        RowState<M> st;
         st.clear();
         const int32_t k_begin = k_lo & ~(kKeys - 1);
         const int32_t n_tiles = k_begin < k_end ? (k_end - k_begin + kKeys - 1) / kKeys : 0;
@@ -208,19 +204,19 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
             const int32_t k0 = k_begin + t * kKeys;
             if (k0 <= w_hi && k0 + kKeys > w_lo) {
                 const char* kb = lds[t & 1][0];
-                f32x16 s[B::kSub];
+                Scores<M> s[B::kSub];
 #pragma unroll
-                for (int n = 0; n < B::kSub; ++n) s[n] = scores<M, DT>(q, kb + n * 32 * R::kBytes, lane, kx);
+                for (int n = 0; n < B::kSub; ++n) scores<M>(s[n], q, kb + n * 32 * R::kBytes, lane, kx);
                 if (k0 < all_lo || k0 + kKeys - 1 > all_hi || k0 < k_lo || k0 + kKeys > k_end) {
 #pragma unroll
                     for (int n = 0; n < B::kSub; ++n)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
-                            const int32_t key = k0 + 32 * n + (r & 3) + 8 * (r >> 2) + 4 * static_cast<int32_t>(h);
-                            if (!(view.sees(key) && key >= k_lo && key < k_end)) s[n][r] = -kInf;
+                            const int32_t key = k0 + 32 * n + static_cast<int32_t>(M::key_of(0, r, h));
+                            if (!(view.sees(key) && key >= k_lo && key < k_end)) s[n].s[0][r] = -kInf;
                         }
                 }
-                accumulate<M, DT, B::kSub>(st, s, a.scale_log2, lds[t & 1][1], vx);
+                accumulate<M, B::kSub>(st, s, scale, lds[t & 1][1], vx);
             }
             if (t + 1 < n_tiles) store_tile((t + 1) & 1);
             if constexpr (PAGED) {
@@ -238,12 +234,12 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
                 for (int d = 0; d < DT / 32; ++d)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) st.o[d][r] = st.l;
-                write_rows<M, QT, DT>(a, st, real, row, q_head, split, lane);
+                write_rows<M, QT>(a, st, real, row, q_head, split, lane);
                 __syncthreads();
                 continue;
             }
         }
-        if (not_finite<DT>(st)) {
+        if (not_finite<M>(st)) {
             for (int r = 0; r < 32; ++r) {
                 if (!__builtin_amdgcn_readlane(real, r)) continue;
                 const uint32_t r_m = tile * 128 + wave * 32 + r, r_head = head * a.group + r_m % a.group;
@@ -262,7 +258,7 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
                 write_row<M>(a, rm, rl, ro, r_row, r_head, split, lane);
             }
         } else {
-            write_rows<M, QT, DT>(a, st, real, row, q_head, split, lane);
+            write_rows<M, QT>(a, st, real, row, q_head, split, lane);
         }
         if constexpr (!PAGED) break;
         __syncthreads();  // the next tile's ranges go where this one's were read

@@ -6,15 +6,18 @@
 namespace objeta {
 namespace dev {
 
-// Joins the parts of one (row, head), a wave each: with M the largest m, l = sum l_s 2^(m_s - M),
-// o = sum o_s 2^(m_s - M) / l.
-template <int QT>
+// Joins the parts of one (row, head), a workgroup each: with M the largest m, l = sum l_s 2^(m_s - M),
+// o = sum o_s 2^(m_s - M) / l. Each part's o is read by as many lanes as hold it four values a
+// lane, so that a workgroup has 1024 / dim parts (of up to 256 dimensions) on their way at once.
+template <int QT, int LANES>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     typedef typename ElemOf<QT>::type elem;
-    const uint32_t lane = threadIdx.x & 63;
-    const uint64_t rh = static_cast<uint64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (rh >= static_cast<uint64_t>(a.n_rows) * a.n_heads) return;
-    const uint32_t row = static_cast<uint32_t>(rh / a.n_heads), head = static_cast<uint32_t>(rh % a.n_heads);
+    constexpr uint32_t kAtOnce = 256 / LANES;
+    __shared__ f32x4 sh_o[256];
+    __shared__ float sh_l[kAtOnce];
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    const uint32_t row = blockIdx.x / a.n_heads, head = blockIdx.x % a.n_heads;
+    const uint64_t rh = blockIdx.x;
     const uint32_t le = count_le(a.cu, a.n_batch + 1, row);
     if (le == 0 || le > a.n_batch) return;
     const uint32_t b = le - 1;
@@ -33,22 +36,28 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
 #pragma unroll
     for (int x = 32; x > 0; x >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x, 64));
     const float ref = top == -kInf ? 0.0f : top;
-    float l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t part = tid / LANES, x = tid % LANES * 4;
+    float l = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-    for (uint32_t s = 0; s < n; ++s) {
+    for (uint32_t s = part; s < n; s += kAtOnce) {
         const uint64_t at = s * step + rh;
         const float f = exp2_hw(a.part_ml[2 * at] - ref);
         l = __builtin_fmaf(a.part_ml[2 * at + 1], f, l);
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-            if (lane + 64 * x < a.dim) o[x] = __builtin_fmaf(a.part[at * a.dim + lane + 64 * x], f, o[x]);
+        if (x < a.dim) o += *reinterpret_cast<const f32x4*>(a.part + at * a.dim + x) * f;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    elem* p = static_cast<elem*>(a.out) + row * a.out_stride + static_cast<uint64_t>(head) * a.dim;
+    sh_o[tid] = o;
+    if (x == 0) sh_l[part] = l;
+    __syncthreads();
+    if (part != 0 || x >= a.dim) return;
 #pragma unroll
-    for (int x = 0; x < 4; ++x)
-        if (lane + 64 * x < a.dim) p[lane + 64 * x] = static_cast<elem>(o[x] * inv);
-    if (a.lse && lane == 0) a.lse[rh] = l == 0.0f ? -kInf : (top + __builtin_amdgcn_logf(l)) * kLn2;
+    for (uint32_t p = 1; p < kAtOnce; ++p) {
+        o += sh_o[p * LANES + tid];
+        l += sh_l[p];
+    }
+    store_out<QT>(static_cast<elem*>(a.out) + row * a.out_stride + static_cast<uint64_t>(head) * a.dim + x,
+                  o * (l == 0.0f ? 0.0f : 1.0f / l));
+    if (a.lse && x == 0) a.lse[rh] = l == 0.0f ? -kInf : (top + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 }  // namespace dev
@@ -59,8 +68,10 @@ namespace {
 
 template <int QT>
 int32_t launch_join(hipStream_t s, const AttnArgs& a, const char* action) {
-    const uint64_t rows = static_cast<uint64_t>(a.n_rows) * a.n_heads;
-    hipLaunchKernelGGL(attn_join_kernel<QT>, dim3(static_cast<uint32_t>((rows + 3) / 4)), dim3(256), 0, s, a);
+    const dim3 grid(a.n_rows * a.n_heads);
+    if (a.dim <= 64) hipLaunchKernelGGL((attn_join_kernel<QT, 16>), grid, dim3(256), 0, s, a);
+    else if (a.dim <= 128) hipLaunchKernelGGL((attn_join_kernel<QT, 32>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_join_kernel<QT, 64>), grid, dim3(256), 0, s, a);
     OBJ_HIP(hipGetLastError(), action);
     return 0;
 }
@@ -128,7 +139,7 @@ int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream
     const uint64_t len = max_len < most ? max_len : most;
     // one wave's 32 rows: each wave reads keys of its own; more: 128 rows share the tiles
     const bool stream_form = rows <= 32;
-    a.n_tiles = static_cast<uint32_t>(stream_form ? (rows + 31) / 32 : (rows + 127) / 128);
+    a.n_tiles = static_cast<uint32_t>(stream_form ? 1 : (rows + 127) / 128);
     // Keys are cut so that there are about 2048 workgroups if every sequence were the
     // longest, in chunks of whole 256 keys.
     const uint64_t units = n_batch * a.n_kv * a.n_tiles;
@@ -144,7 +155,8 @@ int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream
         a.part = static_cast<float*>(ws);
         a.part_ml = a.part + parts * dim;
     }
-    OBJ_TRY(stream_form ? launch_attn_stream(s, dtype, c.dtype, a, action) : launch_attn_cached_block(s, dtype, c.dtype, a, action));
+    OBJ_TRY(stream_form ? launch_attn_stream(s, dtype, c.dtype, static_cast<uint32_t>(rows), a, action)
+                        : launch_attn_cached_block(s, dtype, c.dtype, a, action));
     if (splits == 1) return 0;
     if (dtype == kDtF32) return launch_join<kDtF32>(s, a, action);
     if (dtype == kDtF16) return launch_join<kDtF16>(s, a, action);

@@ -8,30 +8,36 @@ using namespace dev;
 
 namespace {
 
-template <int Q, int K, int DT>
+template <int Q, int K, int DT, int ROWS>
 int32_t launch(hipStream_t s, const AttnArgs& a, const char* action) {
-    const uint64_t x = static_cast<uint64_t>(a.n_splits) * a.n_tiles;
+    const uint64_t groups = static_cast<uint64_t>(a.n_splits) * a.n_batch * a.n_kv;
+    const uint64_t x = (groups + 7) / 8 * 8 * a.n_tiles;
     if (x > 0x7FFFFFFFull) OBJ_FAIL(kInvalidInput, action, "too many workgroups for one launch");
-    hipLaunchKernelGGL((attn_stream_kernel<Q, K, DT>), dim3(static_cast<uint32_t>(x), a.n_kv, a.n_batch), dim3(64 * Stream<K, DT>::kWaves), 0, s, a);
+    hipLaunchKernelGGL((attn_stream_kernel<Q, K, DT, ROWS>), dim3(static_cast<uint32_t>(x)), dim3(64 * Stream<K, DT, ROWS>::kWaves), 0, s, a);
     OBJ_HIP(hipGetLastError(), action);
     return 0;
 }
 
+template <int Q, int K, int ROWS>
+int32_t launch_rows(hipStream_t s, const AttnArgs& a, const char* action) {
+    if (a.dim <= 64) return launch<Q, K, 64, ROWS>(s, a, action);
+    if (a.dim <= 128) return launch<Q, K, 128, ROWS>(s, a, action);
+    return launch<Q, K, 256, ROWS>(s, a, action);
+}
+
 template <int Q, int K>
-int32_t launch_dim(hipStream_t s, const AttnArgs& a, const char* action) {
-    if (a.dim <= 64) return launch<Q, K, 64>(s, a, action);
-    if (a.dim <= 128) return launch<Q, K, 128>(s, a, action);
-    return launch<Q, K, 256>(s, a, action);
+int32_t launch_dim(hipStream_t s, uint32_t rows, const AttnArgs& a, const char* action) {
+    return rows <= 16 ? launch_rows<Q, K, 16>(s, a, action) : launch_rows<Q, K, 32>(s, a, action);
 }
 
 }  // namespace
 
-int32_t launch_attn_stream(hipStream_t s, int32_t q_type, int32_t kv_type, const AttnArgs& a, const char* action) {
-    if (q_type == kDtF16) return launch_dim<kDtF16, kDtF16>(s, a, action);
-    if (q_type == kDtBF16) return launch_dim<kDtBF16, kDtBF16>(s, a, action);
-    if (kv_type == kDtF32) return launch_dim<kDtF32, kDtF32>(s, a, action);
-    if (kv_type == kDtF16) return launch_dim<kDtF32, kDtF16>(s, a, action);
-    return launch_dim<kDtF32, kDtBF16>(s, a, action);
+int32_t launch_attn_stream(hipStream_t s, int32_t q_type, int32_t kv_type, uint32_t rows, const AttnArgs& a, const char* action) {
+    if (q_type == kDtF16) return launch_dim<kDtF16, kDtF16>(s, rows, a, action);
+    if (q_type == kDtBF16) return launch_dim<kDtBF16, kDtBF16>(s, rows, a, action);
+    if (kv_type == kDtF32) return launch_dim<kDtF32, kDtF32>(s, rows, a, action);
+    if (kv_type == kDtF16) return launch_dim<kDtF32, kDtF16>(s, rows, a, action);
+    return launch_dim<kDtF32, kDtBF16>(s, rows, a, action);
 }
 
 }  // namespace objeta

@@ -1,11 +1,11 @@
-// attn_stream.hpp — attention of up to 32 rows of one sequence and key/value head over the
-// cache: decode, and small trees of drafts. Bound by reading keys and values once.
+// attn_stream.hpp — attention of up to 16 or 32 rows of one sequence and key/value head over
+// the cache: decode, and small trees of drafts. Bound by reading keys and values once.
 //
 // Every wave walks key tiles of its own (the chunk's tiles dealt out in turn) with its own
 // part of LDS, so no barrier holds a wave's loads up: the next tile is in flight in registers
 // while the present one is multiplied. The waves' running softmaxes are joined at the end
-// through LDS. The matrix units multiply 32 rows whether or not there are as many; at 16 bits
-// they would keep up with ten times the memory's rate.
+// through LDS. The matrix units multiply 16 or 32 rows whether or not there are as many; at
+// 16 bits they would keep up with ten times the memory's rate.
 #pragma once
 
 #include "attn_tile.hpp"
@@ -13,13 +13,16 @@
 namespace objeta {
 namespace dev {
 
-template <int KT, int DT>
+template <int KT, int DT, int ROWS>
 struct Stream {
-    typedef Rows<KT, DT> R;
+    typedef Rows<KT, DT, ROWS> R;
+    static_assert(64 % R::kUnits == 0 && 64 / R::kUnits <= 8, "the keys of one load in one group of eight");
     static constexpr int kLoads = 32 * R::kUnits / 64;  // 16-byte units of K (and of V) a lane stages
     static constexpr int kWave = 2 * 32 * R::kBytes;    // LDS of a wave: a tile of K and one of V
     static constexpr int kWaves = kWave <= 16384 ? 4 : (kWave <= 32768 ? 2 : 1);
-    static_assert(kWave >= 32 * DT * 4, "o of 32 rows in a wave's part");
+    static_assert(kWave >= ROWS * DT * 4, "o of a wave's rows in its part");
+    // waves a SIMD: two where a wave's part of LDS lets eight be on a CU
+    static constexpr int kPerSimd = kWave <= 16384 ? 2 : 1;
 };
 
 __device__ __forceinline__ void wave_lds_fence() {
@@ -28,19 +31,22 @@ __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <int QT, int KT, int DT>
-__global__ __launch_bounds__((64 * Stream<KT, DT>::kWaves)) void attn_stream_kernel(AttnArgs a) {
-    typedef Math<QT, KT, DT> M;
-    typedef Rows<KT, DT> R;
-    typedef Stream<KT, DT> S;
+template <int QT, int KT, int DT, int ROWS>
+__global__ __launch_bounds__((64 * Stream<KT, DT, ROWS>::kWaves),
+                             (ROWS == 32 ? 1 : Stream<KT, DT, ROWS>::kPerSimd)) void attn_stream_kernel(AttnArgs a) {
+    typedef Math<QT, KT, DT, ROWS> M;
+    typedef Rows<KT, DT, ROWS> R;
+    typedef Stream<KT, DT, ROWS> S;
     constexpr int kWaves = S::kWaves;
     __shared__ alignas(16) char lds[kWaves][S::kWave];
-    __shared__ float sh_m[kWaves][32], sh_l[kWaves][32];
+    __shared__ float sh_m[kWaves][ROWS], sh_l[kWaves][ROWS];
     __shared__ int32_t sh_bad;
 
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-    const uint32_t split = blockIdx.x % a.n_splits, head = blockIdx.y, b = blockIdx.z;
-    uint32_t tile = blockIdx.x / a.n_splits;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane / ROWS, mine = lane % ROWS;
+    const CachedItem item(a, blockIdx.x);
+    if (!item.any) return;
+    const uint32_t split = item.split, head = item.head, b = item.b;
+    uint32_t tile = item.tile;
     const int32_t row0 = a.cu[b], end = a.cu[b + 1], n_q = end - row0;
     if (row0 < 0 || end < row0 || static_cast<uint32_t>(end) > a.n_rows) {
         if (tid == 0) atomicOr(a.err, kErrIndex);
@@ -69,8 +75,8 @@ __global__ __launch_bounds__((64 * Stream<KT, DT>::kWaves)) void attn_stream_ker
     char* v_lds = lds[wave] + 32 * R::kBytes;
     const uint32_t kx = M::k_first(lane), vx = M::v_first(lane);
 
-    for (; static_cast<uint64_t>(tile) * 32 < n_m; tile += a.n_tiles) {
-        const uint32_t m = tile * 32 + (lane & 31);
+    for (; static_cast<uint64_t>(tile) * ROWS < n_m; tile += a.n_tiles) {
+        const uint32_t m = tile * ROWS + mine;
         const bool real = m < n_m;
         const uint32_t i = real ? m / a.group : 0, q_head = head * a.group + (real ? m % a.group : 0);
         const uint64_t row = static_cast<uint64_t>(row0) + i;
@@ -80,16 +86,12 @@ __global__ __launch_bounds__((64 * Stream<KT, DT>::kWaves)) void attn_stream_ker
             if (a.tree) view = RowView{0, len - 1, base, a.tree[row]};
             else view.hi = base + static_cast<int32_t>(i);
         }
-        typename M::frag q[DT / 16];
-        const typename M::qelem* qp =
-            static_cast<const typename M::qelem*>(a.q) + row * a.q_stride + static_cast<uint64_t>(q_head) * a.dim;
-#pragma unroll
-        for (int s = 0; s < DT / 16; ++s) {
-            const uint32_t d = 16 * s + 8 * h;
-            q[s] = (real && d < a.dim) ? M::load_q(qp + d) : M::zero();
-        }
+        typename M::Query q;
+        float scale = a.scale_log2;
+        M::load_q(q, static_cast<const typename M::qelem*>(a.q) + row * a.q_stride + static_cast<uint64_t>(q_head) * a.dim, real,
+                  a.dim, lane, scale);
         if (tid == 0) sh_bad = 0;
-        RowState<DT> st;
+        RowState<M> st;
         st.clear();
 
         // tiles k_lo + 32 (wave + kWaves t)
@@ -101,23 +103,28 @@ __global__ __launch_bounds__((64 * Stream<KT, DT>::kWaves)) void attn_stream_ker
             if (lane < 4 && slot < k_end) p = kv.page_of(static_cast<uint32_t>(slot), bad);
             return p;
         };
+        // Unit u = 64 x + lane of a tile: key u / kUnits. The keys of one x lie in one group of
+        // eight, so in one page: the address is uniform but for the lane's place, the same for all x.
+        const uint32_t l_key = lane / R::kUnits, l_unit = lane % R::kUnits;
+        const uint32_t place = (l_key * a.dim + l_unit * (16 / R::kEs)) * R::kEs;
+        const bool whole = l_unit * (16 / R::kEs) < a.dim;
         auto load_tile = [&](int32_t k0, int32_t pages) {
 #pragma unroll
             for (int x = 0; x < S::kLoads; ++x) {
-                const uint32_t u = x * 64 + lane, key = u / R::kUnits, c = u % R::kUnits;
-                const int32_t page = __shfl(pages, static_cast<int>(key >> 3), 64);
-                const int32_t slot = k0 + static_cast<int32_t>(key);
+                constexpr uint32_t per = 64 / R::kUnits;  // keys of one x
+                const uint32_t key = x * per;
+                const int32_t page = __builtin_amdgcn_readlane(pages, key >> 3);
+                const uint64_t at = kv.paged_at(page, static_cast<uint32_t>(k0) + key);
                 rk[x] = u32x4a{0, 0, 0, 0};
                 rv[x] = u32x4a{0, 0, 0, 0};
-                if (slot < k_end && c * (16 / R::kEs) < a.dim) {
-                    const uint64_t at = kv.paged_at(page, static_cast<uint32_t>(slot)) + c * (16 / R::kEs);
-                    rk[x] = *reinterpret_cast<const u32x4a*>(kv.k + at);
-                    rv[x] = *reinterpret_cast<const u32x4a*>(kv.v + at);
+                if (whole && k0 + static_cast<int32_t>(key + l_key) < k_end) {
+                    rk[x] = *reinterpret_cast<const u32x4a*>(reinterpret_cast<const char*>(kv.k + at) + place);
+                    rv[x] = *reinterpret_cast<const u32x4a*>(reinterpret_cast<const char*>(kv.v + at) + place);
                 }
             }
         };
         const int32_t step = 32 * kWaves;
-        int32_t k0 = k_lo + 32 * static_cast<int32_t>(wave);
+        int32_t k0 = k_lo + 32 * static_cast<int32_t>(__builtin_amdgcn_readfirstlane(wave));
         int32_t pages = 0;
         if (k0 < k_end) {
             load_tile(k0, load_pages(k0));
@@ -135,47 +142,49 @@ __global__ __launch_bounds__((64 * Stream<KT, DT>::kWaves)) void attn_stream_ker
                 if (k_end - k0 > 2 * step) pages = load_pages(k0 + 2 * step);
             }
             wave_lds_fence();
-            f32x16 s[1];
-            s[0] = scores<M, DT>(q, k_lds, lane, kx);
+            Scores<M> s[1];
+            scores<M>(s[0], q, k_lds, lane, kx);
             if (a.tree || k0 + 32 > base + 1 || k0 + 32 > k_end) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int32_t key = k0 + (r & 3) + 8 * (r >> 2) + 4 * static_cast<int32_t>(h);
-                    if (!(view.sees(key) && key < k_end)) s[0][r] = -kInf;
-                }
+                for (int n = 0; n < M::kKeyTiles; ++n)
+#pragma unroll
+                    for (int r = 0; r < M::kRegs; ++r) {
+                        const int32_t key = k0 + static_cast<int32_t>(M::key_of(n, r, h));
+                        if (!(view.sees(key) && key < k_end)) s[0].s[n][r] = -kInf;
+                    }
             }
-            accumulate<M, DT, 1>(st, s, a.scale_log2, v_lds, vx);
+            accumulate<M, 1>(st, s, scale, v_lds, vx);
             wave_lds_fence();
         }
 
         // ---- the waves' results into one: a wave's o goes to its own part of LDS
-        st.l += other_half(st.l);
-        if (h == 0) sh_m[wave][lane] = st.m, sh_l[wave][lane] = st.l;
+        st.l = row_sum<ROWS>(st.l);
+        if (h == 0) sh_m[wave][mine] = st.m, sh_l[wave][mine] = st.l;
         __syncthreads();
         if (bad) atomicOr(&sh_bad, 1);
-        float top = sh_m[0][lane & 31];
+        float top = sh_m[0][mine];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, sh_m[w][lane & 31]);
+        for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, sh_m[w][mine]);
         const float ref = top == -kInf ? 0.0f : top;
         float l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) l += sh_l[w][lane & 31] * exp2_hw(sh_m[w][lane & 31] - ref);
+        for (int w = 0; w < kWaves; ++w) l += sh_l[w][mine] * exp2_hw(sh_m[w][mine] - ref);
         const float f = exp2_hw(st.m - ref);
-        const bool odd = not_finite<DT>(st);
+        const bool odd = not_finite<M>(st);
         if (odd && lane == 0) atomicOr(&sh_bad, 2);
         float* o_lds = reinterpret_cast<float*>(lds[wave]);  // [dimension / 4][row][4]
 #pragma unroll
-        for (int d = 0; d < DT / 32; ++d)
+        for (int d = 0; d < M::kOut; ++d)
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-                *reinterpret_cast<f32x4*>(o_lds + ((8 * d + 2 * r + h) * 32 + (lane & 31)) * 4) =
+            for (int r = 0; r < M::kRegs / 4; ++r)
+                *reinterpret_cast<f32x4*>(o_lds + (out_dim<M>(d, r, h) / 4 * ROWS + mine) * 4) =
                     f32x4{st.o[d][4 * r] * f, st.o[d][4 * r + 1] * f, st.o[d][4 * r + 2] * f, st.o[d][4 * r + 3] * f};
         __syncthreads();
         const int32_t state = sh_bad;
         if (usable && state == 2) {
             // some product met an infinity or NaN: the rows again, key by key (see row_by_row)
-            for (uint32_t r = wave; r < 32; r += kWaves) {
-                const uint32_t r_m = tile * 32 + r;
+            for (uint32_t r = wave; r < ROWS; r += kWaves) {
+                const uint32_t r_m = tile * ROWS + r;
                 if (r_m >= n_m) break;
                 const uint32_t r_head = head * a.group + r_m % a.group, r_i = r_m / a.group;
                 const uint64_t r_row = static_cast<uint64_t>(row0) + r_i;
@@ -193,13 +202,13 @@ __global__ __launch_bounds__((64 * Stream<KT, DT>::kWaves)) void attn_stream_ker
             const bool poison = !usable || (state & 1);
             if (poison) l = __builtin_nanf("");
             const float inv = a.n_splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
-            // this thread: row lane % 32, groups of four dimensions
-            for (uint32_t g = wave * 2 + h; g * 4 < a.dim; g += 2 * kWaves) {
+            // this thread: its row, groups of four dimensions
+            for (uint32_t g = wave * (64 / ROWS) + h; g * 4 < a.dim; g += kWaves * (64 / ROWS)) {
                 f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int w = 0; w < kWaves; ++w)
                     sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w]) +
-                                                           (g * 32 + (lane & 31)) * 4);
+                                                           (g * ROWS + mine) * 4);
                 sum *= inv;
                 if (poison) sum = f32x4{l, l, l, l};
                 if (!real) continue;

@@ -1,26 +1,29 @@
-// attn_tile.hpp — the tile of attention that all its kernels share: 32 query rows of a wave
-// against 32 keys on the matrix cores, with the running softmax.
+// attn_tile.hpp — the tile of attention that all its kernels share: kRows = 32 or 16 query
+// rows of a wave against 32 keys on the matrix cores, with the running softmax.
 //
 // Mathematics, for a row's scores s_j = scale q . k_j in units of log 2: with m a running
 // reference near the largest score, l = sum 2^(s_j - m) and o = sum 2^(s_j - m) v_j; when m
 // grows, l and o take the factor 2^(m - m'). The result is o / l, and ln 2 (m + log2 l).
 //
-// Layout. The scores are computed transposed, S^T = K Q^T: the 32 x 32 result then holds
-// query row n = lane % 32 in its columns, and a lane 16 keys of its one row (the other 16 in
-// lane ^ 32), so that maxima and sums are taken within a lane and across one swap, and
-// rescaling o^T is a factor of the lane. The same registers are the product O^T += V^T P^T's
-// second operand without any exchange: the sum over keys may run in any order, so its index
-// (lane half h, element j) stands for the key 16 t + 8 (j / 4) + 4 h + j % 4 that the lane
-// holds. V^T comes from V's rows in LDS by the transposing 64-bit read, whose 4 x 16 blocks
-// are those four keys.
+// Layout. The scores are computed transposed, S^T = K Q^T: a lane then holds keys of one query
+// row (lane % kRows), and the row's other keys lie in the lanes of the same remainder, so that
+// maxima and sums are taken within a lane and across one or two exchanges, and rescaling o^T
+// is a factor of the lane. The same registers are the product O^T += V^T P^T's second operand
+// without any exchange: the sum over keys may run in any order, so its index (lane part h =
+// lane / kRows, element j) stands for the key that the lane holds there. V^T comes from V's
+// rows in LDS by the transposing 64-bit read, whose blocks of 4 keys x 16 dimensions are what
+// a lane's four consecutive elements name.
 //
 // LDS rows are the keys' rows of 16-byte units; a unit's place within its row is exchanged
-// by an exclusive or with bits of the key (swz_k, swz_v), so that the 16 lanes of a read
-// phase fall into different banks.
+// by an exclusive or with bits of the key (swz_k, swz_v), so that the lanes of a read phase
+// fall into different banks.
 //
-// f16 and bf16 use the 32x32x16 products of their type. With float queries each of these
-// becomes eight 32x32x2 float products over the same fragments (16-bit keys and values
-// converted when read): 1/16 of the rate, but no rounding of q or of the probabilities.
+// Types. f16 and bf16 use the products of their type, probabilities rounded to it. Float
+// queries on a 16-bit cache are split into parts of the cache's type whose sum holds 22 (f16,
+// two parts of the row times a power of two) or 24 bits (bf16, three), each product is exact,
+// and so are the probabilities split: a float result at two or three 16-bit products instead
+// of the eight float ones that a 16-bit product's worth of float products takes at a
+// sixteenth of the rate. Float caches use the float products.
 #pragma once
 
 #include "kv_common.hpp"
@@ -47,8 +50,8 @@ template <int T> struct ElemOf { typedef float type; };
 template <> struct ElemOf<kDtF16> { typedef _Float16 type; };
 template <> struct ElemOf<kDtBF16> { typedef __bf16 type; };
 
-// Rows of DT elements of type KT in LDS.
-template <int KT, int DT>
+// Rows of DT elements of type KT in LDS, read by tiles of ROWS query rows.
+template <int KT, int DT, int ROWS>
 struct Rows {
     static constexpr int kEs = KT == kDtF32 ? 4 : 2;
     static constexpr int kBytes = DT * kEs;
@@ -60,141 +63,215 @@ struct Rows {
         else return (key >> 2) & 3;
     }
     // 16-bit: the 64-byte parts that one transposing read takes from four keys; float: the
-    // 128-byte parts of keys four apart
+    // parts of ROWS dimensions of keys four apart
     static __device__ __forceinline__ uint32_t swz_v(uint32_t key) {
-        if constexpr (KT == kDtF32) return kUnits % 16 == 0 ? ((key >> 2) & 1) << 3 : 0;
+        if constexpr (KT == kDtF32)
+            return kUnits % 16 ? 0 : (ROWS == 32 ? ((key >> 2) & 1) << 3 : ((key >> 2) & 3) << 2);
         else if constexpr (kUnits % 16 == 0) return (key & 3) << 2;
         else if constexpr (kUnits % 8 == 0) return ((key >> 1) & 1) << 2;
         else return 0;
     }
 };
 
+template <int ROWS> struct AccOf { typedef f32x16 type; };
+template <> struct AccOf<16> { typedef f32x4 type; };
+
 // The products of one type of queries (QT) with one type of keys and values (KT).
-template <int QT, int KT, int DT>
+template <int QT, int KT, int DT, int ROWS>
 struct Math {
     static_assert(QT == KT || QT == kDtF32, "float queries, or queries of the cache's type");
-    typedef Rows<KT, DT> R;
-    static constexpr bool kFloat = QT == kDtF32;
+    typedef Rows<KT, DT, ROWS> R;
+    typedef typename AccOf<ROWS>::type acc;
+    static constexpr int kRows = ROWS;
+    static constexpr int kRegs = ROWS == 32 ? 16 : 4;   // of an accumulator
+    static constexpr int kKeyTiles = 32 / ROWS;         // accumulators that hold 32 keys' scores
+    static constexpr int kStep = 8 * (64 / ROWS);       // dimensions (keys) of one product
+    static constexpr int kSteps = DT / kStep;
+    static constexpr int kOut = DT / ROWS;              // accumulators of o
+    static constexpr int kDim = DT;
+    static constexpr bool kFloat = KT == kDtF32;
+    static constexpr int kParts = QT == KT ? 1 : (KT == kDtF16 ? 2 : 3);
     typedef typename ElemOf<QT>::type qelem;
     typedef typename ElemOf<KT>::type kelem;
-    template <int T> struct FragOf { typedef f32x8 type; };
     typedef typename std::conditional<kFloat, f32x8,
                                       typename std::conditional<KT == kDtF16, h16x8, b16x8>::type>::type frag;
+    struct Query {
+        frag f[kParts][kSteps];
+    };
     // f16 probabilities are scaled by 2^7 (with m's slack of 2^8 still below the largest
     // value), which keeps those down to 2^-21 of the largest in its normal range
-    static constexpr float kShift = (!kFloat && KT == kDtF16) ? 7.0f : 0.0f;
+    static constexpr float kShift = KT == kDtF16 ? 7.0f : 0.0f;
 
-    static __device__ __forceinline__ frag zero() {
-        frag f{};
-        return f;
+    static __device__ __forceinline__ acc zero() {
+        acc c;
+#pragma unroll
+        for (int r = 0; r < kRegs; ++r) c[r] = 0.0f;
+        return c;
     }
-    static __device__ __forceinline__ frag load_q(const qelem* p) {
-        if constexpr (kFloat) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
-            return f32x8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
-        } else {
-            return *reinterpret_cast<const frag*>(p);
-        }
-    }
-    static __device__ __forceinline__ f32x16 mma(const frag& a, const frag& b, f32x16 c) {
+    static __device__ __forceinline__ acc mma(const frag& a, const frag& b, acc c) {
         if constexpr (kFloat) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[j], b.v[j], c, 0, 0, 0);
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (ROWS == 32) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a.v[j], b.v[j], c, 0, 0, 0);
+                else c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
+            }
             return c;
         } else if constexpr (KT == kDtF16) {
-            return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+            if constexpr (ROWS == 32) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+            else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
         } else {
-            return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+            if constexpr (ROWS == 32) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+            else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
         }
     }
-    template <class V>
-    static __device__ __forceinline__ frag widen(const V& x) {
-        f32x8 f;
+    // Splits eight floats into the parts of an operand, each the rest's nearest value.
+    template <class Put>
+    static __device__ __forceinline__ void split(const float* x, Put put) {
+        float rest[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f.v[j] = static_cast<float>(x[j]);
-        return f;
-    }
-    // Dimensions 16 s + 8 h .. + 8 of this lane's key (lane % 32 of the tile): K as the first
-    // operand. `row` is the key's LDS row, `x0` its swizzled first unit in bytes.
-    static __device__ __forceinline__ uint32_t k_first(uint32_t lane) {
-        const uint32_t h = lane >> 5, key = lane & 31;
-        return ((KT == kDtF32 ? 2 * h : h) ^ R::swz_k(key)) * 16;
-    }
-    static __device__ __forceinline__ frag lds_k(const char* row, uint32_t x0, int s) {
-        if constexpr (KT == kDtF32) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(row + (x0 ^ (64 * s)));
-            const f32x4 b = *reinterpret_cast<const f32x4*>(row + (x0 ^ (64 * s) ^ 16));
-            return f32x8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
-        } else if constexpr (kFloat) {
-            typedef typename std::conditional<KT == kDtF16, h16x8, b16x8>::type v8;
-            return widen(*reinterpret_cast<const v8*>(row + (x0 ^ (32 * s))));
-        } else {
-            return *reinterpret_cast<const frag*>(row + (x0 ^ (32 * s)));
+        for (int j = 0; j < 8; ++j) rest[j] = x[j];
+#pragma unroll
+        for (int p = 0; p < kParts; ++p) {
+            frag f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                f[j] = static_cast<kelem>(rest[j]);
+                if (p + 1 < kParts) rest[j] -= static_cast<float>(f[j]);
+            }
+            put(p, f);
         }
     }
-    // This lane's place for V: byte offset from a group of 16 keys' first row to the first
-    // of its reads at dimensions 0..31.
-    static __device__ __forceinline__ uint32_t v_first(uint32_t lane) {
-        const uint32_t h = lane >> 5;
-        if constexpr (KT == kDtF32) {
-            return 4 * h * R::kBytes + (R::swz_v(4 * h) * 16) + (lane & 31) * 4;
+    // This lane's part of its row's query: dimensions kStep i + 8 h .. + 8. `scale` takes the
+    // power of two that the row was multiplied by.
+    static __device__ __forceinline__ void load_q(Query& q, const qelem* p, bool real, uint32_t dim, uint32_t lane,
+                                                  float& scale) {
+        const uint32_t h = lane / ROWS;
+        if constexpr (QT != kDtF32) {
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const uint32_t d = kStep * i + 8 * h;
+                frag z{};
+                q.f[0][i] = real && d < dim ? *reinterpret_cast<const frag*>(p + d) : z;
+            }
         } else {
-            const uint32_t l = lane & 15, ds = (lane >> 4) & 1, key = 4 * h + (l >> 2);
+            float x[kSteps][8];
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const uint32_t d = kStep * i + 8 * h;
+                f32x4 a = {0.0f, 0.0f, 0.0f, 0.0f}, b = a;
+                if (real && d < dim) {
+                    a = *reinterpret_cast<const f32x4*>(p + d);
+                    b = *reinterpret_cast<const f32x4*>(p + d + 4);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[i][j] = a[j], x[i][4 + j] = b[j];
+            }
+            if constexpr (KT == kDtF16) {
+                // the row's largest value to [2^13, 2^14): f16's range, with its sums' room
+                float top = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) top = __builtin_fmaxf(top, __builtin_fabsf(x[i][j]));
+#pragma unroll
+                for (int s = ROWS; s < 64; s <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, s, 64));
+                int e = 0;
+                if (top > 0.0f && top < kInf) e = 14 - __builtin_amdgcn_frexp_expf(top);
+                e = e > 120 ? 120 : e;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[i][j] = __builtin_amdgcn_ldexpf(x[i][j], e);
+                scale = __builtin_amdgcn_ldexpf(scale, -e);
+            }
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                if constexpr (kFloat) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) q.f[0][i].v[j] = x[i][j];
+                } else {
+                    split(x[i], [&](int part, const frag& f) { q.f[part][i] = f; });
+                }
+            }
+        }
+    }
+    // Dimensions kStep i + 8 h .. + 8 of this lane's key (lane % ROWS of the tile): K as the
+    // first operand. `row` is the key's LDS row, `x0` its swizzled first unit in bytes.
+    static __device__ __forceinline__ uint32_t k_first(uint32_t lane) {
+        const uint32_t h = lane / ROWS, key = lane % ROWS;
+        return ((kFloat ? 2 * h : h) ^ R::swz_k(key)) * 16;
+    }
+    static __device__ __forceinline__ frag lds_k(const char* row, uint32_t x0, int i) {
+        if constexpr (kFloat) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(row + (x0 ^ (4 * kStep * i)));
+            const f32x4 b = *reinterpret_cast<const f32x4*>(row + (x0 ^ (4 * kStep * i) ^ 16));
+            return f32x8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+        } else {
+            return *reinterpret_cast<const frag*>(row + (x0 ^ (2 * kStep * i)));
+        }
+    }
+    // The key of score register r of tile n, and the keys of element j of a group of kStep
+    // keys (offset from the lane part's first).
+    static __device__ __forceinline__ uint32_t key_of(int n, int r, uint32_t h) {
+        return ROWS == 32 ? (r & 3) + 8 * (r >> 2) + 4 * h : 16 * n + r + 4 * h;
+    }
+    static constexpr int kFar = ROWS == 32 ? 8 : 16;  // elements 4 .. 7 lie this many keys behind 0 .. 3
+    // This lane's place for V: byte offset from a group of kStep keys' first row to the first
+    // of its reads at dimensions 0 .. ROWS.
+    static __device__ __forceinline__ uint32_t v_first(uint32_t lane) {
+        const uint32_t h = lane / ROWS;
+        if constexpr (kFloat) {
+            return 4 * h * R::kBytes + R::swz_v(4 * h) * 16 + (lane % ROWS) * 4;
+        } else {
+            const uint32_t l = lane & 15, ds = ROWS == 32 ? (lane >> 4) & 1 : 0, key = 4 * h + (l >> 2);
             const uint32_t unit = 2 * ds + ((l & 3) >> 1);
             return key * R::kBytes + ((unit ^ R::swz_v(key)) * 16) + (l & 1) * 8;
         }
     }
-    // V^T of 16 keys (rows from `rows` on) at dimensions 32 dd + lane % 32.
+    // V^T of kStep keys (rows from `rows` on) at dimensions ROWS dd + lane % ROWS.
     static __device__ __forceinline__ frag lds_v(const char* rows, uint32_t v0, int dd) {
-        if constexpr (KT == kDtF32) {
+        const char* p = rows + (v0 ^ (ROWS * R::kEs * dd));
+        if constexpr (kFloat) {
             f32x8 f;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                f.v[j] = *reinterpret_cast<const float*>(rows + (v0 ^ (128 * dd)) + (8 * (j / 4) + j % 4) * R::kBytes);
+                f.v[j] = *reinterpret_cast<const float*>(p + (kFar * (j / 4) + j % 4) * R::kBytes);
             return f;
         } else {
-            const char* p = rows + (v0 ^ (64 * dd));
             const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_char*)(p));
             const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(lds_char*)(p + 8 * R::kBytes));
+                (__attribute__((address_space(3))) s16x4*)(lds_char*)(p + kFar * R::kBytes));
             const s16x8 v = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            if constexpr (kFloat) {
-                typedef typename std::conditional<KT == kDtF16, h16x8, b16x8>::type v8;
-                return widen(__builtin_bit_cast(v8, v));
-            } else {
-                return __builtin_bit_cast(frag, v);
-            }
-        }
-    }
-    // Eight probabilities as the second operand: rounded to nearest, as the output is.
-    static __device__ __forceinline__ frag pack(const float* p) {
-        if constexpr (kFloat) {
-            return f32x8{{p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]}};
-        } else {
-            frag f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = static_cast<kelem>(p[j]);
-            return f;
+            return __builtin_bit_cast(frag, v);
         }
     }
 };
 
-// A value and its counterpart 32 lanes away.
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+// A sum or maximum over the lanes that hold one row.
+template <int ROWS>
+__device__ __forceinline__ float row_max(float x) {
+#pragma unroll
+    for (int s = ROWS; s < 64; s <<= 1) x = __builtin_fmaxf(x, __shfl_xor(x, s, 64));
+    return x;
+}
+template <int ROWS>
+__device__ __forceinline__ float row_sum(float x) {
+#pragma unroll
+    for (int s = ROWS; s < 64; s <<= 1) x += __shfl_xor(x, s, 64);
+    return x;
+}
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Running softmax of this lane's row (m and, over this lane's keys only, l), and o^T.
-template <int DT>
+template <class M>
 struct RowState {
-    float m = -kInf, l = 0.0f;
-    f32x16 o[DT / 32];
+    float m, l;
+    typename M::acc o[M::kOut];
     __device__ __forceinline__ void clear() {
         m = -kInf, l = 0.0f;
 #pragma unroll
-        for (int d = 0; d < DT / 32; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][r] = 0.0f;
+        for (int d = 0; d < M::kOut; ++d) o[d] = M::zero();
     }
     __device__ __forceinline__ float reference() const { return m == -kInf ? 0.0f : m; }
     // Takes the factor of a new reference.
@@ -203,9 +280,9 @@ struct RowState {
         m = to;
         l *= f;
 #pragma unroll
-        for (int d = 0; d < DT / 32; ++d)
+        for (int d = 0; d < M::kOut; ++d)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) o[d][r] *= f;
+            for (int r = 0; r < M::kRegs; ++r) o[d][r] *= f;
     }
 };
 
@@ -213,43 +290,68 @@ struct RowState {
 // the types, and rare after the first keys).
 constexpr float kSlack = 8.0f;
 
-// S^T of 32 keys at `rows` (LDS).
-template <class M, int DT>
-__device__ __forceinline__ f32x16 scores(const typename M::frag (&q)[DT / 16], const char* rows, uint32_t lane, uint32_t k0) {
-    f32x16 s;
+// The scores (unscaled) of 32 keys.
+template <class M>
+struct Scores {
+    typename M::acc s[M::kKeyTiles];
+};
+
+// S^T of the 32 keys at `rows` (LDS).
+template <class M>
+__device__ __forceinline__ void scores(Scores<M>& s, const typename M::Query& q, const char* rows, uint32_t lane, uint32_t k0) {
+    const char* row = rows + (lane % M::kRows) * M::R::kBytes;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = 0.0f;
-    const char* row = rows + (lane & 31) * M::R::kBytes;
+    for (int n = 0; n < M::kKeyTiles; ++n) {
+        s.s[n] = M::zero();
 #pragma unroll
-    for (int i = 0; i < DT / 16; ++i) s = M::mma(M::lds_k(row, k0, i), q[i], s);
-    return s;
+        for (int i = 0; i < M::kSteps; ++i) {
+            const typename M::frag k = M::lds_k(row + n * M::kRows * M::R::kBytes, k0, i);
+#pragma unroll
+            for (int p = 0; p < M::kParts; ++p) s.s[n] = M::mma(k, q.f[p][i], s.s[n]);
+        }
+    }
 }
 
-// The softmax step over NS tiles of raw (unscaled, masked to -inf) scores and their values.
-template <class M, int DT, int NS>
-__device__ __forceinline__ void accumulate(RowState<DT>& st, f32x16 (&s)[NS], float scale, const char* v_rows, uint32_t v0) {
-    float top = s[0][0];
+// The softmax step over NS times 32 keys of unscaled scores (unseen ones -inf) and their values.
+template <class M, int NS>
+__device__ __forceinline__ void accumulate(RowState<M>& st, Scores<M> (&s)[NS], float scale, const char* v_rows, uint32_t v0) {
+    float top = -kInf;
 #pragma unroll
     for (int n = 0; n < NS; ++n)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = __builtin_fmaxf(top, s[n][r]);
-    top = __builtin_fmaxf(top, other_half(top)) * scale;
+        for (int t = 0; t < M::kKeyTiles; ++t)
+#pragma unroll
+            for (int r = 0; r < M::kRegs; ++r) top = __builtin_fmaxf(top, s[n].s[t][r]);
+    top = row_max<M::kRows>(top) * scale;
     if (__any(top > st.m + kSlack)) st.raise(__builtin_fmaxf(st.m, top));
     const float off = M::kShift - st.reference();
+    constexpr int kGroups = 32 / M::kStep;  // of kStep keys: two of 16, or one of 32
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < kGroups; ++t) {
             float p[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                p[j] = exp2_hw(__builtin_fmaf(s[n][8 * t + j], scale, off));
+                const float x = M::kRows == 32 ? s[n].s[0][8 * t + j] : s[n].s[j / 4][j % 4];
+                p[j] = exp2_hw(__builtin_fmaf(x, scale, off));
                 st.l += p[j];
             }
-            const typename M::frag pf = M::pack(p);
-            const char* rows = v_rows + (32 * n + 16 * t) * M::R::kBytes;
+            const char* rows = v_rows + (32 * n + M::kStep * t) * M::R::kBytes;
+            if constexpr (M::kFloat) {
+                const f32x8 f = {{p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]}};
 #pragma unroll
-            for (int d = 0; d < DT / 32; ++d) st.o[d] = M::mma(M::lds_v(rows, v0, d), pf, st.o[d]);
+                for (int d = 0; d < M::kOut; ++d) st.o[d] = M::mma(M::lds_v(rows, v0, d), f, st.o[d]);
+            } else {
+                typename M::frag f[M::kParts];  // rounded to nearest, as the output is
+                M::split(p, [&](int part, const typename M::frag& x) { f[part] = x; });
+#pragma unroll
+                for (int d = 0; d < M::kOut; ++d) {
+                    const typename M::frag v = M::lds_v(rows, v0, d);
+#pragma unroll
+                    for (int part = 0; part < M::kParts; ++part) st.o[d] = M::mma(v, f[part], st.o[d]);
+                }
+            }
         }
     }
 }
@@ -272,6 +374,26 @@ struct AttnArgs {
     uint32_t chunk, n_splits, n_tiles;
     float *part, *part_ml;  // [n_splits][n_rows * n_heads][dim], [..][2]
     uint32_t* err;
+};
+
+// Which (sequence, head, split) and row tile a workgroup of a cached call takes. The splits are
+// the slowest index: short sequences have only the first ones, and workgroups go to the eight
+// XCDs in turn, so a fast split index would give the first XCDs most of the work. The groups
+// are turned by one place from split to split, so that no XCD keeps the longest sequences.
+// The row tiles of one group, which read the same keys and values, are eight apart: on one XCD.
+struct CachedItem {
+    uint32_t b, head, split, tile;
+    bool any;
+    __device__ __forceinline__ CachedItem(const AttnArgs& a, uint32_t id) {
+        const uint32_t eight = id / (8 * a.n_tiles), in = id % (8 * a.n_tiles);
+        const uint32_t per = a.n_batch * a.n_kv;
+        const uint32_t g = eight * 8 + ((in + eight * 8 / per) & 7);
+        tile = in >> 3;
+        split = g / per;
+        any = split < a.n_splits;
+        head = g % per % a.n_kv;
+        b = g % per / a.n_kv;
+    }
 };
 
 // What one row sees: keys lo .. hi, and among those from `base` on only the set bits of mask.
@@ -374,48 +496,44 @@ __device__ __forceinline__ uint64_t part_at(const AttnArgs& a, uint32_t split, u
     return (static_cast<uint64_t>(split) * a.n_rows + row) * a.n_heads + head;
 }
 
-// A wave's 32 rows done: normalised output and lse, or (several splits) the parts. Lanes 0-31
-// and 32-63 hold the same rows with different dimensions.
-template <class M, int QT, int DT>
-__device__ __forceinline__ void write_rows(const AttnArgs& a, const RowState<DT>& st, bool real, uint64_t row, uint32_t head,
-                                           uint32_t split, uint32_t lane) {
-    const float l = st.l + other_half(st.l);
-    if (!real) return;
-    const uint32_t h = lane >> 5;
-    if (a.n_splits > 1) {
-        const uint64_t at = part_at(a, split, row, head);
-        float* p = a.part + at * a.dim;
-#pragma unroll
-        for (int d = 0; d < DT / 32; ++d)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint32_t x = 32 * d + 8 * r + 4 * h;
-                if (x < a.dim)
-                    *reinterpret_cast<f32x4*>(p + x) =
-                        f32x4{st.o[d][4 * r], st.o[d][4 * r + 1], st.o[d][4 * r + 2], st.o[d][4 * r + 3]};
-            }
-        if (h == 0) {
-            a.part_ml[2 * at] = st.m - M::kShift;
-            a.part_ml[2 * at + 1] = l;
-        }
-        return;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    typename M::qelem* p = static_cast<typename M::qelem*>(a.out) + row * a.out_stride + static_cast<uint64_t>(head) * a.dim;
-#pragma unroll
-    for (int d = 0; d < DT / 32; ++d)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const uint32_t x = 32 * d + 8 * r + 4 * h;
-            if (x < a.dim)
-                store_out<QT>(p + x, f32x4{st.o[d][4 * r] * inv, st.o[d][4 * r + 1] * inv, st.o[d][4 * r + 2] * inv,
-                                           st.o[d][4 * r + 3] * inv});
-        }
-    if (a.lse && h == 0)
-        a.lse[row * a.n_heads + head] = l == 0.0f ? -kInf : (st.m - M::kShift + __builtin_amdgcn_logf(l)) * kLn2;
+// The first of the four dimensions that accumulator registers 4 r .. 4 r + 3 of o[d] hold.
+template <class M>
+__device__ __forceinline__ uint32_t out_dim(int d, int r, uint32_t h) {
+    return M::kRows * d + (M::kRows == 32 ? 8 * r : 0) + 4 * h;
 }
 
-// The same for one row of row_by_row, by a whole wave (`poison`: NaN instead).
+// A wave's rows done: normalised output and lse, or (several splits) the parts. The lanes of
+// one row hold different dimensions.
+template <class M, int QT>
+__device__ __forceinline__ void write_rows(const AttnArgs& a, const RowState<M>& st, bool real, uint64_t row, uint32_t head,
+                                           uint32_t split, uint32_t lane) {
+    const float l = row_sum<M::kRows>(st.l);
+    if (!real) return;
+    const uint32_t h = lane / M::kRows;
+    const bool parts = a.n_splits > 1;
+    const uint64_t at = parts ? part_at(a, split, row, head) : 0;
+    const float inv = parts ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+    float* pp = a.part + at * a.dim;
+    typename M::qelem* p = static_cast<typename M::qelem*>(a.out) + row * a.out_stride + static_cast<uint64_t>(head) * a.dim;
+#pragma unroll
+    for (int d = 0; d < M::kOut; ++d)
+#pragma unroll
+        for (int r = 0; r < M::kRegs / 4; ++r) {
+            const uint32_t x = out_dim<M>(d, r, h);
+            const f32x4 v = {st.o[d][4 * r] * inv, st.o[d][4 * r + 1] * inv, st.o[d][4 * r + 2] * inv, st.o[d][4 * r + 3] * inv};
+            if (x < a.dim) {
+                if (parts) *reinterpret_cast<f32x4*>(pp + x) = v;
+                else store_out<QT>(p + x, v);
+            }
+        }
+    if (h == 0) {
+        if (parts) a.part_ml[2 * at] = st.m - M::kShift, a.part_ml[2 * at + 1] = l;
+        else if (a.lse)
+            a.lse[row * a.n_heads + head] = l == 0.0f ? -kInf : (st.m - M::kShift + __builtin_amdgcn_logf(l)) * kLn2;
+    }
+}
+
+// The same for one row of row_by_row, by a whole wave.
 template <class M>
 __device__ __forceinline__ void write_row(const AttnArgs& a, float m, float l, const float (&o)[4], uint64_t row,
                                           uint32_t head, uint32_t split, uint32_t lane) {
@@ -435,13 +553,13 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, float m, float l, c
     if (a.lse && lane == 0) a.lse[row * a.n_heads + head] = l == 0.0f ? -kInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-template <int DT>
-__device__ __forceinline__ bool not_finite(const RowState<DT>& st) {
+template <class M>
+__device__ __forceinline__ bool not_finite(const RowState<M>& st) {
     float x = 0.0f;
 #pragma unroll
-    for (int d = 0; d < DT / 32; ++d)
+    for (int d = 0; d < M::kOut; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x = __builtin_fmaf(st.o[d][r], 0.0f, x);
+        for (int r = 0; r < M::kRegs; ++r) x = __builtin_fmaf(st.o[d][r], 0.0f, x);
     return __any(!(x == 0.0f));
 }
 
