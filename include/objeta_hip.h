@@ -936,11 +936,12 @@ int32_t objeta_hip_kv_append_device(objeta_hip_context* ctx, objeta_hip_stream s
  * sees the slots before len - n, and
  *   without d_tree, the slots up to its own (len - n + i);
  *   with d_tree (uint64 [n_rows], n <= 64), slot len - n + j where bit j of its mask is set.
- * A row that sees nothing gets out 0 and lse -inf. d_lse as for prompts. max_rows and
- * max_len: the most rows of an entry and the longest sequence as the host knows them; they
- * only decide how the work is cut, larger ones are computed too. Entries whose sequence,
- * length or pages are out of range, or that have more rows than the sequence tokens, get
- * NaN (bit 2). n_rows * n_q_heads < 2^31; n_batch and n_kv_heads <= 65535. */
+ * A row that sees nothing gets out 0 and lse -inf. d_lse as for prompts. max_rows: no entry
+ * has more rows (any that go past it may come out NaN, with bit 2). max_len: the longest
+ * sequence as the host knows it; it only decides how the work is cut, longer ones are
+ * computed too. Entries whose sequence, length or pages are out of range, or that have more
+ * rows than the sequence tokens, get NaN (bit 2). n_rows * n_q_heads < 2^31;
+ * n_batch <= 65535. */
 int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream stream,
                                       const objeta_hip_kv_cache* cache, uint64_t layer, const int32_t* d_seqs,
                                       const int32_t* d_cu_rows, uint64_t n_batch, uint64_t n_rows, uint64_t max_rows,

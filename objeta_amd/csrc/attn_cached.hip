@@ -50,6 +50,9 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     if (x == 0) sh_l[part] = l;
     __syncthreads();
     if (part != 0 || x >= a.dim) return;
+    // a row past what max_rows allows for has no parts
+    if ((row - lo) * (a.n_heads / a.n_kv) + head % (a.n_heads / a.n_kv) >= static_cast<uint64_t>(a.n_tiles) * a.tile_rows)
+        l = o.x = o.y = o.z = o.w = __builtin_nanf("");
 #pragma unroll
     for (uint32_t p = 1; p < kAtOnce; ++p) {
         o += sh_o[p * LANES + tid];
@@ -139,11 +142,12 @@ int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream
     const uint64_t len = max_len < most ? max_len : most;
     // one wave's 32 rows: each wave reads keys of its own; more: 128 rows share the tiles
     const bool stream_form = rows <= 32;
-    a.n_tiles = static_cast<uint32_t>(stream_form ? 1 : (rows + 127) / 128);
-    // Keys are cut so that there are about 2048 workgroups if every sequence were the
+    a.tile_rows = stream_form ? (rows <= 16 ? 16 : 32) : 128;
+    a.n_tiles = static_cast<uint32_t>((rows + a.tile_rows - 1) / a.tile_rows);
+    // Keys are cut so that there are about 1024 workgroups if every sequence were the
     // longest, in chunks of whole 256 keys.
     const uint64_t units = n_batch * a.n_kv * a.n_tiles;
-    uint64_t splits = (2048 + units - 1) / units;
+    uint64_t splits = (1024 + units - 1) / units;
     uint64_t chunk = ((len + splits - 1) / splits + 255) / 256 * 256;
     splits = (len + chunk - 1) / chunk;
     a.chunk = static_cast<uint32_t>(chunk);

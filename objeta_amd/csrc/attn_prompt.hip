@@ -77,6 +77,8 @@ int32_t objeta_hip_attn_prompt_device(objeta_hip_context* ctx, objeta_hip_stream
     OBJ_TRY(check_attn_rows(action, "k", d_k, n_tokens, k_stride, n_kv_heads, head_dim, es));
     OBJ_TRY(check_attn_rows(action, "v", d_v, n_tokens, v_stride, n_kv_heads, head_dim, es));
     OBJ_TRY(check_attn_rows(action, "out", d_out, n_tokens, out_stride, n_q_heads, head_dim, es));
+    if (k_stride > kMaxKvStride || v_stride > kMaxKvStride)
+        OBJ_FAIL(kInvalidInput, action, strf("k and v strides must not exceed %llu", (unsigned long long)kMaxKvStride));
     const RowSet out{d_out, out_stride * es, n_q_heads * head_dim * es, n_tokens};
     const RowSet in[] = {{d_q, q_stride * es, n_q_heads * head_dim * es, n_tokens},
                          {d_k, k_stride * es, n_kv_heads * head_dim * es, n_tokens},

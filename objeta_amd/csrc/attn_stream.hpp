@@ -16,13 +16,12 @@ namespace dev {
 template <int KT, int DT, int ROWS>
 struct Stream {
     typedef Rows<KT, DT, ROWS> R;
-    static_assert(64 % R::kUnits == 0 && 64 / R::kUnits <= 8, "the keys of one load in one group of eight");
-    static constexpr int kLoads = 32 * R::kUnits / 64;  // 16-byte units of K (and of V) a lane stages
-    static constexpr int kWave = 2 * 32 * R::kBytes;    // LDS of a wave: a tile of K and one of V
-    static constexpr int kWaves = kWave <= 16384 ? 4 : (kWave <= 32768 ? 2 : 1);
+    static constexpr int kLoads = 32 / R::kPer;                // 16-byte units of K (and of V) a lane stages
+    static constexpr int kWave = 32 * (R::kK + R::kV);         // LDS of a wave: a tile of K and one of V
+    static constexpr int kWaves = DT * R::kEs <= 256 ? 4 : (DT * R::kEs <= 512 ? 2 : 1);
     static_assert(kWave >= ROWS * DT * 4, "o of a wave's rows in its part");
     // waves a SIMD: two where a wave's part of LDS lets eight be on a CU
-    static constexpr int kPerSimd = kWave <= 16384 ? 2 : 1;
+    static constexpr int kPerSimd = DT * R::kEs <= 256 ? 2 : 1;
 };
 
 __device__ __forceinline__ void wave_lds_fence() {
@@ -46,7 +45,7 @@ __global__ __launch_bounds__((64 * Stream<KT, DT, ROWS>::kWaves),
     const CachedItem item(a, blockIdx.x);
     if (!item.any) return;
     const uint32_t split = item.split, head = item.head, b = item.b;
-    uint32_t tile = item.tile;
+    const uint32_t tile = item.tile;
     const int32_t row0 = a.cu[b], end = a.cu[b + 1], n_q = end - row0;
     if (row0 < 0 || end < row0 || static_cast<uint32_t>(end) > a.n_rows) {
         if (tid == 0) atomicOr(a.err, kErrIndex);
@@ -72,164 +71,171 @@ __global__ __launch_bounds__((64 * Stream<KT, DT, ROWS>::kWaves),
     const int32_t k_lo = static_cast<int32_t>(c0);
     const int32_t k_end = split + 1 < a.n_splits && c0 + a.chunk < len ? static_cast<int32_t>(c0 + a.chunk) : len;
     char* k_lds = lds[wave];
-    char* v_lds = lds[wave] + 32 * R::kBytes;
-    const uint32_t kx = M::k_first(lane), vx = M::v_first(lane);
+    char* v_lds = lds[wave] + 32 * R::kK;
 
-    for (; static_cast<uint64_t>(tile) * ROWS < n_m; tile += a.n_tiles) {
-        const uint32_t m = tile * ROWS + mine;
-        const bool real = m < n_m;
-        const uint32_t i = real ? m / a.group : 0, q_head = head * a.group + (real ? m % a.group : 0);
-        const uint64_t row = static_cast<uint64_t>(row0) + i;
-        const int32_t base = len - n_q;
-        RowView view{0, -1, 0x7FFFFFFF, 0};
-        if (real && usable) {
-            if (a.tree) view = RowView{0, len - 1, base, a.tree[row]};
-            else view.hi = base + static_cast<int32_t>(i);
+    past_rows<M>(a, tile, ROWS, n_m, row0, head, split);
+    if (static_cast<uint64_t>(tile) * ROWS >= n_m) return;
+    const uint32_t m = tile * ROWS + mine;
+    const bool real = m < n_m;
+    const uint32_t i = real ? m / a.group : 0, q_head = head * a.group + (real ? m % a.group : 0);
+    const uint64_t row = static_cast<uint64_t>(row0) + i;
+    const int32_t base = len - n_q;
+    RowView view{0, -1, 0x7FFFFFFF, 0};
+    if (real && usable) {
+        if (a.tree) view = RowView{0, len - 1, base, a.tree[row]};
+        else view.hi = base + static_cast<int32_t>(i);
+    }
+    typename M::Query q;
+    float scale = a.scale_log2;
+    M::load_q(q, static_cast<const typename M::qelem*>(a.q) + row * a.q_stride + static_cast<uint64_t>(q_head) * a.dim, real,
+              a.dim, lane, scale);
+    M::settle(q);
+    if (tid == 0) sh_bad = 0;
+    RowState<M> st;
+    st.clear();
+
+    // tiles k_lo + 32 (wave + kWaves t)
+    u32x4a rk[S::kLoads], rv[S::kLoads];
+    bool bad = false;
+    auto load_pages = [&](int32_t k0) -> int32_t {  // lane x < 4: the page of keys k0 + 8 x ..
+        int32_t p = 0;
+        const int32_t slot = k0 + static_cast<int32_t>(lane) * 8;
+        if (lane < 4 && slot < k_end) p = kv.entry_of(static_cast<uint32_t>(slot));
+        return p;
+    };
+    // Load x takes the keys x kPer .. of a tile, which lie in one group of eight, so in one page:
+    // the address is uniform but for the lane's place, the same for all x.
+    const uint32_t row_bytes = a.dim * R::kEs, unit = lane % R::kLanes;
+    const uint32_t place = unit * (16 / R::kEs) < a.dim ? lane / R::kLanes * row_bytes + unit * 16 : kNowhere;
+    auto load_tile = [&](int32_t k0, int32_t pages) {
+#pragma unroll
+        for (int x = 0; x < S::kLoads; ++x) {
+            const uint32_t key = x * R::kPer;
+            const int32_t left = k_end - k0 - static_cast<int32_t>(key);  // keys from this one on
+            const uint32_t bytes = left > 0 ? (left < 8 ? left : 8) * row_bytes : 0;
+            const uint64_t at = kv.paged_at(__builtin_amdgcn_readlane(pages, key >> 3), static_cast<uint32_t>(k0) + key);
+            rk[x] = buffer_unit(buffer_of(kv.k + at, bytes), place);
+            rv[x] = buffer_unit(buffer_of(kv.v + at, bytes), place);
         }
-        typename M::Query q;
-        float scale = a.scale_log2;
-        M::load_q(q, static_cast<const typename M::qelem*>(a.q) + row * a.q_stride + static_cast<uint64_t>(q_head) * a.dim, real,
-                  a.dim, lane, scale);
-        if (tid == 0) sh_bad = 0;
-        RowState<M> st;
-        st.clear();
-
-        // tiles k_lo + 32 (wave + kWaves t)
-        u32x4a rk[S::kLoads], rv[S::kLoads];
-        bool bad = false;
-        auto load_pages = [&](int32_t k0) -> int32_t {  // lane x < 4: the page of keys k0 + 8 x ..
-            int32_t p = 0;
-            const int32_t slot = k0 + static_cast<int32_t>(lane) * 8;
-            if (lane < 4 && slot < k_end) p = kv.page_of(static_cast<uint32_t>(slot), bad);
-            return p;
-        };
-        // Unit u = 64 x + lane of a tile: key u / kUnits. The keys of one x lie in one group of
-        // eight, so in one page: the address is uniform but for the lane's place, the same for all x.
-        const uint32_t l_key = lane / R::kUnits, l_unit = lane % R::kUnits;
-        const uint32_t place = (l_key * a.dim + l_unit * (16 / R::kEs)) * R::kEs;
-        const bool whole = l_unit * (16 / R::kEs) < a.dim;
-        auto load_tile = [&](int32_t k0, int32_t pages) {
+    };
+    const uint32_t k_at = lane / R::kLanes * R::kK + unit * 16, v_at = lane / R::kLanes * R::kV + unit * 16;
+    const int32_t step = 32 * kWaves;
+    int32_t k0 = k_lo + 32 * static_cast<int32_t>(__builtin_amdgcn_readfirstlane(wave));
+    int32_t pages = 0;
+    if (k0 < k_end) {
+        pages = load_pages(k0);
+        const int32_t first = kv.checked(pages, bad);
+        if (k_end - k0 > step) pages = load_pages(k0 + step);
+        load_tile(k0, first);
+    }
+    for (; k0 < k_end; k0 = k_end - k0 > step ? k0 + step : k_end) {
+if (R::kLanes == R::kUnits || unit < R::kUnits) {
 #pragma unroll
             for (int x = 0; x < S::kLoads; ++x) {
-                constexpr uint32_t per = 64 / R::kUnits;  // keys of one x
-                const uint32_t key = x * per;
-                const int32_t page = __builtin_amdgcn_readlane(pages, key >> 3);
-                const uint64_t at = kv.paged_at(page, static_cast<uint32_t>(k0) + key);
-                rk[x] = u32x4a{0, 0, 0, 0};
-                rv[x] = u32x4a{0, 0, 0, 0};
-                if (whole && k0 + static_cast<int32_t>(key + l_key) < k_end) {
-                    rk[x] = *reinterpret_cast<const u32x4a*>(reinterpret_cast<const char*>(kv.k + at) + place);
-                    rv[x] = *reinterpret_cast<const u32x4a*>(reinterpret_cast<const char*>(kv.v + at) + place);
+                *reinterpret_cast<u32x4a*>(k_lds + k_at + x * R::kPer * R::kK) = rk[x];
+                *reinterpret_cast<u32x4a*>(v_lds + v_at + x * R::kPer * R::kV) = rv[x];
+            }
+        }
+        if (k_end - k0 > step) {
+            const int32_t now = kv.checked(pages, bad);
+            if (k_end - k0 > 2 * step) pages = load_pages(k0 + 2 * step);
+            load_tile(k0 + step, now);
+        }
+        wave_lds_fence();
+        Scores<M> s;
+        score_rows<M>(s, q, k_lds + M::k_first(lane));
+        if (a.tree || k0 + 32 > base + 1 || k0 + 32 > k_end) {
+#pragma unroll
+            for (int n = 0; n < M::kKeyTiles; ++n)
+#pragma unroll
+                for (int r = 0; r < M::kRegs; ++r) {
+                    const int32_t key = k0 + static_cast<int32_t>(M::key_of(n, r, h));
+                    if (!(view.sees(key) & (key < k_end))) s.s[n][r] = -kInf;
                 }
-            }
-        };
-        const int32_t step = 32 * kWaves;
-        int32_t k0 = k_lo + 32 * static_cast<int32_t>(__builtin_amdgcn_readfirstlane(wave));
-        int32_t pages = 0;
-        if (k0 < k_end) {
-            load_tile(k0, load_pages(k0));
-            if (k_end - k0 > step) pages = load_pages(k0 + step);
         }
-        for (; k0 < k_end; k0 = k_end - k0 > step ? k0 + step : k_end) {
+        take_top<M>(st, s, scale);
+        const float off = M::kShift - st.reference();
 #pragma unroll
-            for (int x = 0; x < S::kLoads; ++x) {
-                const uint32_t u = x * 64 + lane, key = u / R::kUnits, c = u % R::kUnits;
-                *reinterpret_cast<u32x4a*>(k_lds + key * R::kBytes + ((c ^ R::swz_k(key)) << 4)) = rk[x];
-                *reinterpret_cast<u32x4a*>(v_lds + key * R::kBytes + ((c ^ R::swz_v(key)) << 4)) = rv[x];
-            }
-            if (k_end - k0 > step) {
-                load_tile(k0 + step, pages);
-                if (k_end - k0 > 2 * step) pages = load_pages(k0 + 2 * step);
-            }
-            wave_lds_fence();
-            Scores<M> s[1];
-            scores<M>(s[0], q, k_lds, lane, kx);
-            if (a.tree || k0 + 32 > base + 1 || k0 + 32 > k_end) {
-#pragma unroll
-                for (int n = 0; n < M::kKeyTiles; ++n)
-#pragma unroll
-                    for (int r = 0; r < M::kRegs; ++r) {
-                        const int32_t key = k0 + static_cast<int32_t>(M::key_of(n, r, h));
-                        if (!(view.sees(key) && key < k_end)) s[0].s[n][r] = -kInf;
-                    }
-            }
-            accumulate<M, 1>(st, s, scale, v_lds, vx);
-            wave_lds_fence();
+        for (int g = 0; g < kGroups<M>; ++g) {
+            Weights<M> w;
+            weigh<M>(w, st, s, g, scale, off);
+            value_rows<M>(st, w, v_lds + M::v_first(lane), g);
         }
+        wave_lds_fence();
+    }
 
-        // ---- the waves' results into one: a wave's o goes to its own part of LDS
-        st.l = row_sum<ROWS>(st.l);
-        if (h == 0) sh_m[wave][mine] = st.m, sh_l[wave][mine] = st.l;
-        __syncthreads();
-        if (bad) atomicOr(&sh_bad, 1);
-        float top = sh_m[0][mine];
+    const AttnArgs& e = args_again();
+    // ---- the waves' results into one: a wave's o goes to its own part of LDS
+    st.l = row_sum<ROWS>(st.l);
+    if (h == 0) sh_m[wave][mine] = st.m, sh_l[wave][mine] = st.l;
+    __syncthreads();
+    if (bad) atomicOr(&sh_bad, 1);
+    float top = sh_m[0][mine];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, sh_m[w][mine]);
-        const float ref = top == -kInf ? 0.0f : top;
-        float l = 0.0f;
+    for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, sh_m[w][mine]);
+    const float ref = top == -kInf ? 0.0f : top;
+    float l = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) l += sh_l[w][mine] * exp2_hw(sh_m[w][mine] - ref);
-        const float f = exp2_hw(st.m - ref);
-        const bool odd = not_finite<M>(st);
-        if (odd && lane == 0) atomicOr(&sh_bad, 2);
-        float* o_lds = reinterpret_cast<float*>(lds[wave]);  // [dimension / 4][row][4]
+    for (int w = 0; w < kWaves; ++w) l += sh_l[w][mine] * exp2_hw(sh_m[w][mine] - ref);
+    const float f = exp2_hw(st.m - ref);
+    const bool odd = not_finite<M>(st);
+    if (odd && lane == 0) atomicOr(&sh_bad, 2);
+    float* o_lds = reinterpret_cast<float*>(lds[wave]);  // [dimension / 4][row][4]
 #pragma unroll
-        for (int d = 0; d < M::kOut; ++d)
+    for (int d = 0; d < M::kOut; ++d)
 #pragma unroll
-            for (int r = 0; r < M::kRegs / 4; ++r)
-                *reinterpret_cast<f32x4*>(o_lds + (out_dim<M>(d, r, h) / 4 * ROWS + mine) * 4) =
-                    f32x4{st.o[d][4 * r] * f, st.o[d][4 * r + 1] * f, st.o[d][4 * r + 2] * f, st.o[d][4 * r + 3] * f};
-        __syncthreads();
-        const int32_t state = sh_bad;
-        if (usable && state == 2) {
-            // some product met an infinity or NaN: the rows again, key by key (see row_by_row)
-            for (uint32_t r = wave; r < ROWS; r += kWaves) {
-                const uint32_t r_m = tile * ROWS + r;
-                if (r_m >= n_m) break;
-                const uint32_t r_head = head * a.group + r_m % a.group, r_i = r_m / a.group;
-                const uint64_t r_row = static_cast<uint64_t>(row0) + r_i;
-                RowView rv1{0, base + static_cast<int32_t>(r_i), 0x7FFFFFFF, 0};
-                if (a.tree) rv1 = RowView{0, len - 1, base, a.tree[r_row]};
-                float rm, rl, ro[4];
-                row_by_row<M, true, KT>(kv,
-                                        static_cast<const typename M::qelem*>(a.q) + r_row * a.q_stride +
-                                            static_cast<uint64_t>(r_head) * a.dim,
-                                        rv1, k_lo, k_end, a.scale_log2, a.dim, rm, rl, ro);
-                write_row<M>(a, rm, rl, ro, r_row, r_head, split, lane);
-            }
-        } else {
-            if (tid == 0 && (state & 1)) atomicOr(a.err, kErrIndex);
-            const bool poison = !usable || (state & 1);
-            if (poison) l = __builtin_nanf("");
-            const float inv = a.n_splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
-            // this thread: its row, groups of four dimensions
-            for (uint32_t g = wave * (64 / ROWS) + h; g * 4 < a.dim; g += kWaves * (64 / ROWS)) {
-                f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int r = 0; r < M::kRegs / 4; ++r)
+            *reinterpret_cast<f32x4*>(o_lds + (out_dim<M>(d, r, h) / 4 * ROWS + mine) * 4) =
+                f32x4{st.o[d][4 * r] * f, st.o[d][4 * r + 1] * f, st.o[d][4 * r + 2] * f, st.o[d][4 * r + 3] * f};
+    __syncthreads();
+    const int32_t state = sh_bad;
+    if (usable && state == 2) {
+        // some product met an infinity or NaN: the rows again, key by key (see row_by_row)
+        for (uint32_t r = wave; r < ROWS; r += kWaves) {
+            const uint32_t r_m = tile * ROWS + r;
+            if (r_m >= n_m) break;
+            const uint32_t r_head = head * e.group + r_m % e.group, r_i = r_m / e.group;
+            const uint64_t r_row = static_cast<uint64_t>(row0) + r_i;
+            RowView rv1{0, base + static_cast<int32_t>(r_i), 0x7FFFFFFF, 0};
+            if (e.tree) rv1 = RowView{0, len - 1, base, e.tree[r_row]};
+            float rm, rl, ro[4];
+            row_by_row<M, true, KT>(kv,
+                                    static_cast<const typename M::qelem*>(e.q) + r_row * e.q_stride +
+                                        static_cast<uint64_t>(r_head) * e.dim,
+                                    rv1, k_lo, k_end, e.scale_log2, e.dim, rm, rl, ro);
+            write_row<M>(e, rm, rl, ro, r_row, r_head, split, lane);
+        }
+    } else {
+        if (tid == 0 && (state & 1)) atomicOr(e.err, kErrIndex);
+        const bool poison = !usable || (state & 1);
+        if (poison) l = __builtin_nanf("");
+        const float inv = e.n_splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+        // this thread: its row, groups of four dimensions
+        for (uint32_t g = wave * (64 / ROWS) + h; g * 4 < e.dim; g += kWaves * (64 / ROWS)) {
+            f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int w = 0; w < kWaves; ++w)
-                    sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w]) +
-                                                           (g * ROWS + mine) * 4);
-                sum *= inv;
-                if (poison) sum = f32x4{l, l, l, l};
-                if (!real) continue;
-                if (a.n_splits > 1)
-                    *reinterpret_cast<f32x4*>(a.part + part_at(a, split, row, q_head) * a.dim + 4 * g) = sum;
-                else
-                    store_out<QT>(static_cast<typename M::qelem*>(a.out) + row * a.out_stride +
-                                      static_cast<uint64_t>(q_head) * a.dim + 4 * g, sum);
-            }
-            if (real && wave == 0 && h == 0) {
-                if (a.n_splits > 1) {
-                    const uint64_t at = part_at(a, split, row, q_head);
-                    a.part_ml[2 * at] = top - M::kShift;
-                    a.part_ml[2 * at + 1] = l;
-                } else if (a.lse) {
-                    a.lse[row * a.n_heads + q_head] =
-                        l == 0.0f ? -kInf : (top - M::kShift + __builtin_amdgcn_logf(l)) * kLn2;
-                }
+            for (int w = 0; w < kWaves; ++w)
+                sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w]) +
+                                                       (g * ROWS + mine) * 4);
+            sum *= inv;
+            if (poison) sum = f32x4{l, l, l, l};
+            if (!real) continue;
+            if (e.n_splits > 1)
+                *reinterpret_cast<f32x4*>(e.part + part_at(e, split, row, q_head) * e.dim + 4 * g) = sum;
+            else
+                store_out<QT>(static_cast<typename M::qelem*>(e.out) + row * e.out_stride +
+                                  static_cast<uint64_t>(q_head) * e.dim + 4 * g, sum);
+        }
+        if (real && wave == 0 && h == 0) {
+            if (e.n_splits > 1) {
+                const uint64_t at = part_at(e, split, row, q_head);
+                e.part_ml[2 * at] = top - M::kShift;
+                e.part_ml[2 * at + 1] = l;
+            } else if (e.lse) {
+                e.lse[row * e.n_heads + q_head] =
+                    l == 0.0f ? -kInf : (top - M::kShift + __builtin_amdgcn_logf(l)) * kLn2;
             }
         }
-        __syncthreads();  // LDS is used again
     }
 }
 

@@ -14,10 +14,6 @@
 // rows in LDS by the transposing 64-bit read, whose blocks of 4 keys x 16 dimensions are what
 // a lane's four consecutive elements name.
 //
-// LDS rows are the keys' rows of 16-byte units; a unit's place within its row is exchanged
-// by an exclusive or with bits of the key (swz_k, swz_v), so that the lanes of a read phase
-// fall into different banks.
-//
 // Types. f16 and bf16 use the products of their type, probabilities rounded to it. Float
 // queries on a 16-bit cache are split into parts of the cache's type whose sum holds 22 (f16,
 // two parts of the row times a power of two) or 24 bits (bf16, three), each product is exact,
@@ -27,6 +23,8 @@
 #pragma once
 
 #include "kv_common.hpp"
+
+#include <type_traits>
 
 namespace objeta {
 namespace dev {
@@ -50,27 +48,21 @@ template <int T> struct ElemOf { typedef float type; };
 template <> struct ElemOf<kDtF16> { typedef _Float16 type; };
 template <> struct ElemOf<kDtBF16> { typedef __bf16 type; };
 
-// Rows of DT elements of type KT in LDS, read by tiles of ROWS query rows.
+// Rows of DT elements of type KT in LDS, read by tiles of ROWS query rows. A key's row is
+// padded: by 16 bytes, the 16-byte reads of 16 consecutive keys at one column fall into 16
+// different groups of four banks (of 64); by 32 bytes, the 32-byte parts that a transposing
+// read takes from four consecutive keys, and the 32 (ROWS = 16: by 16, the 16) floats of keys
+// four apart, into different banks.
 template <int KT, int DT, int ROWS>
 struct Rows {
     static constexpr int kEs = KT == kDtF32 ? 4 : 2;
     static constexpr int kBytes = DT * kEs;
     static constexpr int kUnits = kBytes / 16;
-    // the units of 16 consecutive keys at one column spread over the 16 units of 64 banks
-    static __device__ __forceinline__ uint32_t swz_k(uint32_t key) {
-        if constexpr (kUnits % 16 == 0) return key & 15;
-        else if constexpr (kUnits % 8 == 0) return (key >> 1) & 7;
-        else return (key >> 2) & 3;
-    }
-    // 16-bit: the 64-byte parts that one transposing read takes from four keys; float: the
-    // parts of ROWS dimensions of keys four apart
-    static __device__ __forceinline__ uint32_t swz_v(uint32_t key) {
-        if constexpr (KT == kDtF32)
-            return kUnits % 16 ? 0 : (ROWS == 32 ? ((key >> 2) & 1) << 3 : ((key >> 2) & 3) << 2);
-        else if constexpr (kUnits % 16 == 0) return (key & 3) << 2;
-        else if constexpr (kUnits % 8 == 0) return ((key >> 1) & 1) << 2;
-        else return 0;
-    }
+    static constexpr int kK = kBytes + 16;
+    static constexpr int kV = kBytes + (KT == kDtF32 && ROWS == 16 ? 16 : 32);
+    // lanes that load one row: a power of two, so that a wave's load lies within eight keys
+    static constexpr int kLanes = kUnits <= 8 ? 8 : (kUnits <= 16 ? 16 : (kUnits <= 32 ? 32 : 64));
+    static constexpr int kPer = 64 / kLanes;  // keys of a wave's load
 };
 
 template <int ROWS> struct AccOf { typedef f32x16 type; };
@@ -195,19 +187,35 @@ struct Math {
             }
         }
     }
-    // Dimensions kStep i + 8 h .. + 8 of this lane's key (lane % ROWS of the tile): K as the
-    // first operand. `row` is the key's LDS row, `x0` its swizzled first unit in bytes.
-    static __device__ __forceinline__ uint32_t k_first(uint32_t lane) {
-        const uint32_t h = lane / ROWS, key = lane % ROWS;
-        return ((kFloat ? 2 * h : h) ^ R::swz_k(key)) * 16;
+    // Waits for the query here. Left in flight into a loop, its first use there would wait
+    // in every turn for whatever loads the turn has on their way.
+    static __device__ __forceinline__ void settle(Query& q) {
+#pragma unroll
+        for (int p = 0; p < kParts; ++p)
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                if constexpr (kFloat) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(q.f[p][i].v[j]));
+                } else {
+                    u32x4a x = __builtin_bit_cast(u32x4a, q.f[p][i]);
+                    asm volatile("" : "+v"(x));
+                    q.f[p][i] = __builtin_bit_cast(frag, x);
+                }
+            }
     }
-    static __device__ __forceinline__ frag lds_k(const char* row, uint32_t x0, int i) {
+    // Dimensions kStep i + 8 h .. + 8 of this lane's key (lane % ROWS of the tile): K as the
+    // first operand. `p` is the tile's first row plus k_first.
+    static __device__ __forceinline__ uint32_t k_first(uint32_t lane) {
+        return lane % ROWS * R::kK + lane / ROWS * (8 * R::kEs);
+    }
+    static __device__ __forceinline__ frag lds_k(const char* p, int i) {
         if constexpr (kFloat) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(row + (x0 ^ (4 * kStep * i)));
-            const f32x4 b = *reinterpret_cast<const f32x4*>(row + (x0 ^ (4 * kStep * i) ^ 16));
+            const f32x4 a = *reinterpret_cast<const f32x4*>(p + 4 * kStep * i);
+            const f32x4 b = *reinterpret_cast<const f32x4*>(p + 4 * kStep * i + 16);
             return f32x8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
         } else {
-            return *reinterpret_cast<const frag*>(row + (x0 ^ (2 * kStep * i)));
+            return *reinterpret_cast<const frag*>(p + 2 * kStep * i);
         }
     }
     // The key of score register r of tile n, and the keys of element j of a group of kStep
@@ -216,49 +224,68 @@ struct Math {
         return ROWS == 32 ? (r & 3) + 8 * (r >> 2) + 4 * h : 16 * n + r + 4 * h;
     }
     static constexpr int kFar = ROWS == 32 ? 8 : 16;  // elements 4 .. 7 lie this many keys behind 0 .. 3
-    // This lane's place for V: byte offset from a group of kStep keys' first row to the first
-    // of its reads at dimensions 0 .. ROWS.
+    // V^T of kStep keys at dimensions ROWS dd + lane % ROWS; `p` is the first key's row plus
+    // v_first.
     static __device__ __forceinline__ uint32_t v_first(uint32_t lane) {
         const uint32_t h = lane / ROWS;
         if constexpr (kFloat) {
-            return 4 * h * R::kBytes + R::swz_v(4 * h) * 16 + (lane % ROWS) * 4;
+            return 4 * h * R::kV + (lane % ROWS) * 4;
         } else {
-            const uint32_t l = lane & 15, ds = ROWS == 32 ? (lane >> 4) & 1 : 0, key = 4 * h + (l >> 2);
-            const uint32_t unit = 2 * ds + ((l & 3) >> 1);
-            return key * R::kBytes + ((unit ^ R::swz_v(key)) * 16) + (l & 1) * 8;
+            const uint32_t l = lane & 15, ds = ROWS == 32 ? (lane >> 4) & 1 : 0;
+            return (4 * h + (l >> 2)) * R::kV + ds * 32 + (l & 3) * 8;
         }
     }
-    // V^T of kStep keys (rows from `rows` on) at dimensions ROWS dd + lane % ROWS.
-    static __device__ __forceinline__ frag lds_v(const char* rows, uint32_t v0, int dd) {
-        const char* p = rows + (v0 ^ (ROWS * R::kEs * dd));
+    static __device__ __forceinline__ frag lds_v(const char* p, int dd) {
+        p += ROWS * R::kEs * dd;
         if constexpr (kFloat) {
             f32x8 f;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                f.v[j] = *reinterpret_cast<const float*>(p + (kFar * (j / 4) + j % 4) * R::kBytes);
+            for (int j = 0; j < 8; ++j) f.v[j] = *reinterpret_cast<const float*>(p + (kFar * (j / 4) + j % 4) * R::kV);
             return f;
         } else {
             const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(lds_char*)(p));
             const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(lds_char*)(p + kFar * R::kBytes));
+                (__attribute__((address_space(3))) s16x4*)(lds_char*)(p + kFar * R::kV));
             const s16x8 v = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
             return __builtin_bit_cast(frag, v);
         }
     }
 };
 
-// A sum or maximum over the lanes that hold one row.
+// x of this lane and of its counterpart 32 (16) lanes away, in either order.
+struct Pair {
+    float a, b;
+};
+__device__ __forceinline__ Pair with_32(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a = r[0], b = r[1];  // a bit cast of a vector's element takes its first
+    return Pair{__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
+}
+__device__ __forceinline__ Pair with_16(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t a = r[0], b = r[1];
+    return Pair{__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
+}
+// A maximum or sum over the lanes that hold one row.
 template <int ROWS>
 __device__ __forceinline__ float row_max(float x) {
-#pragma unroll
-    for (int s = ROWS; s < 64; s <<= 1) x = __builtin_fmaxf(x, __shfl_xor(x, s, 64));
-    return x;
+    if constexpr (ROWS == 16) {
+        const Pair p = with_16(x);
+        x = __builtin_fmaxf(p.a, p.b);
+    }
+    const Pair p = with_32(x);
+    return __builtin_fmaxf(p.a, p.b);
 }
 template <int ROWS>
 __device__ __forceinline__ float row_sum(float x) {
-#pragma unroll
-    for (int s = ROWS; s < 64; s <<= 1) x += __shfl_xor(x, s, 64);
-    return x;
+    if constexpr (ROWS == 16) {
+        const Pair p = with_16(x);
+        x = p.a + p.b;
+    }
+    const Pair p = with_32(x);
+    return p.a + p.b;
 }
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -296,65 +323,102 @@ struct Scores {
     typename M::acc s[M::kKeyTiles];
 };
 
-// S^T of the 32 keys at `rows` (LDS).
+// S^T of 32 keys; `k` is their first row in LDS plus k_first.
 template <class M>
-__device__ __forceinline__ void scores(Scores<M>& s, const typename M::Query& q, const char* rows, uint32_t lane, uint32_t k0) {
-    const char* row = rows + (lane % M::kRows) * M::R::kBytes;
+__device__ __forceinline__ void score_rows(Scores<M>& s, const typename M::Query& q, const char* k) {
 #pragma unroll
     for (int n = 0; n < M::kKeyTiles; ++n) {
         s.s[n] = M::zero();
 #pragma unroll
         for (int i = 0; i < M::kSteps; ++i) {
-            const typename M::frag k = M::lds_k(row + n * M::kRows * M::R::kBytes, k0, i);
+            const typename M::frag f = M::lds_k(k + n * M::kRows * M::R::kK, i);
 #pragma unroll
-            for (int p = 0; p < M::kParts; ++p) s.s[n] = M::mma(k, q.f[p][i], s.s[n]);
+            for (int p = 0; p < M::kParts; ++p) s.s[n] = M::mma(f, q.f[p][i], s.s[n]);
         }
     }
 }
 
-// The softmax step over NS times 32 keys of unscaled scores (unseen ones -inf) and their values.
-template <class M, int NS>
-__device__ __forceinline__ void accumulate(RowState<M>& st, Scores<M> (&s)[NS], float scale, const char* v_rows, uint32_t v0) {
+// The probabilities of group t of kStep keys as an operand.
+template <class M>
+struct Weights {
+    typename M::frag f[M::kParts];
+};
+
+// The fragments of 32 keys (kRows == 32) for all steps of their scores.
+template <class M>
+struct Keys {
+    typename M::frag f[M::kSteps];
+};
+template <class M>
+__device__ __forceinline__ void read_keys(Keys<M>& k, const char* p) {
+#pragma unroll
+    for (int i = 0; i < M::kSteps; ++i) k.f[i] = M::lds_k(p, i);
+}
+template <class M>
+__device__ __forceinline__ void score(Scores<M>& s, const typename M::Query& q, const Keys<M>& k) {
+    s.s[0] = M::zero();
+#pragma unroll
+    for (int i = 0; i < M::kSteps; ++i)
+#pragma unroll
+        for (int p = 0; p < M::kParts; ++p) s.s[0] = M::mma(k.f[i], q.f[p][i], s.s[0]);
+}
+// The fragments of the values of group t (`v`: 32 keys' first row plus v_first), and their
+// products.
+template <class M>
+struct Values {
+    typename M::frag f[M::kOut];
+};
+template <class M>
+__device__ __forceinline__ void read_values(Values<M>& f, const char* v, int t) {
+#pragma unroll
+    for (int d = 0; d < M::kOut; ++d) f.f[d] = M::lds_v(v + M::kStep * t * M::R::kV, d);
+}
+template <class M>
+__device__ __forceinline__ void add_values(RowState<M>& st, const Weights<M>& w, const Values<M>& v) {
+#pragma unroll
+    for (int d = 0; d < M::kOut; ++d)
+#pragma unroll
+        for (int part = 0; part < M::kParts; ++part) st.o[d] = M::mma(v.f[d], w.f[part], st.o[d]);
+}
+
+// The largest score of 32 keys, scaled, over the lanes of a row; raises the reference where it
+// has outgrown it.
+template <class M>
+__device__ __forceinline__ void take_top(RowState<M>& st, const Scores<M>& s, float scale) {
     float top = -kInf;
 #pragma unroll
-    for (int n = 0; n < NS; ++n)
+    for (int t = 0; t < M::kKeyTiles; ++t)
 #pragma unroll
-        for (int t = 0; t < M::kKeyTiles; ++t)
-#pragma unroll
-            for (int r = 0; r < M::kRegs; ++r) top = __builtin_fmaxf(top, s[n].s[t][r]);
+        for (int r = 0; r < M::kRegs; ++r) top = __builtin_fmaxf(top, s.s[t][r]);
     top = row_max<M::kRows>(top) * scale;
     if (__any(top > st.m + kSlack)) st.raise(__builtin_fmaxf(st.m, top));
-    const float off = M::kShift - st.reference();
-    constexpr int kGroups = 32 / M::kStep;  // of kStep keys: two of 16, or one of 32
+}
+
+template <class M>
+__device__ __forceinline__ void weigh(Weights<M>& w, RowState<M>& st, const Scores<M>& s, int t, float scale, float off) {
+    float p[8];
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
+    for (int j = 0; j < 8; ++j) {
+        const float x = M::kRows == 32 ? s.s[0][8 * t + j] : s.s[j / 4 % M::kKeyTiles][j % 4];
+        p[j] = exp2_hw(__builtin_fmaf(x, scale, off));
+        st.l += p[j];
+    }
+    if constexpr (M::kFloat) w.f[0] = f32x8{{p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]}};
+    else M::split(p, [&](int part, const typename M::frag& x) { w.f[part] = x; });  // rounded to nearest, as the output is
+}
+
+// o^T += V^T P^T of group t.
+template <class M>
+__device__ __forceinline__ void value_rows(RowState<M>& st, const Weights<M>& w, const char* v, int t) {
 #pragma unroll
-        for (int t = 0; t < kGroups; ++t) {
-            float p[8];
+    for (int d = 0; d < M::kOut; ++d) {
+        const typename M::frag f = M::lds_v(v + M::kStep * t * M::R::kV, d);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = M::kRows == 32 ? s[n].s[0][8 * t + j] : s[n].s[j / 4][j % 4];
-                p[j] = exp2_hw(__builtin_fmaf(x, scale, off));
-                st.l += p[j];
-            }
-            const char* rows = v_rows + (32 * n + M::kStep * t) * M::R::kBytes;
-            if constexpr (M::kFloat) {
-                const f32x8 f = {{p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7]}};
-#pragma unroll
-                for (int d = 0; d < M::kOut; ++d) st.o[d] = M::mma(M::lds_v(rows, v0, d), f, st.o[d]);
-            } else {
-                typename M::frag f[M::kParts];  // rounded to nearest, as the output is
-                M::split(p, [&](int part, const typename M::frag& x) { f[part] = x; });
-#pragma unroll
-                for (int d = 0; d < M::kOut; ++d) {
-                    const typename M::frag v = M::lds_v(rows, v0, d);
-#pragma unroll
-                    for (int part = 0; part < M::kParts; ++part) st.o[d] = M::mma(v, f[part], st.o[d]);
-                }
-            }
-        }
+        for (int part = 0; part < M::kParts; ++part) st.o[d] = M::mma(f, w.f[part], st.o[d]);
     }
 }
+template <class M>
+constexpr int kGroups = 32 / M::kStep;  // of kStep keys in 32: two of 16, or one of 32
 
 struct AttnArgs {
     const void *q, *k, *v;
@@ -371,7 +435,7 @@ struct AttnArgs {
     const uint64_t* tree;
     uint64_t layer_off;  // elements
     // keys cut over workgroups
-    uint32_t chunk, n_splits, n_tiles;
+    uint32_t chunk, n_splits, n_tiles, tile_rows;
     float *part, *part_ml;  // [n_splits][n_rows * n_heads][dim], [..][2]
     uint32_t* err;
 };
@@ -396,13 +460,24 @@ struct CachedItem {
     }
 };
 
-// What one row sees: keys lo .. hi, and among those from `base` on only the set bits of mask.
+// The kernel's arguments read anew from where the launch left them (each of these kernels has
+// one argument). Used behind a loop, they need no registers during it.
+__device__ __forceinline__ const AttnArgs& args_again() {
+    auto p = (const __attribute__((address_space(4))) AttnArgs*)(__builtin_amdgcn_kernarg_segment_ptr());
+    asm volatile("" : "+s"(p));
+    return *(const AttnArgs*)p;
+}
+
+// What one row sees: keys lo .. hi, and among those from `base` on (64 at most up to hi) only
+// the set bits of mask.
 struct RowView {
     int32_t lo, hi, base;
     uint64_t mask;
     __device__ __forceinline__ bool sees(int32_t key) const {
+        // no short-cut operators: a branch for each of a tile's scores costs more than the tests
         const uint32_t bit = static_cast<uint32_t>(key - base);
-        return key >= lo && key <= hi && (key < base || bit > 63 || ((mask >> bit) & 1));
+        const uint32_t word = static_cast<uint32_t>(bit & 32 ? mask >> 32 : mask);
+        return (key >= lo) & (key <= hi) & ((key < base) | ((word >> (bit & 31)) & 1));
     }
 };
 
@@ -416,13 +491,16 @@ struct KvRows {
     KvView kv;
     uint64_t page_step;  // elements from page to page
     uint32_t dim;
-    // the page of a slot; 0 for one that is none, and *bad
-    __device__ __forceinline__ int32_t page_of(uint32_t slot, bool& bad) const {
-        const int32_t p = table[slot >> kv.shift];
+    // A table entry as it stands: read ahead, it is checked when it is used, so that nothing
+    // waits for it before.
+    __device__ __forceinline__ int32_t entry_of(uint32_t slot) const { return table[slot >> kv.shift]; }
+    // A page that an entry names; 0 for one that is none, and `bad`.
+    __device__ __forceinline__ int32_t checked(int32_t p, bool& bad) const {
         if (page_ok(kv, p)) return p;
         bad = true;
         return 0;
     }
+    __device__ __forceinline__ int32_t page_of(uint32_t slot, bool& bad) const { return checked(entry_of(slot), bad); }
     __device__ __forceinline__ uint64_t paged_at(int32_t page, uint32_t slot) const {
         return static_cast<uint64_t>(static_cast<uint32_t>(page)) * page_step + (slot & ((1u << kv.shift) - 1)) * dim;
     }
@@ -435,6 +513,17 @@ struct KvRows {
         else return v + key * v_stride;
     }
 };
+
+// Loads through a buffer descriptor: a unit at or past `bytes` comes back as zeros with no
+// test and no branch, so a tile's loads are one straight run. `p` is the same in all lanes.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(bytes), 0x00027000);
+}
+__device__ __forceinline__ u32x4a buffer_unit(__amdgpu_buffer_rsrc_t r, uint32_t offset) {
+    return __builtin_bit_cast(u32x4a, __builtin_amdgcn_raw_buffer_load_b128(r, static_cast<int>(offset), 0, 0));
+}
+constexpr uint32_t kNowhere = 0xC0000000u;   // a lane's place past every buffer, with room for the tile's offsets
+constexpr uint64_t kMaxKvStride = 1u << 23;  // elements: 64 rows below kNowhere bytes
 
 // One row computed key by key over the keys it sees in [k0, k1), by a whole wave (a lane has
 // dimensions lane, lane + 64, ...). The matrix products multiply unseen values by a
@@ -551,6 +640,25 @@ __device__ __forceinline__ void write_row(const AttnArgs& a, float m, float l, c
     for (int x = 0; x < 4; ++x)
         if (lane + 64 * x < a.dim) p[lane + 64 * x] = static_cast<typename M::qelem>(o[x] * inv);
     if (a.lse && lane == 0) a.lse[row * a.n_heads + head] = l == 0.0f ? -kInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// Rows of an entry past what max_rows allows for (n_tiles of `rows`): NaN, reported. By the last
+// tile's workgroup; a join writes its own.
+template <class M>
+__device__ __forceinline__ void past_rows(const AttnArgs& a, uint32_t tile, uint32_t rows, uint32_t n_m, int32_t row0,
+                                          uint32_t head, uint32_t split) {
+    const uint64_t room = static_cast<uint64_t>(a.n_tiles) * rows;
+    if (n_m <= room || tile + 1 != a.n_tiles || split) return;
+    if (threadIdx.x == 0) atomicOr(a.err, kErrIndex);
+    if (a.n_splits > 1) return;
+    const float nan = __builtin_nanf("");
+    for (uint64_t m = room; m < n_m; ++m) {
+        const uint64_t row = static_cast<uint64_t>(row0) + m / a.group;
+        const uint32_t q_head = head * a.group + static_cast<uint32_t>(m % a.group);
+        typename M::qelem* p = static_cast<typename M::qelem*>(a.out) + row * a.out_stride + static_cast<uint64_t>(q_head) * a.dim;
+        for (uint32_t d = threadIdx.x; d < a.dim; d += blockDim.x) p[d] = static_cast<typename M::qelem>(nan);
+        if (a.lse && threadIdx.x == 0) a.lse[row * a.n_heads + q_head] = nan;
+    }
 }
 
 template <class M>

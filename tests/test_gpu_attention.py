@@ -423,12 +423,31 @@ def test_cached_long_contexts_are_cut(backend, att, dtype, kv, rows):
 
 
 @pytest.mark.parametrize("rows", [[1, 2], [70, 3]])
-def test_cached_hints_only_cut_the_work(backend, att, rows):
-    """max_rows and max_len below and far above the truth give the same results."""
+def test_cached_bounds_only_cut_the_work(backend, att, rows):
+    """max_len below and far above the truth, and max_rows above it, give the same results."""
     c = Cached(backend, [1500, 900], "bf16", 2, 16, 64, seed=7)
-    for mr, ml in ((1, 1), (1, 100000), (5, 300), (1000, 1500), (64, 1)):
+    for mr, ml in ((70, 1), (70, 100000), (75, 300), (1000, 1500), (72, 257)):
         q, got, lse, cu = run_cached(att, c, [0, 1], rows, "bf16", 8, max_rows=mr, max_len=ml)
         check_cached(c, [0, 1], q, got, lse, cu, "bf16", 8)
+
+
+@pytest.mark.parametrize("rows,max_rows,group", [([4, 9], 4, 4), ([50, 3], 40, 8), ([20, 70], 1, 16)])
+@pytest.mark.parametrize("max_len", [200, 3000])
+def test_cached_more_rows_than_said(backend, rows, max_rows, group, max_len):
+    """Rows past max_rows come out right or NaN and are reported; those within it are right."""
+    att, err = AttentionBackend(backend), MoeExecutor(backend)
+    err.device_error()
+    c = Cached(backend, [1500, 900], "f16", 1, 16, 64, seed=7)
+    q, got, lse, cu = run_cached(att, c, [0, 1], rows, "f16", group, max_rows=max_rows, max_len=max_len)
+    assert err.device_error() == 4
+    full, full_lse = run_cached(att, c, [0, 1], rows, "f16", group, q=q, max_len=max_len)[1:3]
+    for b in range(2):
+        for r in range(cu[b], cu[b + 1]):
+            for h in range(group):
+                gone = np.isnan(got[r, h]).all() and np.isnan(lse[r, h])
+                # the same sums, the keys cut elsewhere: half a step of the output and of p each
+                near = np.all(np.abs(got[r, h] - full[r, h]) <= 4 * 2.0 ** -11) and abs(lse[r, h] - full_lse[r, h]) <= 1e-5
+                assert near or (gone and r - cu[b] >= max_rows), (b, r, h)
 
 
 def test_cached_layers(backend, att):
