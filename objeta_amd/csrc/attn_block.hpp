@@ -43,24 +43,13 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
     KvRows<PAGED, KT> kv;
     bool usable = true;
     if constexpr (PAGED) {
-        const CachedItem item(a, blockIdx.x);
+        const BlockItem item(a, blockIdx.x);
         if (!item.any) return;
         split = item.split, tile = item.tile, head = item.head;
-        const uint32_t b = item.b;
-        row0 = a.cu[b];
-        const int32_t end = a.cu[b + 1];
-        n_q = end - row0;
-        if (row0 < 0 || end < row0 || static_cast<uint32_t>(end) > a.n_rows) {
-            if (threadIdx.x == 0) atomicOr(a.err, kErrIndex);
-            return;
-        }
-        const int32_t seq = a.seqs[b];
-        usable = seq_ok(a.kv, seq);
-        len = usable ? a.kv.lens[seq] : 0;
-        usable = usable && len_ok(a.kv, len) && n_q <= len && (!a.tree || n_q <= 64);
-        if (!usable) len = 0;
-        if (!usable && threadIdx.x == 0 && n_q) atomicOr(a.err, kErrIndex);
-        if (split && static_cast<uint64_t>(split) * a.chunk >= static_cast<uint64_t>(len)) return;
+        row0 = item.row0, n_q = item.n_q, len = item.len;
+        usable = item.usable;
+        const int32_t seq = item.seq;
+        if (!usable && tid == 0) atomicOr(a.err, kErrIndex);
         kv.kv = a.kv;
         kv.table = a.kv.table + static_cast<uint64_t>(usable ? seq : 0) * a.kv.max_pages;
         kv.page_step = (static_cast<uint64_t>(a.n_kv) * a.dim) << a.kv.shift;
@@ -79,7 +68,6 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
     const uint32_t n_m = static_cast<uint32_t>(n_q) * a.group;
 
     if constexpr (PAGED) past_rows<M>(a, tile, 128, n_m, row0, head, split);
-    if (static_cast<uint64_t>(tile) * 128 >= n_m) return;
     // ---- this lane's row
     const uint32_t m = tile * 128 + wave * 32 + (lane & 31);
     bool real = m < n_m;
@@ -114,34 +102,41 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
     M::load_q(q, static_cast<const typename M::qelem*>(a.q) + row * a.q_stride + static_cast<uint64_t>(q_head) * a.dim, real,
               a.dim, lane, scale);
     M::settle(q);
-    // ---- what the wave and the workgroup see
-    const bool sees_any = view.lo <= view.hi;
-    int32_t w_lo = sees_any ? view.lo : 0x7FFFFFFF, w_hi = sees_any ? view.hi : -1;
-    int32_t all_lo = sees_any || !real ? view.lo : 0x7FFFFFFF;  // from here to all_hi every real row sees all
-    int32_t all_hi = real ? (view.base - 1 < view.hi ? view.base - 1 : view.hi) : 0x7FFFFFFF;
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) {
-        const int32_t x = __shfl_xor(w_lo, s, 64), y = __shfl_xor(w_hi, s, 64);
-        const int32_t z = __shfl_xor(all_lo, s, 64), w = __shfl_xor(all_hi, s, 64);
-        w_lo = x < w_lo ? x : w_lo, w_hi = y > w_hi ? y : w_hi;
-        all_lo = z > all_lo ? z : all_lo, all_hi = w < all_hi ? w : all_hi;
-    }
+    // ---- what the workgroup sees, [k_lo, k_end), and what every real row of the wave sees whole
+    int32_t k_lo, k_end, all_lo, all_hi;
     if (tid == 0) sh_bad = 0;
-    if (lane == 0) sh_lo[wave] = w_lo, sh_hi[wave] = w_hi;
-    __syncthreads();
-    int32_t k_lo = sh_lo[0], k_hi = sh_hi[0];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) {
-        k_lo = sh_lo[w] < k_lo ? sh_lo[w] : k_lo;
-        k_hi = sh_hi[w] > k_hi ? sh_hi[w] : k_hi;
-    }
-    k_lo = __builtin_amdgcn_readfirstlane(k_lo), k_hi = __builtin_amdgcn_readfirstlane(k_hi);
-    all_lo = __builtin_amdgcn_readfirstlane(all_lo), all_hi = __builtin_amdgcn_readfirstlane(all_hi);
-    int32_t k_end = k_hi + 1;
     if constexpr (PAGED) {
+        const uint32_t m0 = tile * 128 + __builtin_amdgcn_readfirstlane(wave) * 32;
+        const uint32_t m1 = tile * 128 + 128 < n_m ? tile * 128 + 127 : n_m - 1;
         const int64_t c0 = static_cast<int64_t>(split) * a.chunk, c1 = c0 + a.chunk;
-        if (k_lo < c0) k_lo = static_cast<int32_t>(c0);
+        const int32_t base = len - n_q;
+        k_lo = static_cast<int32_t>(c0);
+        k_end = usable ? (a.tree ? len : base + static_cast<int32_t>(m1 / a.group) + 1) : 0;
         if (split + 1 < a.n_splits && k_end > c1) k_end = static_cast<int32_t>(c1);
+        all_lo = 0;
+        all_hi = a.tree ? base - 1 : base + static_cast<int32_t>(m0 / a.group);
+    } else {
+        const bool sees_any = view.lo <= view.hi;
+        int32_t w_lo = sees_any ? view.lo : 0x7FFFFFFF, w_hi = sees_any ? view.hi : -1;
+        all_lo = sees_any || !real ? view.lo : 0x7FFFFFFF;
+        all_hi = real ? view.hi : 0x7FFFFFFF;
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) {
+            const int32_t x = __shfl_xor(w_lo, s, 64), y = __shfl_xor(w_hi, s, 64);
+            const int32_t z = __shfl_xor(all_lo, s, 64), w = __shfl_xor(all_hi, s, 64);
+            w_lo = x < w_lo ? x : w_lo, w_hi = y > w_hi ? y : w_hi;
+            all_lo = z > all_lo ? z : all_lo, all_hi = w < all_hi ? w : all_hi;
+        }
+        if (lane == 0) sh_lo[wave] = w_lo, sh_hi[wave] = w_hi;
+        __syncthreads();
+        int32_t lo = sh_lo[0], hi = sh_hi[0];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) {
+            lo = sh_lo[w] < lo ? sh_lo[w] : lo;
+            hi = sh_hi[w] > hi ? sh_hi[w] : hi;
+        }
+        k_lo = __builtin_amdgcn_readfirstlane(lo), k_end = __builtin_amdgcn_readfirstlane(hi) + 1;
+        all_lo = __builtin_amdgcn_readfirstlane(all_lo), all_hi = __builtin_amdgcn_readfirstlane(all_hi);
     }
     RowState<M> st;
     st.clear();

@@ -11,7 +11,7 @@ namespace {
 template <int Q, int K, int DT>
 int32_t launch(hipStream_t s, const AttnArgs& a, const char* action) {
     const uint64_t groups = static_cast<uint64_t>(a.n_splits) * a.n_batch * a.n_kv;
-    const uint64_t x = (groups + 7) / 8 * 8 * a.n_tiles;
+    const uint64_t x = groups * a.n_tiles;
     if (x > 0x7FFFFFFFull) OBJ_FAIL(kInvalidInput, action, "too many workgroups for one launch");
     hipLaunchKernelGGL((attn_block_kernel<Q, K, DT, true>), dim3(static_cast<uint32_t>(x)), dim3(256), 0, s, a);
     OBJ_HIP(hipGetLastError(), action);
@@ -21,7 +21,9 @@ int32_t launch(hipStream_t s, const AttnArgs& a, const char* action) {
 template <int Q, int K>
 int32_t launch_dim(hipStream_t s, const AttnArgs& a, const char* action) {
     if (a.dim <= 64) return launch<Q, K, 64>(s, a, action);
+    if (a.dim <= 96) return launch<Q, K, 96>(s, a, action);
     if (a.dim <= 128) return launch<Q, K, 128>(s, a, action);
+    if (a.dim <= 192) return launch<Q, K, 192>(s, a, action);
     return launch<Q, K, 256>(s, a, action);
 }
 

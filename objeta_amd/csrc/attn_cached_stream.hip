@@ -11,7 +11,7 @@ namespace {
 template <int Q, int K, int DT, int ROWS>
 int32_t launch(hipStream_t s, const AttnArgs& a, const char* action) {
     const uint64_t groups = static_cast<uint64_t>(a.n_splits) * a.n_batch * a.n_kv;
-    const uint64_t x = (groups + 7) / 8 * 8 * a.n_tiles;
+    const uint64_t x = (groups + 7) / 8 * 8;
     if (x > 0x7FFFFFFFull) OBJ_FAIL(kInvalidInput, action, "too many workgroups for one launch");
     hipLaunchKernelGGL((attn_stream_kernel<Q, K, DT, ROWS>), dim3(static_cast<uint32_t>(x)), dim3(64 * Stream<K, DT, ROWS>::kWaves), 0, s, a);
     OBJ_HIP(hipGetLastError(), action);

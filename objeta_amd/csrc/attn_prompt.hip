@@ -20,7 +20,9 @@ int32_t launch_prompt(hipStream_t s, const AttnArgs& a, const char* action) {
 template <int T>
 int32_t launch_prompt_dim(hipStream_t s, const AttnArgs& a, const char* action) {
     if (a.dim <= 64) return launch_prompt<T, 64>(s, a, action);
+    if (a.dim <= 96) return launch_prompt<T, 96>(s, a, action);
     if (a.dim <= 128) return launch_prompt<T, 128>(s, a, action);
+    if (a.dim <= 192) return launch_prompt<T, 192>(s, a, action);
     return launch_prompt<T, 256>(s, a, action);
 }
 

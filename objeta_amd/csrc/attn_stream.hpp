@@ -42,10 +42,9 @@ __global__ __launch_bounds__((64 * Stream<KT, DT, ROWS>::kWaves),
     __shared__ int32_t sh_bad;
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane / ROWS, mine = lane % ROWS;
-    const CachedItem item(a, blockIdx.x);
+    const StreamItem item(a, blockIdx.x);
     if (!item.any) return;
-    const uint32_t split = item.split, head = item.head, b = item.b;
-    const uint32_t tile = item.tile;
+    const uint32_t split = item.split, head = item.head, b = item.b, tile = 0;
     const int32_t row0 = a.cu[b], end = a.cu[b + 1], n_q = end - row0;
     if (row0 < 0 || end < row0 || static_cast<uint32_t>(end) > a.n_rows) {
         if (tid == 0) atomicOr(a.err, kErrIndex);

@@ -440,23 +440,77 @@ struct AttnArgs {
     uint32_t* err;
 };
 
-// Which (sequence, head, split) and row tile a workgroup of a cached call takes. The splits are
-// the slowest index: short sequences have only the first ones, and workgroups go to the eight
-// XCDs in turn, so a fast split index would give the first XCDs most of the work. The groups
-// are turned by one place from split to split, so that no XCD keeps the longest sequences.
-// The row tiles of one group, which read the same keys and values, are eight apart: on one XCD.
-struct CachedItem {
-    uint32_t b, head, split, tile;
+// Which (entry, head, split) a workgroup of 16 or 32 rows takes. The splits are the slowest
+// index: short sequences have only the first ones, and workgroups go to the eight XCDs in
+// turn, so a fast split index would give the first XCDs most of the work. The groups are
+// turned by one place from split to split, so that no XCD keeps the longest sequences.
+struct StreamItem {
+    uint32_t b, head, split;
     bool any;
-    __device__ __forceinline__ CachedItem(const AttnArgs& a, uint32_t id) {
-        const uint32_t eight = id / (8 * a.n_tiles), in = id % (8 * a.n_tiles);
-        const uint32_t per = a.n_batch * a.n_kv;
-        const uint32_t g = eight * 8 + ((in + eight * 8 / per) & 7);
-        tile = in >> 3;
+    __device__ __forceinline__ StreamItem(const AttnArgs& a, uint32_t id) {
+        const uint32_t per = a.n_batch * a.n_kv, g = (id & ~7u) + ((id + (id & ~7u) / per) & 7);
         split = g / per;
         any = split < a.n_splits;
         head = g % per % a.n_kv;
         b = g % per / a.n_kv;
+    }
+};
+
+// Which piece of work a workgroup of 128 rows takes, counted over the pieces that there are:
+// entries differ in rows and lengths, and a grid over the largest of both would be mostly
+// empty workgroups, unevenly over the XCDs (8 trees of 9 to 64 drafts: 39 to 64 workgroups on
+// an XCD, the kernel 80 us for 44 us of work on every CU). Each wave reads 64 entries at a
+// time, a lane an entry, and finds the id'th piece in their running sum; what it read of the
+// entry need not be read again.
+struct BlockItem {
+    uint32_t head, split, tile;
+    int32_t row0, n_q, len, seq;
+    bool any, usable;
+    __device__ __forceinline__ BlockItem(const AttnArgs& a, uint32_t id) {
+        const uint32_t lane = threadIdx.x & 63;
+        any = false;
+        for (uint32_t b0 = 0; b0 < a.n_batch; b0 += 64) {
+            const uint32_t b = b0 + lane;
+            int32_t lo = 0, n = 0, s = 0, l = 0;
+            bool ok = true;
+            uint32_t pieces = 0, splits = 1, tiles = 0;
+            if (b < a.n_batch) {
+                lo = a.cu[b];
+                const int32_t hi = a.cu[b + 1];
+                s = a.seqs[b];
+                const bool rows = lo >= 0 && hi >= lo && static_cast<uint32_t>(hi) <= a.n_rows;
+                if (!rows && id == 0) atomicOr(a.err, kErrIndex);
+                n = rows ? hi - lo : 0;
+                ok = seq_ok(a.kv, s);
+                l = ok ? a.kv.lens[s] : 0;
+                ok = ok && len_ok(a.kv, l) && n <= l && (!a.tree || n <= 64);
+                if (!ok) l = 0;
+                tiles = (static_cast<uint32_t>(n) * a.group + 127) / 128;
+                tiles = tiles < a.n_tiles ? tiles : a.n_tiles;
+                splits = (static_cast<uint32_t>(l) + a.chunk - 1) / a.chunk;
+                splits = splits < 1 ? 1 : (splits < a.n_splits ? splits : a.n_splits);
+                pieces = tiles * splits * a.n_kv;
+            }
+            uint32_t sum = pieces;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t o = __shfl_up(sum, d, 64);
+                if (lane >= static_cast<uint32_t>(d)) sum += o;
+            }
+            const uint64_t past = __ballot(sum > id);
+            if (past) {
+                const int at = __builtin_ctzll(past);
+                const uint32_t in = id - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(pieces, at));
+                const uint32_t n_tiles = __builtin_amdgcn_readlane(tiles, at), rest = in / a.n_kv;
+                head = in % a.n_kv, tile = rest % n_tiles, split = rest / n_tiles;
+                row0 = __builtin_amdgcn_readlane(lo, at), n_q = __builtin_amdgcn_readlane(n, at);
+                len = __builtin_amdgcn_readlane(l, at), seq = __builtin_amdgcn_readlane(s, at);
+                usable = __builtin_amdgcn_readlane(static_cast<int32_t>(ok), at) != 0;
+                any = true;
+                return;
+            }
+            id -= __builtin_amdgcn_readlane(sum, 63);
+        }
     }
 };
 
