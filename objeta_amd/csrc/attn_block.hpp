@@ -58,8 +58,10 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
         kv.v = static_cast<const typename M::kelem*>(a.v) + off;
     } else {
         // the last tiles see the most keys: they start first
+        const uint32_t piece = blockIdx.x / a.n_kv;
         head = blockIdx.x % a.n_kv;
-        tile = a.n_tiles - 1 - blockIdx.x / a.n_kv;
+        split = piece % a.n_splits;
+        tile = a.n_tiles - 1 - piece / a.n_splits;
         kv.k = static_cast<const typename M::kelem*>(a.k) + static_cast<uint64_t>(head) * a.dim;
         kv.v = static_cast<const typename M::kelem*>(a.v) + static_cast<uint64_t>(head) * a.dim;
         kv.k_stride = a.k_stride, kv.v_stride = a.v_stride;
@@ -82,8 +84,8 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
         }
     } else {
         if (real) {
-            // the sequence that holds token i: the last start that is <= i
-            uint32_t lo = 0, hi = a.n_batch;  // cu[lo] <= i < cu[hi] once both are known to hold
+            // the sequence that holds token i: the first whose end is past i
+            uint32_t lo = 0, hi = a.n_batch;
             while (lo < hi) {
                 const uint32_t mid = (lo + hi) >> 1;
                 if (a.cu[mid + 1] <= static_cast<int32_t>(i)) lo = mid + 1;
@@ -137,6 +139,14 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
         }
         k_lo = __builtin_amdgcn_readfirstlane(lo), k_end = __builtin_amdgcn_readfirstlane(hi) + 1;
         all_lo = __builtin_amdgcn_readfirstlane(all_lo), all_hi = __builtin_amdgcn_readfirstlane(all_hi);
+        if (a.n_splits > 1 && k_lo < k_end) {
+            const uint32_t n = static_cast<uint32_t>(k_end - k_lo);
+            const uint32_t part = ((n + a.n_splits - 1) / a.n_splits + kKeys - 1) / kKeys * kKeys;
+            const int64_t p0 = static_cast<int64_t>(k_lo & ~(kKeys - 1)) + static_cast<int64_t>(split) * part;
+            const int64_t p1 = split + 1 < a.n_splits ? p0 + part : k_end;
+            k_lo = p0 > k_lo ? static_cast<int32_t>(p0 < k_end ? p0 : k_end) : k_lo;
+            k_end = p1 < k_end ? static_cast<int32_t>(p1) : k_end;
+        }
     }
     RowState<M> st;
     st.clear();

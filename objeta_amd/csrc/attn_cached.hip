@@ -11,7 +11,7 @@ namespace dev {
 // the parts of one (row, head): one where there are many of these with few parts each (9280 of
 // up to 7 parts of 128: 13.6 us, with four waves 18.0), four otherwise (1024 of up to 8: 4.9
 // us, with one 6.8).
-template <int QT, int LANES, int WAVES>
+template <int QT, int LANES, int WAVES, bool PAGED>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     typedef typename ElemOf<QT>::type elem;
     constexpr uint32_t kAtOnce = WAVES * 64 / LANES;
@@ -27,13 +27,18 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
         const uint32_t le = count_le(a.cu, a.n_batch + 1, row);
         any = le != 0 && le <= a.n_batch;
         if (any) {
-            const int32_t lo = a.cu[le - 1], hi = a.cu[le], seq = a.seqs[le - 1];
+            const int32_t lo = a.cu[le - 1], hi = a.cu[le];
             any = lo >= 0 && lo <= static_cast<int32_t>(row) && static_cast<int32_t>(row) < hi &&
                   static_cast<uint32_t>(hi) <= a.n_rows;
-            int32_t len = seq_ok(a.kv, seq) ? a.kv.lens[seq] : 0;
-            if (!len_ok(a.kv, len) || hi - lo > len || (a.tree && hi - lo > 64)) len = 0;
-            n = (static_cast<uint32_t>(len) + a.chunk - 1) / a.chunk;
-            n = !any ? 0 : (n < 1 ? 1 : (n > a.n_splits ? a.n_splits : n));
+            n = a.n_splits;
+            if constexpr (PAGED) {
+                const int32_t seq = a.seqs[le - 1];
+                int32_t len = seq_ok(a.kv, seq) ? a.kv.lens[seq] : 0;
+                if (!len_ok(a.kv, len) || hi - lo > len || (a.tree && hi - lo > 64)) len = 0;
+                n = (static_cast<uint32_t>(len) + a.chunk - 1) / a.chunk;
+                n = n < 1 ? 1 : (n > a.n_splits ? a.n_splits : n);
+            }
+            n = any ? n : 0;
             at_row = row - static_cast<uint32_t>(lo);
         }
     }
@@ -62,10 +67,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
         o += sh_o[p * LANES + tid];
         l += sh_l[tid / LANES + p];
     }
-    // a row past what max_rows allows for has no parts
-    const uint32_t group = a.n_heads / a.n_kv;
-    if (static_cast<uint64_t>(at_row) * group + head % group >= static_cast<uint64_t>(a.n_tiles) * a.tile_rows)
-        l = o.x = o.y = o.z = o.w = __builtin_nanf("");
+    if constexpr (PAGED) {  // a row past what max_rows allows for has no parts
+        const uint32_t group = a.n_heads / a.n_kv;
+        if (static_cast<uint64_t>(at_row) * group + head % group >= static_cast<uint64_t>(a.n_tiles) * a.tile_rows)
+            l = o.x = o.y = o.z = o.w = __builtin_nanf("");
+    }
     store_out<QT>(static_cast<elem*>(a.out) + row * a.out_stride + static_cast<uint64_t>(head) * a.dim + x,
                   o * (l == 0.0f ? 0.0f : 1.0f / l));
     if (a.lse && x == 0) a.lse[rh] = l == 0.0f ? -kInf : (top + __builtin_amdgcn_logf(l)) * kLn2;
@@ -77,23 +83,40 @@ using namespace dev;
 
 namespace {
 
-template <int QT, int LANES>
+template <int QT, int LANES, bool PAGED>
 int32_t launch_join_lanes(hipStream_t s, const AttnArgs& a, const char* action) {
     const uint32_t rows = a.n_rows * a.n_heads;
-    if (a.n_splits <= 16 && rows >= 4096) hipLaunchKernelGGL((attn_join_kernel<QT, LANES, 1>), dim3((rows + 3) / 4), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((attn_join_kernel<QT, LANES, 4>), dim3(rows), dim3(256), 0, s, a);
+    if (a.n_splits <= 16 && rows >= 4096)
+        hipLaunchKernelGGL((attn_join_kernel<QT, LANES, 1, PAGED>), dim3((rows + 3) / 4), dim3(256), 0, s, a);
+    else
+        hipLaunchKernelGGL((attn_join_kernel<QT, LANES, 4, PAGED>), dim3(rows), dim3(256), 0, s, a);
     OBJ_HIP(hipGetLastError(), action);
     return 0;
 }
 
-template <int QT>
+template <int QT, bool PAGED>
 int32_t launch_join(hipStream_t s, const AttnArgs& a, const char* action) {
-    if (a.dim <= 64) return launch_join_lanes<QT, 16>(s, a, action);
-    if (a.dim <= 128) return launch_join_lanes<QT, 32>(s, a, action);
-    return launch_join_lanes<QT, 64>(s, a, action);
+    if (a.dim <= 64) return launch_join_lanes<QT, 16, PAGED>(s, a, action);
+    if (a.dim <= 128) return launch_join_lanes<QT, 32, PAGED>(s, a, action);
+    return launch_join_lanes<QT, 64, PAGED>(s, a, action);
 }
 
 }  // namespace
+
+int32_t attn_parts(objeta_hip_context* ctx, hipStream_t s, AttnArgs& a) {
+    const size_t parts = static_cast<size_t>(a.n_splits) * a.n_rows * a.n_heads;
+    void* ws = nullptr;
+    OBJ_TRY(ensure_workspace(ctx, s, kWsAttn, parts * (a.dim + 2) * sizeof(float), &ws));
+    a.part = static_cast<float*>(ws);
+    a.part_ml = a.part + parts * a.dim;
+    return 0;
+}
+
+int32_t launch_attn_join(hipStream_t s, int32_t dtype, bool paged, const AttnArgs& a, const char* action) {
+    if (dtype == kDtF32) return paged ? launch_join<kDtF32, true>(s, a, action) : launch_join<kDtF32, false>(s, a, action);
+    if (dtype == kDtF16) return paged ? launch_join<kDtF16, true>(s, a, action) : launch_join<kDtF16, false>(s, a, action);
+    return paged ? launch_join<kDtBF16, true>(s, a, action) : launch_join<kDtBF16, false>(s, a, action);
+}
 
 }  // namespace objeta
 
@@ -166,19 +189,10 @@ int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream
     splits = (len + chunk - 1) / chunk;
     a.chunk = static_cast<uint32_t>(chunk);
     a.n_splits = static_cast<uint32_t>(splits);
-    if (splits > 1) {
-        const size_t parts = static_cast<size_t>(splits) * n_rows * n_q_heads;
-        void* ws = nullptr;
-        OBJ_TRY(ensure_workspace(ctx, s, kWsAttn, parts * (dim + 2) * sizeof(float), &ws));
-        a.part = static_cast<float*>(ws);
-        a.part_ml = a.part + parts * dim;
-    }
+    if (splits > 1) OBJ_TRY(attn_parts(ctx, s, a));
     OBJ_TRY(stream_form ? launch_attn_stream(s, dtype, c.dtype, static_cast<uint32_t>(rows), a, action)
                         : launch_attn_cached_block(s, dtype, c.dtype, a, action));
-    if (splits == 1) return 0;
-    if (dtype == kDtF32) return launch_join<kDtF32>(s, a, action);
-    if (dtype == kDtF16) return launch_join<kDtF16>(s, a, action);
-    return launch_join<kDtBF16>(s, a, action);
+    return splits == 1 ? 0 : launch_attn_join(s, dtype, true, a, action);
     OBJ_GUARD_END
 }
 

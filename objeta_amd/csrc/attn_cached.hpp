@@ -1,4 +1,4 @@
-// attn_cached.hpp — the launchers behind objeta_hip_attn_cached_device.
+// attn_cached.hpp — the checks and launchers that both attentions' entry points use.
 #pragma once
 
 #include "attn_tile.hpp"
@@ -9,6 +9,9 @@ namespace objeta {
 int32_t check_attn_rows(const char* action, const char* what, const void* p, uint64_t n, uint64_t stride, uint64_t heads,
                         uint64_t dim, uint64_t size);
 int32_t check_heads(const char* action, uint64_t n_q_heads, uint64_t n_kv_heads, uint64_t n_rows, float scale);
+// Workspace for the parts of a call of several splits, and their join (attn_cached.hip).
+int32_t attn_parts(objeta_hip_context* ctx, hipStream_t s, dev::AttnArgs& a);
+int32_t launch_attn_join(hipStream_t s, int32_t dtype, bool paged, const dev::AttnArgs& a, const char* action);
 // Tiles of 16 rows (rows <= 16) or 32.
 int32_t launch_attn_stream(hipStream_t s, int32_t q_type, int32_t kv_type, uint32_t rows, const dev::AttnArgs& a,
                            const char* action);

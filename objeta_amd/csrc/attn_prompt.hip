@@ -1,5 +1,6 @@
 // attn_prompt.hip — attention over packed prompts (objeta_hip_attn_prompt_device).
 #include "attn_block.hpp"
+#include "attn_cached.hpp"
 #include "kernels.hpp"
 
 #include <cmath>
@@ -10,20 +11,52 @@ using namespace dev;
 
 namespace {
 
+// Parts of the keys that a tile of rows sees, so that few tiles fill the card too: the n with
+// the least time (and a tenth less than one part's), counted in keys that a workgroup alone on its
+// CU takes. Two a CU take 1.37
+// times as long, each; a turn's setup and the parts' way through memory and the join cost what
+// 16-bit products spend on 200 and on 250 + 0.7 a workgroup, float ones on an eighth of that.
+// Sequences are taken to be of their mean length, which is what the host knows; the tiles of a
+// causal one see half of it in the mean, and the longest start first. Measured, one part and the
+// parts chosen: float, 3 x 510 tokens of 8 over 2 heads of 192: 237 us and 114 (5); 777 of 8
+// heads of 64: 64 and 32 (4); bf16 of 128, causal: 1024 tokens of 8 heads 30 and 26 (3), 5000 of
+// 8 over 2 115 and 97 (3); 512 of 32 over 8: 20, with two parts 25 (1).
 template <int T, int DT>
-int32_t launch_prompt(hipStream_t s, const AttnArgs& a, const char* action) {
-    hipLaunchKernelGGL((attn_block_kernel<T, T, DT, false>), dim3(a.n_tiles * a.n_kv), dim3(256), 0, s, a);
+uint32_t prompt_splits(const AttnArgs& a) {
+    constexpr bool two = T != kDtF32 && Block<T, DT>::kPerCu == 2;
+    constexpr double each = two ? 1.37 : 1.0, extra = T == kDtF32 ? 0.125 : 1.0;
+    const uint64_t tiles = static_cast<uint64_t>(a.n_tiles) * a.n_kv, slots = two ? 512 : 256;
+    const double keys = static_cast<double>(a.n_rows) / a.n_batch;
+    uint32_t best = 1;
+    double best_cost = 0.0;
+    for (uint32_t n = 1; n <= 8; ++n) {
+        const uint64_t items = tiles * n, rest = items % slots;
+        double turns = static_cast<double>(items / slots) * each + (rest ? (rest > 256 ? each : 1.0) : 0.0);
+        if (a.causal) turns = __builtin_fmax(turns > 1.0 ? 1.0 + 0.5 * (each - 1.0) : 1.0, 0.5 * each * items / slots);
+        const double setup = static_cast<double>((items + slots - 1) / slots) * 200.0;
+        const double join = n > 1 ? 250.0 + 0.7 * items : 0.0;
+        const double cost = turns * keys / n + extra * (setup + join);
+        if (n == 1 || cost < (best == 1 ? 0.9 : 1.0) * best_cost) best = n, best_cost = cost;
+    }
+    return best;
+}
+
+template <int T, int DT>
+int32_t launch_prompt(objeta_hip_context* ctx, hipStream_t s, AttnArgs& a, const char* action) {
+    a.n_splits = prompt_splits<T, DT>(a);
+    if (a.n_splits > 1) OBJ_TRY(attn_parts(ctx, s, a));
+    hipLaunchKernelGGL((attn_block_kernel<T, T, DT, false>), dim3(a.n_tiles * a.n_splits * a.n_kv), dim3(256), 0, s, a);
     OBJ_HIP(hipGetLastError(), action);
-    return 0;
+    return a.n_splits > 1 ? launch_attn_join(s, T, false, a, action) : 0;
 }
 
 template <int T>
-int32_t launch_prompt_dim(hipStream_t s, const AttnArgs& a, const char* action) {
-    if (a.dim <= 64) return launch_prompt<T, 64>(s, a, action);
-    if (a.dim <= 96) return launch_prompt<T, 96>(s, a, action);
-    if (a.dim <= 128) return launch_prompt<T, 128>(s, a, action);
-    if (a.dim <= 192) return launch_prompt<T, 192>(s, a, action);
-    return launch_prompt<T, 256>(s, a, action);
+int32_t launch_prompt_dim(objeta_hip_context* ctx, hipStream_t s, AttnArgs& a, const char* action) {
+    if (a.dim <= 64) return launch_prompt<T, 64>(ctx, s, a, action);
+    if (a.dim <= 96) return launch_prompt<T, 96>(ctx, s, a, action);
+    if (a.dim <= 128) return launch_prompt<T, 128>(ctx, s, a, action);
+    if (a.dim <= 192) return launch_prompt<T, 192>(ctx, s, a, action);
+    return launch_prompt<T, 256>(ctx, s, a, action);
 }
 
 }  // namespace
@@ -103,13 +136,12 @@ int32_t objeta_hip_attn_prompt_device(objeta_hip_context* ctx, objeta_hip_stream
     a.dim = static_cast<uint32_t>(head_dim);
     a.scale = scale, a.scale_log2 = scale * kLog2e;
     a.causal = causal;
-    a.n_splits = 1;
     a.n_tiles = static_cast<uint32_t>((n_tokens * a.group + 127) / 128);
     a.err = ctx->err_word;
     const hipStream_t s = resolve_stream(ctx, stream);
-    if (dtype == kDtF32) return launch_prompt_dim<kDtF32>(s, a, action);
-    if (dtype == kDtF16) return launch_prompt_dim<kDtF16>(s, a, action);
-    return launch_prompt_dim<kDtBF16>(s, a, action);
+    if (dtype == kDtF32) return launch_prompt_dim<kDtF32>(ctx, s, a, action);
+    if (dtype == kDtF16) return launch_prompt_dim<kDtF16>(ctx, s, a, action);
+    return launch_prompt_dim<kDtBF16>(ctx, s, a, action);
     OBJ_GUARD_END
 }
 

@@ -434,7 +434,8 @@ struct AttnArgs {
     const int32_t* seqs;
     const uint64_t* tree;
     uint64_t layer_off;  // elements
-    // keys cut over workgroups
+    // keys cut over workgroups: of cached sequences in chunks of `chunk`, of a prompt's tile of rows
+    // in n_splits equal parts
     uint32_t chunk, n_splits, n_tiles, tile_rows;
     float *part, *part_ml;  // [n_splits][n_rows * n_heads][dim], [..][2]
     uint32_t* err;
