@@ -13,6 +13,7 @@ namespace objeta {
 namespace dev {
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef int32_t i4 __attribute__((ext_vector_type(4)));
 
 constexpr uint32_t kExtThreads = 1024;
 
@@ -44,30 +45,59 @@ __device__ __forceinline__ uint64_t scan_1024(uint64_t v, uint64_t* sh, uint64_t
 
 // extend's bookkeeping in one workgroup, a thread an entry:
 //   1. what each entry needs (copy on write included), summed over the entries before it;
-//   2. the free pages in index order, as many as are needed;
-//   3. table entries, counts and lengths of the entries that the free pages cover.
+//   2. the free pages in index order, counted by waves that each own a part of the counts;
+//   3. table entries, counts and lengths of the entries that the free pages cover: the thread
+//      that finds the f'th free page finds the entry that takes it.
+// Bound by dependent reads: sequence, length, last page and its count, each some 0.7 us away.
+// The counts of the first kHeld * 1024 pages are read beside them and held as masks; only
+// larger pools are read twice.
 __global__ __launch_bounds__(kExtThreads) void kv_extend_kernel(KvView kv, const int32_t* __restrict__ seqs,
                                                                 const int32_t* __restrict__ counts, uint32_t n,
-                                                                int32_t* __restrict__ free_list,
                                                                 PageCopy* __restrict__ copies,
                                                                 uint32_t* __restrict__ n_copies, uint32_t* err) {
-    __shared__ int32_t sh_seq[kExtThreads], sh_last[kExtThreads];
+    constexpr uint32_t kWaves = kExtThreads / 64, kHeld = 8;
+    __shared__ alignas(16) int32_t sh_seq[kExtThreads], sh_last[kExtThreads];
     __shared__ uint64_t sh_start[kExtThreads + 1];
-    __shared__ int32_t sh_have[kExtThreads];  // first table slot an entry's new pages go to
-    __shared__ uint64_t sh_scan[kExtThreads / 64];
-    __shared__ uint32_t sh_free[kExtThreads / 64], sh_n_copies;
+    __shared__ int32_t sh_have[kExtThreads];    // first table slot an entry's new pages go to
+    __shared__ int32_t sh_filled[kExtThreads];  // rows of the page that its first new page is a copy of; 0: of none
+    __shared__ uint64_t sh_scan[kWaves];
+    __shared__ uint32_t sh_free[kWaves], sh_n_copies;
     const uint32_t i = threadIdx.x, lane = i & 63, wave = i >> 6;
     const uint32_t page = 1u << kv.shift;
     if (i == 0) sh_n_copies = 0;
 
     const int32_t seq = i < n ? seqs[i] : -1;
+    const int32_t count = i < n ? counts[i] : 0;
+    // the counts of this wave's part of the pages
+    const uint64_t part_pages = ((static_cast<uint64_t>(kv.n_pages) + kExtThreads - 1) / kExtThreads) * 64;
+    const uint64_t p0 = wave * part_pages;
+    const uint64_t p1 = p0 + part_pages < kv.n_pages ? p0 + part_pages : kv.n_pages;
+    int32_t ref[kHeld];
+    auto read = [&](uint64_t p) {  // 64 kHeld of them at once
+#pragma unroll
+        for (uint32_t x = 0; x < kHeld; ++x) {
+            const uint64_t at = p + x * 64 + lane;
+            ref[x] = at < p1 ? kv.refs[at] : -1;
+        }
+    };
+    read(p0);
+    const int32_t len0 = i < n && seq_ok(kv, seq) ? kv.lens[seq] : 0;
     sh_seq[i] = seq;
     __syncthreads();
+    // the entries ahead, four at a time: one that names the sequence again is refused
     bool ok = i < n && seq_ok(kv, seq);
-    for (uint32_t j = 0; j < n; ++j)
-        if (j < i && sh_seq[j] == seq) ok = false;
-    const int32_t count = i < n ? counts[i] : 0;
-    const int32_t len = ok ? kv.lens[seq] : 0;
+    auto ahead = [&](const int32_t* sh, int32_t what) {
+        int32_t found = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < n; j += 4) {
+            const i4 x = *reinterpret_cast<const i4*>(sh + j);
+#pragma unroll
+            for (uint32_t y = 0; y < 4; ++y) found += (j + y < i) & (x[y] == what);
+        }
+        return found;
+    };
+    if (wave * 64 < n) ok = ahead(sh_seq, seq) == 0 && ok;
+    const int32_t len = ok ? len0 : 0;
     ok = ok && count >= 0 && len_ok(kv, len) &&
          static_cast<int64_t>(len) + count <= (static_cast<int64_t>(kv.max_pages) << kv.shift);
     const uint32_t filled = static_cast<uint32_t>(len) & (page - 1);
@@ -76,75 +106,85 @@ __global__ __launch_bounds__(kExtThreads) void kv_extend_kernel(KvView kv, const
         part ? kv.table[static_cast<uint64_t>(seq) * kv.max_pages + (static_cast<uint32_t>(len) >> kv.shift)] : -1;
     if (part && !page_ok(kv, last)) ok = false;
     if (i < n && !ok) atomicOr(err, kErrIndex);
-    sh_last[i] = part && ok ? last : -1;
+    const bool shares = part && ok;
+    const int32_t last_refs = shares ? kv.refs[last] : 0;
+    sh_last[i] = shares ? last : -1;
     __syncthreads();
-    bool copy = false;
-    if (part && ok) {
-        int32_t before = 0;  // entries ahead that hold the same page: each took one count from it
-        for (uint32_t j = 0; j < i; ++j) before += sh_last[j] == last;
-        copy = kv.refs[last] - before > 1;
-    }
+    // entries ahead that hold the same page: each took one count from it
+    const bool copy = __any(last_refs > 1) && last_refs - ahead(sh_last, last) > 1;
     const uint32_t have = (static_cast<uint32_t>(len) + page - 1) >> kv.shift;
     const uint32_t want = (static_cast<uint32_t>(len) + static_cast<uint32_t>(count) + page - 1) >> kv.shift;
     const uint64_t need = ok ? want - have + (copy ? 1 : 0) : 0;
+    sh_have[i] = static_cast<int32_t>(copy ? have - 1 : have);
+    sh_filled[i] = copy ? static_cast<int32_t>(filled) : 0;
+    uint64_t held[kHeld];
+    uint32_t mine = 0;
+    auto masks = [&](uint64_t* free) {
+#pragma unroll
+        for (uint32_t x = 0; x < kHeld; ++x) {
+            free[x] = __ballot(ref[x] == 0);
+            mine += __popcll(free[x]);
+        }
+    };
+    masks(held);
     uint64_t total;
     const uint64_t start = scan_1024(need, sh_scan, total);
     sh_start[i] = start;
-    sh_have[i] = static_cast<int32_t>(copy ? have - 1 : have);
     if (i == 0) sh_start[kExtThreads] = total;
-
-    // free pages: wave w counts, then lists, its part of the counts in order
-    const uint64_t part_pages = ((static_cast<uint64_t>(kv.n_pages) + kExtThreads - 1) / kExtThreads) * 64;
-    const uint64_t p0 = wave * part_pages;
-    const uint64_t p1 = p0 + part_pages < kv.n_pages ? p0 + part_pages : kv.n_pages;
-    uint32_t mine = 0;
     if (total) {
-#pragma unroll 8
-        for (uint64_t p = p0; p < p1; p += 64) mine += __popcll(__ballot(p + lane < p1 && kv.refs[p + lane] == 0));
+        uint64_t free[kHeld];
+        for (uint64_t p = p0 + kHeld * 64; p < p1; p += kHeld * 64) {
+            read(p);
+            masks(free);
+        }
     }
     if (lane == 0) sh_free[wave] = mine;
     __syncthreads();
     uint64_t at = 0, n_free = 0;
-    for (uint32_t w = 0; w < kExtThreads / 64; ++w) {
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w) {
         if (w < wave) at += sh_free[w];
         n_free += sh_free[w];
     }
-    if (total && at < total) {
-        for (uint64_t p = p0; p < p1 && at < total; p += 64) {
-            const bool is_free = p + lane < p1 && kv.refs[p + lane] == 0;
-            const uint64_t m = __ballot(is_free);
-            const uint64_t to = at + __popcll(m & ((uint64_t(1) << lane) - 1));
-            if (is_free && to < total) free_list[to] = static_cast<int32_t>(p + lane);
-            at += __popcll(m);
-        }
-    }
     const bool fits = ok && start + need <= n_free;
     if (ok && !fits) atomicOr(err, kErrNoPages);
-    __syncthreads();  // free_list is written, refs are read
 
-    // new pages of the entries that fit: a prefix of the list
-    const uint64_t given = total < n_free ? total : n_free;
-    for (uint64_t f = i; f < given; f += kExtThreads) {
-        uint32_t lo = 0, hi = kExtThreads;  // the entry whose part of the list f lies in: last start <= f with a need
+    // Page p, the f'th free one, to the entry whose part of the list f lies in: the last start
+    // <= f (entries that need nothing lie behind the one that does), if it fits. Only this
+    // wave reads its part of the counts from here on, before it writes them.
+    auto give = [&](uint64_t p, uint64_t f) {
+        uint32_t lo = 0, hi = n;
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) >> 1;
             if (sh_start[mid] <= f) lo = mid;
             else hi = mid;
         }
-        if (sh_start[lo + 1] > n_free) continue;  // an entry that does not fit
-        const int32_t p = free_list[f];
-        const uint64_t slot = static_cast<uint64_t>(sh_have[lo]) + (f - sh_start[lo]);
-        kv.table[static_cast<uint64_t>(sh_seq[lo]) * kv.max_pages + slot] = p;
+        if (sh_start[lo + 1] > n_free) return;
+        const uint64_t slot = f - sh_start[lo];
+        kv.table[static_cast<uint64_t>(sh_seq[lo]) * kv.max_pages + static_cast<uint64_t>(sh_have[lo]) + slot] =
+            static_cast<int32_t>(p);
         kv.refs[p] = 1;
-    }
-    if (fits) {
-        kv.lens[seq] = len + count;
-        if (copy) {
-            atomicSub(&kv.refs[last], 1);
-            copies[atomicAdd(&sh_n_copies, 1u)] =
-                PageCopy{last, free_list[start], static_cast<int32_t>(filled), 0};
+        if (slot == 0 && sh_filled[lo]) {
+            atomicSub(&kv.refs[sh_last[lo]], 1);
+            copies[atomicAdd(&sh_n_copies, 1u)] = PageCopy{sh_last[lo], static_cast<int32_t>(p), sh_filled[lo], 0};
         }
+    };
+    auto give_all = [&](uint64_t p, const uint64_t* free) {
+#pragma unroll
+        for (uint32_t x = 0; x < kHeld; ++x) {
+            const uint64_t to = at + __popcll(free[x] & ((uint64_t(1) << lane) - 1));
+            if ((free[x] >> lane & 1) && to < total) give(p + x * 64 + lane, to);
+            at += __popcll(free[x]);
+        }
+    };
+    if (at < total) give_all(p0, held);
+    for (uint64_t p = p0 + kHeld * 64; p < p1 && at < total; p += kHeld * 64) {
+        uint64_t free[kHeld];
+        read(p);
+        masks(free);
+        give_all(p, free);
     }
+    if (fits) kv.lens[seq] = len + count;
     __syncthreads();
     if (i == 0) *n_copies = sh_n_copies;
 }
@@ -348,13 +388,13 @@ int32_t objeta_hip_kv_extend_device(objeta_hip_context* ctx, objeta_hip_stream s
     const objeta_hip_kv_cache& c = *cache;
     const hipStream_t s = resolve_stream(ctx, stream);
     void* ws = nullptr;
-    const size_t copies = 256, list = copies + kMaxPageOps * sizeof(PageCopy);
-    OBJ_TRY(ensure_workspace(ctx, s, kWsPages, list + static_cast<size_t>(c.n_pages) * 4, &ws));
+    const size_t copies = 256;
+    OBJ_TRY(ensure_workspace(ctx, s, kWsPages, copies + kMaxPageOps * sizeof(PageCopy), &ws));
     char* w = static_cast<char*>(ws);
     uint32_t* n_copies = reinterpret_cast<uint32_t*>(w);
     PageCopy* pc = reinterpret_cast<PageCopy*>(w + copies);
     hipLaunchKernelGGL(kv_extend_kernel, dim3(1), dim3(kExtThreads), 0, s, kv_view(c), d_seqs, d_counts,
-                       static_cast<uint32_t>(n), reinterpret_cast<int32_t*>(w + list), pc, n_copies, ctx->err_word);
+                       static_cast<uint32_t>(n), pc, n_copies, ctx->err_word);
     OBJ_HIP(hipGetLastError(), action);
     // most calls copy nothing and the rest few pages: enough workgroups to fill the device
     // once, fewer where even n copies need fewer
