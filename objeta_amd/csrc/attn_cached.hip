@@ -24,22 +24,18 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     bool any = row < a.n_rows;
     uint32_t n = 0, at_row = 0;
     if (any) {
-        const uint32_t le = count_le(a.cu, a.n_batch + 1, row);
-        any = le != 0 && le <= a.n_batch;
+        const RowEntry<false> entry(a.cu, PAGED ? a.seqs : nullptr, a.n_batch, row);
+        any = entry.any && entry.lo >= 0 && static_cast<uint32_t>(entry.hi) <= a.n_rows;
         if (any) {
-            const int32_t lo = a.cu[le - 1], hi = a.cu[le];
-            any = lo >= 0 && lo <= static_cast<int32_t>(row) && static_cast<int32_t>(row) < hi &&
-                  static_cast<uint32_t>(hi) <= a.n_rows;
             n = a.n_splits;
             if constexpr (PAGED) {
-                const int32_t seq = a.seqs[le - 1];
-                int32_t len = seq_ok(a.kv, seq) ? a.kv.lens[seq] : 0;
-                if (!len_ok(a.kv, len) || hi - lo > len || (a.tree && hi - lo > 64)) len = 0;
+                const int32_t rows = entry.hi - entry.lo;
+                int32_t len = seq_ok(a.kv, entry.seq) ? a.kv.lens[entry.seq] : 0;
+                if (!len_ok(a.kv, len) || rows > len || (a.tree && rows > 64)) len = 0;
                 n = (static_cast<uint32_t>(len) + a.chunk - 1) / a.chunk;
                 n = n < 1 ? 1 : (n > a.n_splits ? a.n_splits : n);
             }
-            n = any ? n : 0;
-            at_row = row - static_cast<uint32_t>(lo);
+            at_row = row - static_cast<uint32_t>(entry.lo);
         }
     }
     const uint64_t step = static_cast<uint64_t>(a.n_rows) * a.n_heads;
