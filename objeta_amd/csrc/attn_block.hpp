@@ -41,13 +41,16 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
     uint32_t tile, head, split = 0;
     int32_t row0 = 0, n_q = static_cast<int32_t>(a.n_rows), len = 0;
     KvRows<PAGED, KT> kv;
-    bool usable = true;
+    uint32_t part = 0;
+    bool usable = true, last_part = true;
     if constexpr (PAGED) {
-        const BlockItem item(a, blockIdx.x);
+        const BlockItem item(a, blockIdx.x, 256 * (QT == kDtF32 ? 1 : B::kPerCu));
         if (!item.any) return;
         split = item.split, tile = item.tile, head = item.head;
         row0 = item.row0, n_q = item.n_q, len = item.len;
         usable = item.usable;
+        part = ((static_cast<uint32_t>(len) + item.splits - 1) / item.splits + kKeys - 1) / kKeys * kKeys;
+        last_part = split + 1 == item.splits;
         const int32_t seq = item.seq;
         if (!usable && tid == 0) atomicOr(a.err, kErrIndex);
         kv.kv = a.kv;
@@ -110,11 +113,11 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
     if constexpr (PAGED) {
         const uint32_t m0 = tile * 128 + __builtin_amdgcn_readfirstlane(wave) * 32;
         const uint32_t m1 = tile * 128 + 128 < n_m ? tile * 128 + 127 : n_m - 1;
-        const int64_t c0 = static_cast<int64_t>(split) * a.chunk, c1 = c0 + a.chunk;
+        const int64_t c0 = static_cast<int64_t>(split) * part, c1 = c0 + part;
         const int32_t base = len - n_q;
-        k_lo = static_cast<int32_t>(c0);
+        k_lo = static_cast<int32_t>(c0 < len ? c0 : len);
         k_end = usable ? (a.tree ? len : base + static_cast<int32_t>(m1 / a.group) + 1) : 0;
-        if (split + 1 < a.n_splits && k_end > c1) k_end = static_cast<int32_t>(c1);
+        if (!last_part && k_end > c1) k_end = static_cast<int32_t>(c1);
         all_lo = 0;
         all_hi = a.tree ? base - 1 : base + static_cast<int32_t>(m0 / a.group);
     } else {
@@ -141,7 +144,7 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
         all_lo = __builtin_amdgcn_readfirstlane(all_lo), all_hi = __builtin_amdgcn_readfirstlane(all_hi);
         if (a.n_splits > 1 && k_lo < k_end) {
             const uint32_t n = static_cast<uint32_t>(k_end - k_lo);
-            const uint32_t part = ((n + a.n_splits - 1) / a.n_splits + kKeys - 1) / kKeys * kKeys;
+            part = ((n + a.n_splits - 1) / a.n_splits + kKeys - 1) / kKeys * kKeys;
             const int64_t p0 = static_cast<int64_t>(k_lo & ~(kKeys - 1)) + static_cast<int64_t>(split) * part;
             const int64_t p1 = split + 1 < a.n_splits ? p0 + part : k_end;
             k_lo = p0 > k_lo ? static_cast<int32_t>(p0 < k_end ? p0 : k_end) : k_lo;

@@ -7,20 +7,18 @@ namespace objeta {
 namespace dev {
 
 // Joins the parts of one (row, head): with M the largest m, l = sum l_s 2^(m_s - M),
-// o = sum o_s 2^(m_s - M) / l. LANES lanes read a part's o, four values each. WAVES waves take
-// the parts of one (row, head): one where there are many of these with few parts each (9280 of
-// up to 7 parts of 128: 13.6 us, with four waves 18.0), four otherwise (1024 of up to 8: 4.9
-// us, with one 6.8).
+// o = sum o_s 2^(m_s - M) / l. LANES lanes read a part's o, four values each, four parts at a
+// time; a wave's lanes hold m, l and weight of 64 parts. WAVES waves take the parts of one
+// (row, head): REPLACE
 template <int QT, int LANES, int WAVES, bool PAGED>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     typedef typename ElemOf<QT>::type elem;
     constexpr uint32_t kAtOnce = WAVES * 64 / LANES;
     __shared__ f32x4 sh_o[256];
-    __shared__ float sh_l[256 / LANES];
     const uint32_t tid = threadIdx.x, lane = tid & 63;
     const uint64_t rh = static_cast<uint64_t>(blockIdx.x) * (4 / WAVES) + tid / (64 * WAVES);
     const uint32_t row = static_cast<uint32_t>(rh / a.n_heads), head = static_cast<uint32_t>(rh % a.n_heads);
-    const uint32_t slot = tid % (64 * WAVES);
+    const uint32_t slot = tid % (64 * WAVES), part = slot / LANES, x = slot % LANES * 4;
     bool any = row < a.n_rows;
     uint32_t n = 0, at_row = 0;
     if (any) {
@@ -32,45 +30,59 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
                 const int32_t rows = entry.hi - entry.lo;
                 int32_t len = seq_ok(a.kv, entry.seq) ? a.kv.lens[entry.seq] : 0;
                 if (!len_ok(a.kv, len) || rows > len || (a.tree && rows > 64)) len = 0;
-                n = (static_cast<uint32_t>(len) + a.chunk - 1) / a.chunk;
-                n = n < 1 ? 1 : (n > a.n_splits ? a.n_splits : n);
+                n = splits_of(len, a.picked ? *a.picked : a.chunk, a.n_splits);
             }
             at_row = row - static_cast<uint32_t>(entry.lo);
         }
     }
     const uint64_t step = static_cast<uint64_t>(a.n_rows) * a.n_heads;
-    float top = -kInf;
-    for (uint32_t s = lane; s < n; s += 64) top = __builtin_fmaxf(top, a.part_ml[2 * (s * step + rh)]);
+    f32x4 v[4], o = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto load = [&](uint32_t s0) {
 #pragma unroll
-    for (int x = 32; x > 0; x >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, x, 64));
+        for (uint32_t y = 0; y < 4; ++y) {
+            const uint32_t s = s0 + part + y * kAtOnce;
+            v[y] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (s < n && x < a.dim) v[y] = *reinterpret_cast<const f32x4*>(a.part + (s * step + rh) * a.dim + x);
+        }
+    };
+    load(0);
+    float m = -kInf, l = 0.0f;
+    if (lane < n) m = a.part_ml[2 * (lane * step + rh)], l = a.part_ml[2 * (lane * step + rh) + 1];
+    float top = m;
+    for (uint32_t s = 64 + lane; s < n; s += 64) top = __builtin_fmaxf(top, a.part_ml[2 * (s * step + rh)]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, d, 64));
     const float ref = top == -kInf ? 0.0f : top;
-    const uint32_t part = slot / LANES, x = slot % LANES * 4;
-    float l = 0.0f;
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (uint32_t s = part; s < n; s += kAtOnce) {
-        const uint64_t at = s * step + rh;
-        const float f = exp2_hw(a.part_ml[2 * at] - ref);
-        l = __builtin_fmaf(a.part_ml[2 * at + 1], f, l);
-        if (x < a.dim) o += *reinterpret_cast<const f32x4*>(a.part + at * a.dim + x) * f;
+    float sum = 0.0f;
+    for (uint32_t base = 0; base < n; base += 64) {
+        if (base) {
+            const uint64_t at = 2 * ((base + lane) * step + rh);
+            m = base + lane < n ? a.part_ml[at] : -kInf, l = base + lane < n ? a.part_ml[at + 1] : 0.0f;
+        }
+        const float w = exp2_hw(m - ref);
+        sum = __builtin_fmaf(l, w, sum);
+        const uint32_t end = n - base < 64 ? n : base + 64;
+        for (uint32_t s0 = base; s0 < end; s0 += 4 * kAtOnce) {
+            if (s0) load(s0);
+#pragma unroll
+            for (uint32_t y = 0; y < 4; ++y) o += v[y] * __shfl(w, static_cast<int>(s0 - base + part + y * kAtOnce), 64);
+        }
     }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d, 64);
     sh_o[tid] = o;
-    if (x == 0) sh_l[tid / LANES] = l;
     __syncthreads();
     if (!any || part != 0 || x >= a.dim) return;
 #pragma unroll
-    for (uint32_t p = 1; p < kAtOnce; ++p) {
-        o += sh_o[p * LANES + tid];
-        l += sh_l[tid / LANES + p];
-    }
+    for (uint32_t p = 1; p < kAtOnce; ++p) o += sh_o[p * LANES + tid];
     if constexpr (PAGED) {  // a row past what max_rows allows for has no parts
         const uint32_t group = a.n_heads / a.n_kv;
         if (static_cast<uint64_t>(at_row) * group + head % group >= static_cast<uint64_t>(a.n_tiles) * a.tile_rows)
-            l = o.x = o.y = o.z = o.w = __builtin_nanf("");
+            sum = o.x = o.y = o.z = o.w = __builtin_nanf("");
     }
     store_out<QT>(static_cast<elem*>(a.out) + row * a.out_stride + static_cast<uint64_t>(head) * a.dim + x,
-                  o * (l == 0.0f ? 0.0f : 1.0f / l));
-    if (a.lse && x == 0) a.lse[rh] = l == 0.0f ? -kInf : (top + __builtin_amdgcn_logf(l)) * kLn2;
+                  o * (sum == 0.0f ? 0.0f : 1.0f / sum));
+    if (a.lse && x == 0) a.lse[rh] = sum == 0.0f ? -kInf : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
 }  // namespace dev
@@ -102,9 +114,10 @@ int32_t launch_join(hipStream_t s, const AttnArgs& a, const char* action) {
 int32_t attn_parts(objeta_hip_context* ctx, hipStream_t s, AttnArgs& a) {
     const size_t parts = static_cast<size_t>(a.n_splits) * a.n_rows * a.n_heads;
     void* ws = nullptr;
-    OBJ_TRY(ensure_workspace(ctx, s, kWsAttn, parts * (a.dim + 2) * sizeof(float), &ws));
+    OBJ_TRY(ensure_workspace(ctx, s, kWsAttn, parts * (a.dim + 2) * sizeof(float) + sizeof(uint32_t), &ws));
     a.part = static_cast<float*>(ws);
     a.part_ml = a.part + parts * a.dim;
+    if (a.pick) a.picked = reinterpret_cast<uint32_t*>(a.part_ml + 2 * parts);
     return 0;
 }
 
@@ -182,9 +195,13 @@ int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream
     const uint64_t units = n_batch * a.n_kv * a.n_tiles;
     uint64_t splits = (1024 + units - 1) / units;
     uint64_t chunk = ((len + splits - 1) / splits + 255) / 256 * 256;
+    // Few keys in one piece: the join costs more than the waves' longer way (560 keys of one
+    // sequence, bf16: 10.5 us against 11.1; 700: 11.3 and 11.2; 260: 7.9 and 10.9).
+    if (stream_form && len <= 576) chunk = 768;
     splits = (len + chunk - 1) / chunk;
     a.chunk = static_cast<uint32_t>(chunk);
     a.n_splits = static_cast<uint32_t>(splits);
+    a.pick = !stream_form && splits > 1 && n_batch <= 64;
     if (splits > 1) OBJ_TRY(attn_parts(ctx, s, a));
     OBJ_TRY(stream_form ? launch_attn_stream(s, dtype, c.dtype, static_cast<uint32_t>(rows), a, action)
                         : launch_attn_cached_block(s, dtype, c.dtype, a, action));

@@ -434,9 +434,11 @@ struct AttnArgs {
     const int32_t* seqs;
     const uint64_t* tree;
     uint64_t layer_off;  // elements
-    // keys cut over workgroups: of cached sequences in chunks of `chunk`, of a prompt's tile of rows
-    // in n_splits equal parts
-    uint32_t chunk, n_splits, n_tiles, tile_rows;
+    // keys cut over workgroups: of cached sequences in equal parts of about `chunk`, of a prompt's
+    // tile of rows in n_splits equal ones. pick: the kernel takes a chunk that fills the card,
+    // and leaves it in *picked for the join.
+    uint32_t chunk, n_splits, n_tiles, tile_rows, pick;
+    uint32_t* picked;
     float *part, *part_ml;  // [n_splits][n_rows * n_heads][dim], [..][2]
     uint32_t* err;
 };
@@ -457,30 +459,45 @@ struct StreamItem {
     }
 };
 
+// Into how many parts a sequence's keys are cut.
+__device__ __forceinline__ uint32_t splits_of(int32_t len, uint32_t chunk, uint32_t most) {
+    const uint32_t n = (static_cast<uint32_t>(len) + chunk - 1) / chunk;
+    return n < 1 ? 1 : (n < most ? n : most);
+}
+
 // Which piece of work a workgroup of 128 rows takes, counted over the pieces that there are:
 // entries differ in rows and lengths, and a grid over the largest of both would be mostly
 // empty workgroups, unevenly over the XCDs (8 trees of 9 to 64 drafts: 39 to 64 workgroups on
 // an XCD, the kernel 80 us for 44 us of work on every CU). Each wave reads 64 entries at a
 // time, a lane an entry, and finds the id'th piece in their running sum; what it read of the
-// entry need not be read again.
+// entry need not be read again. Up to 64 entries it also chooses the chunk, which the host
+// could only choose for the longest: REPLACE
 struct BlockItem {
-    uint32_t head, split, tile;
+    uint32_t head, split, tile, splits;
     int32_t row0, n_q, len, seq;
     bool any, usable;
-    __device__ __forceinline__ BlockItem(const AttnArgs& a, uint32_t id) {
+    static __device__ __forceinline__ uint32_t total(uint32_t v) {
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+        return __builtin_amdgcn_readfirstlane(v);
+    }
+    // `slots` workgroups run at a time.
+    __device__ __forceinline__ BlockItem(const AttnArgs& a, uint32_t id, uint32_t slots) {
         const uint32_t lane = threadIdx.x & 63;
+        uint32_t chunk = a.chunk;
+        const bool first = id == 0;
         any = false;
         for (uint32_t b0 = 0; b0 < a.n_batch; b0 += 64) {
             const uint32_t b = b0 + lane;
             int32_t lo = 0, n = 0, s = 0, l = 0;
             bool ok = true;
-            uint32_t pieces = 0, splits = 1, tiles = 0;
+            uint32_t tiles = 0;
             if (b < a.n_batch) {
                 lo = a.cu[b];
                 const int32_t hi = a.cu[b + 1];
                 s = a.seqs[b];
                 const bool rows = lo >= 0 && hi >= lo && static_cast<uint32_t>(hi) <= a.n_rows;
-                if (!rows && id == 0) atomicOr(a.err, kErrIndex);
+                if (!rows && first) atomicOr(a.err, kErrIndex);
                 n = rows ? hi - lo : 0;
                 ok = seq_ok(a.kv, s);
                 l = ok ? a.kv.lens[s] : 0;
@@ -488,10 +505,24 @@ struct BlockItem {
                 if (!ok) l = 0;
                 tiles = (static_cast<uint32_t>(n) * a.group + 127) / 128;
                 tiles = tiles < a.n_tiles ? tiles : a.n_tiles;
-                splits = (static_cast<uint32_t>(l) + a.chunk - 1) / a.chunk;
-                splits = splits < 1 ? 1 : (splits < a.n_splits ? splits : a.n_splits);
-                pieces = tiles * splits * a.n_kv;
             }
+            if (a.pick) {
+                // pieces of `chunk` keys are to be at most what runs at once, or a multiple of
+                // it where the tiles alone are more than three quarters
+                const uint32_t one = total(tiles * a.n_kv);
+                const uint32_t room = (one * 4 / 3 + slots) / slots * slots;
+                float keys = static_cast<float>(tiles * a.n_kv) * static_cast<float>((static_cast<uint32_t>(l) + 63) / 64);
+#pragma unroll
+                for (int d = 32; d > 0; d >>= 1) keys += __shfl_xor(keys, d, 64);
+                const uint32_t least = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(keys / static_cast<float>(room))) + 1;
+                for (uint32_t k = 8; k <= 16; k += k < 12 ? 1 : 2) {
+                    chunk = least * 8 * k;
+                    chunk = chunk < 256 ? 256 : chunk;
+                    if (total(tiles * a.n_kv * splits_of(l, chunk, a.n_splits)) <= room) break;
+                }
+                if (first && threadIdx.x == 0) *a.picked = chunk;
+            }
+            const uint32_t parts = splits_of(l, chunk, a.n_splits), pieces = tiles * parts * a.n_kv;
             uint32_t sum = pieces;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
@@ -504,6 +535,7 @@ struct BlockItem {
                 const uint32_t in = id - (__builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(pieces, at));
                 const uint32_t n_tiles = __builtin_amdgcn_readlane(tiles, at), rest = in / a.n_kv;
                 head = in % a.n_kv, tile = rest % n_tiles, split = rest / n_tiles;
+                splits = __builtin_amdgcn_readlane(parts, at);
                 row0 = __builtin_amdgcn_readlane(lo, at), n_q = __builtin_amdgcn_readlane(n, at);
                 len = __builtin_amdgcn_readlane(l, at), seq = __builtin_amdgcn_readlane(s, at);
                 usable = __builtin_amdgcn_readlane(static_cast<int32_t>(ok), at) != 0;
