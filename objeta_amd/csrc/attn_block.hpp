@@ -16,15 +16,19 @@ namespace dev {
 template <int KT, int DT>
 struct Block {
     typedef Rows<KT, DT, 32> R;
-    static constexpr int kKeys = R::kBytes <= 512 ? 64 : 32;
+    static constexpr int kKeys = KT != kDtF32x3 && R::kBytes <= 512 ? 64 : 32;
     static constexpr int kSub = kKeys / 32;
     static constexpr int kLoads = kKeys / (4 * R::kPer);  // 16-byte units of K (and of V) a thread stages
     static constexpr int kTileK = kKeys * R::kK, kTileV = kKeys * R::kV;
-    static_assert(KT == kDtF32 || kSub == 2, "16-bit tiles are two steps");
+    static_assert(R::kEs == 4 || kSub == 2, "16-bit tiles are two steps");
     static constexpr int kLds = 2 * (kTileK + kTileV);
     // two workgroups a CU where LDS and registers allow it
     static constexpr int kPerCu = kLds <= 73728 ? 2 : 1;
 };
+
+// How float keys and values are taken: in parts where two tiles of them fit LDS.
+template <int KT, int DT>
+constexpr int block_type = KT == kDtF32 && DT <= 192 ? kDtF32x3 : KT;
 
 template <int QT, int KT, int DT, bool PAGED>
 __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) void attn_block_kernel(AttnArgs a) {
@@ -176,18 +180,44 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
     const uint32_t w_key = __builtin_amdgcn_readfirstlane(wave) * R::kPer;
     const uint32_t k_row = static_cast<uint32_t>(PAGED ? a.dim : kv.k_stride) * R::kEs;  // bytes
     const uint32_t v_row = static_cast<uint32_t>(PAGED ? a.dim : kv.v_stride) * R::kEs;
-    const uint32_t unit = lane % R::kLanes, l_key = lane / R::kLanes;
+    // lanes past a row's last unit take one again, and store it again
+    const uint32_t l_unit = lane % R::kLanes, l_key = lane / R::kLanes;
+    const uint32_t unit = l_unit < R::kUnits ? l_unit : l_unit - (R::kLanes - R::kUnits);
     // a unit behind the head's last dimension reads nothing, wherever its row is
     const bool inside = unit * (16 / R::kEs) < a.dim;
     const uint32_t k_place = inside ? l_key * k_row + unit * 16 : kNowhere;
     const uint32_t v_place = inside ? l_key * v_row + unit * 16 : kNowhere;
-    auto load_tile = [&](int32_t t) {
+    // K (V) of tile t to registers; zeros behind the last key
+    auto load = [&](u32x4a* r, const typename M::kelem* base, uint64_t stride, uint32_t row, uint32_t at_lane, int32_t t) {
         const int32_t t0 = k_begin + t * kKeys;
         if constexpr (PAGED) {
 #pragma unroll
             for (int x = 0; x < B::kLoads; ++x) {
                 const uint32_t key = x * 4 * R::kPer + w_key;
                 const int32_t left = k_end - t0 - static_cast<int32_t>(key);  // keys from this one on
+                const uint32_t bytes = __builtin_amdgcn_readfirstlane(left < 0 ? 0 : (left > 8 ? 8 : left)) * row;
+                const uint64_t at = kv.paged_at(__builtin_amdgcn_readfirstlane(ring[t & 3][key >> 3]),
+                                                static_cast<uint32_t>(t0) + key);
+                r[x] = buffer_unit(buffer_of(base + at, bytes), at_lane);
+            }
+        } else {
+            const int32_t left = k_end - t0;
+            // (to a scalar register: the clamp is a vector instruction)
+            const uint32_t rows = __builtin_amdgcn_readfirstlane(left < 0 ? 0 : (left > kKeys ? kKeys : left));
+            const auto b = buffer_of(base + static_cast<uint64_t>(t0) * stride, rows * row);
+#pragma unroll
+            for (int x = 0; x < B::kLoads; ++x) r[x] = buffer_unit(b, at_lane + (x * 4 * R::kPer + w_key) * row);
+        }
+    };
+    auto load_k = [&](int32_t t) { load(rk, kv.k, kv.k_stride, k_row, k_place, t); };
+    auto load_v = [&](int32_t t) { load(rv, kv.v, kv.v_stride, v_row, v_place, t); };
+    auto load_tile = [&](int32_t t) {  // both of a tile that there is
+        const int32_t t0 = k_begin + t * kKeys;
+        if constexpr (PAGED) {
+#pragma unroll
+            for (int x = 0; x < B::kLoads; ++x) {
+                const uint32_t key = x * 4 * R::kPer + w_key;
+                const int32_t left = k_end - t0 - static_cast<int32_t>(key);
                 const uint32_t bytes = left > 0 ? (left < 8 ? left : 8) * k_row : 0;
                 const uint64_t at = kv.paged_at(__builtin_amdgcn_readfirstlane(ring[t & 3][key >> 3]),
                                                 static_cast<uint32_t>(t0) + key);
@@ -207,14 +237,28 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
             }
         }
     };
-    const uint32_t k_at = (wave * R::kPer + l_key) * R::kK + unit * 16, v_at = (wave * R::kPer + l_key) * R::kV + unit * 16;
-    auto store_tile = [&](int buf) {
-        if (R::kLanes == R::kUnits || unit < R::kUnits) {
+    const uint32_t place = unit * (16 / R::kEs * R::kLs);
+    const uint32_t k_at = (wave * R::kPer + l_key) * R::kK + place, v_at = (wave * R::kPer + l_key) * R::kV + place;
+    auto store_unit = [&](char* to, u32x4a x) {
+        if constexpr (KT == kDtF32x3) {
+            const f32x4 y = __builtin_bit_cast(f32x4, x);
+            float rest[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-            for (int x = 0; x < B::kLoads; ++x) {
-                *reinterpret_cast<u32x4a*>(lds_k[buf] + k_at + x * 4 * R::kPer * R::kK) = rk[x];
-                *reinterpret_cast<u32x4a*>(lds_v[buf] + v_at + x * 4 * R::kPer * R::kV) = rv[x];
+            for (int p = 0; p < 3; ++p) {
+                const uint32_t a = take_bf16(rest[0], rest[1]), b = take_bf16(rest[2], rest[3]);
+                *reinterpret_cast<uint2*>(to + p * R::kPart) = uint2{a, b};
             }
+        } else {
+            *reinterpret_cast<u32x4a*>(to) = x;
+        }
+    };
+    auto store_k = [&](int buf, int x) { store_unit(lds_k[buf] + k_at + x * 4 * R::kPer * R::kK, rk[x]); };
+    auto store_v = [&](int buf, int x) { store_unit(lds_v[buf] + v_at + x * 4 * R::kPer * R::kV, rv[x]); };
+    auto store_tile = [&](int buf) {
+#pragma unroll
+        for (int x = 0; x < B::kLoads; ++x) {
+            store_k(buf, x);
+            store_v(buf, x);
         }
     };
     const uint32_t k_first = M::k_first(lane), v_first = M::v_first(lane);
@@ -234,7 +278,7 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
     // holds the next 32's, and then those at k_after), values half a step; without the scheduling
     // barriers the compiler moves the reads back to their products, and each waits for LDS. The
     // workgroup meets where the step's last values have been read.
-    constexpr bool kAhead = !M::kFloat && (M::kParts == 1 || DT <= 128);
+    constexpr bool kAhead = !M::kFloat && M::kKvParts == 1 && (M::kParts == 1 || DT <= 128);
     Keys<M> keys;
     auto step = [&](Scores<M>& cur, Scores<M>& next, const char* v, const char* k) {
         Weights<M> w0, w1;
@@ -264,63 +308,135 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
             value_rows<M>(st, w1, v, 1);
         }
     };
-    // Tile t lies in LDS buffer t % 2, tile t + 1 in registers, and the scores of tile t's first
-    // 32 keys are there.
-    if (n_tiles) {
-        if constexpr (PAGED) {
-            const int32_t p0 = load_pages(0), p1 = load_pages(1), p2 = load_pages(2);
-            store_pages(0, p0);
-            store_pages(1, p1);
-            store_pages(2, p2);
+    if constexpr (M::kKvParts == 3) {
+        // K runs a tile ahead of V: a turn multiplies tile t's values and tile t + 1's keys, and
+        // writes the parts of tile t + 1's values and tile t + 2's keys, all of it independent,
+        // so that it meets once. The turn goes by groups of the six products of three fragments,
+        // the next group's fragments read ahead; splitting and softmax are dealt out between
+        // the groups, in the shadow of their products. A turn of 192 dimensions takes 8470 cycles of
+        // which the products are 4608: a wave alone on its SIMD issues some 1000 instructions in it,
+        // and waits for loads (1300 less without them). Float products would take 12288.
+        if (n_tiles) {
+            if constexpr (PAGED) {
+#pragma unroll
+                for (int32_t t = 0; t < 4; ++t) store_pages(t, load_pages(t));
+                __syncthreads();
+            }
+            load_tile(0);
+            store_tile(0);
+            load_k(1);
+#pragma unroll
+            for (int x = 0; x < B::kLoads; ++x) store_k(1, x);
+            load_k(2);
+            load_v(1);
+        }
+        __syncthreads();
+        if (n_tiles) score_rows<M>(sc[0], q, lds_k[0] + k_first);
+        constexpr int kGroups = M::kSteps + 2 * M::kOut;
+        for (int32_t t = 0; t < n_tiles; ++t) {
+            const int32_t k0 = k_begin + t * kKeys;
+            if (k0 < all_lo || k0 + kKeys - 1 > all_hi || k0 < k_lo || k0 + kKeys > k_end) mask(sc[0], k0);
+            const int32_t ahead = load_pages(t + 4);
+            const char* k = lds_k[(t + 1) & 1] + k_first;
+            const char* v = lds_v[t & 1] + v_first;
+            typename M::frag f[2][3];
+            auto read = [&](typename M::frag* to, int g) {
+                const int d = (g - M::kSteps) % M::kOut, half = (g - M::kSteps) / M::kOut;
+#pragma unroll
+                for (int x = 0; x < 3; ++x)
+                    to[x] = g < M::kSteps ? M::lds_k(k, g, x) : M::lds_v(v + M::kStep * half * R::kV, d, x);
+            };
+            Weights<M> w[2];
+            read(f[0], 0);
+            take_top<M>(st, sc[0], scale);
+            const float off = M::kShift - st.reference();
+            sc[1].s[0] = M::zero();
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) {
+                if (g + 1 < kGroups) read(f[(g + 1) & 1], g + 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int x = 2; x >= 0; --x)
+#pragma unroll
+                    for (int p = 2 - x; p >= 0; --p) {
+                        if (g < M::kSteps) sc[1].s[0] = M::mma(f[g & 1][x], q.f[p][g], sc[1].s[0]);
+                        else st.o[(g - M::kSteps) % M::kOut] = M::mma(f[g & 1][x], w[(g - M::kSteps) / M::kOut].f[p],
+                                                                     st.o[(g - M::kSteps) % M::kOut]);
+                    }
+#pragma unroll
+                for (int x = 0; x < B::kLoads; ++x) {
+                    if (g == x * M::kSteps / B::kLoads) store_k(t & 1, x);
+                    if (g == M::kSteps + x * 2 * M::kOut / B::kLoads) store_v((t + 1) & 1, x);
+                }
+                if (g == M::kSteps / 2) weigh<M>(w[0], st, sc[0], 0, scale, off);
+                if (g == M::kSteps - 1) load_k(t + 3);
+                if (g == M::kSteps) weigh<M>(w[1], st, sc[0], 1, scale, off);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            sc[0] = sc[1];
+            load_v(t + 2);
+            store_pages(t + 4, ahead);
             __syncthreads();
         }
-        load_tile(0);
-        store_tile(0);
-        if (n_tiles > 1) load_tile(1);
-    }
-    __syncthreads();
-    if (n_tiles) {
-        const char* k = lds_k[0] + k_first;
-        if constexpr (kAhead) {
-            read_keys<M>(keys, k);
-            score<M>(sc[0], q, keys);
-            read_keys<M>(keys, k + 32 * R::kK);
-        } else {
-            score_rows<M>(sc[0], q, k);
+    } else {
+        // Tile t lies in LDS buffer t % 2, tile t + 1 in registers, and the scores of tile t's first
+        // 32 keys are there.
+        if (n_tiles) {
+            if constexpr (PAGED) {
+                const int32_t p0 = load_pages(0), p1 = load_pages(1), p2 = load_pages(2);
+                store_pages(0, p0);
+                store_pages(1, p1);
+                store_pages(2, p2);
+                __syncthreads();
+            }
+            load_tile(0);
+            store_tile(0);
+            if (n_tiles > 1) load_tile(1);
         }
-    }
-    for (int32_t t = 0; t < n_tiles; ++t) {
-        int32_t ahead = 0;
-        if (PAGED && t + 3 < n_tiles) ahead = load_pages(t + 3);
-        if (t + 1 < n_tiles) store_tile((t + 1) & 1);
-        if (t + 2 < n_tiles) load_tile(t + 2);
-        const int32_t k0 = k_begin + t * kKeys;
-        const bool masked = k0 < all_lo || k0 + kKeys - 1 > all_hi || k0 < k_lo || k0 + kKeys > k_end;
-        const char* v = lds_v[t & 1] + v_first;
-        const char* kn = lds_k[(t + 1) & 1] + k_first;  // behind the last tile: whatever is there, for scores nobody uses
-        if constexpr (kAhead) {
-            // the first step's meeting: tile t + 1 is in LDS; the second's: tile t is read
-            if (masked) mask(sc[0], k0);
-            step(sc[0], sc[1], v, kn);
-            if (masked) mask(sc[1], k0 + 32);
-            if constexpr (PAGED) {
-                if (t + 3 < n_tiles) store_pages(t + 3, ahead);
+        __syncthreads();
+        if (n_tiles) {
+            const char* k = lds_k[0] + k_first;
+            if constexpr (kAhead) {
+                read_keys<M>(keys, k);
+                score<M>(sc[0], q, keys);
+                read_keys<M>(keys, k + 32 * R::kK);
+            } else {
+                score_rows<M>(sc[0], q, k);
             }
-            step(sc[1], sc[0], v + 32 * R::kV, kn + 32 * R::kK);
-        } else {
-            if constexpr (B::kSub == 2) {
+        }
+        for (int32_t t = 0; t < n_tiles; ++t) {
+            int32_t ahead = 0;
+            if (PAGED && t + 3 < n_tiles) ahead = load_pages(t + 3);
+            if (t + 1 < n_tiles) store_tile((t + 1) & 1);
+            if (t + 2 < n_tiles) load_tile(t + 2);
+            const int32_t k0 = k_begin + t * kKeys;
+            const bool masked = k0 < all_lo || k0 + kKeys - 1 > all_hi || k0 < k_lo || k0 + kKeys > k_end;
+            const char* v = lds_v[t & 1] + v_first;
+            const char* kn = lds_k[(t + 1) & 1] + k_first;  // behind the last tile: whatever is there, for scores nobody uses
+            if constexpr (kAhead) {
+                // the first step's meeting: tile t + 1 is in LDS; the second's: tile t is read
                 if (masked) mask(sc[0], k0);
-                step(sc[0], sc[1], v, lds_k[t & 1] + k_first + 32 * R::kK);
+                step(sc[0], sc[1], v, kn);
+                if (masked) mask(sc[1], k0 + 32);
+                if constexpr (PAGED) {
+                    if (t + 3 < n_tiles) store_pages(t + 3, ahead);
+                }
+                step(sc[1], sc[0], v + 32 * R::kV, kn + 32 * R::kK);
+            } else {
+                if constexpr (B::kSub == 2) {
+                    if (masked) mask(sc[0], k0);
+                    step(sc[0], sc[1], v, lds_k[t & 1] + k_first + 32 * R::kK);
+                }
+                __syncthreads();  // tile t + 1 is in LDS
+                constexpr int last = B::kSub - 1, other = 1 - last;
+                if (masked) mask(sc[last], k0 + 32 * last);
+                step(sc[last], sc[other], v + last * 32 * R::kV, kn);
+                if constexpr (B::kSub == 1) sc[0] = sc[1];
+                if constexpr (PAGED) {
+                    if (t + 3 < n_tiles) store_pages(t + 3, ahead);
+                }
+                __syncthreads();  // tile t is read
             }
-            __syncthreads();  // tile t + 1 is in LDS
-            constexpr int last = B::kSub - 1, other = 1 - last;
-            if (masked) mask(sc[last], k0 + 32 * last);
-            step(sc[last], sc[other], v + last * 32 * R::kV, kn);
-            if constexpr (B::kSub == 1) sc[0] = sc[1];
-            if constexpr (PAGED) {
-                if (t + 3 < n_tiles) store_pages(t + 3, ahead);
-            }
-            __syncthreads();  // tile t is read
         }
     }
     const AttnArgs& e = args_again();

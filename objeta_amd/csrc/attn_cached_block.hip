@@ -13,7 +13,7 @@ int32_t launch(hipStream_t s, const AttnArgs& a, const char* action) {
     const uint64_t groups = static_cast<uint64_t>(a.n_splits) * a.n_batch * a.n_kv;
     const uint64_t x = groups * a.n_tiles;
     if (x > 0x7FFFFFFFull) OBJ_FAIL(kInvalidInput, action, "too many workgroups for one launch");
-    hipLaunchKernelGGL((attn_block_kernel<Q, K, DT, true>), dim3(static_cast<uint32_t>(x)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((attn_block_kernel<Q, block_type<K, DT>, DT, true>), dim3(static_cast<uint32_t>(x)), dim3(256), 0, s, a);
     OBJ_HIP(hipGetLastError(), action);
     return 0;
 }

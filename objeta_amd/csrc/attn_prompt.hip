@@ -12,30 +12,31 @@ using namespace dev;
 namespace {
 
 // Parts of the keys that a tile of rows sees, so that few tiles fill the card too: the n with
-// the least time (and a tenth less than one part's), counted in keys that a workgroup alone on its
-// CU takes. Two a CU take 1.37
-// times as long, each; a turn's setup and the parts' way through memory and the join cost what
-// 16-bit products spend on 200 and on 250 + 0.7 a workgroup, float ones on an eighth of that.
-// Sequences are taken to be of their mean length, which is what the host knows; the tiles of a
-// causal one see half of it in the mean, and the longest start first. Measured, one part and the
-// parts chosen: float, 3 x 510 tokens of 8 over 2 heads of 192: 237 us and 114 (5); 777 of 8
-// heads of 64: 64 and 32 (4); bf16 of 128, causal: 1024 tokens of 8 heads 30 and 26 (3), 5000 of
-// 8 over 2 115 and 97 (3); 512 of 32 over 8: 20, with two parts 25 (1).
+// the least time, counted in cycles (and a tenth less than one part's). A key takes a workgroup
+// alone on its CU 0.39 DT cycles in 16 bits, 1.4 DT in float parts, 2.9 DT in float products;
+// two a CU take 1.37 times as long, each. A workgroup's setup, and the parts' way through memory
+// to the join, are as measured. Sequences are taken to be of their mean length, which is what
+// the host knows; a tile may see two of them, and the tiles of a causal one see half of it in
+// the mean. Measured, one part and the parts chosen: float, 1530 tokens of 8 over 2 heads of
+// 192: 187 us and 116 (2); 777 of 8 heads of 64: 40 and 25 (4); bf16 of 128, causal: 1024 tokens
+// of 8 heads 30 and 26 (4), 5000 of 8 over 2 115 and 97 (3); 512 of 32 over 8: 20, with two
+// parts 25 (1).
 template <int T, int DT>
 uint32_t prompt_splits(const AttnArgs& a) {
     constexpr bool two = T != kDtF32 && Block<T, DT>::kPerCu == 2;
-    constexpr double each = two ? 1.37 : 1.0, extra = T == kDtF32 ? 0.125 : 1.0;
+    constexpr double each = two ? 1.37 : 1.0;
+    constexpr double key = DT * (T != kDtF32 ? 0.39 : (block_type<T, DT> == kDtF32x3 ? 1.4 : 2.9));
+    constexpr double setup = T != kDtF32 ? 2000.0 + 62.0 * DT : 8000.0 + 120.0 * DT;
     const uint64_t tiles = static_cast<uint64_t>(a.n_tiles) * a.n_kv, slots = two ? 512 : 256;
-    const double keys = static_cast<double>(a.n_rows) / a.n_batch;
+    const double mean = static_cast<double>(a.n_rows) / a.n_batch, longest = a.n_batch > 1 ? 2.0 * mean : mean;
     uint32_t best = 1;
     double best_cost = 0.0;
     for (uint32_t n = 1; n <= 8; ++n) {
         const uint64_t items = tiles * n, rest = items % slots;
-        double turns = static_cast<double>(items / slots) * each + (rest ? (rest > 256 ? each : 1.0) : 0.0);
-        if (a.causal) turns = __builtin_fmax(turns > 1.0 ? 1.0 + 0.5 * (each - 1.0) : 1.0, 0.5 * each * items / slots);
-        const double setup = static_cast<double>((items + slots - 1) / slots) * 200.0;
-        const double join = n > 1 ? 250.0 + 0.7 * items : 0.0;
-        const double cost = turns * keys / n + extra * (setup + join);
+        const double turns = static_cast<double>(items / slots) * each + (rest ? (rest > 256 ? each : 1.0) : 0.0);
+        const double keys = __builtin_fmax(longest * (items > 256 ? 0.5 + 0.5 * each : 1.0), turns * mean * (a.causal ? 0.5 : 1.0));
+        const double join = n > 1 ? 12000.0 + 0.4 * DT * items : 0.0;
+        const double cost = key * keys / n + setup * ((items + slots - 1) / slots) + join;
         if (n == 1 || cost < (best == 1 ? 0.9 : 1.0) * best_cost) best = n, best_cost = cost;
     }
     return best;
@@ -45,7 +46,7 @@ template <int T, int DT>
 int32_t launch_prompt(objeta_hip_context* ctx, hipStream_t s, AttnArgs& a, const char* action) {
     a.n_splits = prompt_splits<T, DT>(a);
     if (a.n_splits > 1) OBJ_TRY(attn_parts(ctx, s, a));
-    hipLaunchKernelGGL((attn_block_kernel<T, T, DT, false>), dim3(a.n_tiles * a.n_splits * a.n_kv), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((attn_block_kernel<T, block_type<T, DT>, DT, false>), dim3(a.n_tiles * a.n_splits * a.n_kv), dim3(256), 0, s, a);
     OBJ_HIP(hipGetLastError(), action);
     return a.n_splits > 1 ? launch_attn_join(s, T, false, a, action) : 0;
 }

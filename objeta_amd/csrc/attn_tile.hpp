@@ -19,7 +19,9 @@
 // two parts of the row times a power of two) or 24 bits (bf16, three), each product is exact,
 // and so are the probabilities split: a float result at two or three 16-bit products instead
 // of the eight float ones that a 16-bit product's worth of float products takes at a
-// sixteenth of the rate. Float caches use the float products.
+// sixteenth of the rate. So are float keys and values where 128 rows share the work (three
+// parts by three of bf16, without the three products below 2^-24: six 16-bit ones; a value
+// below 2^-102 loses its last part); else floats use the float products.
 #pragma once
 
 #include "kv_common.hpp"
@@ -47,6 +49,9 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f
 template <int T> struct ElemOf { typedef float type; };
 template <> struct ElemOf<kDtF16> { typedef _Float16 type; };
 template <> struct ElemOf<kDtBF16> { typedef __bf16 type; };
+// Float keys and values that lie in LDS as three bf16 parts each.
+constexpr int kDtF32x3 = 3;
+static_assert(kDtF32x3 != kDtF32 && kDtF32x3 != kDtF16 && kDtF32x3 != kDtBF16, "a type of its own");
 
 // Rows of DT elements of type KT in LDS, read by tiles of ROWS query rows. A key's row is
 // padded: by 16 bytes, the 16-byte reads of 16 consecutive keys at one column fall into 16
@@ -55,15 +60,29 @@ template <> struct ElemOf<kDtBF16> { typedef __bf16 type; };
 // four apart, into different banks.
 template <int KT, int DT, int ROWS>
 struct Rows {
-    static constexpr int kEs = KT == kDtF32 ? 4 : 2;
+    static constexpr int kEs = KT == kDtF32 || KT == kDtF32x3 ? 4 : 2;  // of an element in memory
     static constexpr int kBytes = DT * kEs;
     static constexpr int kUnits = kBytes / 16;
-    static constexpr int kK = kBytes + 16;
-    static constexpr int kV = kBytes + (KT == kDtF32 && ROWS == 16 ? 16 : 32);
+    static constexpr int kLs = KT == kDtF32 ? 4 : 2;  // of an element of a part in LDS
+    static constexpr int kParts = KT == kDtF32x3 ? 3 : 1;
+    static constexpr int kPart = DT * kLs;  // bytes from part to part of a row in LDS
+    static constexpr int kK = kParts * kPart + 16;
+    static constexpr int kV = kParts * kPart + (KT == kDtF32 && ROWS == 16 ? 16 : 32);
     // lanes that load one row: a power of two, so that a wave's load lies within eight keys
     static constexpr int kLanes = kUnits <= 8 ? 8 : (kUnits <= 16 ? 16 : (kUnits <= 32 ? 32 : 64));
     static constexpr int kPer = 64 / kLanes;  // keys of a wave's load
 };
+
+// Two floats rounded to bf16, side by side; x and y keep the rest. By words: left to
+// conversions of single values, the compiler makes each of them twice.
+__device__ __forceinline__ uint32_t take_bf16(float& x, float& y) {
+    typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const uint32_t pair = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, b16x2));
+    x -= __builtin_bit_cast(float, pair << 16);
+    y -= __builtin_bit_cast(float, pair & 0xFFFF0000u);
+    return pair;
+}
 
 template <int ROWS> struct AccOf { typedef f32x16 type; };
 template <> struct AccOf<16> { typedef f32x4 type; };
@@ -82,9 +101,13 @@ struct Math {
     static constexpr int kOut = DT / ROWS;              // accumulators of o
     static constexpr int kDim = DT;
     static constexpr bool kFloat = KT == kDtF32;
-    static constexpr int kParts = QT == KT ? 1 : (KT == kDtF16 ? 2 : 3);
+    static constexpr int kParts = QT == KT ? 1 : (KT == kDtF16 ? 2 : 3);  // of a query's and a probability's
+    static constexpr int kKvParts = R::kParts;                            // of a key's and a value's
+    // whether the product of these parts counts: of three and three, those above 2^-24
+    static constexpr bool counts(int kv, int q) { return kKvParts == 1 || kv + q < 3; }
     typedef typename ElemOf<QT>::type qelem;
     typedef typename ElemOf<KT>::type kelem;
+    typedef typename std::conditional<KT == kDtF16, _Float16, __bf16>::type pelem;  // of parts
     typedef typename std::conditional<kFloat, f32x8,
                                       typename std::conditional<KT == kDtF16, h16x8, b16x8>::type>::type frag;
     struct Query {
@@ -125,9 +148,16 @@ struct Math {
 #pragma unroll
         for (int p = 0; p < kParts; ++p) {
             frag f;
+            if constexpr (kParts == 3) {
+                u32x4a words;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) words[j] = take_bf16(rest[2 * j], rest[2 * j + 1]);
+                put(p, __builtin_bit_cast(frag, words));
+                continue;
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                f[j] = static_cast<kelem>(rest[j]);
+                f[j] = static_cast<pelem>(rest[j]);
                 if (p + 1 < kParts) rest[j] -= static_cast<float>(f[j]);
             }
             put(p, f);
@@ -207,9 +237,10 @@ struct Math {
     // Dimensions kStep i + 8 h .. + 8 of this lane's key (lane % ROWS of the tile): K as the
     // first operand. `p` is the tile's first row plus k_first.
     static __device__ __forceinline__ uint32_t k_first(uint32_t lane) {
-        return lane % ROWS * R::kK + lane / ROWS * (8 * R::kEs);
+        return lane % ROWS * R::kK + lane / ROWS * (8 * R::kLs);
     }
-    static __device__ __forceinline__ frag lds_k(const char* p, int i) {
+    static __device__ __forceinline__ frag lds_k(const char* p, int i, int part = 0) {
+        p += part * R::kPart;
         if constexpr (kFloat) {
             const f32x4 a = *reinterpret_cast<const f32x4*>(p + 4 * kStep * i);
             const f32x4 b = *reinterpret_cast<const f32x4*>(p + 4 * kStep * i + 16);
@@ -235,8 +266,8 @@ struct Math {
             return (4 * h + (l >> 2)) * R::kV + ds * 32 + (l & 3) * 8;
         }
     }
-    static __device__ __forceinline__ frag lds_v(const char* p, int dd) {
-        p += ROWS * R::kEs * dd;
+    static __device__ __forceinline__ frag lds_v(const char* p, int dd, int part = 0) {
+        p += part * R::kPart + ROWS * R::kLs * dd;
         if constexpr (kFloat) {
             f32x8 f;
 #pragma unroll
@@ -331,9 +362,13 @@ __device__ __forceinline__ void score_rows(Scores<M>& s, const typename M::Query
         s.s[n] = M::zero();
 #pragma unroll
         for (int i = 0; i < M::kSteps; ++i) {
-            const typename M::frag f = M::lds_k(k + n * M::kRows * M::R::kK, i);
 #pragma unroll
-            for (int p = 0; p < M::kParts; ++p) s.s[n] = M::mma(f, q.f[p][i], s.s[n]);
+            for (int x = 0; x < M::kKvParts; ++x) {
+                const typename M::frag f = M::lds_k(k + n * M::kRows * M::R::kK, i, x);
+#pragma unroll
+                for (int p = 0; p < M::kParts; ++p)
+                    if (M::counts(x, p)) s.s[n] = M::mma(f, q.f[p][i], s.s[n]);
+            }
         }
     }
 }
@@ -412,9 +447,13 @@ template <class M>
 __device__ __forceinline__ void value_rows(RowState<M>& st, const Weights<M>& w, const char* v, int t) {
 #pragma unroll
     for (int d = 0; d < M::kOut; ++d) {
-        const typename M::frag f = M::lds_v(v + M::kStep * t * M::R::kV, d);
 #pragma unroll
-        for (int part = 0; part < M::kParts; ++part) st.o[d] = M::mma(f, w.f[part], st.o[d]);
+        for (int x = 0; x < M::kKvParts; ++x) {
+            const typename M::frag f = M::lds_v(v + M::kStep * t * M::R::kV, d, x);
+#pragma unroll
+            for (int p = 0; p < M::kParts; ++p)
+                if (M::counts(x, p)) st.o[d] = M::mma(f, w.f[p], st.o[d]);
+        }
     }
 }
 template <class M>
