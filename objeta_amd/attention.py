@@ -14,7 +14,7 @@ import numpy as np
 
 from . import _lib
 from ._lib import KvCacheDesc, RopeParams, RopePlan
-from .api import HipBackend, _addr, _addr_or_none, check
+from .api import HipBackend, _addr, check
 
 ELEMENT_TYPES = {"f32": 0, "f16": 1, "bf16": 2}
 ELEMENT_BYTES = {"f32": 4, "f16": 2, "bf16": 2}
@@ -29,7 +29,13 @@ def _choice(table: dict, name, what: str) -> int:
 
 
 def _dtype(name) -> int:
-    return _choice(ELEMENT_TYPES, name, "element type")
+    code = ELEMENT_TYPES.get(name)
+    return _choice(ELEMENT_TYPES, name, "element type") if code is None else code
+
+
+def _at(v):
+    """An address as the C call takes it; integers and None go as they are, which is cheapest."""
+    return v if type(v) is int or v is None else _addr(v)
 
 
 class Rope:
@@ -46,7 +52,8 @@ class Rope:
         p = RopeParams(theta, rotary_dim, _choice(_LAYOUTS, layout, "layout"), _choice(_SCALINGS, scaling, "scaling"), 0,
                        factor, original_context, beta_fast, beta_slow, 0.0 if amplitude is None else amplitude)
         self.plan = RopePlan()
-        check(_lib.load().objeta_hip_rope_init(C.byref(p), C.byref(self.plan)))
+        self._ref = C.byref(self.plan)
+        check(_lib.load().objeta_hip_rope_init(C.byref(p), self._ref))
         self.rotary_dim = rotary_dim
 
     def turns(self) -> np.ndarray:
@@ -81,6 +88,7 @@ class KvCache:
         self.desc = KvCacheDesc(_addr(self.d_k), _addr(self.d_v), _addr(self.d_page_table), _addr(self.d_seq_lens),
                                 _addr(self.d_ref_counts), code, n_layers, n_pages, n_kv_heads, page_size, head_dim, n_seqs,
                                 max_pages)
+        self._ref = C.byref(self.desc)
 
     def append_device(self, layer: int, d_seqs, d_cu_rows, n_batch: int, n_rows: int, dtype: str, d_k, d_v,
                       rope: Rope | None = None, d_positions=None, d_q=None, d_q_out=None, n_q_heads: int = 0,
@@ -90,32 +98,32 @@ class KvCache:
         extend_device), keys and, with d_q, queries rotated on the way."""
         row, q_row = self.n_kv_heads * self.head_dim, n_q_heads * self.head_dim
         check(self.L.objeta_hip_kv_append_device(
-            self.backend.ctx, stream, C.byref(self.desc), layer, _addr(d_seqs), _addr(d_cu_rows), n_batch, n_rows,
-            _dtype(dtype), _addr(d_k), row if k_stride is None else k_stride, _addr(d_v),
-            row if v_stride is None else v_stride, None if rope is None else C.byref(rope.plan),
-            _addr_or_none(d_positions), _addr_or_none(d_q), q_row if q_stride is None else q_stride, n_q_heads,
-            _dtype(dtype if q_out_dtype is None else q_out_dtype), _addr_or_none(d_q_out),
+            self.backend.ctx, stream, self._ref, layer, _at(d_seqs), _at(d_cu_rows), n_batch, n_rows,
+            _dtype(dtype), _at(d_k), row if k_stride is None else k_stride, _at(d_v),
+            row if v_stride is None else v_stride, None if rope is None else rope._ref,
+            _at(d_positions), _at(d_q), q_row if q_stride is None else q_stride, n_q_heads,
+            _dtype(dtype if q_out_dtype is None else q_out_dtype), _at(d_q_out),
             q_row if q_out_stride is None else q_out_stride))
 
     def extend_device(self, d_seqs, d_counts, n: int, stream=None) -> None:
         """Room for d_counts[i] more tokens of sequence d_seqs[i]; a shared last page is copied."""
-        check(self.L.objeta_hip_kv_extend_device(self.backend.ctx, stream, C.byref(self.desc), _addr(d_seqs),
-                                                 _addr(d_counts), n))
+        check(self.L.objeta_hip_kv_extend_device(self.backend.ctx, stream, self._ref, _at(d_seqs),
+                                                 _at(d_counts), n))
 
     def fork_device(self, d_src, d_dst, n: int, stream=None) -> None:
         """Sequence d_dst[i] becomes d_src[i] as it was before the call, on shared pages."""
-        check(self.L.objeta_hip_kv_fork_device(self.backend.ctx, stream, C.byref(self.desc), _addr(d_src), _addr(d_dst),
+        check(self.L.objeta_hip_kv_fork_device(self.backend.ctx, stream, self._ref, _at(d_src), _at(d_dst),
                                                n))
 
     def compact_device(self, d_seqs, d_drafts, d_keep, d_kept, n: int, max_keep: int, stream=None) -> None:
         """Of the last d_drafts[i] tokens of sequence d_seqs[i], those with the d_kept[i] ascending
         indices d_keep[i] stay and move together; the others are dropped."""
-        check(self.L.objeta_hip_kv_compact_device(self.backend.ctx, stream, C.byref(self.desc), _addr(d_seqs),
-                                                  _addr(d_drafts), _addr_or_none(d_keep), _addr(d_kept), n, max_keep))
+        check(self.L.objeta_hip_kv_compact_device(self.backend.ctx, stream, self._ref, _at(d_seqs),
+                                                  _at(d_drafts), _at(d_keep), _at(d_kept), n, max_keep))
 
     def free_device(self, d_seqs, n: int, stream=None) -> None:
         """Sequence d_seqs[i] releases its pages and is empty."""
-        check(self.L.objeta_hip_kv_free_device(self.backend.ctx, stream, C.byref(self.desc), _addr(d_seqs), n))
+        check(self.L.objeta_hip_kv_free_device(self.backend.ctx, stream, self._ref, _at(d_seqs), n))
 
 
 class AttentionBackend:
@@ -132,10 +140,10 @@ class AttentionBackend:
         """Rotary positions for queries and (n_k_heads > 0) keys in one launch."""
         q_row, k_row = n_q_heads * head_dim, n_k_heads * head_dim
         check(self.L.objeta_hip_rope_device(
-            self.backend.ctx, stream, C.byref(rope.plan), _addr(d_positions), n_tokens, head_dim, _dtype(dtype),
-            _dtype(dtype if out_dtype is None else out_dtype), _addr(d_q), q_row if q_stride is None else q_stride,
-            _addr(d_q_out), q_row if q_out_stride is None else q_out_stride, n_q_heads, _addr_or_none(d_k),
-            k_row if k_stride is None else k_stride, _addr_or_none(d_k_out),
+            self.backend.ctx, stream, rope._ref, _at(d_positions), n_tokens, head_dim, _dtype(dtype),
+            _dtype(dtype if out_dtype is None else out_dtype), _at(d_q), q_row if q_stride is None else q_stride,
+            _at(d_q_out), q_row if q_out_stride is None else q_out_stride, n_q_heads, _at(d_k),
+            k_row if k_stride is None else k_stride, _at(d_k_out),
             k_row if k_out_stride is None else k_out_stride, n_k_heads))
 
     def prompt_device(self, dtype: str, d_q, d_k, d_v, d_out, n_q_heads: int, n_kv_heads: int, head_dim: int,
@@ -145,11 +153,11 @@ class AttentionBackend:
         """Attention over packed sequences; scale None is head_dim ** -0.5."""
         q_row, kv_row = n_q_heads * head_dim, n_kv_heads * head_dim
         check(self.L.objeta_hip_attn_prompt_device(
-            self.backend.ctx, stream, _dtype(dtype), _addr(d_q), q_row if q_stride is None else q_stride, n_q_heads,
-            _addr(d_k), kv_row if k_stride is None else k_stride, _addr(d_v), kv_row if v_stride is None else v_stride,
-            n_kv_heads, head_dim, n_tokens, _addr(d_cu_seqlens), n_seqs, 1 if causal else 0,
-            head_dim ** -0.5 if scale is None else scale, _addr(d_out), q_row if out_stride is None else out_stride,
-            _addr_or_none(d_lse)))
+            self.backend.ctx, stream, _dtype(dtype), _at(d_q), q_row if q_stride is None else q_stride, n_q_heads,
+            _at(d_k), kv_row if k_stride is None else k_stride, _at(d_v), kv_row if v_stride is None else v_stride,
+            n_kv_heads, head_dim, n_tokens, _at(d_cu_seqlens), n_seqs, 1 if causal else 0,
+            head_dim ** -0.5 if scale is None else scale, _at(d_out), q_row if out_stride is None else out_stride,
+            _at(d_lse)))
 
     def cached_device(self, cache: KvCache, layer: int, d_seqs, d_cu_rows, n_batch: int, n_rows: int, max_rows: int,
                       max_len: int, dtype: str, d_q, d_out, n_q_heads: int, d_tree=None, scale: float | None = None,
@@ -158,7 +166,7 @@ class AttentionBackend:
         d_tree among an entry's own rows. scale None is head_dim ** -0.5."""
         q_row = n_q_heads * cache.head_dim
         check(self.L.objeta_hip_attn_cached_device(
-            self.backend.ctx, stream, C.byref(cache.desc), layer, _addr(d_seqs), _addr(d_cu_rows), n_batch, n_rows,
-            max_rows, max_len, _dtype(dtype), _addr(d_q), q_row if q_stride is None else q_stride, n_q_heads,
-            _addr_or_none(d_tree), cache.head_dim ** -0.5 if scale is None else scale, _addr(d_out),
-            q_row if out_stride is None else out_stride, _addr_or_none(d_lse)))
+            self.backend.ctx, stream, cache._ref, layer, _at(d_seqs), _at(d_cu_rows), n_batch, n_rows,
+            max_rows, max_len, _dtype(dtype), _at(d_q), q_row if q_stride is None else q_stride, n_q_heads,
+            _at(d_tree), cache.head_dim ** -0.5 if scale is None else scale, _at(d_out),
+            q_row if out_stride is None else out_stride, _at(d_lse)))
