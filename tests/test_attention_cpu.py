@@ -143,6 +143,13 @@ def test_prompt_refuses(lib, ctx, kw, text):
     refused(lib, call_prompt(lib, ctx, **kw), INVALID, text)
 
 
+@pytest.mark.parametrize("kw", [{"ks": (1 << 23) + 8, "n": 2}, {"vs": 1 << 24, "n": 2}])
+def test_prompt_refuses_wide_rows(lib, ctx, kw):
+    """Rows of keys and values no further apart than 2^23 elements."""
+    far = dict(q=1 << 45, k=1 << 46, v=3 << 45, out=1 << 47)
+    refused(lib, call_prompt(lib, ctx, **far, **kw), INVALID, "strides must not exceed")
+
+
 def cache(**kw):
     a = dict(k=0x7000000000, v=0x7100000000, page_table=0x7200000000, seq_lens=0x7200100000, ref_counts=0x7200200000, dtype=2,
              n_layers=2, n_pages=64, n_kv_heads=2, page_size=16, head_dim=64, n_seqs=4, max_pages=16)
