@@ -883,7 +883,10 @@ int32_t objeta_hip_rope_device(objeta_hip_context* ctx, objeta_hip_stream stream
  * last one, or under indices out of order) are left as they were. What lies in places a
  * row does not see, infinities and NaN included, does not reach it. scale > 0. Sums and
  * softmax are held in float; 16-bit types round the probabilities to their type before the
- * product with v (float: not). out may not overlap q, k or v. n_tokens * n_q_heads < 2^31. */
+ * product with v (float: not; float keys and values may be multiplied as three bf16 parts
+ * each, 24 bits together, of which a value below 2^-102 loses the last). Where the tiles of
+ * rows are few, keys are cut over workgroups whose parts lie in the stream's workspace. out
+ * may not overlap q, k or v. k_stride, v_stride <= 2^23. n_tokens * n_q_heads < 2^31. */
 int32_t objeta_hip_attn_prompt_device(objeta_hip_context* ctx, objeta_hip_stream stream, int32_t dtype,
                                       const void* d_q, uint64_t q_stride, uint64_t n_q_heads, const void* d_k,
                                       uint64_t k_stride, const void* d_v, uint64_t v_stride, uint64_t n_kv_heads,
