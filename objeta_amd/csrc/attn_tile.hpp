@@ -510,7 +510,8 @@ __device__ __forceinline__ uint32_t splits_of(int32_t len, uint32_t chunk, uint3
 // an XCD, the kernel 80 us for 44 us of work on every CU). Each wave reads 64 entries at a
 // time, a lane an entry, and finds the id'th piece in their running sum; what it read of the
 // entry need not be read again. Up to 64 entries it also chooses the chunk, which the host
-// could only choose for the longest: REPLACE
+// could only choose for the longest (8 trees over 2000 to 7001 tokens: parts of at most 896 keys
+// instead of 1024, the kernel 52.5 us instead of 55.5, the join 10 instead of 11.4).
 struct BlockItem {
     uint32_t head, split, tile, splits;
     int32_t row0, n_q, len, seq;

@@ -15,6 +15,7 @@ constexpr uint32_t kErrIndex = 4u;    // device error word, bit 2: an index outs
 constexpr uint32_t kErrNoPages = 8u;  // bit 3: not enough free pages
 constexpr uint64_t kMaxHeadDim = 256;
 constexpr uint64_t kMaxPageOps = 1024;  // entries of one page operation
+constexpr uint64_t kMaxTokens = 0x7FFF0000u;  // of a sequence: 32-bit sums of a key's index and a tile's keys stay below 2^31
 
 inline bool dtype_ok(int32_t t) { return t == kDtF32 || t == kDtF16 || t == kDtBF16; }
 inline uint64_t dtype_size(int32_t t) { return t == kDtF32 ? 4 : 2; }

@@ -260,7 +260,7 @@ int32_t check_kv(const objeta_hip_kv_cache* c, const char* action) {
     if (reinterpret_cast<uintptr_t>(c->k) % 16 || reinterpret_cast<uintptr_t>(c->v) % 16)
         OBJ_FAIL(kInvalidInput, action, "cache k and v must be 16-byte aligned");
     if (c->n_pages > 0x7FFFFFFFu || c->n_seqs > 0x7FFFFFFFu || c->n_kv_heads > 65535u || c->n_layers > 65535u ||
-        static_cast<uint64_t>(c->max_pages) * c->page_size > 0x7FFFFFFFu ||
+        static_cast<uint64_t>(c->max_pages) * c->page_size > kMaxTokens ||
         static_cast<double>(c->n_layers) * c->n_pages * c->n_kv_heads * c->page_size * c->head_dim > 1e14)
         OBJ_FAIL(kInvalidInput, action, "cache too large");
     return 0;

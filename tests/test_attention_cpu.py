@@ -143,6 +143,12 @@ def test_prompt_refuses(lib, ctx, kw, text):
     refused(lib, call_prompt(lib, ctx, **kw), INVALID, text)
 
 
+def test_prompt_refuses_most_rows(lib, ctx):
+    """A key's index and a tile's keys add up in 32 bits: some room is left below 2^31."""
+    refused(lib, call_prompt(lib, ctx, n=0x7FFF0000 // 8 + 1), INVALID, "2^31")
+    refused(lib, call_cached(lib, ctx, cache(max_pages=0x7FFF0000 // 16 + 1)), INVALID, "too large")
+
+
 @pytest.mark.parametrize("kw", [{"ks": (1 << 23) + 8, "n": 2}, {"vs": 1 << 24, "n": 2}])
 def test_prompt_refuses_wide_rows(lib, ctx, kw):
     """Rows of keys and values no further apart than 2^23 elements."""

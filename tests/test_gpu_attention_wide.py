@@ -68,6 +68,15 @@ def test_cached_cuts_that_fill_the_card(backend, att, dtype, kv, lens, rows, hea
     assert np.array_equal(got, again[1]) and np.array_equal(lse, again[2])
 
 
+@pytest.mark.parametrize("dtype,kv", [("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_cached_more_parts_than_lanes(backend, att, dtype, kv, rows):
+    c = Cached(backend, [20000, 16640, 16385, 16384, 90], kv, 1, 64, 40, seed=27)
+    for seqs in ([0, 1, 2, 3, 4], [2], [3, 4]):
+        q, got, lse, cu = run_cached(att, c, seqs, [rows] * len(seqs), dtype, 1)
+        check_cached(c, seqs, q, got, lse, cu, dtype, 1)
+
+
 @pytest.mark.parametrize("dtype,kv", [("bf16", "bf16"), ("f32", "f32"), ("f32", "bf16")])
 @pytest.mark.parametrize("batch,rows", [(130, 1), (300, 2), (70, 16)])
 def test_cached_joins_of_many_rows(backend, att, dtype, kv, batch, rows):
