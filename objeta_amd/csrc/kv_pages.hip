@@ -219,7 +219,9 @@ __device__ __forceinline__ bool named_before(const int32_t* __restrict__ ids, ui
     return __syncthreads_or(same);
 }
 
-// fork, first half: counts of the pages that change hands, and the sources' tables as they
+// fork in two launches: with everything held in registers by one workgroup it is one, and no
+// faster (24 x 2 sequences of 94 pages: 6.0 us against 3.3 and 2.6).
+// First half: counts of the pages that change hands, and the sources' tables as they
 // are now (rows [n][max_pages], then lengths [n]; -1 for an entry that is left out).
 __global__ __launch_bounds__(256) void kv_fork_stage_kernel(KvView kv, const int32_t* __restrict__ src,
                                                             const int32_t* __restrict__ dst, int32_t* __restrict__ rows,

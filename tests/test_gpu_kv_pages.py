@@ -284,3 +284,19 @@ def test_append_bad_indices_and_repeats(backend):
     r.cache.d_page_table.upload(table)
     r.m.error = 4
     r.compare("pages")
+
+
+@pytest.mark.parametrize("max_pages", [2730, 2731, 8192, 8193])
+def test_fork_of_long_tables(backend, max_pages):
+    """Around the size up to which one workgroup holds all tables: shared, exchanged, onto one that
+    held pages of its own, an entry refused among them."""
+    r = Rig(backend, 7, pages=14000, page=8, seqs=6, max_pages=max_pages, layers=1, heads=1, dim=8)
+    r.extend([0, 1, 2], [8 * 2700 + 3, 8 * 2000, 17])
+    r.fork([0, 1, 2], [3, 4, 1])
+    r.compare("three")
+    r.fork([0, 3, 9], [1, 0, 2])
+    r.compare("onto pages of its own, back, and a bad one")
+    r.fork([1, 4, 0], [4, 1, 4])
+    r.compare("exchange, and one destination twice")
+    r.fork([2], [2])
+    r.compare("itself")
