@@ -110,7 +110,6 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
     float scale = a.scale_log2;
     M::load_q(q, static_cast<const typename M::qelem*>(a.q) + row * a.q_stride + static_cast<uint64_t>(q_head) * a.dim, real,
               a.dim, lane, scale);
-    M::settle(q);
     // ---- what the workgroup sees, [k_lo, k_end), and what every real row of the wave sees whole
     int32_t k_lo, k_end, all_lo, all_hi;
     if (tid == 0) sh_bad = 0;
@@ -326,6 +325,7 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
                 __syncthreads();
             }
             load_tile(0);
+            M::settle(q);
             store_tile(0);
             load_k(1);
 #pragma unroll
@@ -393,6 +393,7 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
                 __syncthreads();
             }
             load_tile(0);
+            M::settle(q);
             store_tile(0);
             if (n_tiles > 1) load_tile(1);
         }

@@ -498,6 +498,23 @@ struct StreamItem {
     }
 };
 
+// The sum over the lanes up to this one, by moves within rows of 16 and broadcasts of their last
+// lanes: a few cycles each, where an exchange through LDS takes some sixty.
+template <class T>
+__device__ __forceinline__ T sum_to_lane(T v) {
+    auto add = [&](auto move) {
+        const int x = move(__builtin_bit_cast(int, v));
+        v += __builtin_bit_cast(T, x);
+    };
+    add([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false); });  // row_shr:1
+    add([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false); });
+    add([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false); });
+    add([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false); });
+    add([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false); });  // row_bcast:15 to rows 1 and 3
+    add([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false); });  // row_bcast:31 to rows 2 and 3
+    return v;
+}
+
 // Into how many parts a sequence's keys are cut.
 __device__ __forceinline__ uint32_t splits_of(int32_t len, uint32_t chunk, uint32_t most) {
     const uint32_t n = (static_cast<uint32_t>(len) + chunk - 1) / chunk;
@@ -516,11 +533,7 @@ struct BlockItem {
     uint32_t head, split, tile, splits;
     int32_t row0, n_q, len, seq;
     bool any, usable;
-    static __device__ __forceinline__ uint32_t total(uint32_t v) {
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
-        return __builtin_amdgcn_readfirstlane(v);
-    }
+    static __device__ __forceinline__ uint32_t total(uint32_t v) { return __builtin_amdgcn_readlane(sum_to_lane(v), 63); }
     // `slots` workgroups run at a time.
     __device__ __forceinline__ BlockItem(const AttnArgs& a, uint32_t id, uint32_t slots) {
         const uint32_t lane = threadIdx.x & 63;
@@ -552,9 +565,8 @@ struct BlockItem {
                 const uint32_t one = total(tiles * a.n_kv);
                 const uint32_t room = (one * 4 / 3 + slots) / slots * slots;
                 float keys = static_cast<float>(tiles * a.n_kv) * static_cast<float>((static_cast<uint32_t>(l) + 63) / 64);
-#pragma unroll
-                for (int d = 32; d > 0; d >>= 1) keys += __shfl_xor(keys, d, 64);
-                const uint32_t least = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(keys / static_cast<float>(room))) + 1;
+                keys = sum_to_lane(keys);
+                const uint32_t least = __builtin_amdgcn_readlane(static_cast<uint32_t>(keys / static_cast<float>(room)), 63) + 1;
                 for (uint32_t k = 8; k <= 16; k += k < 12 ? 1 : 2) {
                     chunk = least * 8 * k;
                     chunk = chunk < 256 ? 256 : chunk;
@@ -563,12 +575,7 @@ struct BlockItem {
                 if (first && threadIdx.x == 0) *a.picked = chunk;
             }
             const uint32_t parts = splits_of(l, chunk, a.n_splits), pieces = tiles * parts * a.n_kv;
-            uint32_t sum = pieces;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint32_t o = __shfl_up(sum, d, 64);
-                if (lane >= static_cast<uint32_t>(d)) sum += o;
-            }
+            const uint32_t sum = sum_to_lane(pieces);
             const uint64_t past = __ballot(sum > id);
             if (past) {
                 const int at = __builtin_ctzll(past);
