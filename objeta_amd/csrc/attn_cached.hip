@@ -196,6 +196,8 @@ int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream
     // longest, in chunks of whole 256 keys.
     const uint64_t units = n_batch * a.n_kv * a.n_tiles;
     uint64_t splits = (1024 + units - 1) / units;
+    const uint64_t room = most_parts(n_rows, n_q_heads, dim);
+    splits = splits < room ? splits : room;
     uint64_t chunk = ((len + splits - 1) / splits + 255) / 256 * 256;
     // Few keys in one piece: the join costs more than the waves' longer way (560 keys of one
     // sequence, bf16: 10.5 us against 11.1; 700: 11.3 and 11.2; 260: 7.9 and 10.9).

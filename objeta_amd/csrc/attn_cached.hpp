@@ -9,6 +9,12 @@ namespace objeta {
 int32_t check_attn_rows(const char* action, const char* what, const void* p, uint64_t n, uint64_t stride, uint64_t heads,
                         uint64_t dim, uint64_t size);
 int32_t check_heads(const char* action, uint64_t n_q_heads, uint64_t n_kv_heads, uint64_t n_rows, float scale);
+// The most parts that keep their workspace within 1 GiB: rows that belong to no sequence count too,
+// and a batch padded far would ask for more than it uses.
+inline uint64_t most_parts(uint64_t n_rows, uint64_t n_heads, uint64_t dim) {
+    const uint64_t most = (uint64_t(1) << 30) / (n_rows * n_heads * (dim + 2) * sizeof(float));
+    return most < 1 ? 1 : most;
+}
 // Workspace for the parts of a call of several splits, and their join (attn_cached.hip).
 int32_t attn_parts(objeta_hip_context* ctx, hipStream_t s, dev::AttnArgs& a);
 int32_t launch_attn_join(hipStream_t s, int32_t dtype, bool paged, const dev::AttnArgs& a, const char* action);

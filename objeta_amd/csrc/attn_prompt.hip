@@ -44,7 +44,9 @@ uint32_t prompt_splits(const AttnArgs& a) {
 
 template <int T, int DT>
 int32_t launch_prompt(objeta_hip_context* ctx, hipStream_t s, AttnArgs& a, const char* action) {
+    const uint64_t room = most_parts(a.n_rows, a.n_heads, a.dim);
     a.n_splits = prompt_splits<T, DT>(a);
+    if (a.n_splits > room) a.n_splits = static_cast<uint32_t>(room);
     if (a.n_splits > 1) OBJ_TRY(attn_parts(ctx, s, a));
     hipLaunchKernelGGL((attn_block_kernel<T, block_type<T, DT>, DT, false>), dim3(a.n_tiles * a.n_splits * a.n_kv), dim3(256), 0, s, a);
     OBJ_HIP(hipGetLastError(), action);

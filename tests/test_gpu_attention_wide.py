@@ -90,6 +90,26 @@ def test_cached_joins_of_many_rows(backend, att, dtype, kv, batch, rows):
         check_cached(c, [seqs[b]], q[cu[b]:cu[b + 1]], got[cu[b]:cu[b + 1]], lse[cu[b]:cu[b + 1]], [0, rows], dtype, nq)
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_cached_batch_padded_far(backend, att, rows):
+    """100 thousand rows of which one entry has a few: the padding is left alone."""
+    be, n, nq = backend, 100000, 16
+    c = Cached(backend, [3000], "f16", 1, 16, 64, seed=28)
+    q = to_type(np.random.default_rng(29).standard_normal((rows, nq, 64)), "f16")
+    d_q, out = be.alloc(n * nq * 64 * 2), be.alloc(n * nq * 64 * 2)
+    d_q.upload(q)
+    edge = np.full((rows + 8, nq, 64), FILL, np.float16)
+    out.upload(edge)
+    lse = be.to_device(np.full((n, nq), FILL, np.float32))
+    att.cached_device(c.cache, 0, be.to_device(np.array([0], np.int32)), be.to_device(np.array([0, rows], np.int32)), 1, n, rows, 3000,
+                      "f16", d_q, out, nq, d_lse=lse)
+    be.synchronize()
+    got = out.download(np.float16, edge.size).reshape(edge.shape).astype(np.float64)
+    l = lse.download(np.float32, n * nq).reshape(n, nq)
+    check_cached(c, [0], q, got[:rows], l[:rows].astype(np.float64), [0, rows], "f16", nq)
+    assert np.all(got[rows:] == FILL) and np.all(l[rows:] == FILL)
+
+
 def test_cached_replays_choose_their_own_cuts(backend, att):
     """A captured call of many rows on lengths that changed since: each replay as an eager call."""
     be, st = backend, backend.stream(1)
