@@ -820,7 +820,9 @@ int32_t objeta_hip_st_deepseek_router(const objeta_hip_st_model* model, uint64_t
  * kernels before any access they lead to: an index outside its table sets bit 2 of the
  * device error word (objeta_hip_device_error), page allocation without free pages bit 3.
  * The entry point says what becomes of the work concerned. Calls allocate nothing once
- * a call as large has run on their stream, and may be captured after it. Graphs
+ * a call of the same sizes (max_rows and max_len among them) has run on their stream, and
+ * may be captured after it; a smaller call may cut its keys into more parts and need more.
+ * A captured call that finds no workspace of its size is refused (Unsupported). Graphs
  * captured on one stream share that stream's workspace: their replays are ordered one
  * after the other, as calls on the stream are. */
 
