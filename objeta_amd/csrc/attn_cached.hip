@@ -193,16 +193,31 @@ int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream
     a.tile_rows = stream_form ? (rows <= 16 ? 16 : 32) : 128;
     a.n_tiles = static_cast<uint32_t>((rows + a.tile_rows - 1) / a.tile_rows);
     // Keys are cut so that there are about 1024 workgroups if every sequence were the
-    // longest, in chunks of whole 256 keys.
+    // longest, in chunks of at least 256 keys; of two tiles a wave where all workgroups then
+    // have a CU to themselves (4000 keys of one sequence, float cache: 14.7 us against 22.4;
+    // 30000 keys, which then have not, 46.0 against 37.3).
     const uint64_t units = n_batch * a.n_kv * a.n_tiles;
     uint64_t splits = (1024 + units - 1) / units;
     const uint64_t room = most_parts(n_rows, n_q_heads, dim);
     splits = splits < room ? splits : room;
-    uint64_t chunk = ((len + splits - 1) / splits + 255) / 256 * 256;
-    // Few keys in one piece: the join costs more than the waves' longer way (560 keys of one
-    // sequence, bf16: 10.5 us against 11.1; 700: 11.3 and 11.2; 260: 7.9 and 10.9).
-    if (stream_form && len <= 576) chunk = 768;
+    const bool float_cache = c.dtype == kDtF32, can_wide = stream_form && a.tile_rows == 16;
+    const uint64_t waves = stream_waves(static_cast<int>((dim <= 64 ? 64 : (dim <= 128 ? 128 : 256)) * dtype_size(c.dtype)));
+    const uint64_t whole = stream_form ? 64 * waves : 256;
+    uint64_t chunk = ((len + splits - 1) / splits + whole - 1) / whole * whole;
+    if (chunk < 256 && !(can_wide && units * ((len + whole - 1) / whole) <= 256)) chunk = 256;
+    // Few keys, some tiles a wave, stay in one piece: the join costs more than the waves' longer
+    // way (bf16, one sequence: 700 keys 10.1 us against 11.5, 1000 11.9 and 11.7; float queries 700
+    // 11.8 and 12.6, 1000 14.3 and 12.7; 40 sequences of 300 to 900 14.7 and 18.6; float cache, one
+    // of 130 keys 11.9 and 12.9, of 260 15.6 and 12.9). With a workgroup or more a CU anyway, more
+    // keys do (float cache, 100 of 200 to 500: 43 and 54).
+    if (stream_form) {
+        uint64_t few = 576;
+        if (units <= 256 && can_wide) few = 64 * waves * (float_cache ? 2 : (units < 64 ? 3 : 4));
+        else if (units <= 256) few = 32 * waves * (float_cache ? 2 : 4);
+        if (len <= few) chunk = few;
+    }
     splits = (len + chunk - 1) / chunk;
+    a.wide = can_wide && units * splits <= 256;
     a.chunk = static_cast<uint32_t>(chunk);
     a.n_splits = static_cast<uint32_t>(splits);
     a.pick = !stream_form && splits > 1 && n_batch <= 64;

@@ -8,26 +8,28 @@ using namespace dev;
 
 namespace {
 
-template <int Q, int K, int DT, int ROWS>
+template <int Q, int K, int DT, int ROWS, bool WIDE>
 int32_t launch(hipStream_t s, const AttnArgs& a, const char* action) {
     const uint64_t groups = static_cast<uint64_t>(a.n_splits) * a.n_batch * a.n_kv;
     const uint64_t x = (groups + 7) / 8 * 8;
     if (x > 0x7FFFFFFFull) OBJ_FAIL(kInvalidInput, action, "too many workgroups for one launch");
-    hipLaunchKernelGGL((attn_stream_kernel<Q, K, DT, ROWS>), dim3(static_cast<uint32_t>(x)), dim3(64 * Stream<K, DT, ROWS>::kWaves), 0, s, a);
+    hipLaunchKernelGGL((attn_stream_kernel<Q, K, DT, ROWS, WIDE>), dim3(static_cast<uint32_t>(x)),
+                       dim3(64 * Stream<K, DT, ROWS, WIDE>::kWaves), 0, s, a);
     OBJ_HIP(hipGetLastError(), action);
     return 0;
 }
 
-template <int Q, int K, int ROWS>
+template <int Q, int K, int ROWS, bool WIDE>
 int32_t launch_rows(hipStream_t s, const AttnArgs& a, const char* action) {
-    if (a.dim <= 64) return launch<Q, K, 64, ROWS>(s, a, action);
-    if (a.dim <= 128) return launch<Q, K, 128, ROWS>(s, a, action);
-    return launch<Q, K, 256, ROWS>(s, a, action);
+    if (a.dim <= 64) return launch<Q, K, 64, ROWS, WIDE>(s, a, action);
+    if (a.dim <= 128) return launch<Q, K, 128, ROWS, WIDE>(s, a, action);
+    return launch<Q, K, 256, ROWS, WIDE>(s, a, action);
 }
 
 template <int Q, int K>
 int32_t launch_dim(hipStream_t s, uint32_t rows, const AttnArgs& a, const char* action) {
-    return rows <= 16 ? launch_rows<Q, K, 16>(s, a, action) : launch_rows<Q, K, 32>(s, a, action);
+    if (rows > 16) return launch_rows<Q, K, 32, false>(s, a, action);
+    return a.wide ? launch_rows<Q, K, 16, true>(s, a, action) : launch_rows<Q, K, 16, false>(s, a, action);
 }
 
 }  // namespace

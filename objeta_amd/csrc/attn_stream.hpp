@@ -13,12 +13,15 @@
 namespace objeta {
 namespace dev {
 
-template <int KT, int DT, int ROWS>
+// WIDE: twice the waves, for few workgroups that each have a CU to themselves (517 keys of one
+// sequence in one piece, bf16: 8.9 us against 10.4), where more would wait for one another (32
+// sequences of 301 to 8192: 46.5 against 42.6).
+template <int KT, int DT, int ROWS, bool WIDE>
 struct Stream {
     typedef Rows<KT, DT, ROWS> R;
     static constexpr int kLoads = 32 / R::kPer;                // 16-byte units of K (and of V) a lane stages
     static constexpr int kWave = 32 * (R::kK + R::kV);         // LDS of a wave: a tile of K and one of V
-    static constexpr int kWaves = DT * R::kEs <= 256 ? 4 : (DT * R::kEs <= 512 ? 2 : 1);
+    static constexpr int kWaves = stream_waves(DT * R::kEs) * (WIDE ? 2 : 1);
     static_assert(kWave >= ROWS * DT * 4, "o of a wave's rows in its part");
     // waves a SIMD: two where a wave's part of LDS lets eight be on a CU
     static constexpr int kPerSimd = DT * R::kEs <= 256 ? 2 : 1;
@@ -30,12 +33,12 @@ __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-template <int QT, int KT, int DT, int ROWS>
-__global__ __launch_bounds__((64 * Stream<KT, DT, ROWS>::kWaves),
-                             (ROWS == 32 ? 1 : Stream<KT, DT, ROWS>::kPerSimd)) void attn_stream_kernel(AttnArgs a) {
+template <int QT, int KT, int DT, int ROWS, bool WIDE>
+__global__ __launch_bounds__((64 * Stream<KT, DT, ROWS, WIDE>::kWaves),
+                             (ROWS == 32 ? 1 : Stream<KT, DT, ROWS, WIDE>::kPerSimd)) void attn_stream_kernel(AttnArgs a) {
     typedef Math<QT, KT, DT, ROWS> M;
     typedef Rows<KT, DT, ROWS> R;
-    typedef Stream<KT, DT, ROWS> S;
+    typedef Stream<KT, DT, ROWS, WIDE> S;
     constexpr int kWaves = S::kWaves;
     __shared__ alignas(16) char lds[kWaves][S::kWave];
     __shared__ float sh_m[kWaves][ROWS], sh_l[kWaves][ROWS];
@@ -128,7 +131,7 @@ __global__ __launch_bounds__((64 * Stream<KT, DT, ROWS>::kWaves),
         load_tile(k0, first);
     }
     for (; k0 < k_end; k0 = k_end - k0 > step ? k0 + step : k_end) {
-if (R::kLanes == R::kUnits || unit < R::kUnits) {
+        if (R::kLanes == R::kUnits || unit < R::kUnits) {
 #pragma unroll
             for (int x = 0; x < S::kLoads; ++x) {
                 *reinterpret_cast<u32x4a*>(k_lds + k_at + x * R::kPer * R::kK) = rk[x];

@@ -475,12 +475,16 @@ struct AttnArgs {
     uint64_t layer_off;  // elements
     // keys cut over workgroups: of cached sequences in equal parts of about `chunk`, of a prompt's
     // tile of rows in n_splits equal ones. pick: the kernel takes a chunk that fills the card,
-    // and leaves it in *picked for the join.
-    uint32_t chunk, n_splits, n_tiles, tile_rows, pick;
+    // and leaves it in *picked for the join. wide: workgroups of twice the waves.
+    uint32_t chunk, n_splits, n_tiles, tile_rows, pick, wide;
     uint32_t* picked;
     float *part, *part_ml;  // [n_splits][n_rows * n_heads][dim], [..][2]
     uint32_t* err;
 };
+
+// Waves of a workgroup of 16 or 32 rows, by the bytes of a head's row: as many as LDS lets two such
+// workgroups have on a CU (one, of the largest rows of 32).
+constexpr int stream_waves(int row_bytes) { return row_bytes <= 256 ? 4 : (row_bytes <= 512 ? 2 : 1); }
 
 // Which (entry, head, split) a workgroup of 16 or 32 rows takes. The splits are the slowest
 // index: short sequences have only the first ones, and workgroups go to the eight XCDs in
