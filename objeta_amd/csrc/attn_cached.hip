@@ -207,12 +207,13 @@ int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream
     if (chunk < 256 && !(can_wide && units * ((len + whole - 1) / whole) <= 256)) chunk = 256;
     // Few keys, some tiles a wave, stay in one piece: the join costs more than the waves' longer
     // way (bf16, one sequence: 700 keys 10.1 us against 11.5, 1000 11.9 and 11.7; float queries 700
-    // 11.8 and 12.6, 1000 14.3 and 12.7; 40 sequences of 300 to 900 14.7 and 18.6; float cache, one
-    // of 130 keys 11.9 and 12.9, of 260 15.6 and 12.9). With a workgroup or more a CU anyway, more
-    // keys do (float cache, 100 of 200 to 500: 43 and 54).
+    // 11.8 and 12.6, 1000 14.3 and 12.7; 40 sequences of 300 to 900 14.7 and 18.6, 64 of 300 to 2000
+    // 32.2 and 38.8; float cache, one of 130 keys 11.9 and 12.9, of 260 15.6 and 12.9). With a
+    // workgroup or more a CU anyway, more keys do (float cache, 100 of 200 to 500: 43 and 54).
     if (stream_form) {
         uint64_t few = 576;
-        if (units <= 256 && can_wide) few = 64 * waves * (float_cache ? 2 : (units < 64 ? 3 : 4));
+        const uint64_t tiles = float_cache ? 2 : (units < 64 ? 3 : (units < 128 ? 4 : units / 32));
+        if (units <= 256 && can_wide) few = 64 * waves * tiles;
         else if (units <= 256) few = 32 * waves * (float_cache ? 2 : 4);
         if (len <= few) chunk = few;
     }
