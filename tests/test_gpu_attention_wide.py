@@ -68,6 +68,18 @@ def test_cached_cuts_that_fill_the_card(backend, att, dtype, kv, lens, rows, hea
     assert np.array_equal(got, again[1]) and np.array_equal(lse, again[2])
 
 
+@pytest.mark.parametrize("dtype,kv,dim", [(*p, 64) for p in PAIRS] + [("f32", "f32", 128), ("f32", "f32", 256), ("f16", "f16", 256)])
+@pytest.mark.parametrize("lens,heads,group", [([767], 1, 4), ([769, 768], 2, 1), ([255, 256, 257], 1, 16), ([127, 128, 129, 385], 1, 1),
+                                              ([1023, 1024] * 10, 4, 2), ([1025] * 16 + [3], 4, 1), ([500, 20] * 35, 4, 1),
+                                              ([513, 385], 2, 20)])
+def test_cached_decode_around_the_cuts(backend, att, dtype, kv, dim, lens, heads, group):
+    """One piece or several, workgroups of one or both sizes, 16 or 32 rows a tile."""
+    c = Cached(backend, lens, kv, heads, 16, dim, seed=19)
+    seqs = list(range(len(lens)))
+    q, got, lse, cu = run_cached(att, c, seqs, [1] * len(lens), dtype, heads * group)
+    check_cached(c, seqs, q, got, lse, cu, dtype, heads * group)
+
+
 @pytest.mark.parametrize("dtype,kv", [("bf16", "bf16"), ("f32", "f32")])
 @pytest.mark.parametrize("rows", [1, 40])
 def test_cached_more_parts_than_lanes(backend, att, dtype, kv, rows):
