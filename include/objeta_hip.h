@@ -812,9 +812,9 @@ int32_t objeta_hip_st_deepseek_router(const objeta_hip_st_model* model, uint64_t
  * has a counterpart in it.
  *
  * Element types are OBJETA_HIP_DT_F32 / _F16 / _BF16. head_dim is a multiple of 8 up to
- * 256. Strides count elements from one token to the next; a token's heads lie behind one
- * another. Attention reads rows of 16-byte aligned addresses (base and stride). Query
- * head h reads key/value head h / (n_q_heads / n_kv_heads).
+ * 256. Strides count elements from one token to the next (of a single token: unused); a
+ * token's heads lie behind one another. Attention reads rows of 16-byte aligned addresses
+ * (base and stride). Query head h reads key/value head h / (n_q_heads / n_kv_heads).
  *
  * Indices on the device (cu_seqlens, sequences, lengths, page tables) are checked by the
  * kernels before any access they lead to: an index outside its table sets bit 2 of the

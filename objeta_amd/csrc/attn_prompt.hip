@@ -111,6 +111,12 @@ int32_t objeta_hip_attn_prompt_device(objeta_hip_context* ctx, objeta_hip_stream
     if (n_tokens == 0 || n_seqs == 0) return 0;
     if (!d_cu_seqlens) OBJ_FAIL(kInvalidInput, action, "cu_seqlens are NULL");
     const uint64_t es = dtype_size(dtype);
+    // one row has no next one: its strides may be anything, and the kernels take a row's stride
+    // for the bytes that there are to read
+    if (n_tokens == 1) {
+        q_stride = out_stride = n_q_heads * head_dim;
+        k_stride = v_stride = n_kv_heads * head_dim;
+    }
     OBJ_TRY(check_attn_rows(action, "q", d_q, n_tokens, q_stride, n_q_heads, head_dim, es));
     OBJ_TRY(check_attn_rows(action, "k", d_k, n_tokens, k_stride, n_kv_heads, head_dim, es));
     OBJ_TRY(check_attn_rows(action, "v", d_v, n_tokens, v_stride, n_kv_heads, head_dim, es));

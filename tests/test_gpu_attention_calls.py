@@ -1,0 +1,44 @@
+"""Calls of rotary positions, appends and attention at the edges of what they take: strides of one
+row, batches with empty entries, batches without entries, more workgroups than one launch holds, and
+row indices out of order."""
+import numpy as np
+import pytest
+
+from attn_reference import NP, attend, download, frequencies, from_type, lse_bound, rotate, rotate_bound, to_type
+from objeta_amd import AttentionBackend, KvCache, MoeExecutor, Rope
+from test_gpu_attention import FILL, TYPES, Cached, check_cached, run_cached
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def att(backend):
+    MoeExecutor(backend).device_error()
+    yield AttentionBackend(backend)
+    assert MoeExecutor(backend).device_error() == 0
+
+
+def ints(be, v):
+    return be.to_device(np.array(v, np.int32).ravel())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim", [64, 200, 256])
+@pytest.mark.parametrize("q_stride,k_stride,v_stride,out_stride", [(0, 0, 0, 0), (8, 8, 4, 12), (1, 2, 24, 7), (1 << 22, 1 << 22, 1 << 23, 5),
+                                                                   (9, (1 << 23) + 8, 1 << 24, 1 << 30)])
+def test_prompt_of_one_token_has_no_strides(backend, att, dtype, dim, q_stride, k_stride, v_stride, out_stride):
+    """There is no second row for a stride to lead to."""
+    rng, nq, nk = np.random.default_rng(40), 4, 2
+    q, k, v = (to_type(rng.standard_normal((1, h, dim)), dtype) for h in (nq, nk, nk))
+    out = backend.to_device(to_type(np.full(q.shape, FILL), dtype))
+    lse = backend.to_device(np.full((1, nq), FILL, np.float32))
+    att.prompt_device(dtype, *(backend.to_device(x) for x in (q, k, v)), out, nq, nk, dim, 1, ints(backend, [0, 1]), 1, d_lse=lse,
+                      q_stride=q_stride, k_stride=k_stride, v_stride=v_stride, out_stride=out_stride)
+    backend.synchronize()
+    got, got_lse = download(out, dtype, q.shape), lse.download(np.float32, nq)
+    scale = np.float64(np.float32(dim ** -0.5))
+    for h in range(nq):
+        q64, k64, v64 = (from_type(x, dtype) for x in (q[:, h], k[:, h // 2], v[:, h // 2]))
+        want, want_lse, bound = attend(q64, k64, v64, np.ones((1, 1), bool), scale, dtype, dtype)
+        assert np.all(np.abs(got[:, h] - want) <= bound)
+        assert abs(got_lse[h] - want_lse[0]) <= lse_bound(want_lse, dim, scale * (np.abs(q64) @ np.abs(k64).T).max())[0]
