@@ -925,7 +925,7 @@ typedef struct {
  * them. With `rope`, keys are rotated by d_positions[row] first (a draft's position need
  * not be its slot); with d_q also queries, q [n_rows][n_q_heads][head_dim] to q_out
  * (q_out_dtype; in place as for objeta_hip_rope_device), in the same launch. A sequence
- * that the batch names twice takes its last entry's rows. Keys and values of no entry, or
+ * that the batch names twice takes the rows of its last entry that has any. Keys and values of no entry, or
  * whose slot has no page (bit 2), are not written; queries of every row are. Sources may
  * not overlap the cache. */
 int32_t objeta_hip_kv_append_device(objeta_hip_context* ctx, objeta_hip_stream stream, const objeta_hip_kv_cache* cache,

@@ -79,9 +79,9 @@ __device__ __forceinline__ uint32_t count_le(const int32_t* __restrict__ cu, uin
 }
 
 // The batch entry that holds row r, found by a whole wave. `any`: there is one; `again` (where
-// LATER): a later entry names the same sequence. seqs may be NULL. Up to 63 entries lie in the lanes after one read, since
-// such reads are what small kernels wait for (a join of 32 rows: 4.4 us, with a search and
-// reads of its own for the entry's bounds 4.9).
+// LATER): a later entry that has rows names the same sequence. seqs may be NULL. Up to 63 entries
+// lie in the lanes after one read, since such reads are what small kernels wait for (a join of 32
+// rows: 4.4 us, with a search and reads of its own for the entry's bounds 4.9).
 template <bool LATER>
 struct RowEntry {
     int32_t lo, hi, seq;
@@ -93,20 +93,23 @@ struct RowEntry {
         lo = hi = 0, seq = -1, again = false;
         if (n_batch < 64) {
             const int32_t start = cu[lane <= n_batch ? lane : n_batch], s = seqs ? seqs[lane < n_batch ? lane : n_batch - 1] : -1;
+            int32_t end = 0;  // read beside the starts, so that no wait is added
+            if (LATER) end = cu[lane < n_batch ? lane + 1 : n_batch];
             const uint32_t le = __popcll(__ballot(lane <= n_batch && start <= r));
             any = le != 0 && le <= n_batch;
             if (!any) return;
             b = le - 1;
             lo = __builtin_amdgcn_readlane(start, b), hi = __builtin_amdgcn_readlane(start, le);
             seq = __builtin_amdgcn_readlane(s, b);
-            if (LATER) again = __ballot(lane > b && lane < n_batch && s == seq) != 0;
+            if (LATER) again = __ballot(lane > b && lane < n_batch && s == seq && end > start) != 0;
         } else {
             const uint32_t le = count_le(cu, n_batch + 1, r);
             any = le != 0 && le <= n_batch;
             if (!any) return;
             b = le - 1;
             lo = cu[b], hi = cu[le], seq = seqs ? seqs[b] : -1;
-            for (uint32_t i = b + 1; LATER && i < n_batch; i += 64) again |= __ballot(i + lane < n_batch && seqs[i + lane] == seq) != 0;
+            for (uint32_t i = b + 1; LATER && i < n_batch; i += 64)
+                again |= __ballot(i + lane < n_batch && seqs[i + lane] == seq && cu[i + lane + 1] > cu[i + lane]) != 0;
         }
         any = lo <= r && r < hi;
     }

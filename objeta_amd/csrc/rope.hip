@@ -168,7 +168,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
     if (a.ck) {
         const int64_t r = static_cast<int64_t>(t);
         const RowEntry<true> entry(a.cu, a.seqs, a.n_batch, r);
-        keep = entry.any && !entry.again;  // a later entry of the same sequence writes these slots
+        keep = entry.any && !entry.again;  // a later entry's rows of the same sequence take these slots
         if (keep) {
             bool ok = seq_ok(a.kv, entry.seq);
             const int32_t len = ok ? a.kv.lens[entry.seq] : 0;

@@ -42,3 +42,36 @@ def test_prompt_of_one_token_has_no_strides(backend, att, dtype, dim, q_stride, 
         want, want_lse, bound = attend(q64, k64, v64, np.ones((1, 1), bool), scale, dtype, dtype)
         assert np.all(np.abs(got[:, h] - want) <= bound)
         assert abs(got_lse[h] - want_lse[0]) <= lse_bound(want_lse, dim, scale * (np.abs(q64) @ np.abs(k64).T).max())[0]
+
+
+@pytest.mark.parametrize("batch", [2, 5, 62, 63, 64, 65, 130])
+@pytest.mark.parametrize("dim", [16, 40])
+def test_append_with_empty_entries_of_named_sequences(backend, att, batch, dim):
+    """Entries without rows write nothing, so they take nothing from an entry ahead that names their
+    sequence: a batch padded to a fixed count, and one that repeats a sequence with rows and without."""
+    be, rng = backend, np.random.default_rng(batch)
+    page, used = 8, (batch + 1) // 2
+    c = KvCache(be, 1, used, 2, page, dim, used, 1, dtype="f32")
+    table = rng.permutation(used).astype(np.int32).reshape(used, 1)
+    lens = rng.integers(2, page + 1, used).astype(np.int32)
+    pool = np.full((used, 2, page, dim), FILL, np.float32)
+    for d, x in ((c.d_page_table, table), (c.d_seq_lens, lens), (c.d_ref_counts, np.ones(used, np.int32)), (c.d_k, pool), (c.d_v, pool)):
+        d.upload(x)
+    again = batch - used  # empty entries: of every sequence in turn, the first one's among them
+    for seqs, rows in ((list(range(used)) + list(range(again)), [1] * used + [0] * again),
+                       (list(range(used)) + [0] * again, [2] * used + [0] * again),
+                       ([0] + list(range(1, used)) + [0] + [0] * (again - 1), [2] * used + [1] + [0] * (again - 1))):
+        n, cu = sum(rows), np.concatenate(([0], np.cumsum(rows)))
+        k, v = (rng.standard_normal((n, 2, dim)).astype(np.float32) for _ in range(2))
+        c.d_k.upload(pool)
+        c.d_v.upload(pool)
+        c.append_device(0, ints(be, seqs), ints(be, cu), batch, n, "f32", be.to_device(k), be.to_device(v))
+        be.synchronize()
+        want_k, want_v = pool.copy(), pool.copy()
+        last = {s: b for b, s in enumerate(seqs) if rows[b]}  # the last entry with rows
+        for s, b in last.items():
+            for i in range(rows[b]):
+                at = lens[s] - rows[b] + i
+                want_k[table[s, 0], :, at], want_v[table[s, 0], :, at] = k[cu[b] + i], v[cu[b] + i]
+        assert np.array_equal(c.d_k.download(np.float32, pool.size).reshape(pool.shape), want_k)
+        assert np.array_equal(c.d_v.download(np.float32, pool.size).reshape(pool.shape), want_v)
