@@ -458,8 +458,8 @@ int32_t objeta_hip_kv_append_device(objeta_hip_context* ctx, objeta_hip_stream s
         OBJ_FAIL(kInvalidInput, action, "dtype must be F32, F16 or BF16");
     if (n_q_heads > 65535) OBJ_FAIL(kInvalidInput, action, "n_q_heads must be 0 to 65535");
     if (n_rows >= (uint64_t(1) << 31) || n_batch >= (uint64_t(1) << 31)) OBJ_FAIL(kInvalidInput, action, "too many rows");
-    if (n_rows == 0 || n_batch == 0) return 0;
-    if (!d_seqs || !d_cu_rows) OBJ_FAIL(kInvalidInput, action, "sequences or cu_rows are NULL");
+    if (n_rows == 0 || (n_batch == 0 && n_q_heads == 0)) return 0;
+    if (n_batch && (!d_seqs || !d_cu_rows)) OBJ_FAIL(kInvalidInput, action, "sequences or cu_rows are NULL");
     if (rope && !d_positions) OBJ_FAIL(kInvalidInput, action, "positions are NULL");
     const uint64_t in = dtype_size(dtype);
     OBJ_TRY(check_tensor(action, "k", d_k, n_rows, k_stride, nk, dim, in));
@@ -485,16 +485,19 @@ int32_t objeta_hip_kv_append_device(objeta_hip_context* ctx, objeta_hip_stream s
     RopeArgs a{};
     set_rope(a, rope);
     a.pos = d_positions;
-    a.nq = static_cast<uint32_t>(n_q_heads), a.nk = a.nv = cache->n_kv_heads;
+    a.nq = static_cast<uint32_t>(n_q_heads);
     a.dim = cache->head_dim;
     if (n_q_heads) a.q = d_q, a.q_out = d_q_out, a.q_stride = q_stride, a.q_out_stride = q_out_stride;
-    a.k = d_k, a.k_stride = k_stride, a.v = d_v, a.v_stride = v_stride;
     a.q_out_type = n_q_heads ? q_out_dtype : dtype;
     a.k_out_type = cache->dtype;
-    a.ck = cache->k, a.cv = cache->v;
-    a.layer_off = layer * cache->n_pages * nk * cache->page_size * dim;
-    a.kv = kv_view(*cache);
-    a.seqs = d_seqs, a.cu = d_cu_rows, a.n_batch = static_cast<uint32_t>(n_batch);
+    if (n_batch) {  // without entries the keys and values are nobody's: queries alone
+        a.nk = a.nv = cache->n_kv_heads;
+        a.k = d_k, a.k_stride = k_stride, a.v = d_v, a.v_stride = v_stride;
+        a.ck = cache->k, a.cv = cache->v;
+        a.layer_off = layer * cache->n_pages * nk * cache->page_size * dim;
+        a.kv = kv_view(*cache);
+        a.seqs = d_seqs, a.cu = d_cu_rows, a.n_batch = static_cast<uint32_t>(n_batch);
+    }
     a.err = ctx->err_word;
     return launch_rope(resolve_stream(ctx, stream), dtype, n_rows, a, action);
     OBJ_GUARD_END

@@ -75,3 +75,26 @@ def test_append_with_empty_entries_of_named_sequences(backend, att, batch, dim):
                 want_k[table[s, 0], :, at], want_v[table[s, 0], :, at] = k[cu[b] + i], v[cu[b] + i]
         assert np.array_equal(c.d_k.download(np.float32, pool.size).reshape(pool.shape), want_k)
         assert np.array_equal(c.d_v.download(np.float32, pool.size).reshape(pool.shape), want_v)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rotated", [True, False])
+def test_append_of_no_entries_rotates_queries(backend, att, dtype, rotated):
+    """Queries of every row are written, also where no entry names any."""
+    rng, n, nq, dim = np.random.default_rng(41), 5, 3, 32
+    c = KvCache(backend, 1, 2, 1, 8, dim, 1, 2, dtype="f16")
+    pool = rng.standard_normal((2, 8, dim)).astype(np.float16)
+    c.d_k.upload(pool)
+    c.d_v.upload(pool)
+    q, k = (to_type(rng.standard_normal((n, h, dim)), dtype) for h in (nq, 1))
+    pos = np.arange(n, dtype=np.int32) + 900
+    out, d_k = backend.to_device(to_type(np.full(q.shape, FILL), dtype)), backend.to_device(k)
+    c.append_device(0, None, None, 0, n, dtype, d_k, d_k, rope=Rope(dim) if rotated else None, d_positions=ints(backend, pos),
+                    d_q=backend.to_device(q), d_q_out=out, n_q_heads=nq)
+    backend.synchronize()
+    q64 = from_type(q, dtype)
+    want = rotate(q64, pos, frequencies(dim, 10000.0), "half") if rotated else q64
+    bound = rotate_bound(q64, dim, "half", dtype, 1.0, want) + 905 * 3e-15 * 10 if rotated else 0
+    assert np.all(np.abs(download(out, dtype, q.shape) - want) <= bound)
+    for d in (c.d_k, c.d_v):
+        assert np.array_equal(d.download(np.float16, pool.size).reshape(pool.shape), pool)
