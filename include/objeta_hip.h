@@ -924,10 +924,10 @@ typedef struct {
  * become the last slots of the sequence: objeta_hip_kv_extend_device has made room for
  * them. With `rope`, keys are rotated by d_positions[row] first (a draft's position need
  * not be its slot); with d_q also queries, q [n_rows][n_q_heads][head_dim] to q_out
- * (q_out_dtype; in place as for objeta_hip_rope_device), in the same launch. A sequence
- * that the batch names twice takes the rows of its last entry that has any. Keys and values of no entry, or
- * whose slot has no page (bit 2), are not written; queries of every row are. Sources may
- * not overlap the cache. */
+ * (q_out_dtype; in place as for objeta_hip_rope_device; n_q_heads 0: none, and d_q and
+ * d_q_out NULL), in the same launch. A sequence that the batch names twice takes the rows
+ * of its last entry that has any. Keys and values of no entry, or whose slot has no page
+ * (bit 2), are not written; queries of every row are. Sources may not overlap the cache. */
 int32_t objeta_hip_kv_append_device(objeta_hip_context* ctx, objeta_hip_stream stream, const objeta_hip_kv_cache* cache,
                                     uint64_t layer, const int32_t* d_seqs, const int32_t* d_cu_rows, uint64_t n_batch,
                                     uint64_t n_rows, int32_t dtype, const void* d_k, uint64_t k_stride, const void* d_v,

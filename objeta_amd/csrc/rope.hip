@@ -457,6 +457,7 @@ int32_t objeta_hip_kv_append_device(objeta_hip_context* ctx, objeta_hip_stream s
     if (!dtype_ok(dtype) || (n_q_heads && !dtype_ok(q_out_dtype)))
         OBJ_FAIL(kInvalidInput, action, "dtype must be F32, F16 or BF16");
     if (n_q_heads > 65535) OBJ_FAIL(kInvalidInput, action, "n_q_heads must be 0 to 65535");
+    if (n_q_heads == 0 && (d_q || d_q_out)) OBJ_FAIL(kInvalidInput, action, "q or q_out without n_q_heads");
     if (n_rows >= (uint64_t(1) << 31) || n_batch >= (uint64_t(1) << 31)) OBJ_FAIL(kInvalidInput, action, "too many rows");
     if (n_rows == 0 || (n_batch == 0 && n_q_heads == 0)) return 0;
     if (n_batch && (!d_seqs || !d_cu_rows)) OBJ_FAIL(kInvalidInput, action, "sequences or cu_rows are NULL");

@@ -211,6 +211,12 @@ def test_append_refuses(lib, ctx, kw, text):
     refused(lib, call_append(lib, ctx, **kw), INVALID, text)
 
 
+@pytest.mark.parametrize("kw", [{"nq": 0}, {"nq": 0, "q": None}, {"nq": 0, "qo": None}, {"nq": 0, "rows": 0}])
+def test_append_refuses_queries_without_heads(lib, ctx, kw):
+    """Queries that would be left as they are without a word: their count was forgotten."""
+    refused(lib, call_append(lib, ctx, **kw), INVALID, "without n_q_heads")
+
+
 @pytest.mark.parametrize("kw,text", [
     ({"layer": 2}, "out of bounds"), ({"dtype": 9}, "dtype"), ({"nq": 3}, "multiple"), ({"scale": 0.0}, "scale"), ({"batch": 65536}, "65535"),
     ({"seqs": None}, "sequences"), ({"mr": 0}, "max_rows"), ({"ml": 0}, "max_len"), ({"q": A + 4}, "16-byte"), ({"os": 508}, "stride"),
