@@ -48,7 +48,7 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
     uint32_t part = 0;
     bool usable = true, last_part = true;
     if constexpr (PAGED) {
-        const BlockItem item(a, blockIdx.x, 256 * (QT == kDtF32 ? 1 : B::kPerCu));
+        const BlockItem item(a, a.first + blockIdx.x, 256 * (QT == kDtF32 ? 1 : B::kPerCu));
         if (!item.any) return;
         split = item.split, tile = item.tile, head = item.head;
         row0 = item.row0, n_q = item.n_q, len = item.len;
@@ -65,8 +65,8 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
         kv.v = static_cast<const typename M::kelem*>(a.v) + off;
     } else {
         // the last tiles see the most keys: they start first
-        const uint32_t piece = blockIdx.x / a.n_kv;
-        head = blockIdx.x % a.n_kv;
+        const uint32_t id = a.first + blockIdx.x, piece = id / a.n_kv;
+        head = id % a.n_kv;
         split = piece % a.n_splits;
         tile = a.n_tiles - 1 - piece / a.n_splits;
         kv.k = static_cast<const typename M::kelem*>(a.k) + static_cast<uint64_t>(head) * a.dim;

@@ -11,11 +11,7 @@ namespace {
 template <int Q, int K, int DT>
 int32_t launch(hipStream_t s, const AttnArgs& a, const char* action) {
     const uint64_t groups = static_cast<uint64_t>(a.n_splits) * a.n_batch * a.n_kv;
-    const uint64_t x = groups * a.n_tiles;
-    if (x > 0x7FFFFFFFull) OBJ_FAIL(kInvalidInput, action, "too many workgroups for one launch");
-    hipLaunchKernelGGL((attn_block_kernel<Q, block_type<K, DT>, DT, true>), dim3(static_cast<uint32_t>(x)), dim3(256), 0, s, a);
-    OBJ_HIP(hipGetLastError(), action);
-    return 0;
+    return launch_groups(attn_block_kernel<Q, block_type<K, DT>, DT, true>, groups * a.n_tiles, 256, s, a, action);
 }
 
 template <int Q, int K>

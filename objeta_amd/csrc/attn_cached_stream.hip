@@ -11,12 +11,8 @@ namespace {
 template <int Q, int K, int DT, int ROWS, bool WIDE>
 int32_t launch(hipStream_t s, const AttnArgs& a, const char* action) {
     const uint64_t groups = static_cast<uint64_t>(a.n_splits) * a.n_batch * a.n_kv;
-    const uint64_t x = (groups + 7) / 8 * 8;
-    if (x > 0x7FFFFFFFull) OBJ_FAIL(kInvalidInput, action, "too many workgroups for one launch");
-    hipLaunchKernelGGL((attn_stream_kernel<Q, K, DT, ROWS, WIDE>), dim3(static_cast<uint32_t>(x)),
-                       dim3(64 * Stream<K, DT, ROWS, WIDE>::kWaves), 0, s, a);
-    OBJ_HIP(hipGetLastError(), action);
-    return 0;
+    return launch_groups(attn_stream_kernel<Q, K, DT, ROWS, WIDE>, (groups + 7) / 8 * 8, 64 * Stream<K, DT, ROWS, WIDE>::kWaves, s, a,
+                         action);
 }
 
 template <int Q, int K, int ROWS, bool WIDE>

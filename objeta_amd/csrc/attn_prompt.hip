@@ -48,8 +48,8 @@ int32_t launch_prompt(objeta_hip_context* ctx, hipStream_t s, AttnArgs& a, const
     a.n_splits = prompt_splits<T, DT>(a);
     if (a.n_splits > room) a.n_splits = static_cast<uint32_t>(room);
     if (a.n_splits > 1) OBJ_TRY(attn_parts(ctx, s, a));
-    hipLaunchKernelGGL((attn_block_kernel<T, block_type<T, DT>, DT, false>), dim3(a.n_tiles * a.n_splits * a.n_kv), dim3(256), 0, s, a);
-    OBJ_HIP(hipGetLastError(), action);
+    const uint64_t groups = static_cast<uint64_t>(a.n_tiles) * a.n_splits * a.n_kv;
+    OBJ_TRY(launch_groups(attn_block_kernel<T, block_type<T, DT>, DT, false>, groups, 256, s, a, action));
     return a.n_splits > 1 ? launch_attn_join(s, T, false, a, action) : 0;
 }
 

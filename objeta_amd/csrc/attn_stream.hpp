@@ -45,7 +45,7 @@ __global__ __launch_bounds__((64 * Stream<KT, DT, ROWS, WIDE>::kWaves),
     __shared__ int32_t sh_bad;
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane / ROWS, mine = lane % ROWS;
-    const StreamItem item(a, blockIdx.x);
+    const StreamItem item(a, a.first + blockIdx.x);
     if (!item.any) return;
     const uint32_t split = item.split, head = item.head, b = item.b, tile = 0;
     const int32_t row0 = a.cu[b], end = a.cu[b + 1], n_q = end - row0;

@@ -477,6 +477,7 @@ struct AttnArgs {
     // tile of rows in n_splits equal ones. pick: the kernel takes a chunk that fills the card,
     // and leaves it in *picked for the join. wide: workgroups of twice the waves.
     uint32_t chunk, n_splits, n_tiles, tile_rows, pick, wide;
+    uint32_t first;  // the launch's first workgroup
     uint32_t* picked;
     float *part, *part_ml;  // [n_splits][n_rows * n_heads][dim], [..][2]
     uint32_t* err;

@@ -17,6 +17,11 @@ constexpr uint64_t kMaxHeadDim = 256;
 constexpr uint64_t kMaxPageOps = 1024;  // entries of one page operation
 constexpr uint64_t kMaxTokens = 0x7FFF0000u;  // of a sequence: 32-bit sums of a key's index and a tile's keys stay below 2^31
 
+// Workgroups of one launch: a grid of 2^32 threads and more in a dimension runs fewer workgroups
+// than asked for, without an error. More go in several launches, each told its first one; a
+// multiple of the XCDs.
+constexpr uint64_t kMostGroups = uint64_t(1) << 22;
+
 inline bool dtype_ok(int32_t t) { return t == kDtF32 || t == kDtF16 || t == kDtBF16; }
 inline uint64_t dtype_size(int32_t t) { return t == kDtF32 ? 4 : 2; }
 inline bool head_dim_ok(uint64_t d) { return d >= 8 && d <= kMaxHeadDim && d % 8 == 0; }

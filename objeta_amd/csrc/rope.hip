@@ -34,7 +34,7 @@ struct RopeArgs {
     uint64_t layer_off;  // elements
     KvView kv;
     const int32_t *seqs, *cu;
-    uint32_t n_batch;
+    uint32_t n_batch, first;  // first: the launch's first token
     uint32_t* err;
 };
 
@@ -105,7 +105,7 @@ __device__ __forceinline__ void cos_sin(uint64_t place, float& c, float& s) {
 
 template <int IN, bool VEC>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
-    const uint64_t t = blockIdx.x;
+    const uint64_t t = static_cast<uint64_t>(a.first) + blockIdx.x;
     const uint32_t rotated = (a.half + 3) >> 2;                      // units of four pairs
     const uint32_t tail = a.dim - 2 * a.half, copied = (tail + 7) >> 3;  // units of eight elements
     uint32_t units = rotated + copied;
@@ -309,7 +309,7 @@ void launch_typed(hipStream_t s, int32_t dtype, dim3 grid, const RopeArgs& a) {
     else hipLaunchKernelGGL((rope_kernel<kDtBF16, VEC>), grid, dim3(256), 0, s, a);
 }
 
-int32_t launch_rope(hipStream_t s, int32_t dtype, uint64_t n_tokens, const RopeArgs& a, const char* action) {
+int32_t launch_rope(hipStream_t s, int32_t dtype, uint64_t n_tokens, RopeArgs& a, const char* action) {
     const uint64_t in = dtype_size(dtype), qo = dtype_size(a.q_out_type), ko = dtype_size(a.k_out_type);
     // four elements at once where every row starts on their boundary and the parts are whole
     bool vec = a.half % 4 == 0;
@@ -323,10 +323,14 @@ int32_t launch_rope(hipStream_t s, int32_t dtype, uint64_t n_tokens, const RopeA
     const uint32_t units = a.nv && rotated + tail < a.dim / 8 ? a.dim / 8 : rotated + tail;
     const uint64_t turns = (a.nq + a.nk + a.nv + 256 / units - 1) / (256 / units), room = 1024 / n_tokens;
     const uint64_t y = room < 1 ? 1 : (room < turns ? room : turns);
-    const dim3 grid(static_cast<uint32_t>(n_tokens), static_cast<uint32_t>(y));
-    if (vec) launch_typed<true>(s, dtype, grid, a);
-    else launch_typed<false>(s, dtype, grid, a);
-    OBJ_HIP(hipGetLastError(), action);
+    for (uint64_t first = 0; first < n_tokens; first += kMostGroups) {
+        const uint64_t n = n_tokens - first < kMostGroups ? n_tokens - first : kMostGroups;
+        const dim3 grid(static_cast<uint32_t>(n), static_cast<uint32_t>(y));
+        a.first = static_cast<uint32_t>(first);
+        if (vec) launch_typed<true>(s, dtype, grid, a);
+        else launch_typed<false>(s, dtype, grid, a);
+        OBJ_HIP(hipGetLastError(), action);
+    }
     return 0;
 }
 

@@ -98,3 +98,67 @@ def test_append_of_no_entries_rotates_queries(backend, att, dtype, rotated):
     assert np.all(np.abs(download(out, dtype, q.shape) - want) <= bound)
     for d in (c.d_k, c.d_v):
         assert np.array_equal(d.download(np.float16, pool.size).reshape(pool.shape), pool)
+
+
+MANY = (1 << 24) + 5  # tokens: a workgroup of 256 threads each is past 2^32 threads
+
+
+def places_of(n):
+    """Rows at the ends and around where a launch may end."""
+    at = {0, 1, n - 1, n - 2, n // 2}
+    for p in (1 << 20, 1 << 22, 1 << 23, 1 << 24):
+        at |= {p - 1, p, p + 1}
+    return sorted(x for x in at if 0 <= x < n)
+
+
+def test_rope_of_more_tokens_than_a_launch_holds(backend, att):
+    rng, dim = np.random.default_rng(45), 8
+    x = np.resize(rng.standard_normal((4099, dim)).astype(np.float16), (MANY, dim))
+    pos = np.arange(MANY, dtype=np.int32)
+    d = backend.to_device(x)
+    att.rope_device(Rope(dim), backend.to_device(pos), MANY, dim, d, d, 1, dtype="f16")
+    backend.synchronize()
+    at = places_of(MANY)
+    got = np.stack([d.download(np.float16, dim, offset=p * dim * 2) for p in at]).astype(np.float64)[:, None]
+    x64 = x[at].astype(np.float64)[:, None]
+    want = rotate(x64, pos[at], frequencies(dim, 10000.0), "half")
+    assert np.all(np.abs(got - want) <= rotate_bound(x64, dim, "half", "f16", 1.0, want) + MANY * 3e-15 * 10)
+
+
+def test_append_of_more_tokens_than_a_launch_holds(backend, att):
+    rng, dim, page = np.random.default_rng(46), 8, 256
+    x = np.resize(rng.standard_normal((4099, 1, dim)).astype(np.float16), (MANY, 1, dim))
+    n_pages = -(-MANY // page)
+    c = KvCache(backend, 1, n_pages + 1, 1, page, dim, 2, n_pages, dtype="f16")
+    c.d_page_table.upload(np.arange(n_pages + 1, dtype=np.int32))  # the second sequence's one page behind the first's
+    c.d_seq_lens.upload(np.array([MANY - 3, 2], np.int32))
+    d = backend.to_device(x)
+    c.append_device(0, ints(backend, [0, 1]), ints(backend, [0, MANY - 3, MANY - 1]), 2, MANY, "f16", d, d)  # the last row is nobody's
+    backend.synchronize()
+    for p in (p for p in places_of(MANY) if p < MANY - 1):
+        slot = p if p < MANY - 3 else n_pages * page + p - (MANY - 3)
+        for pool in (c.d_k, c.d_v):
+            assert np.array_equal(pool.download(np.float16, dim, offset=slot * dim * 2), x[p, 0]), p
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_cached_more_workgroups_than_a_launch_holds(backend, att, rows):
+    """65535 entries over 300 key/value heads, nearly all of them empty."""
+    batch, heads, dim = 65535, 300, 8
+    c = Cached(backend, [50, 41], "f16", heads, 8, dim, seed=47)
+    seqs = np.zeros(batch, np.int32)
+    counts = np.zeros(batch, np.int64)
+    seqs[-1], seqs[70] = 1, 1
+    counts[0], counts[70], counts[-1] = rows, 1, rows
+    cu = np.concatenate(([0], np.cumsum(counts)))
+    n = int(cu[-1])
+    q = to_type(np.random.default_rng(48).standard_normal((n, heads, dim)), "f16")
+    out = backend.to_device(np.full(q.shape, FILL, np.float16))
+    lse = backend.to_device(np.full((n, heads), FILL, np.float32))
+    att.cached_device(c.cache, 0, backend.to_device(seqs), ints(backend, cu), batch, n, rows, 50, "f16", backend.to_device(q), out, heads,
+                      d_lse=lse)
+    backend.synchronize()
+    got, l = download(out, "f16", q.shape), lse.download(np.float32, n * heads).reshape(n, heads).astype(np.float64)
+    for b in (0, 70, batch - 1):
+        lo, hi = cu[b], cu[b + 1]
+        check_cached(c, [seqs[b]], q[lo:hi], got[lo:hi], l[lo:hi], [0, hi - lo], "f16", heads)
