@@ -91,13 +91,7 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
         }
     } else {
         if (real) {
-            // the sequence that holds token i: the first whose end is past i
-            uint32_t lo = 0, hi = a.n_batch;
-            while (lo < hi) {
-                const uint32_t mid = (lo + hi) >> 1;
-                if (a.cu[mid + 1] <= static_cast<int32_t>(i)) lo = mid + 1;
-                else hi = mid;
-            }
+            const uint32_t lo = first_unended(a.n_batch, [&](uint32_t x) { return a.cu[x + 1] <= static_cast<int32_t>(i); });
             int32_t s = 0, e = 0;
             if (lo < a.n_batch) s = a.cu[lo], e = a.cu[lo + 1];
             const bool in = lo < a.n_batch && s <= static_cast<int32_t>(i) && static_cast<int32_t>(i) < e;

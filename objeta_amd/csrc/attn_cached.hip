@@ -23,19 +23,21 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     const uint32_t slot = tid % (64 * WAVES), part = slot / LANES, x = slot % LANES * 4;
     bool any = row < a.n_rows;
     uint32_t n = 0, at_row = 0;
-    if (any) {
-        const RowEntry<false> entry(a.cu, PAGED ? a.seqs : nullptr, a.n_batch, row);
-        any = entry.any && entry.lo >= 0 && static_cast<uint32_t>(entry.hi) <= a.n_rows;
+    if constexpr (PAGED) {
         if (any) {
-            n = a.n_splits;
-            if constexpr (PAGED) {
+            const RowEntry<false> entry(a.cu, a.seqs, a.n_batch, row);
+            any = entry.any && entry.lo >= 0 && static_cast<uint32_t>(entry.hi) <= a.n_rows;
+            if (any) {
                 const int32_t rows = entry.hi - entry.lo;
                 int32_t len = seq_ok(a.kv, entry.seq) ? a.kv.lens[entry.seq] : 0;
                 if (!len_ok(a.kv, len) || rows > len || (a.tree && rows > 64)) len = 0;
                 n = splits_of(len, a.picked ? *a.picked : a.chunk, a.n_splits);
+                at_row = row - static_cast<uint32_t>(entry.lo);
             }
-            at_row = row - static_cast<uint32_t>(entry.lo);
         }
+    } else {
+        any = any && TokenRange(a.cu, a.n_batch, a.n_rows, static_cast<int32_t>(row)).any;
+        if (any) n = a.n_splits;
     }
     const uint64_t step = static_cast<uint64_t>(a.n_rows) * a.n_heads;
     f32x4 v[4], o = {0.0f, 0.0f, 0.0f, 0.0f};

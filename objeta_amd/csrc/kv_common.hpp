@@ -83,10 +83,46 @@ __device__ __forceinline__ uint32_t count_le(const int32_t* __restrict__ cu, uin
     return c;
 }
 
+// The sequence of packed prompts that holds a token: the first of n whose end is past it, where
+// `ended(b)` tells that sequence b's is not. The attention kernel and the join of its parts ask the
+// same questions, so that they agree where the indices are in no order too.
+template <class Ended>
+__device__ __forceinline__ uint32_t first_unended(uint32_t n, Ended ended) {
+    uint32_t lo = 0, hi = n;
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (ended(mid)) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// That sequence's tokens [lo, hi), found for token r by a whole wave; up to 63 sequences lie in the
+// lanes after one read. `any`: it holds r, and its tokens are among the n_rows.
+struct TokenRange {
+    int32_t lo, hi;
+    bool any;
+    __device__ __forceinline__ TokenRange(const int32_t* __restrict__ cu, uint32_t n, uint32_t n_rows, int32_t r) {
+        const uint32_t lane = threadIdx.x & 63;
+        uint32_t b;
+        lo = hi = 0;
+        if (n < 64) {
+            const int32_t start = cu[lane <= n ? lane : n];
+            const uint64_t past = __ballot(start <= r) >> 1;
+            b = first_unended(n, [&](uint32_t x) { return (past >> x & 1) != 0; });
+            if (b < n) lo = __builtin_amdgcn_readlane(start, b), hi = __builtin_amdgcn_readlane(start, b + 1);
+        } else {
+            b = first_unended(n, [&](uint32_t x) { return cu[x + 1] <= r; });
+            if (b < n) lo = cu[b], hi = cu[b + 1];
+        }
+        any = b < n && 0 <= lo && lo <= r && r < hi && static_cast<uint32_t>(hi) <= n_rows;
+    }
+};
+
 // The batch entry that holds row r, found by a whole wave. `any`: there is one; `again` (where
-// LATER): a later entry that has rows names the same sequence. seqs may be NULL. Up to 63 entries
-// lie in the lanes after one read, since such reads are what small kernels wait for (a join of 32
-// rows: 4.4 us, with a search and reads of its own for the entry's bounds 4.9).
+// LATER): a later entry that has rows names the same sequence. Up to 63 entries lie in the lanes
+// after one read, since such reads are what small kernels wait for (a join of 32 rows: 4.4 us, with
+// a search and reads of its own for the entry's bounds 4.9).
 template <bool LATER>
 struct RowEntry {
     int32_t lo, hi, seq;
@@ -97,7 +133,7 @@ struct RowEntry {
         uint32_t b;
         lo = hi = 0, seq = -1, again = false;
         if (n_batch < 64) {
-            const int32_t start = cu[lane <= n_batch ? lane : n_batch], s = seqs ? seqs[lane < n_batch ? lane : n_batch - 1] : -1;
+            const int32_t start = cu[lane <= n_batch ? lane : n_batch], s = seqs[lane < n_batch ? lane : n_batch - 1];
             int32_t end = 0;  // read beside the starts, so that no wait is added
             if (LATER) end = cu[lane < n_batch ? lane + 1 : n_batch];
             const uint32_t le = __popcll(__ballot(lane <= n_batch && start <= r));
@@ -112,7 +148,7 @@ struct RowEntry {
             any = le != 0 && le <= n_batch;
             if (!any) return;
             b = le - 1;
-            lo = cu[b], hi = cu[le], seq = seqs ? seqs[b] : -1;
+            lo = cu[b], hi = cu[le], seq = seqs[b];
             for (uint32_t i = b + 1; LATER && i < n_batch; i += 64)
                 again |= __ballot(i + lane < n_batch && seqs[i + lane] == seq && cu[i + lane + 1] > cu[i + lane]) != 0;
         }

@@ -100,6 +100,52 @@ def test_append_of_no_entries_rotates_queries(backend, att, dtype, rotated):
         assert np.array_equal(d.download(np.float16, pool.size).reshape(pool.shape), pool)
 
 
+def sequence_of(cu, i):
+    """The sequence that holds token i: the first, by bisection, whose end is past it."""
+    lo, hi = 0, len(cu) - 1
+    while lo < hi:
+        mid = (lo + hi) // 2
+        if cu[mid + 1] <= i:
+            lo = mid + 1
+        else:
+            hi = mid
+    return lo if lo < len(cu) - 1 and cu[lo] <= i < cu[lo + 1] else None
+
+
+@pytest.mark.parametrize("n,heads,dim", [(6000, 1, 64), (40, 1, 64)])  # in parts, and whole
+@pytest.mark.parametrize("cu", [[1, 0, 1, 0, 6001], [-2, 0, -1, 0, 39], [5, 2, 30, 10, 38], [0, 30, 10, 20, 35],
+                                [0, 7, 3, 1, 20, 2, 30, 33, 12], [9, 1, 5, 2, 7], [0, 5, -3, 10, 20, 30], [2, 1] * 40 + [0, 33],
+                                [0, 39] + [12] * 70 + [30, 8] * 3])
+def test_prompt_indices_out_of_order(backend, n, heads, dim, cu):
+    """Rows that belong to no sequence are left as they were, whether the keys are cut over workgroups
+    or not, and whatever an earlier call left behind."""
+    att, err = AttentionBackend(backend), MoeExecutor(backend)
+    rng = np.random.default_rng(44)
+    q = to_type(rng.standard_normal((n, heads, dim)), "bf16")
+    d = backend.to_device(q)
+
+    def call(cu):
+        out = backend.to_device(to_type(np.full(q.shape, FILL), "bf16"))
+        lse = backend.to_device(np.full((n, heads), FILL, np.float32))
+        att.prompt_device("bf16", d, d, d, out, heads, heads, dim, n, ints(backend, cu), len(cu) - 1, causal=False, d_lse=lse)
+        backend.synchronize()
+        return download(out, "bf16", q.shape), lse.download(np.float32, n * heads)
+    call(np.linspace(0, n, 5).astype(int))
+    err.device_error()
+    got, lse = call(cu)
+    of = [sequence_of(cu, i) for i in range(n)]
+    real = [i for i in range(n) if of[i] is not None and cu[of[i]] >= 0 and cu[of[i] + 1] <= n]
+    touched = [i for i in range(n) if not np.all(got[i] == FILL)]
+    assert touched == real and [i for i in range(n) if lse[i] != FILL] == real
+    assert err.device_error() == (4 if any(of[i] is not None for i in set(range(n)) - set(real)) else 0)
+    x = from_type(q, "bf16")[:, 0]
+    for s in sorted({of[i] for i in real}):
+        lo, hi = cu[s], cu[s + 1]
+        mine = [i for i in real if of[i] == s]
+        want, _, bound = attend(x[mine], x[lo:hi], x[lo:hi], np.ones((len(mine), hi - lo), bool), 0.125, "bf16", "bf16")
+        assert np.all(np.abs(got[mine, 0] - want) <= bound)
+
+
 MANY = (1 << 24) + 5  # tokens: a workgroup of 256 threads each is past 2^32 threads
 
 
