@@ -545,6 +545,14 @@ struct BlockItem {
         uint32_t chunk = a.chunk;
         const bool first = id == 0;
         any = false;
+        if (first && a.n_batch > 64) {  // it finds its piece early: row ranges behind are its to check too
+            bool bad = false;
+            for (uint32_t b = 64 + threadIdx.x; b < a.n_batch; b += blockDim.x) {
+                const int32_t lo = a.cu[b], hi = a.cu[b + 1];
+                bad |= lo < 0 || hi < lo || static_cast<uint32_t>(hi) > a.n_rows;
+            }
+            if (bad) atomicOr(a.err, kErrIndex);
+        }
         for (uint32_t b0 = 0; b0 < a.n_batch; b0 += 64) {
             const uint32_t b = b0 + lane;
             int32_t lo = 0, n = 0, s = 0, l = 0;

@@ -100,6 +100,33 @@ def test_append_of_no_entries_rotates_queries(backend, att, dtype, rotated):
         assert np.array_equal(d.download(np.float16, pool.size).reshape(pool.shape), pool)
 
 
+@pytest.mark.parametrize("rows,long", [(40, False), (40, True), (2, False), (2, True)])
+@pytest.mark.parametrize("at,value", [(0, -1), (1, 1 << 20), (63, 1 << 20), (64, -4), (65, 1 << 30), (100, 1 << 20), (129, -1), (130, 1 << 20)])
+def test_cached_bad_row_indices_anywhere_are_reported(backend, rows, long, at, value):
+    """A row index out of range, in any place of a batch past a wave's lanes, sets the bit; the entries
+    ahead of it are computed."""
+    att, err = AttentionBackend(backend), MoeExecutor(backend)
+    err.device_error()
+    c = Cached(backend, [3000 if long else 90, 60], "f16", 1, 16, 64, seed=42)
+    seqs = [b % 2 for b in range(130)]
+    cu = np.arange(131) * rows
+    n = int(cu[-1])
+    q = to_type(np.random.default_rng(43).standard_normal((n, 1, 64)), "f16")
+    bad = cu.copy()
+    bad[at] = value
+    out = backend.to_device(np.full(q.shape, FILL, np.float16))
+    lse = backend.to_device(np.full((n, 1), FILL, np.float32))
+    att.cached_device(c.cache, 0, ints(backend, seqs), ints(backend, bad), 130, n, rows, max(c.lens), "f16", backend.to_device(q), out,
+                      1, d_lse=lse)
+    backend.synchronize()
+    assert err.device_error() == 4
+    if value >= 0:  # (starts below all rows move the ones behind up by one entry)
+        got, l = download(out, "f16", q.shape), lse.download(np.float32, n).reshape(n, 1).astype(np.float64)
+        for b in {0, at // 2, at - 2} & set(range(max(at - 1, 0))):
+            lo, hi = cu[b], cu[b + 1]
+            check_cached(c, [seqs[b]], q[lo:hi], got[lo:hi], l[lo:hi], [0, rows], "f16", 1)
+
+
 def sequence_of(cu, i):
     """The sequence that holds token i: the first, by bisection, whose end is past it."""
     lo, hi = 0, len(cu) - 1
