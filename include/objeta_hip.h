@@ -947,8 +947,8 @@ int32_t objeta_hip_kv_append_device(objeta_hip_context* ctx, objeta_hip_stream s
  * sequence as the host knows it; it only decides how the work is cut, longer ones are
  * computed too. Entries whose sequence, length or pages are out of range, or that have more
  * rows than the sequence tokens, get NaN (bit 2). Row indices out of range or order set bit 2;
- * the rows that they name, and rows behind them, may be left as they were.
- * n_rows * n_q_heads <= 2^31 - 2^16; n_batch <= 65535. */
+ * what the rows that they name, and rows behind them, hold is then undefined.
+ * n_rows * n_q_heads <= 2^31 - 2^16; n_batch <= 65535, times the cache's heads below 2^31. */
 int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream stream,
                                       const objeta_hip_kv_cache* cache, uint64_t layer, const int32_t* d_seqs,
                                       const int32_t* d_cu_rows, uint64_t n_batch, uint64_t n_rows, uint64_t max_rows,

@@ -10,8 +10,11 @@ namespace {
 
 template <int Q, int K, int DT>
 int32_t launch(hipStream_t s, const AttnArgs& a, const char* action) {
-    const uint64_t groups = static_cast<uint64_t>(a.n_splits) * a.n_batch * a.n_kv;
-    return launch_groups(attn_block_kernel<Q, block_type<K, DT>, DT, true>, groups * a.n_tiles, 256, s, a, action);
+    // tiles that there can be: of every entry as many as the longest one's, and no more than all
+    // rows fill and one that is not full for every entry with rows
+    const uint64_t most = static_cast<uint64_t>(a.n_batch) * a.n_tiles, with_rows = a.n_batch < a.n_rows ? a.n_batch : a.n_rows;
+    const uint64_t full = static_cast<uint64_t>(a.n_rows) * a.group / 128 + with_rows, tiles = full < most ? full : most;
+    return launch_groups(attn_block_kernel<Q, block_type<K, DT>, DT, true>, tiles * a.n_splits * a.n_kv, 256, s, a, action);
 }
 
 template <int Q, int K>

@@ -235,3 +235,42 @@ def test_cached_more_workgroups_than_a_launch_holds(backend, att, rows):
     for b in (0, 70, batch - 1):
         lo, hi = cu[b], cu[b + 1]
         check_cached(c, [seqs[b]], q[lo:hi], got[lo:hi], l[lo:hi], [0, hi - lo], "f16", heads)
+
+
+@pytest.mark.parametrize("dtype,kv", [("bf16", "bf16"), ("f32", "f32")])
+@pytest.mark.parametrize("batch", [24, 90])
+def test_cached_chunk_beside_decode(backend, att, dtype, kv, batch):
+    """One chunk of a prompt and single tokens of other sequences, some of them long, in one call."""
+    rng = np.random.default_rng(batch)
+    lens = [2300, 9000, 6100] + rng.integers(1, 700, 9).tolist()
+    c = Cached(backend, lens, kv, 1, 16, 64, seed=49)
+    seqs = [0] + [1 + b % 11 for b in range(batch - 1)]
+    rows = [1000] + [1] * (batch - 1)
+    q, got, lse, cu = run_cached(att, c, seqs, rows, dtype, 2)
+    check_cached(c, seqs[:14] + seqs[-3:], np.concatenate([q[:1013], q[cu[-4]:cu[-1]]]), np.concatenate([got[:1013], got[cu[-4]:cu[-1]]]),
+                 np.concatenate([lse[:1013], lse[cu[-4]:cu[-1]]]), list(cu[:15]) + [1014, 1015, 1016], dtype, 2)
+
+
+def test_cached_many_entries_and_padding(backend, att):
+    """A million rows of room, of which few entries of many have some: no more workgroups are asked
+    for than there can be work for."""
+    batch, heads, dim, n = 2048, 128, 8, 1 << 20
+    c = Cached(backend, [300, 41], "f16", heads, 8, dim, seed=50)
+    seqs, counts = np.zeros(batch, np.int32), np.zeros(batch, np.int64)
+    seqs[70], counts[0], counts[70], counts[-1] = 1, 40, 35, 200
+    cu = np.concatenate(([0], np.cumsum(counts)))
+    used = int(cu[-1])
+    q = to_type(np.random.default_rng(51).standard_normal((used, heads, dim)), "f16")
+    d_q, out = backend.alloc(n * heads * dim * 2), backend.alloc(n * heads * dim * 2)
+    edge = np.full((used + 8, heads, dim), FILL, np.float16)
+    d_q.upload(q)
+    out.upload(edge)
+    lse = backend.to_device(np.full((n, heads), FILL, np.float32))
+    att.cached_device(c.cache, 0, backend.to_device(seqs), ints(backend, cu), batch, n, n, 300, "f16", d_q, out, heads, d_lse=lse)
+    backend.synchronize()
+    got = from_type(out.download(np.float16, edge.size).reshape(edge.shape), "f16")
+    l = lse.download(np.float32, n * heads).reshape(n, heads)
+    for b in (0, 70, batch - 1):
+        lo, hi = cu[b], cu[b + 1]
+        check_cached(c, [seqs[b]], q[lo:hi], got[lo:hi], l[lo:hi].astype(np.float64), [0, hi - lo], "f16", heads)
+    assert np.all(got[used:] == FILL) and np.all(l[used:] == FILL)
