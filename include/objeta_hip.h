@@ -883,7 +883,9 @@ int32_t objeta_hip_rope_device(objeta_hip_context* ctx, objeta_hip_stream stream
  * q, out [n_tokens][n_q_heads][head_dim], k, v [n_tokens][n_kv_heads][head_dim], all of
  * `dtype`; d_lse [n_tokens][n_q_heads] float, nullable. Rows of no sequence (behind the
  * last one, or under indices out of order) are left as they were. What lies in places a
- * row does not see, infinities and NaN included, does not reach it. scale > 0. Sums and
+ * row does not see, infinities and NaN included, does not reach it; rows near places that
+ * hold any are computed a second time, so that such a call takes two to five times as long
+ * (float calls whose keys or queries are infinite throughout: some 25 times). scale > 0. Sums and
  * softmax are held in float; 16-bit types round the probabilities to their type before the
  * product with v (float: not; float keys and values may be multiplied as three bf16 parts
  * each, 24 bits together, of which a value below 2^-102 loses the last). Where the tiles of
@@ -942,7 +944,8 @@ int32_t objeta_hip_kv_append_device(objeta_hip_context* ctx, objeta_hip_stream s
  * sees the slots before len - n, and
  *   without d_tree, the slots up to its own (len - n + i);
  *   with d_tree (uint64 [n_rows], n <= 64), slot len - n + j where bit j of its mask is set.
- * A row that sees nothing gets out 0 and lse -inf. d_lse as for prompts. max_rows: no entry
+ * A row that sees nothing gets out 0 and lse -inf. Infinities and NaN, and d_lse, as for
+ * prompts. max_rows: no entry
  * has more rows (any that go past it may come out NaN, with bit 2). max_len: the longest
  * sequence as the host knows it; it only decides how the work is cut, longer ones are
  * computed too. Entries whose sequence, length or pages are out of range, or that have more

@@ -8,7 +8,7 @@
 // tile but one travel in registers.
 #pragma once
 
-#include "attn_tile.hpp"
+#include "attn_careful.hpp"
 
 namespace objeta {
 namespace dev {
@@ -39,7 +39,8 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
     __shared__ alignas(16) char lds_k[2][B::kTileK], lds_v[2][B::kTileV];
     __shared__ int32_t sh_lo[4], sh_hi[4];
     __shared__ int32_t ring[4][8];  // page ids of a tile's groups of eight keys
-    __shared__ int32_t sh_bad;
+    __shared__ int32_t sh_bad;       // bit 0: a bad page; bit 1: a result that is not finite
+    __shared__ uint32_t sh_odd[3];   // second pass: keys of a tile without parts; whether values are marked
 
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
     uint32_t tile, head, split = 0;
@@ -438,41 +439,51 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
         }
     }
     const AttnArgs& e = args_again();
-    if constexpr (PAGED) {
-        if (bad) sh_bad = 1;
-        __syncthreads();
-        if (!usable || sh_bad) {
-            if (tid == 0 && sh_bad) atomicOr(e.err, kErrIndex);
-            st.l = __builtin_nanf("");
+    if (PAGED && bad) atomicOr(&sh_bad, 1);
+    if (not_finite<M>(st) && lane == 0) atomicOr(&sh_bad, 2);
+    __syncthreads();
+    const int32_t state = sh_bad;
+    if (PAGED && (!usable || (state & 1))) {
+        if (tid == 0 && (state & 1)) atomicOr(e.err, kErrIndex);
+        st.l = __builtin_nanf("");
 #pragma unroll
-            for (int d = 0; d < DT / 32; ++d)
+        for (int d = 0; d < DT / 32; ++d)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) st.o[d][r] = st.l;
-            write_rows<M, QT>(e, st, real, row, q_head, split, lane);
-            return;
+            for (int r = 0; r < 16; ++r) st.o[d][r] = st.l;
+    } else if (state) {
+        // some product met an infinity or NaN: the tiles again, one at a time (see attn_careful.hpp)
+        const auto* q_row = static_cast<const typename M::qelem*>(e.q) + row * e.q_stride + static_cast<uint64_t>(q_head) * e.dim;
+        const bool q_odd = query_without_parts<M, KT>(q_row, e.dim);
+        Specials<M> specials{};
+        st.clear();
+        for (int32_t t = 0; t < n_tiles; ++t) {
+            __syncthreads();  // the tile before is read
+            if (tid < 3) sh_odd[tid] = 0;
+            store_pages(t, load_pages(t));
+            __syncthreads();
+            load_tile(t);
+#pragma unroll
+            for (int x = 0; x < B::kLoads; ++x) {
+                const uint32_t key = x * 4 * R::kPer + wave * R::kPer + l_key;
+                store_k(0, x);
+                if (M::kParts > 1 && key_without_parts<KT>(rk[x]) != 0) atomicOr(&sh_odd[key >> 5], 1u << (key & 31));
+                u32x4a marks;
+                if (take_specials<KT>(rv[x], marks) != 0) sh_odd[2] = 1;
+                store_values<M, KT>(lds_v[0] + v_at + x * 4 * R::kPer * R::kV, rv[x]);
+                store_marks<M, KT>(lds_v[1] + v_at + x * 4 * R::kPer * R::kV, marks);
+            }
+            __syncthreads();
+#pragma unroll 1
+            for (int sub = 0; sub < kKeys / 32; ++sub) {
+                const Seen seen =
+                    careful_step<M>(st, q, q_row, q_odd, kv, view, k_begin + t * kKeys + 32 * sub, k_lo, k_end, sh_odd[sub], scale, e.dim,
+                                    lds_k[0] + k_first + sub * 32 * R::kK, lds_v[0] + v_first + sub * 32 * R::kV);
+                if (sh_odd[2]) add_specials<M>(specials, seen, lds_v[1] + v_first + sub * 32 * R::kV);
+            }
         }
+        apply_specials<M>(st, specials);
     }
-    if (not_finite<M>(st)) {
-        for (int r = 0; r < 32; ++r) {
-            if (!__builtin_amdgcn_readlane(real, r)) continue;
-            const uint32_t r_m = tile * 128 + wave * 32 + r, r_head = head * e.group + r_m % e.group;
-            const uint64_t r_row = static_cast<uint64_t>(row0) + r_m / e.group;
-            RowView rv1{__builtin_amdgcn_readlane(view.lo, r), __builtin_amdgcn_readlane(view.hi, r),
-                        __builtin_amdgcn_readlane(view.base, r), 0};
-            rv1.mask = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int32_t>(view.mask), r)) |
-                       static_cast<uint64_t>(static_cast<uint32_t>(
-                           __builtin_amdgcn_readlane(static_cast<int32_t>(view.mask >> 32), r)))
-                           << 32;
-            float rm, rl, ro[4];
-            row_by_row<M, PAGED, KT>(kv,
-                                     static_cast<const typename M::qelem*>(e.q) + r_row * e.q_stride +
-                                         static_cast<uint64_t>(r_head) * e.dim,
-                                     rv1, k_lo, k_end, e.scale_log2, e.dim, rm, rl, ro);
-            write_row<M>(e, rm, rl, ro, r_row, r_head, split, lane);
-        }
-    } else {
-        write_rows<M, QT>(e, st, real, row, q_head, split, lane);
-    }
+    write_rows<M, QT>(e, st, real, row, q_head, split, lane);
 }
 
 }  // namespace dev

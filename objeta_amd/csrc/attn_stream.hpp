@@ -8,7 +8,7 @@
 // 16 bits they would keep up with ten times the memory's rate.
 #pragma once
 
-#include "attn_tile.hpp"
+#include "attn_careful.hpp"
 
 namespace objeta {
 namespace dev {
@@ -35,7 +35,7 @@ __device__ __forceinline__ void wave_lds_fence() {
 
 template <int QT, int KT, int DT, int ROWS, bool WIDE>
 __global__ __launch_bounds__((64 * Stream<KT, DT, ROWS, WIDE>::kWaves),
-                             (ROWS == 32 ? 1 : Stream<KT, DT, ROWS, WIDE>::kPerSimd)) void attn_stream_kernel(AttnArgs a) {
+                             (ROWS == 32 ? (KT == kDtF16 && DT == 64 ? 3 : 1) : Stream<KT, DT, ROWS, WIDE>::kPerSimd)) void attn_stream_kernel(AttnArgs a) {
     typedef Math<QT, KT, DT, ROWS> M;
     typedef Rows<KT, DT, ROWS> R;
     typedef Stream<KT, DT, ROWS, WIDE> S;
@@ -168,75 +168,120 @@ __global__ __launch_bounds__((64 * Stream<KT, DT, ROWS, WIDE>::kWaves),
 
     const AttnArgs& e = args_again();
     // ---- the waves' results into one: a wave's o goes to its own part of LDS
-    st.l = row_sum<ROWS>(st.l);
-    if (h == 0) sh_m[wave][mine] = st.m, sh_l[wave][mine] = st.l;
-    __syncthreads();
-    if (bad) atomicOr(&sh_bad, 1);
-    float top = sh_m[0][mine];
+    float top, l;
+    auto meet = [&]() -> int32_t {
+        st.l = row_sum<ROWS>(st.l);
+        if (h == 0) sh_m[wave][mine] = st.m, sh_l[wave][mine] = st.l;
+        __syncthreads();
+        if (bad) atomicOr(&sh_bad, 1);
+        top = sh_m[0][mine];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, sh_m[w][mine]);
-    const float ref = top == -kInf ? 0.0f : top;
-    float l = 0.0f;
+        for (int w = 1; w < kWaves; ++w) top = __builtin_fmaxf(top, sh_m[w][mine]);
+        const float ref = top == -kInf ? 0.0f : top;
+        l = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) l += sh_l[w][mine] * exp2_hw(sh_m[w][mine] - ref);
-    const float f = exp2_hw(st.m - ref);
-    const bool odd = not_finite<M>(st);
-    if (odd && lane == 0) atomicOr(&sh_bad, 2);
-    float* o_lds = reinterpret_cast<float*>(lds[wave]);  // [dimension / 4][row][4]
+        for (int w = 0; w < kWaves; ++w) l += sh_l[w][mine] * exp2_hw(sh_m[w][mine] - ref);
+        const float f = exp2_hw(st.m - ref);
+        if (not_finite<M>(st) && lane == 0) atomicOr(&sh_bad, 2);
+        float* o_lds = reinterpret_cast<float*>(lds[wave]);  // [dimension / 4][row][4]
 #pragma unroll
-    for (int d = 0; d < M::kOut; ++d)
+        for (int d = 0; d < M::kOut; ++d)
 #pragma unroll
-        for (int r = 0; r < M::kRegs / 4; ++r)
-            *reinterpret_cast<f32x4*>(o_lds + (out_dim<M>(d, r, h) / 4 * ROWS + mine) * 4) =
-                f32x4{st.o[d][4 * r] * f, st.o[d][4 * r + 1] * f, st.o[d][4 * r + 2] * f, st.o[d][4 * r + 3] * f};
-    __syncthreads();
-    const int32_t state = sh_bad;
+            for (int r = 0; r < M::kRegs / 4; ++r)
+                *reinterpret_cast<f32x4*>(o_lds + (out_dim<M>(d, r, h) / 4 * ROWS + mine) * 4) =
+                    f32x4{st.o[d][4 * r] * f, st.o[d][4 * r + 1] * f, st.o[d][4 * r + 2] * f, st.o[d][4 * r + 3] * f};
+        __syncthreads();
+        return sh_bad;
+    };
+    const int32_t state = meet();
     if (usable && state == 2) {
-        // some product met an infinity or NaN: the rows again, key by key (see row_by_row)
-        for (uint32_t r = wave; r < ROWS; r += kWaves) {
-            const uint32_t r_m = tile * ROWS + r;
-            if (r_m >= n_m) break;
-            const uint32_t r_head = head * e.group + r_m % e.group, r_i = r_m / e.group;
-            const uint64_t r_row = static_cast<uint64_t>(row0) + r_i;
-            RowView rv1{0, base + static_cast<int32_t>(r_i), 0x7FFFFFFF, 0};
-            if (e.tree) rv1 = RowView{0, len - 1, base, e.tree[r_row]};
-            float rm, rl, ro[4];
-            row_by_row<M, true, KT>(kv,
-                                    static_cast<const typename M::qelem*>(e.q) + r_row * e.q_stride +
-                                        static_cast<uint64_t>(r_head) * e.dim,
-                                    rv1, k_lo, k_end, e.scale_log2, e.dim, rm, rl, ro);
-            write_row<M>(e, rm, rl, ro, r_row, r_head, split, lane);
-        }
-    } else {
-        if (tid == 0 && (state & 1)) atomicOr(e.err, kErrIndex);
-        const bool poison = !usable || (state & 1);
-        if (poison) l = __builtin_nanf("");
-        const float inv = e.n_splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
-        // this thread: its row, groups of four dimensions
-        for (uint32_t g = wave * (64 / ROWS) + h; g * 4 < e.dim; g += kWaves * (64 / ROWS)) {
-            f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        // some product met an infinity or NaN: the wave's tiles again, one at a time (see
+        // attn_careful.hpp). The others' parts of LDS are not read before the next meeting.
+        const auto* q_row = static_cast<const typename M::qelem*>(e.q) + row * e.q_stride + static_cast<uint64_t>(q_head) * e.dim;
+        const bool q_odd = query_without_parts<M, KT>(q_row, e.dim);
+        Specials<M> specials{};
+        st.clear();
+        for (int32_t t0 = k_lo + 32 * static_cast<int32_t>(__builtin_amdgcn_readfirstlane(wave)); t0 < k_end;
+             t0 = k_end - t0 > step ? t0 + step : k_end) {
+            const int32_t t_pages = kv.checked(load_pages(t0), bad);
+            // two units of K and V at a time, for the registers' sake
+            auto unit_of = [&](const typename M::kelem* pool, uint32_t x) {
+                const uint32_t key = x * R::kPer;
+                const int32_t left = k_end - t0 - static_cast<int32_t>(key);
+                const uint32_t bytes = left > 0 ? (left < 8 ? left : 8) * row_bytes : 0;
+                const uint64_t at = kv.paged_at(__builtin_amdgcn_readlane(t_pages, key >> 3), static_cast<uint32_t>(t0) + key);
+                return buffer_unit(buffer_of(pool + at, bytes), place);
+            };
+            uint32_t odd = 0, marked = 0;
+            wave_lds_fence();  // the tile before is read
+#pragma unroll 1
+            for (uint32_t x = 0; x < static_cast<uint32_t>(S::kLoads); x += 2) {
+                u32x4a uk[2], uv[2], marks;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w)
-                sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w]) +
-                                                       (g * ROWS + mine) * 4);
-            sum *= inv;
-            if (poison) sum = f32x4{l, l, l, l};
-            if (!real) continue;
-            if (e.n_splits > 1)
-                *reinterpret_cast<f32x4*>(e.part + part_at(e, split, row, q_head) * e.dim + 4 * g) = sum;
-            else
-                store_out<QT>(static_cast<typename M::qelem*>(e.out) + row * e.out_stride +
-                                  static_cast<uint64_t>(q_head) * e.dim + 4 * g, sum);
-        }
-        if (real && wave == 0 && h == 0) {
-            if (e.n_splits > 1) {
-                const uint64_t at = part_at(e, split, row, q_head);
-                e.part_ml[2 * at] = top - M::kShift;
-                e.part_ml[2 * at + 1] = l;
-            } else if (e.lse) {
-                e.lse[row * e.n_heads + q_head] =
-                    l == 0.0f ? -kInf : (top - M::kShift + __builtin_amdgcn_logf(l)) * kLn2;
+                for (uint32_t y = 0; y < 2; ++y) uk[y] = unit_of(kv.k, x + y), uv[y] = unit_of(kv.v, x + y);
+#pragma unroll
+                for (uint32_t y = 0; y < 2; ++y) {
+                    if constexpr (M::kParts > 1)
+                        odd |= static_cast<uint32_t>(key_without_parts<KT>(uk[y]) != 0) << ((x + y) * R::kPer + lane / R::kLanes);
+                    marked |= take_specials<KT>(uv[y], marks);
+                    *reinterpret_cast<u32x4a*>(k_lds + k_at + (x + y) * R::kPer * R::kK) = uk[y];
+                    *reinterpret_cast<u32x4a*>(v_lds + v_at + (x + y) * R::kPer * R::kV) = uv[y];
+                }
             }
+#pragma unroll
+            for (int y = 1; y < 64; y <<= 1) odd |= __shfl_xor(odd, y, 64);
+            wave_lds_fence();
+            const Seen seen = careful_step<M>(st, q, q_row, q_odd, kv, view, t0, k_lo, k_end, __builtin_amdgcn_readfirstlane(odd),
+                                              scale, e.dim, k_lds + M::k_first(lane), v_lds + M::v_first(lane));
+            if (__any(marked != 0)) {  // the values' marks in their place
+                wave_lds_fence();
+#pragma unroll 1
+                for (uint32_t x = 0; x < static_cast<uint32_t>(S::kLoads); x += 2) {
+                    u32x4a uv[2], marks;
+#pragma unroll
+                    for (uint32_t y = 0; y < 2; ++y) uv[y] = unit_of(kv.v, x + y);
+#pragma unroll
+                    for (uint32_t y = 0; y < 2; ++y) {
+                        take_specials<KT>(uv[y], marks);
+                        *reinterpret_cast<u32x4a*>(v_lds + v_at + (x + y) * R::kPer * R::kV) = marks;
+                    }
+                }
+                wave_lds_fence();
+                add_specials<M>(specials, seen, v_lds + M::v_first(lane));
+            }
+        }
+        wave_lds_fence();
+        apply_specials<M>(st, specials);
+        meet();
+    }
+    if (tid == 0 && (state & 1)) atomicOr(e.err, kErrIndex);
+    const bool poison = !usable || (state & 1);
+    if (poison) l = __builtin_nanf("");
+    const float inv = e.n_splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+    // this thread: its row, groups of four dimensions
+    for (uint32_t g = wave * (64 / ROWS) + h; g * 4 < e.dim; g += kWaves * (64 / ROWS)) {
+        f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w)
+            sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds[w]) +
+                                                   (g * ROWS + mine) * 4);
+        sum *= inv;
+        if (poison) sum = f32x4{l, l, l, l};
+        if (!real) continue;
+        if (e.n_splits > 1)
+            *reinterpret_cast<f32x4*>(e.part + part_at(e, split, row, q_head) * e.dim + 4 * g) = sum;
+        else
+            store_out<QT>(static_cast<typename M::qelem*>(e.out) + row * e.out_stride +
+                              static_cast<uint64_t>(q_head) * e.dim + 4 * g, sum);
+    }
+    if (real && wave == 0 && h == 0) {
+        if (e.n_splits > 1) {
+            const uint64_t at = part_at(e, split, row, q_head);
+            e.part_ml[2 * at] = top - M::kShift;
+            e.part_ml[2 * at + 1] = l;
+        } else if (e.lse) {
+            e.lse[row * e.n_heads + q_head] =
+                l == 0.0f ? -kInf : (top - M::kShift + __builtin_amdgcn_logf(l)) * kLn2;
         }
     }
 }

@@ -416,17 +416,17 @@ __device__ __forceinline__ void add_values(RowState<M>& st, const Weights<M>& w,
         for (int part = 0; part < M::kParts; ++part) st.o[d] = M::mma(v.f[d], w.f[part], st.o[d]);
 }
 
-// The largest score of 32 keys, scaled, over the lanes of a row; raises the reference where it
-// has outgrown it.
+// The largest score of 32 keys, scaled, over the lanes of a row; raises the reference, `lift` above
+// the largest, where that has outgrown it by more than `slack`.
 template <class M>
-__device__ __forceinline__ void take_top(RowState<M>& st, const Scores<M>& s, float scale) {
+__device__ __forceinline__ void take_top(RowState<M>& st, const Scores<M>& s, float scale, float slack = kSlack, float lift = 0.0f) {
     float top = -kInf;
 #pragma unroll
     for (int t = 0; t < M::kKeyTiles; ++t)
 #pragma unroll
         for (int r = 0; r < M::kRegs; ++r) top = __builtin_fmaxf(top, s.s[t][r]);
-    top = row_max<M::kRows>(top) * scale;
-    if (__any(top > st.m + kSlack)) st.raise(__builtin_fmaxf(st.m, top));
+    top = row_max<M::kRows>(top) * scale + lift;
+    if (__any(top > st.m + slack)) st.raise(__builtin_fmaxf(st.m, top));
 }
 
 template <class M>
@@ -672,50 +672,6 @@ __device__ __forceinline__ u32x4a buffer_unit(__amdgpu_buffer_rsrc_t r, uint32_t
 constexpr uint32_t kNowhere = 0xC0000000u;   // a lane's place past every buffer, with room for the tile's offsets
 constexpr uint64_t kMaxKvStride = 1u << 23;  // elements: 64 rows below kNowhere bytes
 
-// One row computed key by key over the keys it sees in [k0, k1), by a whole wave (a lane has
-// dimensions lane, lane + 64, ...). The matrix products multiply unseen values by a
-// probability of 0, which an infinity or NaN there turns into NaN; a wave whose result is
-// not finite comes here, where unseen places are not touched.
-template <class M, bool PAGED, int KT>
-__device__ __forceinline__ void row_by_row(const KvRows<PAGED, KT>& kv, const typename M::qelem* q, const RowView& view,
-                                           int32_t k0, int32_t k1, float scale, uint32_t dim, float& m, float& l,
-                                           float (&o)[4]) {
-    const uint32_t lane = threadIdx.x & 63;
-    float qv[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-        const uint32_t d = lane + 64 * x;
-        qv[x] = d < dim ? static_cast<float>(q[d]) : 0.0f;
-        o[x] = 0.0f;
-    }
-    m = -kInf, l = 0.0f;
-    bool bad = false;
-    for (int32_t j = k0; j < k1; ++j) {
-        if (!view.sees(j)) continue;
-        const auto* kr = kv.k_row(static_cast<uint32_t>(j), bad);
-        const auto* vr = kv.v_row(static_cast<uint32_t>(j), bad);
-        float dot = 0.0f, vv[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const uint32_t d = lane + 64 * x;
-            vv[x] = 0.0f;
-            if (d < dim) {
-                dot = __builtin_fmaf(qv[x], static_cast<float>(kr[d]), dot);
-                vv[x] = static_cast<float>(vr[d]);
-            }
-        }
-#pragma unroll
-        for (int s = 32; s > 0; s >>= 1) dot += __shfl_xor(dot, s, 64);
-        const float sc = dot * scale;
-        const float top = __builtin_fmaxf(m, sc), ref = top == -kInf ? 0.0f : top;
-        const float f = exp2_hw(m - ref), p = exp2_hw(sc - ref);
-        l = l * f + p;
-#pragma unroll
-        for (int x = 0; x < 4; ++x) o[x] = o[x] * f + p * vv[x];
-        m = top;
-    }
-}
-
 // Writes four consecutive output values.
 template <int QT>
 __device__ __forceinline__ void store_out(typename ElemOf<QT>::type* p, f32x4 v) {
@@ -767,26 +723,6 @@ __device__ __forceinline__ void write_rows(const AttnArgs& a, const RowState<M>&
         else if (a.lse)
             a.lse[row * a.n_heads + head] = l == 0.0f ? -kInf : (st.m - M::kShift + __builtin_amdgcn_logf(l)) * kLn2;
     }
-}
-
-// The same for one row of row_by_row, by a whole wave.
-template <class M>
-__device__ __forceinline__ void write_row(const AttnArgs& a, float m, float l, const float (&o)[4], uint64_t row,
-                                          uint32_t head, uint32_t split, uint32_t lane) {
-    if (a.n_splits > 1) {
-        const uint64_t at = part_at(a, split, row, head);
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-            if (lane + 64 * x < a.dim) a.part[at * a.dim + lane + 64 * x] = o[x];
-        if (lane == 0) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
-        return;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    typename M::qelem* p = static_cast<typename M::qelem*>(a.out) + row * a.out_stride + static_cast<uint64_t>(head) * a.dim;
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-        if (lane + 64 * x < a.dim) p[lane + 64 * x] = static_cast<typename M::qelem>(o[x] * inv);
-    if (a.lse && lane == 0) a.lse[row * a.n_heads + head] = l == 0.0f ? -kInf : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // Rows of an entry past what max_rows allows for (n_tiles of `rows`): NaN, reported. By the last
