@@ -454,6 +454,7 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
         // some product met an infinity or NaN: the tiles again, one at a time (see attn_careful.hpp)
         const auto* q_row = static_cast<const typename M::qelem*>(e.q) + row * e.q_stride + static_cast<uint64_t>(q_head) * e.dim;
         const bool q_odd = query_without_parts<M, KT>(q_row, e.dim);
+        const float lift = lift_of<KT>(static_cast<uint32_t>(PAGED ? len : n_q));
         Specials<M> specials{};
         st.clear();
         for (int32_t t = 0; t < n_tiles; ++t) {
@@ -476,7 +477,7 @@ __global__ __launch_bounds__(256, (QT == kDtF32 ? 1 : Block<KT, DT>::kPerCu)) vo
 #pragma unroll 1
             for (int sub = 0; sub < kKeys / 32; ++sub) {
                 const Seen seen =
-                    careful_step<M>(st, q, q_row, q_odd, kv, view, k_begin + t * kKeys + 32 * sub, k_lo, k_end, sh_odd[sub], scale, e.dim,
+                    careful_step<M>(st, q, q_row, q_odd, kv, view, k_begin + t * kKeys + 32 * sub, k_lo, k_end, sh_odd[sub], scale, lift, e.dim,
                                     lds_k[0] + k_first + sub * 32 * R::kK, lds_v[0] + v_first + sub * 32 * R::kV);
                 if (sh_odd[2]) add_specials<M>(specials, seen, lds_v[1] + v_first + sub * 32 * R::kV);
             }

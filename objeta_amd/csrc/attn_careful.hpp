@@ -6,8 +6,9 @@
 // So the second pass stages such values as zeros and marks them in a matrix of their own (1 for
 // inf, 64 for -inf, 4096 for NaN): its product with the rows' masks counts, for each row and
 // dimension, what of each kind the row sees among 32 keys, exactly. Scores of a key or a query that
-// has no parts are computed in floats, a row a lane. m is kept 32 above the largest score (values of
-// f16, whose sums have the room: at it), so that sums of large finite values stay finite too.
+// has no parts are computed in floats, a row a lane. m is kept above the largest score by the
+// logarithm of the keys' number (values of f16, whose sums have the room: at it), so that sums of
+// large finite values stay finite too, over all parts and waves.
 //
 // It walks the same tiles, one at a time; what it costs over the first pass is bounded by that, and
 // by one row's dot product a lane for each key without parts.
@@ -215,11 +216,17 @@ __device__ __forceinline__ void apply_specials(RowState<M>& st, const Specials<M
         }
 }
 
+// How far above the largest score m is kept where a row sees at most `keys` keys.
+template <int KT>
+__device__ __forceinline__ float lift_of(uint32_t keys) {
+    return KT == kDtF16 || keys == 0 ? 0.0f : static_cast<float>(32 - __builtin_clz(keys));
+}
+
 // 32 keys of the second pass: `k` and `v` are their staged rows plus k_first and v_first.
 template <class M, bool PAGED, int KT>
 __device__ __forceinline__ Seen careful_step(RowState<M>& st, const typename M::Query& q, const typename M::qelem* q_row, bool q_odd,
                                              const KvRows<PAGED, KT>& kv, const RowView& view, int32_t key0, int32_t k_lo,
-                                             int32_t k_end, uint32_t odd, float scale, uint32_t dim, const char* k, const char* v) {
+                                             int32_t k_end, uint32_t odd, float scale, float lift, uint32_t dim, const char* k, const char* v) {
     uint32_t h = (threadIdx.x & 63) / M::kRows;
     asm volatile("" : "+v"(h));  // nothing of this pass is computed ahead of it
     Scores<M> s;
@@ -239,7 +246,7 @@ __device__ __forceinline__ Seen careful_step(RowState<M>& st, const typename M::
             if (!sees) s.s[n][r] = -kInf;
             __builtin_amdgcn_sched_barrier(0);
         }
-    take_top<M>(st, s, scale, 0.0f, KT == kDtF16 ? 0.0f : 32.0f);
+    take_top<M>(st, s, scale, 0.0f, lift);
     const float off = M::kShift - st.reference();
 #pragma unroll
     for (int g = 0; g < kGroups<M>; ++g) {

@@ -199,6 +199,7 @@ __global__ __launch_bounds__((64 * Stream<KT, DT, ROWS, WIDE>::kWaves),
         // attn_careful.hpp). The others' parts of LDS are not read before the next meeting.
         const auto* q_row = static_cast<const typename M::qelem*>(e.q) + row * e.q_stride + static_cast<uint64_t>(q_head) * e.dim;
         const bool q_odd = query_without_parts<M, KT>(q_row, e.dim);
+        const float lift = lift_of<KT>(static_cast<uint32_t>(len));
         Specials<M> specials{};
         st.clear();
         for (int32_t t0 = k_lo + 32 * static_cast<int32_t>(__builtin_amdgcn_readfirstlane(wave)); t0 < k_end;
@@ -232,7 +233,7 @@ __global__ __launch_bounds__((64 * Stream<KT, DT, ROWS, WIDE>::kWaves),
             for (int y = 1; y < 64; y <<= 1) odd |= __shfl_xor(odd, y, 64);
             wave_lds_fence();
             const Seen seen = careful_step<M>(st, q, q_row, q_odd, kv, view, t0, k_lo, k_end, __builtin_amdgcn_readfirstlane(odd),
-                                              scale, e.dim, k_lds + M::k_first(lane), v_lds + M::v_first(lane));
+                                              scale, lift, e.dim, k_lds + M::k_first(lane), v_lds + M::v_first(lane));
             if (__any(marked != 0)) {  // the values' marks in their place
                 wave_lds_fence();
 #pragma unroll 1

@@ -158,6 +158,34 @@ def test_cached_large_finite_values(backend, att, dtype, kv):
             assert np.all(np.abs(got[lo:hi, 0] - out) <= bound)
 
 
+@pytest.mark.parametrize("rows", [1, 9, 40])
+def test_cached_large_values_of_unlikely_keys(backend, att, rows):
+    """A key 2^-100 as likely as the others still counts where its value is 2^126, in a pass that was not
+    finite for another dimension's sake."""
+    n, dim = 200, 64
+    c = Cached(backend, [n], "f32", 1, 16, dim, seed=63)
+    at = np.arange(n)
+    place = (0, c.table[0, at // 16], slice(None), at % 16)
+    k, v = np.zeros((n, 1, dim), np.float32), np.random.default_rng(64).standard_normal((n, 1, dim)).astype(np.float32)
+    k[7, 0, 0] = -100 * np.log(2) * 8  # times 1/8 and a query of 1: e^-69.3 = 2^-100
+    v[7, 0, 3], v[9, 0, 5] = 2.0 ** 126, np.inf
+    c.k[place], c.v[place] = k, v
+    c.upload()
+    q = np.ones((rows + 2, 1, dim), np.float32)
+    _, got, lse, _ = run_cached(att, c, [0], [rows], "f32", 1, q=q)
+    for i in range(rows):
+        seen = n - rows + i + 1
+        s = np.zeros(seen)
+        s[7] = 0.125 * float(k[7, 0, 0])
+        p = np.exp(s)
+        want = (p @ np.where(np.isfinite(v[:seen, 0]), v[:seen, 0], 0).astype(np.float64)) / p.sum()
+        # the score's roundings (72 of its 69.3, and its logarithm's) and the sums over up to 200 keys
+        size = (p @ np.abs(np.where(np.isfinite(v[:seen, 0]), v[:seen, 0], 0)).astype(np.float64)) / p.sum()
+        bound = size * 2.0 ** -24 * (2 * (80 * 70 + 4 * 70 + seen + 16))
+        ok = np.arange(dim) != 5
+        assert np.all(np.abs(got[i, 0] - want)[ok] <= bound[ok]) and got[i, 0, 5] == np.inf
+
+
 @pytest.mark.parametrize("dtype,n,dim", [("bf16", 8192, 128), ("f16", 8192, 64), ("f32", 4096, 128), ("f32", 4096, 256)])
 @pytest.mark.parametrize("what", ["one value", "all values", "one key"])
 def test_specials_cost_a_few_passes(backend, att, dtype, n, dim, what):
