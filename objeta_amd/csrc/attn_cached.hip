@@ -180,7 +180,7 @@ int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream
     a.n_heads = static_cast<uint32_t>(n_q_heads), a.n_kv = c.n_kv_heads;
     a.group = a.n_heads / a.n_kv;
     a.dim = c.head_dim;
-    a.scale = scale, a.scale_log2 = scale * kLog2e;
+    a.scale_log2 = scale * kLog2e;
     a.kv = kv_view(c);
     a.layer_off = layer * c.n_pages * c.n_kv_heads * c.page_size * dim;
     a.err = ctx->err_word;

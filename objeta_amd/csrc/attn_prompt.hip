@@ -143,7 +143,7 @@ int32_t objeta_hip_attn_prompt_device(objeta_hip_context* ctx, objeta_hip_stream
     a.n_heads = static_cast<uint32_t>(n_q_heads), a.n_kv = static_cast<uint32_t>(n_kv_heads);
     a.group = a.n_heads / a.n_kv;
     a.dim = static_cast<uint32_t>(head_dim);
-    a.scale = scale, a.scale_log2 = scale * kLog2e;
+    a.scale_log2 = scale * kLog2e;
     a.causal = causal;
     a.n_tiles = static_cast<uint32_t>((n_tokens * a.group + 127) / 128);
     a.err = ctx->err_word;

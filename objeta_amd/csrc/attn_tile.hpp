@@ -99,7 +99,6 @@ struct Math {
     static constexpr int kStep = 8 * (64 / ROWS);       // dimensions (keys) of one product
     static constexpr int kSteps = DT / kStep;
     static constexpr int kOut = DT / ROWS;              // accumulators of o
-    static constexpr int kDim = DT;
     static constexpr bool kFloat = KT == kDtF32;
     static constexpr int kParts = QT == KT ? 1 : (KT == kDtF16 ? 2 : 3);  // of a query's and a probability's
     static constexpr int kKvParts = R::kParts;                            // of a key's and a value's
@@ -466,7 +465,7 @@ struct AttnArgs {
     uint64_t q_stride, k_stride, v_stride, out_stride;  // elements; k and v of packed prompts
     const int32_t* cu;
     uint32_t n_batch, n_rows, n_heads, n_kv, group, dim;
-    float scale, scale_log2;
+    float scale_log2;  // times log2 e
     int32_t causal;
     // paged
     KvView kv;
@@ -654,10 +653,6 @@ struct KvRows {
     __device__ __forceinline__ const elem* k_row(uint32_t key, bool& bad) const {
         if constexpr (PAGED) return k + paged_at(page_of(key, bad), key);
         else return k + key * k_stride;
-    }
-    __device__ __forceinline__ const elem* v_row(uint32_t key, bool& bad) const {
-        if constexpr (PAGED) return v + paged_at(page_of(key, bad), key);
-        else return v + key * v_stride;
     }
 };
 
