@@ -864,9 +864,10 @@ typedef struct {
 int32_t objeta_hip_rope_init(const objeta_hip_rope_params* params, objeta_hip_rope* out);
 
 /* Rotary positions for the queries and, unless n_k_heads is 0, the keys of n_tokens
- * tokens in one launch: q [n_tokens][n_q_heads][head_dim] (token stride q_stride) by the
+ * tokens in one launch (past 2^22 tokens: of that many each): q [n_tokens][n_q_heads][head_dim] (token stride q_stride) by the
  * angles of d_positions[t] (int32, any value), written to q_out; k likewise. Types:
- * `dtype` in, `out_dtype` out; computed in float, angles exact to 2^-32 of a turn. An
+ * `dtype` in, `out_dtype` out; computed in float: a position's place on the circle is
+ * exact to 2^-32 of a turn, its angle from the nearest quarter a float (to 2^-28 of one). An
  * output may be its own input (same address, stride and type); otherwise outputs may not
  * overlap inputs or one another. Pointers aligned to their element type. */
 int32_t objeta_hip_rope_device(objeta_hip_context* ctx, objeta_hip_stream stream, const objeta_hip_rope* rope,
@@ -948,7 +949,8 @@ int32_t objeta_hip_kv_append_device(objeta_hip_context* ctx, objeta_hip_stream s
  * prompts. max_rows: no entry
  * has more rows (any that go past it may come out NaN, with bit 2). max_len: the longest
  * sequence as the host knows it; it only decides how the work is cut, longer ones are
- * computed too. Entries whose sequence, length or pages are out of range, or that have more
+ * computed too. (Entries of up to 32 rows and heads are cut as if all were that long: far
+ * above the truth, as in a call captured for a context's limit, few workgroups do the work.) Entries whose sequence, length or pages are out of range, or that have more
  * rows than the sequence tokens, get NaN (bit 2). Row indices out of range or order set bit 2;
  * what the rows that they name, and rows behind them, hold is then undefined.
  * n_rows * n_q_heads <= 2^31 - 2^16; n_batch <= 65535, times the cache's heads below 2^31. */
@@ -971,7 +973,8 @@ int32_t objeta_hip_attn_cached_device(objeta_hip_context* ctx, objeta_hip_stream
 int32_t objeta_hip_kv_extend_device(objeta_hip_context* ctx, objeta_hip_stream stream, const objeta_hip_kv_cache* cache,
                                     const int32_t* d_seqs, const int32_t* d_counts, uint64_t n);
 /* fork: sequence d_dst[i] becomes d_src[i] as it was before the call, on shared pages; what
- * it held is released. A destination may be another entry's source (beams in a new order). */
+ * it held is released. A destination may be another entry's source (beams in a new order). A table
+ * entry of a source that names no page is handed on as -1 (bit 2). */
 int32_t objeta_hip_kv_fork_device(objeta_hip_context* ctx, objeta_hip_stream stream, const objeta_hip_kv_cache* cache,
                                   const int32_t* d_src, const int32_t* d_dst, uint64_t n);
 /* compact: of the last d_drafts[i] tokens of sequence d_seqs[i], the d_kept[i] ones with the
