@@ -4,7 +4,7 @@ row indices out of order."""
 import numpy as np
 import pytest
 
-from attn_reference import NP, attend, download, frequencies, from_type, lse_bound, rotate, rotate_bound, to_type
+from attn_reference import attend, download, frequencies, from_type, lse_bound, rotate, rotate_bound, to_type
 from objeta_amd import AttentionBackend, KvCache, MoeExecutor, Rope
 from test_gpu_attention import FILL, TYPES, Cached, check_cached, run_cached
 

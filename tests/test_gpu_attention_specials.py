@@ -8,7 +8,7 @@ import zlib
 import numpy as np
 import pytest
 
-from attn_reference import NP, attend, download, from_type, lse_bound, to_type
+from attn_reference import attend, from_type, lse_bound, to_type
 from objeta_amd import AttentionBackend, MoeExecutor
 from objeta_amd.api import check
 from test_gpu_attention import PAIRS, TYPES, Cached, run_cached, run_prompt, tree_masks
