@@ -989,6 +989,79 @@ int32_t objeta_hip_kv_compact_device(objeta_hip_context* ctx, objeta_hip_stream 
 int32_t objeta_hip_kv_free_device(objeta_hip_context* ctx, objeta_hip_stream stream, const objeta_hip_kv_cache* cache,
                                   const int32_t* d_seqs, uint64_t n);
 
+/* ------------------------------------- norms, 8-bit products, log probabilities */
+/* What a decoder layer runs between its attention and its experts, and what is read off
+ * the answers: the norm ahead of each half, with the codes that the next product reads;
+ * rows quantized to 8 bits; the product in 8-bit integers; log probabilities. The reference
+ * has none of these on its device path.
+ *
+ * Element types are OBJETA_HIP_DT_F32 / _F16 / _BF16. Strides count elements from one row to
+ * the next (of a single row: unused), at least the row's elements and below 2^31. Pointers are
+ * aligned to their element type, codes to nothing; rows may begin anywhere. An output may not
+ * overlap an input or another output, but for those named below. Calls allocate nothing (log
+ * probabilities: once a call of the same sizes has run on their stream) and may be captured.
+ * Results are the same bits each time. */
+
+/* 8-bit codes of a row y of floats.
+ * INT8: s = max |y| / 127 (a float; one a row), code = y / s rounded to the nearest, halves to even,
+ *   in exact arithmetic, within -127 .. 127 (only where s has lost bits as a subnormal number can
+ *   a quotient lie outside). A row of zeros has s 0 and codes 0, one that holds an
+ *   infinity or NaN s NaN and codes 0, so that every product with it is NaN.
+ * FP8: F8_E4M3 bytes with an E8M0 byte for each block of 128 as objeta_hip_act_quant_fp8_device
+ *   leaves them. */
+enum { OBJETA_HIP_CODES_NONE = 0, OBJETA_HIP_CODES_INT8 = 1, OBJETA_HIP_CODES_FP8 = 2 };
+
+/* The RMS norm of n_tokens rows of `hidden` elements (1 .. 65536) with the residual's addition:
+ *   h = x + residual                                   (float; d_residual NULL: h = x)
+ *   y_i = h_i (weight_i + weight_offset) / sqrt(sum_j h_j^2 / hidden + eps)
+ * d_residual_out (nullable) receives h rounded to residual_dtype, and it is this that is normed;
+ * it may be d_residual itself (address and stride). d_out (nullable) receives y rounded to
+ * out_dtype; it may be d_x itself where the types' sizes agree. `codes` other than NONE: d_codes
+ * [n_tokens][hidden] bytes (codes_stride) and d_scales (INT8 float [n_tokens], FP8 bytes
+ * [n_tokens][hidden / 128], hidden a multiple of 128) of y rounded to float; they do not
+ * depend on out_dtype. One output at least is given. y is computed in 64 bits and rounded
+ * once (16-bit types: from its float). eps >= 0; with eps 0 a row of zeros gives NaN. */
+int32_t objeta_hip_rms_norm_device(objeta_hip_context* ctx, objeta_hip_stream stream, uint64_t n_tokens, uint64_t hidden,
+                                   int32_t dtype, const void* d_x, uint64_t x_stride, int32_t weight_dtype,
+                                   const void* d_weight, float weight_offset, double eps, int32_t residual_dtype,
+                                   const void* d_residual, uint64_t residual_stride, void* d_residual_out,
+                                   uint64_t residual_out_stride, int32_t out_dtype, void* d_out, uint64_t out_stride,
+                                   int32_t codes, void* d_codes, uint64_t codes_stride, void* d_scales);
+
+/* Rows of a matrix (a weight's channels, tokens) to int8 codes with a scale a row: INT8 above.
+ * x [n_rows][cols] of `dtype`, cols 1 .. 65536. */
+int32_t objeta_hip_quantize_rows_i8_device(objeta_hip_context* ctx, objeta_hip_stream stream, uint64_t n_rows, uint64_t cols,
+                                           int32_t dtype, const void* d_x, uint64_t x_stride, int8_t* d_codes,
+                                           uint64_t codes_stride, float* d_scales);
+
+/* The product of tokens and channels in 8-bit integers:
+ *   out[t][r] = float(sum_k a[t][k] w[r][k]) * a_scales[t] * w_scales[r] (+ bias[r])
+ * a [n_tokens][cols], w [rows][cols] int8 (-128 .. 127), scales and bias (nullable) float, out
+ * [n_tokens][rows] of out_dtype. The sum is exact; it, both products, the addition and the last
+ * rounding to a 16-bit type are each rounded to nearest, in this order, so that results do not
+ * depend on the sizes of a batch. cols 1 .. 131071, rows < 2^24, n_tokens <= 2^20 - 16. Rows that
+ * begin at multiples of 16 bytes (addresses and strides) are read fastest. */
+int32_t objeta_hip_i8_product_device(objeta_hip_context* ctx, objeta_hip_stream stream, uint64_t n_tokens, uint64_t rows,
+                                     uint64_t cols, const int8_t* d_a, uint64_t a_stride, const float* d_a_scales,
+                                     const int8_t* d_w, uint64_t w_stride, const float* d_w_scales, const float* d_bias,
+                                     int32_t out_dtype, void* d_out, uint64_t out_stride);
+
+/* Log probabilities of rows of logits [n_rows][vocab] under p = softmax(scale * logits):
+ *   d_token_log_probs [n_rows][n_given] = ln p of d_tokens [n_rows][n_given] (int32; -1: none, 0;
+ *     others outside the vocab: NaN, and bit 2 of the device error word); n_given 0: both NULL
+ *   d_lse [n_rows] (nullable) = ln sum exp(scale * logits)
+ *   d_entropy [n_rows] (nullable) = -sum p ln p
+ *   d_top_ids, d_top_log_probs [n_rows][n_top] (the second nullable; n_top 0: both NULL; at most 32
+ *     and the vocab): the n_top largest logits, the largest first, equal ones by the lowest
+ *     index, and their ln p
+ * Logits of -infinity have ln p -inf; a row of nothing else lse -inf and entropy 0. A row that
+ * holds NaN or +infinity has NaN for lse, entropy and every ln p; NaN ranks below -infinity.
+ * scale > 0 (1 / temperature). Sums are held in float, references in units of ln 2. */
+int32_t objeta_hip_log_probs_device(objeta_hip_context* ctx, objeta_hip_stream stream, uint64_t n_rows, uint64_t vocab,
+                                    int32_t dtype, const void* d_logits, uint64_t stride, float scale, const int32_t* d_tokens,
+                                    uint64_t n_given, float* d_token_log_probs, float* d_lse, float* d_entropy, uint64_t n_top,
+                                    int32_t* d_top_ids, float* d_top_log_probs);
+
 #ifdef __cplusplus
 }
 #endif

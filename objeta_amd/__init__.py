@@ -8,7 +8,8 @@ from .api import (DeviceBuffer, ExpertCache, ExpertCacheKey, ExpertTable, Expert
                   HipBackendBuilder, HipError, HostExpertSet, MoeExecutor, PinnedHostBuffer, QGemvShape, QuantBackend, QuantFormat, check,
                   discover_devices)
 from .attention import AttentionBackend, KvCache, Rope
+from .dense import DenseBackend
 
-__all__ = ["AttentionBackend", "DeviceBuffer", "ExpertCache", "ExpertCacheKey", "ExpertTable", "ExpertTensorKind", "HipBackend",
+__all__ = ["AttentionBackend", "DenseBackend", "DeviceBuffer", "ExpertCache", "ExpertCacheKey", "ExpertTable", "ExpertTensorKind", "HipBackend",
            "HipBackendBuilder", "HipError", "HostExpertSet", "KvCache", "MoeExecutor", "PinnedHostBuffer", "QGemvShape", "QuantBackend", "QuantFormat", "Rope", "check",
            "discover_devices"]

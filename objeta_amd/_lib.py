@@ -224,6 +224,11 @@ SIGNATURES = {
     "objeta_hip_kv_fork_device": (I32, [P, P, P, P, P, U64]),
     "objeta_hip_kv_compact_device": (I32, [P, P, P, P, P, P, P, U64, U64]),
     "objeta_hip_kv_free_device": (I32, [P, P, P, P, U64]),
+    "objeta_hip_rms_norm_device": (I32, [P, P, U64, U64, I32, P, U64, I32, P, F32, F64, I32, P, U64, P, U64, I32, P, U64,
+                                         I32, P, U64, P]),
+    "objeta_hip_quantize_rows_i8_device": (I32, [P, P, U64, U64, I32, P, U64, P, U64, P]),
+    "objeta_hip_i8_product_device": (I32, [P, P, U64, U64, U64, P, U64, P, P, U64, P, P, I32, P, U64]),
+    "objeta_hip_log_probs_device": (I32, [P, P, U64, U64, I32, P, U64, F32, P, U64, P, P, P, U64, P, P]),
 }
 
 

@@ -1,0 +1,127 @@
+// dense_common.hpp — what the norm, the 8-bit product and the log probabilities share: host
+// checks of their tensors, the context's device made current, element loads and wave sums.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "kv_common.hpp"
+
+namespace objeta {
+
+// Makes the context's device current for a call and gives the caller's back.
+class OnDevice {
+public:
+    explicit OnDevice(int device) {
+        if (hipGetDevice(&before_) != hipSuccess || before_ == device) before_ = -1;
+        else status_ = hipSetDevice(device);
+    }
+    ~OnDevice() {
+        if (before_ >= 0) (void)hipSetDevice(before_);
+    }
+    OnDevice(const OnDevice&) = delete;
+    hipError_t status() const { return status_; }
+
+private:
+    int before_ = -1;
+    hipError_t status_ = hipSuccess;
+};
+
+// Rows of `width` elements of `size` bytes, `stride` elements apart (one row: unused).
+inline RowSet row_set(const void* p, uint64_t n, uint64_t stride, uint64_t width, uint64_t size) {
+    return RowSet{p, (n > 1 ? stride : width) * size, width * size, n};
+}
+int32_t check_dense_rows(const char* action, const char* what, const void* p, uint64_t n, uint64_t stride, uint64_t width,
+                         uint64_t size);
+// That `out` overlaps none of the others; it may be others[own] itself (own -1: none).
+int32_t check_dense_apart(const char* action, const char* what, const RowSet& out, const RowSet* others, int n, int own);
+
+#if defined(__HIPCC__)
+namespace dev {
+
+// Sixteen and eight bytes at an address of any alignment: this target's global loads take them.
+typedef uint32_t any_u32x4 __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t any_u32x2 __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t reg_u32x4 __attribute__((ext_vector_type(4)));
+
+// Eight elements as they lie in memory; 16-bit types fill `a` alone.
+struct Raw8 {
+    reg_u32x4 a, b;
+};
+
+// Eight elements of row `p` from element i on, of which n are there (others 0).
+template <class E>
+__device__ __forceinline__ Raw8 load_some(const E* p, uint32_t n) {
+    Raw8 r{};
+    E* x = reinterpret_cast<E*>(&r);
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i)
+        if (i < n) x[i] = p[i];
+    return r;
+}
+__device__ __forceinline__ Raw8 load_raw8(int32_t type, const void* base, uint64_t at, uint32_t n) {
+    if (type == kDtF32) {
+        const uint32_t* p = static_cast<const uint32_t*>(base) + at;
+        if (n < 8) return load_some(p, n);
+        return Raw8{*reinterpret_cast<const any_u32x4*>(p), *reinterpret_cast<const any_u32x4*>(p + 4)};
+    }
+    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+    if (n < 8) return load_some(p, n);
+    return Raw8{*reinterpret_cast<const any_u32x4*>(p), reg_u32x4{0, 0, 0, 0}};
+}
+__device__ __forceinline__ void to_floats(int32_t type, const Raw8& r, float (&x)[8]) {
+    if (type == kDtF32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __uint_as_float(r.a[i]), x[4 + i] = __uint_as_float(r.b[i]);
+    } else if (type == kDtBF16) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(r.a[i] << 16), x[2 * i + 1] = __uint_as_float(r.a[i] & 0xFFFF0000u);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(r.a[i])));
+            x[2 * i + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(r.a[i] >> 16)));
+        }
+    }
+}
+__device__ __forceinline__ uint32_t bits_of(int32_t type, float x) {  // a 16-bit type's bits, rounded to nearest even
+    return type == kDtBF16 ? static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<__bf16>(x)))
+                           : static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<_Float16>(x)));
+}
+__device__ __forceinline__ float rounded_to(int32_t type, float x) {
+    if (type == kDtF32) return x;
+    return type == kDtBF16 ? static_cast<float>(static_cast<__bf16>(x)) : static_cast<float>(static_cast<_Float16>(x));
+}
+__device__ __forceinline__ void store_floats(int32_t type, void* base, uint64_t at, uint32_t n, const float (&x)[8]) {
+    if (type == kDtF32) {
+        float* p = static_cast<float*>(base) + at;
+        if (n >= 8) {
+            reg_u32x4 a, b;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[i] = __float_as_uint(x[i]), b[i] = __float_as_uint(x[4 + i]);
+            *reinterpret_cast<any_u32x4*>(p) = a;
+            *reinterpret_cast<any_u32x4*>(p + 4) = b;
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                if (i < n) p[i] = x[i];
+        }
+        return;
+    }
+    uint16_t* p = static_cast<uint16_t*>(base) + at;
+    reg_u32x4 a;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = bits_of(type, x[2 * i]) | bits_of(type, x[2 * i + 1]) << 16;
+    if (n >= 8) {
+        *reinterpret_cast<any_u32x4*>(p) = a;
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i)
+            if (i < n) p[i] = static_cast<uint16_t>(a[i / 2] >> (16 * (i & 1)));
+    }
+}
+
+}  // namespace dev
+#endif
+
+}  // namespace objeta

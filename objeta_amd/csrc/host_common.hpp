@@ -82,7 +82,8 @@ enum WsSlot : int {
     kWsStack = 7,     // routing results and expert tables of the cached decode stack
     kWsPages = 8,     // free pages, copies and staged tables of the cache's page operations
     kWsAttn = 9,      // partial sums of attention over a cache cut along its length
-    kWsSlots = 10
+    kWsLogProbs = 10,  // sums and best tokens of rows cut over workgroups
+    kWsSlots = 11
 };
 
 // The scratch of one stream. Calls on different streams of a context may be in

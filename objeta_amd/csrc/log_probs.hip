@@ -1,0 +1,498 @@
+// log_probs.hip — log probabilities of given tokens, with the entropy and the best alternatives.
+//
+// With z = scale x, m = max z: S = sum exp(z - m), lse = m + ln S, log p_i = z_i - lse and
+// H = ln S - sum exp(z - m) (z - m) / S, in one pass: a thread keeps a reference R (its largest z so
+// far, in units of ln 2), s = sum 2^(z - R) and t = sum 2^(z - R) (z - R), and moves both when R grows:
+// with d = R - R', s' = 2^d s and t' = 2^d (t + d s).
+//
+// The best N: a thread also keeps the largest x of each stretch it read (up to 16). The N-th largest
+// of the threads' maxima bounds the N-th best from below, so only the few stretches that reach it are
+// read again, and what reaches it there is ranked. A value's key is its bits in their order above the
+// complement of its index: equal values go by the lowest index. Where too many values reach the bound
+// (ties, all of the best in few threads), the N-th value is found bit by bit over the row instead.
+//
+// Bound: HBM where rows are many; few rows are cut over workgroups, whose parts a second launch joins.
+#include "dense_common.hpp"
+#include "kernels.hpp"
+
+namespace objeta {
+namespace dev {
+
+constexpr uint32_t kLpThreads = 256;
+constexpr uint32_t kLpVecs = 4;      // 16-byte loads of a thread in flight
+constexpr uint32_t kLpStretches = 16;
+constexpr uint32_t kLpMostTop = 32;
+constexpr uint32_t kLpMostCandidates = 1024;  // no less than kLpMostTop^2, for the join
+// References lie between -2^24 and 2^24, where rounding one moves its largest term by a factor of two
+// at most. Threads whose values are all lower add nothing to a row within; a row whose largest is
+// outside is summed a second time about that value itself.
+constexpr float kLpFar = 16777216.0f;
+
+struct LpArgs {
+    const void* x;
+    uint64_t stride;
+    uint64_t first;  // the launch's first row
+    uint32_t n_rows, vocab, n_given, n_top, parts, part_size;
+    float scale, c;  // c = scale / ln 2
+    const int32_t* tokens;
+    float *lp, *lse, *entropy, *top;
+    int32_t* ids;
+    float4* stats;   // [rows][parts]: m, R, s, t
+    uint64_t* keys;  // [rows][parts][n_top], the best first, 0 behind the last
+    uint32_t* err;
+};
+
+// A float's bits in the order of floats; NaN below all.
+__device__ __forceinline__ uint32_t ordered(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);  // -0 is 0
+    if (x != x) return 0;
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t o) { return __uint_as_float(o >> 31 ? o & 0x7FFFFFFFu : ~o); }
+constexpr uint32_t kOrderedInf = 0x007FFFFFu;  // of -infinity
+
+template <int TYPE> struct LpElem { static constexpr uint32_t kPer = TYPE == kDtF32 ? 4 : 8; };  // elements of 16 bytes
+
+template <int TYPE>
+__device__ __forceinline__ float lp_at(const void* row, uint64_t i) {
+    if constexpr (TYPE == kDtF32) return static_cast<const float*>(row)[i];
+    const uint16_t b = static_cast<const uint16_t*>(row)[i];
+    return TYPE == kDtBF16 ? __uint_as_float(static_cast<uint32_t>(b) << 16) : static_cast<float>(__builtin_bit_cast(_Float16, b));
+}
+template <int TYPE>
+__device__ __forceinline__ void lp_floats(const reg_u32x4& r, float* x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (TYPE == kDtF32) x[i] = __uint_as_float(r[i]);
+        else if constexpr (TYPE == kDtBF16) x[2 * i] = __uint_as_float(r[i] << 16), x[2 * i + 1] = __uint_as_float(r[i] & 0xFFFF0000u);
+        else {
+            x[2 * i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(r[i])));
+            x[2 * i + 1] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(r[i] >> 16)));
+        }
+    }
+}
+// 16 bytes from element i on, -infinity behind `end`.
+template <int TYPE>
+__device__ __forceinline__ reg_u32x4 lp_load(const void* row, uint32_t i, uint32_t end) {
+    constexpr uint32_t kPer = LpElem<TYPE>::kPer;
+    const char* p = static_cast<const char*>(row) + static_cast<uint64_t>(i) * (16 / kPer);
+    if (i + kPer <= end) return *reinterpret_cast<const any_u32x4*>(p);
+    reg_u32x4 r;
+    if constexpr (TYPE == kDtF32) {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) r[j] = i + j < end ? reinterpret_cast<const uint32_t*>(p)[j] : 0xFF800000u;
+    } else {
+        constexpr uint32_t inf = TYPE == kDtBF16 ? 0xFF80u : 0xFC00u;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t a = i + 2 * j < end ? reinterpret_cast<const uint16_t*>(p)[2 * j] : inf;
+            const uint32_t b = i + 2 * j + 1 < end ? reinterpret_cast<const uint16_t*>(p)[2 * j + 1] : inf;
+            r[j] = a | b << 16;
+        }
+    }
+    return r;
+}
+
+// Sums about a reference, and their join.
+struct LpSums {
+    float m, ref, s, t;
+    __device__ __forceinline__ void move(float to) {
+        const float d = __builtin_fmaxf(ref - to, -1000.0f);
+        const float f = __builtin_amdgcn_exp2f(d);
+        t = f * __builtin_fmaf(d, s, t);
+        s *= f;
+        ref = to;
+    }
+    __device__ __forceinline__ void join(LpSums o) {
+        const float to = __builtin_fmaxf(ref, o.ref);
+        move(to);
+        o.move(to);
+        m = __builtin_fmaxf(m, o.m);
+        s += o.s;
+        t += o.t;
+    }
+    __device__ __forceinline__ LpSums from(int off) const {
+        return LpSums{__shfl_xor(m, off, 64), __shfl_xor(ref, off, 64), __shfl_xor(s, off, 64), __shfl_xor(t, off, 64)};
+    }
+};
+
+struct LpShared {
+    LpSums sums[kLpThreads / 64];
+    uint32_t max[kLpThreads];
+    uint64_t keys[kLpMostCandidates];
+    uint64_t best[kLpMostTop];
+    uint32_t hist[256];
+    uint32_t count, bound, digit, wave[kLpThreads / 64];
+};
+
+__device__ __forceinline__ LpSums lp_join_all(LpSums v, LpShared& sh) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v.join(v.from(off));
+    if ((threadIdx.x & 63) == 0) sh.sums[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = sh.sums[0];
+    for (uint32_t i = 1; i < kLpThreads / 64; ++i) v.join(sh.sums[i]);
+    __syncthreads();
+    return v;
+}
+
+// sh.keys[0 .. n) to sh.best, the n_top largest in order, 0 behind the last; keys differ.
+__device__ __forceinline__ void lp_rank(LpShared& sh, uint32_t n, uint32_t n_top) {
+    if (threadIdx.x < kLpMostTop) sh.best[threadIdx.x] = 0;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += kLpThreads) {
+        const uint64_t k = sh.keys[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < n && rank < n_top; ++j) rank += sh.keys[j] > k;
+        if (rank < n_top) sh.best[rank] = k;
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ uint64_t lp_key(uint32_t value, uint32_t index) {
+    return static_cast<uint64_t>(value) << 32 | static_cast<uint32_t>(~index);
+}
+
+// Appends to sh.keys the elements of [lo, hi) whose ordered value is `value`, the lowest indices
+// first, until there are `want` keys.
+template <int TYPE>
+__device__ void lp_fill(const void* row, uint32_t lo, uint32_t hi, uint32_t value, uint32_t want, LpShared& sh) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (uint32_t i = lo; i < hi; i += kLpThreads) {
+        const uint32_t have = sh.count;
+        if (have >= want) break;
+        const uint32_t at = i + threadIdx.x;
+        const bool hit = at < hi && ordered(lp_at<TYPE>(row, at)) == value;
+        const uint64_t hits = __ballot(hit);
+        if (lane == 0) sh.wave[wave] = __popcll(hits);
+        __syncthreads();
+        uint32_t place = have + __popcll(hits & ((uint64_t(1) << lane) - 1)), all = have;
+        for (uint32_t w = 0; w < kLpThreads / 64; ++w) {
+            if (w < wave) place += sh.wave[w];
+            all += sh.wave[w];
+        }
+        if (hit && place < want) sh.keys[place] = lp_key(value, at);
+        __syncthreads();
+        if (threadIdx.x == 0) sh.count = all < want ? all : want;
+        __syncthreads();
+    }
+}
+
+// The n_top best above -infinity of [lo, hi) by the digits of their values; there are more than n_top.
+template <int TYPE>
+__device__ void lp_by_digits(const void* row, uint32_t lo, uint32_t hi, uint32_t n_top, LpShared& sh) {
+    uint32_t prefix = 0, want = n_top;  // values whose upper digits are the prefix's: `want` of them are among the best
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        sh.hist[threadIdx.x] = 0;
+        __syncthreads();
+        for (uint32_t i = lo + threadIdx.x; i < hi; i += kLpThreads) {
+            const uint32_t o = ordered(lp_at<TYPE>(row, i));
+            if (o > kOrderedInf && (shift == 24 || o >> (shift + 8) == prefix >> (shift + 8))) atomicAdd(&sh.hist[o >> shift & 255], 1u);
+        }
+        __syncthreads();
+        uint32_t above = 0;
+        for (uint32_t d = threadIdx.x + 1; d < 256; ++d) above += sh.hist[d];
+        if (above < want && above + sh.hist[threadIdx.x] >= want) sh.digit = threadIdx.x, sh.bound = want - above;
+        __syncthreads();
+        prefix |= sh.digit << shift;
+        want = sh.bound;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) sh.count = 0;
+    __syncthreads();
+    for (uint32_t i = lo + threadIdx.x; i < hi; i += kLpThreads) {
+        const uint32_t o = ordered(lp_at<TYPE>(row, i));
+        if (o > prefix) sh.keys[atomicAdd(&sh.count, 1u)] = lp_key(o, i);  // n_top - want of them
+    }
+    __syncthreads();
+    lp_fill<TYPE>(row, lo, hi, prefix, n_top, sh);
+}
+
+// What a row's sums and best come to.
+template <int TYPE>
+__device__ void lp_finish(const LpArgs& a, uint64_t r, LpSums v, LpShared& sh) {
+    const void* row = static_cast<const char*>(a.x) + r * a.stride * (16 / LpElem<TYPE>::kPer);
+    const uint32_t tid = threadIdx.x;
+    const bool none = v.m == -__builtin_inff() && v.s == v.s;  // (the sum is NaN where the row holds one)
+    const bool again = v.m != -__builtin_inff() && !(v.ref > -kLpFar && v.ref < kLpFar);
+    if (again) {
+        LpSums u{v.m, 0.0f, 0.0f, 0.0f};
+        for (uint32_t i = tid; i < a.vocab; i += kLpThreads) {
+            const float d = (lp_at<TYPE>(row, i) - v.m) * a.c, e = __builtin_amdgcn_exp2f(d);
+            u.s += e;
+            u.t = __builtin_fmaf(e, __builtin_fmaxf(d, -200.0f), u.t);
+        }
+        v = lp_join_all(u, sh);
+    }
+    constexpr float kLn2 = 0.693147180559945309f;
+    const float log_s = __builtin_amdgcn_logf(v.s);  // of base 2
+    const float more = (again ? log_s : log_s + __builtin_fmaf(-v.m, a.c, v.ref)) * kLn2;  // ln sum exp(z - m)
+    auto not_above_0 = [](float p) { return p > 0.0f ? 0.0f : p; };  // NaN stays
+    auto log_prob = [&](float x) {
+        return none ? -__builtin_inff() : not_above_0(__builtin_fmaf(x - v.m, a.scale, -more));
+    };
+    if (tid == 0) {
+        if (a.lse) a.lse[r] = none ? -__builtin_inff() : __builtin_fmaf(v.m, a.scale, more);
+        if (a.entropy) a.entropy[r] = none ? 0.0f : -not_above_0((v.t / v.s - log_s) * kLn2);
+    }
+    if (a.lp)
+        for (uint32_t g = tid; g < a.n_given; g += kLpThreads) {
+            const int32_t token = a.tokens[r * a.n_given + g];
+            float p = 0.0f;
+            if (static_cast<uint32_t>(token) < a.vocab) {
+                p = log_prob(lp_at<TYPE>(row, token));
+            } else if (token != -1) {
+                p = __builtin_nanf("");
+                atomicOr(a.err, kErrIndex);
+            }
+            a.lp[r * a.n_given + g] = p;
+        }
+    if (a.n_top) {
+        // sh.best holds the values above -infinity; the others by their indices
+        if (sh.best[a.n_top - 1] == 0) {
+            if (tid == 0) {
+                uint32_t n = 0;
+                while (n < a.n_top && sh.best[n]) sh.keys[n] = sh.best[n], ++n;
+                sh.count = n;
+            }
+            __syncthreads();
+            lp_fill<TYPE>(row, 0, a.vocab, kOrderedInf, a.n_top, sh);
+            lp_fill<TYPE>(row, 0, a.vocab, 0, a.n_top, sh);
+            if (tid < a.n_top) sh.best[tid] = sh.keys[tid];
+            __syncthreads();
+        }
+        if (tid < a.n_top) {
+            const uint64_t k = sh.best[tid];
+            const uint32_t index = ~static_cast<uint32_t>(k);
+            if (a.ids) a.ids[r * a.n_top + tid] = static_cast<int32_t>(index);
+            if (a.top) a.top[r * a.n_top + tid] = k >> 32 ? log_prob(unordered(static_cast<uint32_t>(k >> 32))) : __builtin_nanf("");
+        }
+    }
+}
+
+template <int TYPE, bool TOP, bool ENTROPY>
+__global__ __launch_bounds__(kLpThreads) void lp_part_kernel(LpArgs a) {
+    constexpr uint32_t kPer = LpElem<TYPE>::kPer, kStep = kLpThreads * kPer, kTurn = kLpVecs * kStep;
+    __shared__ LpShared sh;
+    __shared__ float stretch[TOP ? kLpStretches : 1][kLpThreads];
+    const uint64_t r = a.first + blockIdx.x;
+    const uint32_t part = blockIdx.y, tid = threadIdx.x;
+    const uint32_t lo = part * a.part_size, hi = a.vocab - lo < a.part_size ? a.vocab : lo + a.part_size;
+    const void* row = static_cast<const char*>(a.x) + r * a.stride * (16 / kPer);
+    const uint32_t turns = (hi - lo + kTurn - 1) / kTurn, per = (turns + kLpStretches - 1) / kLpStretches;
+
+    const float ninf = -__builtin_inff();
+    LpSums v{ninf, -kLpFar, 0.0f, 0.0f};
+    float longest = ninf;
+    reg_u32x4 next[kLpVecs];
+#pragma unroll
+    for (uint32_t u = 0; u < kLpVecs; ++u) next[u] = lp_load<TYPE>(row, lo + u * kStep + tid * kPer, hi);
+    for (uint32_t turn = 0; turn < turns; ++turn) {
+        float x[kLpVecs][kPer];
+#pragma unroll
+        for (uint32_t u = 0; u < kLpVecs; ++u) lp_floats<TYPE>(next[u], x[u]);
+        if (turn + 1 < turns) {
+#pragma unroll
+            for (uint32_t u = 0; u < kLpVecs; ++u) next[u] = lp_load<TYPE>(row, lo + (turn + 1) * kTurn + u * kStep + tid * kPer, hi);
+        }
+        float m = ninf;
+#pragma unroll
+        for (uint32_t u = 0; u < kLpVecs; ++u)
+#pragma unroll
+            for (uint32_t i = 0; i < kPer; ++i) m = __builtin_fmaxf(m, x[u][i]);
+        longest = __builtin_fmaxf(longest, m);
+        if (TOP && (turn % per == per - 1 || turn + 1 == turns)) {
+            stretch[turn / per][tid] = longest;
+            longest = ninf;
+        }
+        if (m > v.m) {
+            v.m = m;
+            v.move(__builtin_fmaxf(m * a.c, -kLpFar));
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kLpVecs; ++u)
+#pragma unroll
+            for (uint32_t i = 0; i < kPer; ++i) {
+                const float d = __builtin_fmaf(x[u][i], a.c, -v.ref), e = __builtin_amdgcn_exp2f(d);
+                v.s += e;
+                if (ENTROPY) v.t = __builtin_fmaf(e, __builtin_fmaxf(d, -200.0f), v.t);
+            }
+    }
+    const float mine = v.m;
+    v = lp_join_all(v, sh);
+
+    if constexpr (TOP) {
+        // The n_top-th largest of the threads' maxima.
+        const uint32_t key = ordered(mine);
+        sh.max[tid] = key;
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+        uint32_t rank = 0;
+        for (uint32_t i = 0; i < kLpThreads; ++i) rank += sh.max[i] > key || (sh.max[i] == key && i < tid);
+        if (rank == a.n_top - 1) sh.bound = key;
+        __syncthreads();
+        uint32_t bound = sh.bound;
+        if (bound <= kOrderedInf) bound = kOrderedInf + 1;
+        if (key >= bound) {
+            for (uint32_t g = 0; g * per < turns; ++g) {
+                if (ordered(stretch[g][tid]) < bound) continue;
+                const uint32_t end = (g + 1) * per < turns ? (g + 1) * per : turns;
+                for (uint32_t turn = g * per; turn < end; ++turn)
+#pragma unroll
+                    for (uint32_t u = 0; u < kLpVecs; ++u) {
+                        const uint32_t at = lo + turn * kTurn + u * kStep + tid * kPer;
+                        float x[kPer];
+                        lp_floats<TYPE>(lp_load<TYPE>(row, at, hi), x);
+#pragma unroll
+                        for (uint32_t i = 0; i < kPer; ++i) {
+                            const uint32_t o = ordered(x[i]);
+                            if (o < bound) continue;
+                            const uint32_t place = atomicAdd(&sh.count, 1u);
+                            if (place < kLpMostCandidates) sh.keys[place] = lp_key(o, at + i);
+                        }
+                    }
+            }
+        }
+        __syncthreads();
+        if (sh.count > kLpMostCandidates) lp_by_digits<TYPE>(row, lo, hi, a.n_top, sh);
+        lp_rank(sh, sh.count, a.n_top);
+    }
+    if (a.parts == 1) {
+        lp_finish<TYPE>(a, r, v, sh);
+        return;
+    }
+    const uint64_t at = r * a.parts + part;
+    if (tid == 0) a.stats[at] = make_float4(v.m, v.ref, v.s, v.t);
+    if (TOP && tid < a.n_top) a.keys[at * a.n_top + tid] = sh.best[tid];
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(kLpThreads) void lp_join_kernel(LpArgs a) {
+    __shared__ LpShared sh;
+    const uint64_t r = a.first + blockIdx.x;
+    const uint32_t tid = threadIdx.x;
+    LpSums v{-__builtin_inff(), -kLpFar, 0.0f, 0.0f};
+    if (tid < a.parts) {
+        const float4 p = a.stats[r * a.parts + tid];
+        v = LpSums{p.x, p.y, p.z, p.w};
+    }
+    v = lp_join_all(v, sh);
+    if (a.n_top) {
+        // A part's first key is its best; with n_top parts or more the n_top-th of these bounds the rest.
+        const uint64_t* keys = a.keys + r * a.parts * a.n_top;
+        if (tid < a.parts) sh.keys[tid] = keys[static_cast<uint64_t>(tid) * a.n_top];
+        __syncthreads();
+        lp_rank(sh, a.parts, a.n_top);
+        const uint64_t bound = sh.best[a.n_top - 1];
+        if (tid == 0) sh.count = 0;
+        __syncthreads();
+        if (tid < a.parts)
+            for (uint32_t i = 0; i < a.n_top; ++i) {
+                const uint64_t k = keys[static_cast<uint64_t>(tid) * a.n_top + i];
+                if (k == 0 || k < bound) break;
+                sh.keys[atomicAdd(&sh.count, 1u)] = k;  // of at most n_top parts n_top each
+            }
+        __syncthreads();
+        lp_rank(sh, sh.count, a.n_top);
+    }
+    lp_finish<TYPE>(a, r, v, sh);
+}
+
+}  // namespace dev
+
+using namespace dev;
+
+namespace {
+
+template <int TYPE>
+void launch_parts(hipStream_t s, dim3 grid, const LpArgs& a) {
+    if (a.n_top && a.entropy) hipLaunchKernelGGL((lp_part_kernel<TYPE, true, true>), grid, dim3(kLpThreads), 0, s, a);
+    else if (a.n_top) hipLaunchKernelGGL((lp_part_kernel<TYPE, true, false>), grid, dim3(kLpThreads), 0, s, a);
+    else if (a.entropy) hipLaunchKernelGGL((lp_part_kernel<TYPE, false, true>), grid, dim3(kLpThreads), 0, s, a);
+    else hipLaunchKernelGGL((lp_part_kernel<TYPE, false, false>), grid, dim3(kLpThreads), 0, s, a);
+    if (a.parts > 1) hipLaunchKernelGGL((lp_join_kernel<TYPE>), dim3(grid.x), dim3(kLpThreads), 0, s, a);
+}
+
+int32_t launch_lp(hipStream_t s, int32_t type, LpArgs a, const char* action) {
+    for (a.first = 0; a.first < a.n_rows; a.first += kMostGroups) {
+        const uint64_t n = a.n_rows - a.first;
+        const dim3 grid(static_cast<uint32_t>(n < kMostGroups ? n : kMostGroups), a.parts);
+        if (type == kDtF32) launch_parts<kDtF32>(s, grid, a);
+        else if (type == kDtF16) launch_parts<kDtF16>(s, grid, a);
+        else launch_parts<kDtBF16>(s, grid, a);
+        OBJ_HIP(hipGetLastError(), action);
+    }
+    return 0;
+}
+
+}  // namespace
+
+}  // namespace objeta
+
+using namespace objeta;
+
+extern "C" {
+
+int32_t objeta_hip_log_probs_device(objeta_hip_context* ctx, objeta_hip_stream stream, uint64_t n_rows, uint64_t vocab,
+                                    int32_t dtype, const void* d_logits, uint64_t stride, float scale, const int32_t* d_tokens,
+                                    uint64_t n_given, float* d_token_log_probs, float* d_lse, float* d_entropy, uint64_t n_top,
+                                    int32_t* d_top_ids, float* d_top_log_probs) {
+    OBJ_GUARD_BEGIN
+    const char* action = "log_probs_device";
+    OBJ_TRY(check_ctx(ctx, action));
+    if (vocab == 0 || vocab > kMaxTokens) OBJ_FAIL(kInvalidInput, action, "vocab must be 1 to 2^31 - 2^16");
+    if (!dtype_ok(dtype)) OBJ_FAIL(kInvalidInput, action, "dtype must be F32, F16 or BF16");
+    if (!(scale > 0.0f && scale < 1e30f)) OBJ_FAIL(kInvalidInput, action, "scale must be positive and finite");
+    if (n_given > 1024) OBJ_FAIL(kInvalidInput, action, "at most 1024 given tokens a row");
+    if (n_top > kLpMostTop || n_top > vocab) OBJ_FAIL(kInvalidInput, action, "n_top must be at most 32 and the vocab");
+    if (n_rows >= (uint64_t(1) << 31)) OBJ_FAIL(kInvalidInput, action, "too many rows");
+    if ((n_given != 0) != (d_token_log_probs != nullptr) || (n_given != 0) != (d_tokens != nullptr))
+        OBJ_FAIL(kInvalidInput, action, "given tokens and their log probabilities come together with n_given");
+    if (n_top != 0 && !d_top_ids) OBJ_FAIL(kInvalidInput, action, "top ids are NULL");
+    if (n_top == 0 && (d_top_ids || d_top_log_probs)) OBJ_FAIL(kInvalidInput, action, "top outputs with n_top 0");
+    if (!n_given && !n_top && !d_lse && !d_entropy) OBJ_FAIL(kInvalidInput, action, "no output is given");
+    if (n_rows == 0) return 0;
+    const uint64_t es = dtype_size(dtype);
+    OBJ_TRY(check_dense_rows(action, "logits", d_logits, n_rows, stride, vocab, es));
+    RowSet sets[7] = {row_set(d_logits, n_rows, stride, vocab, es), row_set(d_tokens, 1, 0, n_rows * n_given, 4)};
+    int n_sets = 2;
+    const struct { const char* what; const void* p; uint64_t n; } outs[5] = {
+        {"token log probs", d_token_log_probs, n_given}, {"lse", d_lse, 1}, {"entropy", d_entropy, 1},
+        {"top ids", d_top_ids, n_top}, {"top log probs", d_top_log_probs, n_top}};
+    if (d_tokens) OBJ_TRY(check_dense_rows(action, "tokens", d_tokens, 1, 0, n_given, 4));
+    for (const auto& o : outs) {
+        if (!o.p) continue;
+        OBJ_TRY(check_dense_rows(action, o.what, o.p, 1, 0, o.n, 4));
+        const RowSet set = row_set(o.p, 1, 0, n_rows * o.n, 4);
+        OBJ_TRY(check_dense_apart(action, o.what, set, sets, n_sets, -1));
+        sets[n_sets++] = set;
+    }
+    const OnDevice on(ctx->device);
+    OBJ_HIP(on.status(), action);
+    const hipStream_t s = resolve_stream(ctx, stream);
+    LpArgs a{};
+    a.x = d_logits, a.stride = n_rows > 1 ? stride : 0;
+    a.n_rows = static_cast<uint32_t>(n_rows), a.vocab = static_cast<uint32_t>(vocab);
+    a.n_given = static_cast<uint32_t>(n_given), a.n_top = static_cast<uint32_t>(n_top);
+    a.scale = scale, a.c = static_cast<float>(scale * 1.4426950408889634074);
+    a.tokens = d_tokens, a.lp = d_token_log_probs, a.lse = d_lse, a.entropy = d_entropy, a.ids = d_top_ids, a.top = d_top_log_probs;
+    a.err = ctx->err_word;
+    const uint32_t turn = kLpThreads * kLpVecs * (dtype == kDtF32 ? 4 : 8);
+    const uint64_t most = (vocab + turn - 1) / turn, want = 1024 / n_rows;
+    uint64_t parts = want < 1 ? 1 : (want < most ? want : most);
+    if (parts > kLpThreads) parts = kLpThreads;
+    const uint64_t size = ((vocab + parts - 1) / parts + turn - 1) / turn * turn;
+    a.part_size = static_cast<uint32_t>(size);
+    a.parts = static_cast<uint32_t>((vocab + size - 1) / size);
+    if (a.parts > 1) {
+        void* ws = nullptr;
+        const size_t n = static_cast<size_t>(n_rows) * a.parts;
+        OBJ_TRY(ensure_workspace(ctx, s, kWsLogProbs, n * (sizeof(float4) + 8 * n_top), &ws));
+        a.stats = static_cast<float4*>(ws);
+        a.keys = reinterpret_cast<uint64_t*>(a.stats + n);
+    }
+    return launch_lp(s, dtype, a, action);
+    OBJ_GUARD_END
+}
+
+}  // extern "C"
