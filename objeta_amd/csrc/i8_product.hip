@@ -7,6 +7,8 @@
 #include "dense_common.hpp"
 #include "kernels.hpp"
 
+#include <cmath>
+
 namespace objeta {
 namespace dev {
 
@@ -43,49 +45,57 @@ __device__ __forceinline__ void store_one(int32_t type, void* out, uint64_t at, 
     else static_cast<uint16_t*>(out)[at] = static_cast<uint16_t>(bits_of(type, x));
 }
 
-// Few tokens: a workgroup takes 16 channels and 16 NT tokens, its waves share the columns. The
+// Few tokens: a workgroup takes 16 NC channels and 16 NT tokens, its waves share the columns. The
 // matrix instruction's operands are sixteen codes of a channel (lane % 16) and of a token, columns
 // 16 (lane / 16) on; channels' codes come straight from memory, each once, U loads ahead.
-template <int WAVES, int NT, int U, bool WHOLE>
+template <int WAVES, int NC, int NT, int U, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES) void i8_stream_kernel(I8Args a) {
-    __shared__ i32x4 part[WAVES][NT][64];
+    __shared__ i32x4 part[WAVES][NC * NT][64];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t r0 = 16 * blockIdx.x, t0 = 16 * NT * blockIdx.y;
-    const uint32_t r = r0 + (lane & 15) < a.rows ? r0 + (lane & 15) : a.rows - 1;
-    const int8_t* w = a.w + r * a.w_stride;
-    const int8_t* x[NT];
+    const uint32_t r0 = 16 * NC * blockIdx.x, t0 = 16 * NT * blockIdx.y;
+    const int8_t *w[NC], *x[NT];
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+        const uint32_t r = r0 + 16 * n + (lane & 15);
+        w[n] = a.w + (r < a.rows ? r : a.rows - 1) * a.w_stride;
+    }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const uint32_t t = t0 + 16 * n + (lane & 15);
         x[n] = a.a + (t < a.n_tokens ? t : a.n_tokens - 1) * a.a_stride;
     }
-    i32x4 nw[U], nx[U][NT];
+    i32x4 nw[U][NC], nx[U][NT];
     auto load = [&](uint32_t k) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const uint32_t at = k + 64 * u + 16 * (lane >> 4);
             if constexpr (WHOLE) {  // past the last column: channels' codes 0, tokens' any
                 const bool in = at < a.cols;
-                const i32x4 v = __builtin_bit_cast(i32x4, *reinterpret_cast<const any_u32x4*>(w + (in ? at : 0)));
-                nw[u] = in ? v : i32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int n = 0; n < NC; ++n) {
+                    const i32x4 v = __builtin_bit_cast(i32x4, *reinterpret_cast<const any_u32x4*>(w[n] + (in ? at : 0)));
+                    nw[u][n] = in ? v : i32x4{0, 0, 0, 0};
+                }
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
                     nx[u][n] = __builtin_bit_cast(i32x4, *reinterpret_cast<const any_u32x4*>(x[n] + (in ? at : 0)));
             } else {
-                nw[u] = load_codes(w, at, a.cols);
+#pragma unroll
+                for (int n = 0; n < NC; ++n) nw[u][n] = load_codes(w[n], at, a.cols);
 #pragma unroll
                 for (int n = 0; n < NT; ++n) nx[u][n] = load_codes(x[n], at, a.cols);
             }
         }
     };
-    i32x4 sum[NT] = {};
+    i32x4 sum[NC][NT] = {};
     constexpr uint32_t kStep = 64 * U * WAVES;
     load(64 * U * wave);
     for (uint32_t k = 64 * U * wave; k < a.cols; k += kStep) {
-        i32x4 cw[U], cx[U][NT];
+        i32x4 cw[U][NC], cx[U][NT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            cw[u] = nw[u];
+#pragma unroll
+            for (int n = 0; n < NC; ++n) cw[u][n] = nw[u][n];
 #pragma unroll
             for (int n = 0; n < NT; ++n) cx[u][n] = nx[u][n];
         }
@@ -93,38 +103,49 @@ __global__ __launch_bounds__(64 * WAVES) void i8_stream_kernel(I8Args a) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) sum[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cw[u], cx[u][n], sum[n], 0, 0, 0);
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) sum[c][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cw[u][c], cx[u][n], sum[c][n], 0, 0, 0);
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n) part[wave][n][lane] = sum[n];
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) part[wave][c * NT + n][lane] = sum[c][n];
     __syncthreads();
-    for (uint32_t n = wave; n < NT; n += WAVES) {
-        i32x4 s = part[0][n][lane];
-        for (int i = 1; i < WAVES; ++i) s += part[i][n][lane];
-        const uint32_t t = t0 + 16 * n + (lane & 15);
+    for (uint32_t i = wave; i < NC * NT; i += WAVES) {
+        i32x4 s = part[0][i][lane];
+        for (int v = 1; v < WAVES; ++v) s += part[v][i][lane];
+        const uint32_t t = t0 + 16 * (i % NT) + (lane & 15);
         if (t >= a.n_tokens) continue;
         const float sa = a.sa[t];
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t c = r0 + 4 * (lane >> 4) + i;
-            if (c < a.rows) store_one(a.out_type, a.out, t * a.out_stride + c, scaled(s[i], sa, a.sw[c], a.bias, a.bias ? a.bias[c] : 0.0f));
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t c = r0 + 16 * (i / NT) + 4 * (lane >> 4) + j;
+            if (c < a.rows) store_one(a.out_type, a.out, t * a.out_stride + c, scaled(s[j], sa, a.sw[c], a.bias, a.bias ? a.bias[c] : 0.0f));
         }
     }
 }
 
-// Many tokens: a workgroup computes 32 TC WC channels by 32 TT WT tokens over 128 columns at a time.
-// These lie twice in LDS, rows of 128 bytes whose 16-byte chunks are exchanged by the row's last three
-// bits (chunk c of row r at c ^ (r & 7)), so that eight lanes that read one chunk of eight rows, or
-// write a row, touch all banks. The next columns travel through registers: written to the other
-// half midway, while those behind them are asked for.
-template <int WC, int WT, int TC, int TT, bool WHOLE>
-__global__ __launch_bounds__(64 * WC * WT) void i8_tile_kernel(I8Args a, uint32_t tiles_c, uint32_t tiles_t) {
-    constexpr uint32_t kThreads = 64 * WC * WT, kC = 32 * TC * WC, kT = 32 * TT * WT;
-    constexpr uint32_t kPer = kThreads / 8, kLoads = (kC + kT) / kPer, kLoadsC = kC / kPer;
+// More tokens: a workgroup computes 32 TC WC channels by 32 TT WT tokens, 128 KG columns a step; each
+// of KG groups of WC WT waves takes 128 of these, and the groups' sums are added at the end. A group's
+// columns lie twice in LDS, rows of 128 bytes whose 16-byte chunks are exchanged by the row (chunk c of
+// row r at c ^ (r / 2 % 8)), so that sixteen lanes that read one chunk of sixteen rows, or write two rows, touch all
+// 64 banks (a read of a wave: 4.4 cycles; exchanged by r % 8 it took 8.1, of rows as they are 32; a
+// write 13). The next AHEAD steps' columns travel in registers: the first of them
+// is written to the other half midway, and those behind the last are asked for in its place.
+template <int WC, int WT, int TC, int TT, int KG, int AHEAD, bool WHOLE>
+__global__ __launch_bounds__(64 * WC * WT * KG, 2) void i8_tile_kernel(I8Args a, uint32_t tiles_c, uint32_t tiles_t) {
+    constexpr uint32_t kGroup = 64 * WC * WT, kC = 32 * TC * WC, kT = 32 * TT * WT;
+    constexpr uint32_t kPer = kGroup / 8, kLoads = (kC + kT) / kPer, kLoadsC = kC / kPer;
     constexpr uint32_t kHalf = (kC + kT) * 128;
-    static_assert(kC % kPer == 0 && kT % kPer == 0 && TC % 2 == 0, "whole loads, pairs of channel tiles");
-    static_assert(2 * kHalf >= WC * WT * 32 * 68 * 4, "a wave's piece of the results fits");
-    __shared__ __attribute__((aligned(16))) char lds[2 * kHalf];
+    constexpr uint32_t kPitch = TC > 1 ? 68 : 36;  // words of a row of results
+    // Eight waves, two of a SIMD: they take turns, one multiplying while the other moves operands.
+    constexpr bool kTurns = WC * WT * KG == 8;
+    constexpr uint32_t kSums = (KG - 1) * kGroup * TC * TT * 64, kPieces = WC * WT * 32 * kPitch * 4;
+    constexpr uint32_t kBytes = 2 * KG * kHalf > kSums + kPieces ? 2 * KG * kHalf : kSums + kPieces;
+    static_assert(kC % kPer == 0 && kT % kPer == 0, "whole loads");
+    __shared__ __attribute__((aligned(16))) char lds[kBytes];
+    __shared__ float sh_sw[kC], sh_bias[kC], sh_sa[kT];
 
     // Workgroups of one XCD take tiles next to one another: eight tiles of tokens by some of channels.
     const uint32_t tiles = tiles_c * tiles_t, each = (tiles + 7) / 8;
@@ -134,7 +155,7 @@ __global__ __launch_bounds__(64 * WC * WT) void i8_tile_kernel(I8Args a, uint32_
     const uint32_t high = tiles_t - 8 * group < 8 ? tiles_t - 8 * group : 8;
     const uint32_t c0 = in / high * kC, t0 = (8 * group + in % high) * kT;
 
-    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t tid = threadIdx.x % kGroup, lane = tid & 63, wave = tid >> 6, kg = threadIdx.x / kGroup;
     const uint32_t wc = wave % WC, wt = wave / WC;
     const uint32_t chunk = tid & 7, first = tid >> 3;
 
@@ -151,88 +172,173 @@ __global__ __launch_bounds__(64 * WC * WT) void i8_tile_kernel(I8Args a, uint32_
         const uint32_t r = first + kPer * (j < kLoadsC ? j : j - kLoadsC), n = j < kLoadsC ? rows_c : rows_t;
         from[j] = (r < n ? r : n - 1) * static_cast<uint32_t>(j < kLoadsC ? a.w_stride : a.a_stride);
     }
-    i32x4 stage[kLoads];
-    auto load = [&](uint32_t k0) {
-        const uint32_t k = k0 + 16 * chunk;
+    i32x4 stage[AHEAD][kLoads];
+    auto load = [&](i32x4 (&v)[kLoads], uint32_t step, uint32_t j0, uint32_t j1) {
+        const uint32_t k = 128 * (step * KG + kg) + 16 * chunk;
 #pragma unroll
-        for (uint32_t j = 0; j < kLoads; ++j) {
+        for (uint32_t j = j0; j < j1; ++j) {
             if constexpr (WHOLE) {  // columns past the last are out of the buffer's range: zeros
                 const int at = k < a.cols ? static_cast<int>(from[j] + k) : -1;
-                stage[j] = __builtin_bit_cast(i32x4, j < kLoadsC ? __builtin_amdgcn_raw_buffer_load_b128(rs_c, at, 0, 0)
-                                                                 : __builtin_amdgcn_raw_buffer_load_b128(rs_t, at, 0, 0));
+                v[j] = __builtin_bit_cast(i32x4, j < kLoadsC ? __builtin_amdgcn_raw_buffer_load_b128(rs_c, at, 0, 0)
+                                                             : __builtin_amdgcn_raw_buffer_load_b128(rs_t, at, 0, 0));
             } else {
-                stage[j] = load_codes((j < kLoadsC ? base_c : base_t) + from[j], k, a.cols);
+                v[j] = load_codes((j < kLoadsC ? base_c : base_t) + from[j], k, a.cols);
             }
         }
     };
-    const uint32_t to = first * 128 + 16 * (chunk ^ (first & 7));
-    auto put = [&](uint32_t half) {
+    char* const mine = lds + kg * 2 * kHalf;
+    auto put = [&](const i32x4 (&v)[kLoads], uint32_t half, uint32_t j0, uint32_t j1) {
 #pragma unroll
-        for (uint32_t j = 0; j < kLoads; ++j) *reinterpret_cast<i32x4*>(lds + half * kHalf + to + j * kPer * 128) = stage[j];
+        for (uint32_t j = j0; j < j1; ++j) {
+            const uint32_t turn = kPer % 16 ? (first + kPer * j) / 2 % 8 : first / 2 % 8;
+            *reinterpret_cast<i32x4*>(mine + half * kHalf + (first + kPer * j) * 128 + 16 * (chunk ^ turn)) = v[j];
+        }
     };
 
-    const uint32_t at_c = (wc * 32 * TC + (lane & 31)) * 128 + 16 * ((lane >> 5) ^ (lane & 7));
-    const uint32_t at_t = (kC + wt * 32 * TT + (lane & 31)) * 128 + 16 * ((lane >> 5) ^ (lane & 7));
+    const uint32_t at_c = (wc * 32 * TC + (lane & 31)) * 128 + 16 * ((lane >> 5) ^ (lane / 2 % 8));
+    const uint32_t at_t = (kC + wt * 32 * TT + (lane & 31)) * 128 + 16 * ((lane >> 5) ^ (lane / 2 % 8));
     i32x16 sum[TC][TT] = {};
-    const uint32_t steps = (a.cols + 127) / 128;
-    load(0);
-    put(0);
-    if (steps > 1) load(128);
+    const uint32_t steps = (a.cols + 128 * KG - 1) / (128 * KG);
+    load(stage[0], 0, 0, kLoads);
+    for (uint32_t i = threadIdx.x; i < kC; i += kGroup * KG) {
+        const bool there = i < rows_c;
+        sh_sw[i] = there ? a.sw[c0 + i] : 0.0f;
+        sh_bias[i] = there && a.bias ? a.bias[c0 + i] : 0.0f;
+    }
+    for (uint32_t i = threadIdx.x; i < kT; i += kGroup * KG) sh_sa[i] = i < rows_t ? a.sa[t0 + i] : 0.0f;
+    put(stage[0], 0, 0, kLoads);
+    // (Loads keep their order, so that a wait for one step's leaves the later ones in flight.)
+#pragma unroll
+    for (uint32_t d = 0; d < AHEAD; ++d) {
+        load(stage[d], 1 + d, 0, kLoads);
+        __builtin_amdgcn_sched_barrier(0);
+    }
     __syncthreads();
-    for (uint32_t s = 0; s < steps; ++s) {
+    i32x4 c[2][TC], t[2][TT];  // operands of two quarters
+    auto take = [&](uint32_t half, uint32_t q) {
+#pragma unroll
+        for (uint32_t i = 0; i < TC; ++i) c[q & 1][i] = *reinterpret_cast<const i32x4*>(mine + half * kHalf + (at_c ^ (32 * q)) + i * 4096);
+#pragma unroll
+        for (uint32_t i = 0; i < TT; ++i) t[q & 1][i] = *reinterpret_cast<const i32x4*>(mine + half * kHalf + (at_t ^ (32 * q)) + i * 4096);
+    };
+    auto multiply = [&](uint32_t q) {
+#pragma unroll
+        for (uint32_t i = 0; i < TC; ++i)
+#pragma unroll
+            for (uint32_t n = 0; n < TT; ++n)
+                sum[i][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(c[q & 1][i], t[q & 1][n], sum[i][n], 0, 0, 0);
+    };
+    auto meet = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto step = [&](i32x4 (&v)[kLoads], uint32_t s) {
         const uint32_t half = s & 1;
+        if constexpr (kTurns) {
 #pragma unroll
-        for (uint32_t q = 0; q < 4; ++q) {
-            i32x4 c[TC], t[TT];
+            for (uint32_t h = 0; h < 2; ++h) {
+                take(half, 2 * h);
+                take(half, 2 * h + 1);
+                put(v, half ^ 1, h * kLoads / 2, (h + 1) * kLoads / 2);
+                load(v, s + 1 + AHEAD, h * kLoads / 2, (h + 1) * kLoads / 2);
+                meet();
+                __builtin_amdgcn_s_setprio(1);
+                multiply(0);
+                multiply(1);
+                __builtin_amdgcn_s_setprio(0);
+                meet();
+            }
+        } else {
 #pragma unroll
-            for (uint32_t i = 0; i < TC; ++i) c[i] = *reinterpret_cast<const i32x4*>(lds + half * kHalf + (at_c ^ (32 * q)) + i * 4096);
+            for (uint32_t q = 0; q < 4; ++q) {
+                if (q < 3) {
+                    take(half, q + 1);
+                } else {
+                    __syncthreads();
+                    take(half ^ 1, 0);
+                }
+                if (q == 1) {
+                    put(v, half ^ 1, 0, kLoads);
+                    __builtin_amdgcn_sched_barrier(0);
+                    load(v, s + 1 + AHEAD, 0, kLoads);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(q);
+            }
+        }
+    };
+    const bool second = kTurns && __builtin_amdgcn_readfirstlane(threadIdx.x) >= 256;
+    if (second) meet();
+    if constexpr (!kTurns) take(0, 0);
+    // Whole groups of AHEAD steps, then what is left: a way out of the loop's middle would leave the
+    // order of loads unknown at its top.
+    uint32_t s = 0;
+    for (; s + AHEAD <= steps; s += AHEAD)
 #pragma unroll
-            for (uint32_t i = 0; i < TT; ++i) t[i] = *reinterpret_cast<const i32x4*>(lds + half * kHalf + (at_t ^ (32 * q)) + i * 4096);
+        for (uint32_t d = 0; d < AHEAD; ++d) step(stage[d], s + d);
+#pragma unroll
+    for (uint32_t d = 0; d + 1 < AHEAD; ++d)
+        if (s + d < steps) step(stage[d], s + d);
+    if (kTurns && !second) meet();
+    __syncthreads();
+
+    if constexpr (KG > 1) {
+        i32x4* others = reinterpret_cast<i32x4*>(lds + kPieces);
+        auto at = [&](uint32_t g, uint32_t i, uint32_t n, uint32_t v) { return ((((g - 1) * TC + i) * TT + n) * 4 + v) * kGroup + tid; };
+#pragma unroll
+        for (uint32_t i = 0; i < TC; ++i)
+#pragma unroll
+            for (uint32_t n = 0; n < TT; ++n)
+#pragma unroll
+                for (uint32_t v = 0; v < 4; ++v)
+                    if (kg) others[at(kg, i, n, v)] = i32x4{sum[i][n][4 * v], sum[i][n][4 * v + 1], sum[i][n][4 * v + 2], sum[i][n][4 * v + 3]};
+        __syncthreads();
+        if (kg) return;
+#pragma unroll
+        for (uint32_t g = 1; g < KG; ++g)
 #pragma unroll
             for (uint32_t i = 0; i < TC; ++i)
 #pragma unroll
-                for (uint32_t n = 0; n < TT; ++n) sum[i][n] = __builtin_amdgcn_mfma_i32_32x32x32_i8(c[i], t[n], sum[i][n], 0, 0, 0);
-            if (q == 1 && s + 1 < steps) {
-                put(half ^ 1);
-                if (s + 2 < steps) load(128 * (s + 2));
-            }
-        }
-        __syncthreads();
+                for (uint32_t n = 0; n < TT; ++n)
+#pragma unroll
+                    for (uint32_t v = 0; v < 4; ++v) {
+                        const i32x4 o = others[at(g, i, n, v)];
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e) sum[i][n][4 * v + e] += o[e];
+                    }
     }
 
-    // Results by way of LDS, 32 tokens by 64 channels of a wave at a time, so that eight lanes write
-    // 64 neighbouring channels of a token. (A lane of the product holds channels 8 g + 4 (lane / 32) +
-    // 0 .. 3 of token lane % 32.)
-    int32_t* piece = reinterpret_cast<int32_t*>(lds) + wave * 32 * 68;
+    // Results by way of LDS, 32 tokens by 64 (32) channels of a wave at a time, so that eight (four)
+    // lanes write neighbouring channels of a token. (A lane of the product holds channels
+    // 8 g + 4 (lane / 32) + 0 .. 3 of token lane % 32.)
+    int32_t* piece = reinterpret_cast<int32_t*>(lds) + wave * 32 * kPitch;
 #pragma unroll
     for (uint32_t n = 0; n < TT; ++n)
 #pragma unroll
-        for (uint32_t p = 0; p < TC / 2; ++p) {
+        for (uint32_t p = 0; p < TC; p += 2) {
+            const uint32_t tiles_here = p + 1 < TC ? 2 : 1, lanes = 4 * tiles_here;  // of a token's row
 #pragma unroll
-            for (uint32_t i = 0; i < 2; ++i)
+            for (uint32_t i = 0; i < tiles_here; ++i)
 #pragma unroll
                 for (uint32_t g = 0; g < 4; ++g)
-                    *reinterpret_cast<i32x4*>(piece + (lane & 31) * 68 + 32 * i + 8 * g + 4 * (lane >> 5)) =
-                        i32x4{sum[2 * p + i][n][4 * g], sum[2 * p + i][n][4 * g + 1], sum[2 * p + i][n][4 * g + 2], sum[2 * p + i][n][4 * g + 3]};
-            const uint32_t c = c0 + wc * 32 * TC + 64 * p + 8 * (lane & 7);
-            const uint32_t left = c < a.rows ? (a.rows - c < 8 ? a.rows - c : 8) : 0;
+                    *reinterpret_cast<i32x4*>(piece + (lane & 31) * kPitch + 32 * i + 8 * g + 4 * (lane >> 5)) =
+                        i32x4{sum[p + i][n][4 * g], sum[p + i][n][4 * g + 1], sum[p + i][n][4 * g + 2], sum[p + i][n][4 * g + 3]};
+            const uint32_t at = 8 * (lane % lanes), in_c = wc * 32 * TC + 32 * p + at;
+            const uint32_t left = in_c < rows_c ? (rows_c - in_c < 8 ? rows_c - in_c : 8) : 0;
             float sw[8], bias[8];
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                sw[i] = i < left ? a.sw[c + i] : 0.0f;
-                bias[i] = i < left && a.bias ? a.bias[c + i] : 0.0f;
-            }
+            for (uint32_t i = 0; i < 8; ++i) sw[i] = sh_sw[in_c + i], bias[i] = sh_bias[in_c + i];
 #pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) {
-                const uint32_t row = 8 * j + (lane >> 3), t = t0 + wt * 32 * TT + 32 * n + row;
-                if (t >= a.n_tokens || !left) continue;
-                const i32x4 u = *reinterpret_cast<const i32x4*>(piece + row * 68 + 8 * (lane & 7));
-                const i32x4 v = *reinterpret_cast<const i32x4*>(piece + row * 68 + 8 * (lane & 7) + 4);
-                const float sa = a.sa[t];
+            for (uint32_t j = 0; j < lanes / 2; ++j) {
+                const uint32_t row = j * (64 / lanes) + lane / lanes, in_t = wt * 32 * TT + 32 * n + row;
+                const i32x4 u = *reinterpret_cast<const i32x4*>(piece + row * kPitch + at);
+                const i32x4 v = *reinterpret_cast<const i32x4*>(piece + row * kPitch + at + 4);
+                const float sa = sh_sa[in_t];
                 float y[8];
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i) y[i] = scaled(i < 4 ? u[i & 3] : v[i & 3], sa, sw[i], a.bias, bias[i]);
-                store_floats(a.out_type, a.out, t * a.out_stride + c, left, y);
+                if (in_t < rows_t && left) store_floats(a.out_type, a.out, (t0 + in_t) * a.out_stride + c0 + in_c, left, y);
             }
         }
 }
@@ -245,35 +351,81 @@ namespace {
 
 constexpr uint64_t kMaxCols = 131071;  // sums of products of codes from -128 on stay below 2^31
 
-template <int NT, int U>
+template <int WAVES, int NC, int NT, int U>
 void launch_stream(hipStream_t s, const I8Args& a, bool whole) {
-    const dim3 grid((a.rows + 15) / 16, (a.n_tokens + 16 * NT - 1) / (16 * NT));
-    if (whole) hipLaunchKernelGGL((i8_stream_kernel<4, NT, U, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((i8_stream_kernel<4, NT, U, false>), grid, dim3(256), 0, s, a);
+    const dim3 grid((a.rows + 16 * NC - 1) / (16 * NC), (a.n_tokens + 16 * NT - 1) / (16 * NT)), block(64 * WAVES);
+    if (whole) hipLaunchKernelGGL((i8_stream_kernel<WAVES, NC, NT, U, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((i8_stream_kernel<WAVES, NC, NT, U, false>), grid, block, 0, s, a);
 }
 
-template <int WC, int WT, int TC, int TT>
-void launch_tile(hipStream_t s, const I8Args& a, bool whole) {
+template <int WC, int WT, int TC, int TT, int KG, int AHEAD, bool WHOLE>
+void launch_tile(hipStream_t s, const I8Args& a) {
     const uint32_t tc = (a.rows + 32 * TC * WC - 1) / (32 * TC * WC), tt = (a.n_tokens + 32 * TT * WT - 1) / (32 * TT * WT);
-    const dim3 grid((tc * tt + 7) / 8 * 8), block(64 * WC * WT);
-    if (whole) hipLaunchKernelGGL((i8_tile_kernel<WC, WT, TC, TT, true>), grid, block, 0, s, a, tc, tt);
-    else hipLaunchKernelGGL((i8_tile_kernel<WC, WT, TC, TT, false>), grid, block, 0, s, a, tc, tt);
+    hipLaunchKernelGGL((i8_tile_kernel<WC, WT, TC, TT, KG, AHEAD, WHOLE>), dim3((tc * tt + 7) / 8 * 8), dim3(64 * WC * WT * KG), 0, s, a, tc, tt);
+}
+
+// What a tile costs, in us, measured over batches of 17 to 8192 tokens and matrices of 512 to 151936
+// channels by 2048 to 14336 columns: `fixed` around the columns; for 128 columns `low` where a CU has one
+// workgroup and few others run, `full` a workgroup of a full card, where the products of real codes
+// draw the clock down (8192^3: 450 us, of zeros 318). `resident` workgroups share a CU.
+struct TileCost {
+    uint32_t channels, tokens, resident;
+    double fixed, low, full;
+};
+enum : int { kTile256, kTile128x256, kTile128, kTile64x128, kTile64, kTile32x64, kTile32, kTiles };
+constexpr TileCost kTileCosts[kTiles] = {
+    {256, 256, 1, 6.7, 1.03, 1.70}, {128, 256, 1, 5.1, 0.85, 1.15}, {128, 128, 2, 3.7, 0.65, 0.60}, {64, 128, 3, 3.9, 0.42, 0.39},
+    {64, 64, 4, 3.6, 0.30, 0.23},   {32, 64, 1, 4.2, 0.21, 0.22},   {32, 32, 1, 4.9, 0.15, 0.16},
+};
+
+// The tile that would take the least time: large ones do the most products for what they load, but
+// few of them leave CUs idle, and rounds of them the last one part empty (2048 tokens of 4096 to
+// 4096: 256 x 256 47 us, 128 x 256 43; 4096 tokens: 65 and 84. 64 tokens of 14336 to 4096: 64 x 64 38,
+// 32 x 32 with eight groups along the columns 22; 64 of 4096 to 14336: 18 and 37).
+int best_tile(const I8Args& a) {
+    const double steps = (a.cols + 127) / 128;
+    int best = 0;
+    double least = 0;
+    for (int i = 0; i < kTiles; ++i) {
+        const TileCost& c = kTileCosts[i];
+        const double tiles = static_cast<double>((a.rows + c.channels - 1) / c.channels) * ((a.n_tokens + c.tokens - 1) / c.tokens);
+        const double each = ceil(tiles / 256);  // of the CU with most
+        double us;
+        if (c.resident > 1) {
+            const double step = each * c.full > c.low ? each * c.full : c.low;
+            us = c.fixed + steps * step;
+        } else {
+            const double busy = tiles < 256 ? tiles / 256 : 1;
+            us = each * (c.fixed + steps * (c.low + (c.full - c.low) * busy));
+        }
+        if (i == 0 || us < least) best = i, least = us;
+    }
+    return best;
 }
 
 int32_t launch_i8(hipStream_t s, const I8Args& a, const char* action) {
     // Whole chunks of 16 codes, each at a multiple of 16 bytes.
     const bool whole = (a.cols | a.a_stride | a.w_stride | reinterpret_cast<uintptr_t>(a.a) | reinterpret_cast<uintptr_t>(a.w)) % 16 == 0;
     const bool near = a.a_stride < (1u << 22) && a.w_stride < (1u << 22);  // a tile's rows within a buffer's 32-bit range
-    const uint64_t big = static_cast<uint64_t>((a.rows + 255) / 256) * ((a.n_tokens + 255) / 256);
-    if (!near || a.n_tokens <= 64) {
-        if (a.n_tokens <= 16) launch_stream<1, 4>(s, a, whole);
-        else if (a.n_tokens <= 32) launch_stream<2, 4>(s, a, whole);
-        else if (a.n_tokens <= 48) launch_stream<3, 2>(s, a, whole);
-        else launch_stream<4, 2>(s, a, whole);
-    } else if (big >= 128) {
-        launch_tile<2, 4, 4, 2>(s, a, whole);
+    if (a.n_tokens <= 16 || !near) {
+        // 16 channels a workgroup where these are few, 32 otherwise, whose tokens' codes are read half as
+        // often (one token, 4096 of 14336 columns: 12.9 and 18.0 us; 151936 of 4096: 123 and 109)
+        if (a.rows <= 8192) launch_stream<8, 1, 1, 4>(s, a, whole);
+        else launch_stream<8, 2, 1, 2>(s, a, whole);
+    } else if (!whole) {
+        const bool many = static_cast<uint64_t>((a.rows + 127) / 128) * ((a.n_tokens + 127) / 128) >= 256;
+        if (many) launch_tile<2, 2, 2, 2, 1, 1, false>(s, a);
+        else launch_tile<2, 2, 1, 1, 1, 2, false>(s, a);
     } else {
-        launch_tile<2, 2, 2, 2>(s, a, whole);
+        switch (best_tile(a)) {
+            case kTile256: launch_tile<2, 4, 4, 2, 1, 1, true>(s, a); break;
+            case kTile128x256: launch_tile<2, 4, 2, 2, 1, 2, true>(s, a); break;
+            case kTile128: launch_tile<2, 2, 2, 2, 1, 2, true>(s, a); break;
+            case kTile64x128: launch_tile<2, 2, 1, 2, 1, 3, true>(s, a); break;
+            case kTile64: launch_tile<2, 2, 1, 1, 1, 3, true>(s, a); break;
+            case kTile32x64: launch_tile<1, 2, 1, 1, 4, 2, true>(s, a); break;
+            default: launch_tile<1, 1, 1, 1, 8, 3, true>(s, a); break;
+        }
     }
     OBJ_HIP(hipGetLastError(), action);
     return 0;
