@@ -83,7 +83,8 @@ enum WsSlot : int {
     kWsPages = 8,     // free pages, copies and staged tables of the cache's page operations
     kWsAttn = 9,      // partial sums of attention over a cache cut along its length
     kWsLogProbs = 10,  // sums and best tokens of rows cut over workgroups
-    kWsSlots = 11
+    kWsCodes = 11,     // 8-bit rows copied to whole chunks
+    kWsSlots = 12
 };
 
 // The scratch of one stream. Calls on different streams of a context may be in

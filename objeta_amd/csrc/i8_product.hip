@@ -8,6 +8,7 @@
 #include "kernels.hpp"
 
 #include <cmath>
+#include <type_traits>
 
 namespace objeta {
 namespace dev {
@@ -24,12 +25,43 @@ struct I8Args {
     int32_t out_type;
 };
 
-// Sixteen codes of a row from column k on; columns past the last are 0.
-__device__ __forceinline__ i32x4 load_codes(const int8_t* row, uint32_t k, uint32_t cols) {
-    if (k + 16 <= cols) return __builtin_bit_cast(i32x4, *reinterpret_cast<const any_u32x4*>(row + k));
+typedef uint32_t word_u32x4 __attribute__((ext_vector_type(4), aligned(4)));
+
+__device__ __forceinline__ i32x4 load16(const int8_t* p) { return __builtin_bit_cast(i32x4, *reinterpret_cast<const word_u32x4*>(p)); }
+
+// Rows that begin anywhere: loads off a word's boundary take twice as long, so that the whole words
+// around sixteen codes are read and moved together when they are used.
+struct Raw16 {
+    i32x4 v;
+    uint32_t w;
+};
+// The words of the sixteen codes at base + off, base a multiple of 4; a fifth one where they reach into it.
+__device__ __forceinline__ Raw16 load_raw16(const int8_t* base, uint32_t off) {
+    const int8_t* p = base + (off & ~3u);
+    return Raw16{load16(p), *reinterpret_cast<const uint32_t*>(base + ((off & ~3u) + (off & 3 ? 16 : 12)))};
+}
+__device__ __forceinline__ i32x4 straight(const Raw16& r, uint32_t off) {
+    const uint32_t a = r.v[0], b = r.v[1], c = r.v[2], d = r.v[3], n = off & 3;
+    return i32x4{static_cast<int32_t>(__builtin_amdgcn_alignbyte(b, a, n)), static_cast<int32_t>(__builtin_amdgcn_alignbyte(c, b, n)),
+                 static_cast<int32_t>(__builtin_amdgcn_alignbyte(d, c, n)), static_cast<int32_t>(__builtin_amdgcn_alignbyte(r.w, d, n))};
+}
+// Sixteen codes moved down by n, zeros behind them.
+__device__ __forceinline__ i32x4 moved(const i32x4& v, uint32_t n) {
+    uint64_t lo = static_cast<uint32_t>(v[0]) | static_cast<uint64_t>(static_cast<uint32_t>(v[1])) << 32;
+    uint64_t hi = static_cast<uint32_t>(v[2]) | static_cast<uint64_t>(static_cast<uint32_t>(v[3])) << 32;
+    const uint32_t bits = 8 * (n & 7);
+    if (n >= 16) lo = hi = 0;
+    if (n >= 8) lo = hi, hi = 0;
+    if (bits) lo = lo >> bits | hi << (64 - bits), hi >>= bits;
+    return i32x4{static_cast<int32_t>(lo), static_cast<int32_t>(lo >> 32), static_cast<int32_t>(hi), static_cast<int32_t>(hi >> 32)};
+}
+// Where a row's sixteen codes from column k on are read: past its last sixteen, there (and moved down).
+__device__ __forceinline__ uint32_t read_at(uint32_t k, uint32_t cols) { return k + 16 <= cols ? k : cols - 16; }
+// Codes of a row of fewer than sixteen.
+__device__ __forceinline__ i32x4 load_few(const int8_t* row, uint32_t k, uint32_t cols) {
     uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
-    for (uint32_t i = 0; i < 16; ++i)
+    for (uint32_t i = 0; i < 15; ++i)
         if (k + i < cols) v[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + i])) << (8 * (i % 4));
     return i32x4{static_cast<int32_t>(v[0]), static_cast<int32_t>(v[1]), static_cast<int32_t>(v[2]), static_cast<int32_t>(v[3])};
 }
@@ -51,61 +83,64 @@ __device__ __forceinline__ void store_one(int32_t type, void* out, uint64_t at, 
 template <int WAVES, int NC, int NT, int U, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES) void i8_stream_kernel(I8Args a) {
     __shared__ i32x4 part[WAVES][NC * NT][64];
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t r0 = 16 * NC * blockIdx.x, t0 = 16 * NT * blockIdx.y;
-    const int8_t *w[NC], *x[NT];
+    constexpr int kRows = NC + NT;
+    const int8_t* row[kRows];  // channels, then tokens (the last one again past it)
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-        const uint32_t r = r0 + 16 * n + (lane & 15);
-        w[n] = a.w + (r < a.rows ? r : a.rows - 1) * a.w_stride;
+    for (int n = 0; n < kRows; ++n) {
+        const uint32_t i = (n < NC ? r0 + 16 * n : t0 + 16 * (n - NC)) + (lane & 15), all = n < NC ? a.rows : a.n_tokens;
+        row[n] = (n < NC ? a.w : a.a) + (i < all ? i : all - 1) * (n < NC ? a.w_stride : a.a_stride);
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const uint32_t t = t0 + 16 * n + (lane & 15);
-        x[n] = a.a + (t < a.n_tokens ? t : a.n_tokens - 1) * a.a_stride;
-    }
-    i32x4 nw[U][NC], nx[U][NT];
+    typedef typename std::conditional<WHOLE, i32x4, Raw16>::type Raw;
+    Raw next[U][kRows];
     auto load = [&](uint32_t k) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const uint32_t at = k + 64 * u + 16 * (lane >> 4);
-            if constexpr (WHOLE) {  // past the last column: channels' codes 0, tokens' any
-                const bool in = at < a.cols;
+        for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int n = 0; n < NC; ++n) {
-                    const i32x4 v = __builtin_bit_cast(i32x4, *reinterpret_cast<const any_u32x4*>(w[n] + (in ? at : 0)));
-                    nw[u][n] = in ? v : i32x4{0, 0, 0, 0};
+            for (int n = 0; n < kRows; ++n) {
+                const uint32_t at = k + 64 * u + 16 * (lane >> 4);
+                if constexpr (WHOLE) {
+                    next[u][n] = load16(row[n] + (at < a.cols ? at : 0));
+                } else if (a.cols >= 16) {
+                    const uint64_t p = reinterpret_cast<uint64_t>(row[n]);
+                    next[u][n] = load_raw16(reinterpret_cast<const int8_t*>(p & ~uint64_t(3)), static_cast<uint32_t>(p & 3) + read_at(at, a.cols));
+                } else {
+                    next[u][n] = Raw16{load_few(row[n], at, a.cols), 0};
                 }
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    nx[u][n] = __builtin_bit_cast(i32x4, *reinterpret_cast<const any_u32x4*>(x[n] + (in ? at : 0)));
-            } else {
-#pragma unroll
-                for (int n = 0; n < NC; ++n) nw[u][n] = load_codes(w[n], at, a.cols);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) nx[u][n] = load_codes(x[n], at, a.cols);
             }
+    };
+    // past the last column: channels' codes 0, tokens' any
+    auto codes = [&](const Raw& r, int n, uint32_t k, uint32_t at) {
+        if constexpr (WHOLE) {
+            return n < NC && at >= a.cols ? i32x4{0, 0, 0, 0} : r;
+        } else {
+            if (a.cols < 16) return r.v;
+            const uint32_t from = read_at(at, a.cols);
+            const i32x4 v = straight(r, static_cast<uint32_t>(reinterpret_cast<uint64_t>(row[n])) + from);
+            return k + 64 <= a.cols ? v : moved(v, at - from);
         }
     };
     i32x4 sum[NC][NT] = {};
     constexpr uint32_t kStep = 64 * U * WAVES;
     load(64 * U * wave);
     for (uint32_t k = 64 * U * wave; k < a.cols; k += kStep) {
-        i32x4 cw[U][NC], cx[U][NT];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-            for (int n = 0; n < NC; ++n) cw[u][n] = nw[u][n];
-#pragma unroll
-            for (int n = 0; n < NT; ++n) cx[u][n] = nx[u][n];
-        }
-        if (k + kStep < a.cols) load(k + kStep);
+        Raw now[U][kRows];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
+            for (int n = 0; n < kRows; ++n) now[u][n] = next[u][n];
+        if (k + kStep < a.cols) load(k + kStep);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            i32x4 v[kRows];
+#pragma unroll
+            for (int n = 0; n < kRows; ++n) v[n] = codes(now[u][n], n, k + 64 * u, k + 64 * u + 16 * (lane >> 4));
+#pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int n = 0; n < NT; ++n) sum[c][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(cw[u][c], cx[u][n], sum[c][n], 0, 0, 0);
+                for (int n = 0; n < NT; ++n) sum[c][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[c], v[NC + n], sum[c][n], 0, 0, 0);
+        }
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -155,7 +190,8 @@ __global__ __launch_bounds__(64 * WC * WT * KG, 2) void i8_tile_kernel(I8Args a,
     const uint32_t high = tiles_t - 8 * group < 8 ? tiles_t - 8 * group : 8;
     const uint32_t c0 = in / high * kC, t0 = (8 * group + in % high) * kT;
 
-    const uint32_t tid = threadIdx.x % kGroup, lane = tid & 63, wave = tid >> 6, kg = threadIdx.x / kGroup;
+    const uint32_t tid = threadIdx.x % kGroup, lane = tid & 63, wave = tid >> 6;
+    const uint32_t kg = __builtin_amdgcn_readfirstlane(threadIdx.x / kGroup);
     const uint32_t wc = wave % WC, wt = wave / WC;
     const uint32_t chunk = tid & 7, first = tid >> 3;
 
@@ -172,8 +208,13 @@ __global__ __launch_bounds__(64 * WC * WT * KG, 2) void i8_tile_kernel(I8Args a,
         const uint32_t r = first + kPer * (j < kLoadsC ? j : j - kLoadsC), n = j < kLoadsC ? rows_c : rows_t;
         from[j] = (r < n ? r : n - 1) * static_cast<uint32_t>(j < kLoadsC ? a.w_stride : a.a_stride);
     }
-    i32x4 stage[AHEAD][kLoads];
-    auto load = [&](i32x4 (&v)[kLoads], uint32_t step, uint32_t j0, uint32_t j1) {
+    typedef typename std::conditional<WHOLE, i32x4, Raw16>::type Raw;
+    typedef Raw Stage[kLoads];
+    Stage stage[AHEAD];
+    // (rows that begin anywhere are addressed from the word ahead of the first)
+    const uint32_t low_c = reinterpret_cast<uint64_t>(base_c) & 3, low_t = reinterpret_cast<uint64_t>(base_t) & 3;
+    const uint32_t last = a.cols < 16 ? 0 : a.cols - 16;
+    auto load = [&](Stage& v, uint32_t step, uint32_t j0, uint32_t j1) {
         const uint32_t k = 128 * (step * KG + kg) + 16 * chunk;
 #pragma unroll
         for (uint32_t j = j0; j < j1; ++j) {
@@ -182,16 +223,25 @@ __global__ __launch_bounds__(64 * WC * WT * KG, 2) void i8_tile_kernel(I8Args a,
                 v[j] = __builtin_bit_cast(i32x4, j < kLoadsC ? __builtin_amdgcn_raw_buffer_load_b128(rs_c, at, 0, 0)
                                                              : __builtin_amdgcn_raw_buffer_load_b128(rs_t, at, 0, 0));
             } else {
-                v[j] = load_codes((j < kLoadsC ? base_c : base_t) + from[j], k, a.cols);
+                const uint32_t low = j < kLoadsC ? low_c : low_t;
+                v[j] = load_raw16((j < kLoadsC ? base_c : base_t) - low, low + from[j] + (k < last ? k : last));
             }
         }
     };
     char* const mine = lds + kg * 2 * kHalf;
-    auto put = [&](const i32x4 (&v)[kLoads], uint32_t half, uint32_t j0, uint32_t j1) {
+    auto put = [&](const Stage& v, uint32_t step, uint32_t j0, uint32_t j1) {
 #pragma unroll
         for (uint32_t j = j0; j < j1; ++j) {
             const uint32_t turn = kPer % 16 ? (first + kPer * j) / 2 % 8 : first / 2 % 8;
-            *reinterpret_cast<i32x4*>(mine + half * kHalf + (first + kPer * j) * 128 + 16 * (chunk ^ turn)) = v[j];
+            i32x4 x;
+            if constexpr (WHOLE) {
+                x = v[j];
+            } else {
+                const uint32_t k0 = 128 * (step * KG + kg), k = k0 + 16 * chunk, at = k < last ? k : last;
+                x = straight(v[j], (j < kLoadsC ? low_c : low_t) + from[j] + at);
+                if (k0 + 128 > a.cols) x = moved(x, k - at);
+            }
+            *reinterpret_cast<i32x4*>(mine + (step & 1) * kHalf + (first + kPer * j) * 128 + 16 * (chunk ^ turn)) = x;
         }
     };
 
@@ -233,14 +283,14 @@ __global__ __launch_bounds__(64 * WC * WT * KG, 2) void i8_tile_kernel(I8Args a,
         __syncthreads();
         __builtin_amdgcn_sched_barrier(0);
     };
-    auto step = [&](i32x4 (&v)[kLoads], uint32_t s) {
+    auto step = [&](Stage& v, uint32_t s) {
         const uint32_t half = s & 1;
         if constexpr (kTurns) {
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
                 take(half, 2 * h);
                 take(half, 2 * h + 1);
-                put(v, half ^ 1, h * kLoads / 2, (h + 1) * kLoads / 2);
+                put(v, s + 1, h * kLoads / 2, (h + 1) * kLoads / 2);
                 load(v, s + 1 + AHEAD, h * kLoads / 2, (h + 1) * kLoads / 2);
                 meet();
                 __builtin_amdgcn_s_setprio(1);
@@ -259,7 +309,7 @@ __global__ __launch_bounds__(64 * WC * WT * KG, 2) void i8_tile_kernel(I8Args a,
                     take(half ^ 1, 0);
                 }
                 if (q == 1) {
-                    put(v, half ^ 1, 0, kLoads);
+                    put(v, s + 1, 0, kLoads);
                     __builtin_amdgcn_sched_barrier(0);
                     load(v, s + 1 + AHEAD, 0, kLoads);
                 }
@@ -343,6 +393,19 @@ __global__ __launch_bounds__(64 * WC * WT * KG, 2) void i8_tile_kernel(I8Args a,
         }
 }
 
+// Rows that begin anywhere copied to multiples of 16 bytes, zeros up to these behind them.
+__global__ __launch_bounds__(256) void i8_straighten_kernel(const int8_t* from, uint64_t stride, uint32_t rows, uint32_t cols, int8_t* to) {
+    const uint32_t chunks = (cols + 15) / 16;
+    const uint64_t all = static_cast<uint64_t>(rows) * chunks;
+    for (uint64_t i = static_cast<uint64_t>(blockIdx.x) * 256 + threadIdx.x; i < all; i += static_cast<uint64_t>(gridDim.x) * 256) {
+        const uint32_t r = static_cast<uint32_t>(i / chunks), k = 16 * static_cast<uint32_t>(i % chunks), at = read_at(k, cols);
+        const uint64_t p = reinterpret_cast<uint64_t>(from + r * stride);
+        const uint32_t off = static_cast<uint32_t>(p & 3) + at;
+        const i32x4 v = straight(load_raw16(reinterpret_cast<const int8_t*>(p & ~uint64_t(3)), off), off);
+        reinterpret_cast<i32x4*>(to)[i] = at == k ? v : moved(v, k - at);
+    }
+}
+
 }  // namespace dev
 
 using namespace dev;
@@ -363,6 +426,12 @@ void launch_tile(hipStream_t s, const I8Args& a) {
     const uint32_t tc = (a.rows + 32 * TC * WC - 1) / (32 * TC * WC), tt = (a.n_tokens + 32 * TT * WT - 1) / (32 * TT * WT);
     hipLaunchKernelGGL((i8_tile_kernel<WC, WT, TC, TT, KG, AHEAD, WHOLE>), dim3((tc * tt + 7) / 8 * 8), dim3(64 * WC * WT * KG), 0, s, a, tc, tt);
 }
+// (Rows that begin anywhere need registers for moving them and load one step ahead.)
+template <int WC, int WT, int TC, int TT, int KG, int AHEAD>
+void launch_either(hipStream_t s, const I8Args& a, bool whole) {
+    if (whole) launch_tile<WC, WT, TC, TT, KG, AHEAD, true>(s, a);
+    else launch_tile<WC, WT, TC, TT, KG, 1, false>(s, a);
+}
 
 // What a tile costs, in us, measured over batches of 17 to 8192 tokens and matrices of 512 to 151936
 // channels by 2048 to 14336 columns: `fixed` around the columns; for 128 columns `low` where a CU has one
@@ -382,11 +451,12 @@ constexpr TileCost kTileCosts[kTiles] = {
 // few of them leave CUs idle, and rounds of them the last one part empty (2048 tokens of 4096 to
 // 4096: 256 x 256 47 us, 128 x 256 43; 4096 tokens: 65 and 84. 64 tokens of 14336 to 4096: 64 x 64 38,
 // 32 x 32 with eight groups along the columns 22; 64 of 4096 to 14336: 18 and 37).
-int best_tile(const I8Args& a) {
+int best_tile(const I8Args& a, bool whole) {
     const double steps = (a.cols + 127) / 128;
-    int best = 0;
+    const int first = whole ? kTile256 : kTile128x256;
+    int best = first;
     double least = 0;
-    for (int i = 0; i < kTiles; ++i) {
+    for (int i = first; i < kTiles; ++i) {
         const TileCost& c = kTileCosts[i];
         const double tiles = static_cast<double>((a.rows + c.channels - 1) / c.channels) * ((a.n_tokens + c.tokens - 1) / c.tokens);
         const double each = ceil(tiles / 256);  // of the CU with most
@@ -398,33 +468,52 @@ int best_tile(const I8Args& a) {
             const double busy = tiles < 256 ? tiles / 256 : 1;
             us = each * (c.fixed + steps * (c.low + (c.full - c.low) * busy));
         }
-        if (i == 0 || us < least) best = i, least = us;
+        if (i == first || us < least) best = i, least = us;
     }
     return best;
 }
 
-int32_t launch_i8(hipStream_t s, const I8Args& a, const char* action) {
-    // Whole chunks of 16 codes, each at a multiple of 16 bytes.
-    const bool whole = (a.cols | a.a_stride | a.w_stride | reinterpret_cast<uintptr_t>(a.a) | reinterpret_cast<uintptr_t>(a.w)) % 16 == 0;
+// Whole chunks of 16 codes, each at a multiple of 16 bytes.
+bool whole_chunks(const I8Args& a) {
+    return (a.cols | a.a_stride | a.w_stride | reinterpret_cast<uintptr_t>(a.a) | reinterpret_cast<uintptr_t>(a.w)) % 16 == 0;
+}
+
+// Rows that begin anywhere cost the tiles moves of all they load: where tokens and channels are many,
+// both are copied to a workspace first (4000 tokens and channels of 4003 columns: 131 us, with the
+// copies 85; 512 tokens, 14336 channels of 4095: 71 with them, 65 without).
+constexpr uint64_t kMostStraight = uint64_t(1) << 30;
+int32_t straighten(objeta_hip_context* ctx, hipStream_t s, I8Args& a, const char* action) {
+    const uint64_t pitch = (static_cast<uint64_t>(a.cols) + 15) / 16 * 16, n = a.n_tokens, r = a.rows;
+    if (n * r < 800 * (n + r) || a.cols < 16 || (n + r) * pitch > kMostStraight) return 0;
+    if (!workspace_ready(ctx, s, kWsCodes, (n + r) * pitch)) return 0;  // captured without one: read as they are
+    void* ws = nullptr;
+    OBJ_TRY(ensure_workspace(ctx, s, kWsCodes, (n + r) * pitch, &ws));
+    int8_t* to = static_cast<int8_t*>(ws);
+    hipLaunchKernelGGL(i8_straighten_kernel, dim3(2048), dim3(256), 0, s, a.a, a.a_stride, a.n_tokens, a.cols, to);
+    hipLaunchKernelGGL(i8_straighten_kernel, dim3(2048), dim3(256), 0, s, a.w, a.w_stride, a.rows, a.cols, to + n * pitch);
+    OBJ_HIP(hipGetLastError(), action);
+    a.a = to, a.w = to + n * pitch, a.a_stride = a.w_stride = pitch, a.cols = static_cast<uint32_t>(pitch);
+    return 0;
+}
+
+int32_t launch_i8(objeta_hip_context* ctx, hipStream_t s, I8Args a, const char* action) {
+    if (!whole_chunks(a)) OBJ_TRY(straighten(ctx, s, a, action));
+    const bool whole = whole_chunks(a);
     const bool near = a.a_stride < (1u << 22) && a.w_stride < (1u << 22);  // a tile's rows within a buffer's 32-bit range
-    if (a.n_tokens <= 16 || !near) {
+    if (a.n_tokens <= 16 || !near || a.cols < 16) {
         // 16 channels a workgroup where these are few, 32 otherwise, whose tokens' codes are read half as
         // often (one token, 4096 of 14336 columns: 12.9 and 18.0 us; 151936 of 4096: 123 and 109)
         if (a.rows <= 8192) launch_stream<8, 1, 1, 4>(s, a, whole);
         else launch_stream<8, 2, 1, 2>(s, a, whole);
-    } else if (!whole) {
-        const bool many = static_cast<uint64_t>((a.rows + 127) / 128) * ((a.n_tokens + 127) / 128) >= 256;
-        if (many) launch_tile<2, 2, 2, 2, 1, 1, false>(s, a);
-        else launch_tile<2, 2, 1, 1, 1, 2, false>(s, a);
     } else {
-        switch (best_tile(a)) {
+        switch (best_tile(a, whole)) {
             case kTile256: launch_tile<2, 4, 4, 2, 1, 1, true>(s, a); break;
-            case kTile128x256: launch_tile<2, 4, 2, 2, 1, 2, true>(s, a); break;
-            case kTile128: launch_tile<2, 2, 2, 2, 1, 2, true>(s, a); break;
-            case kTile64x128: launch_tile<2, 2, 1, 2, 1, 3, true>(s, a); break;
-            case kTile64: launch_tile<2, 2, 1, 1, 1, 3, true>(s, a); break;
-            case kTile32x64: launch_tile<1, 2, 1, 1, 4, 2, true>(s, a); break;
-            default: launch_tile<1, 1, 1, 1, 8, 3, true>(s, a); break;
+            case kTile128x256: launch_either<2, 4, 2, 2, 1, 2>(s, a, whole); break;
+            case kTile128: launch_either<2, 2, 2, 2, 1, 2>(s, a, whole); break;
+            case kTile64x128: launch_either<2, 2, 1, 2, 1, 3>(s, a, whole); break;
+            case kTile64: launch_either<2, 2, 1, 1, 1, 3>(s, a, whole); break;
+            case kTile32x64: launch_either<1, 2, 1, 1, 4, 2>(s, a, whole); break;
+            default: launch_either<1, 1, 1, 1, 8, 3>(s, a, whole); break;
         }
     }
     OBJ_HIP(hipGetLastError(), action);
@@ -469,7 +558,7 @@ int32_t objeta_hip_i8_product_device(objeta_hip_context* ctx, objeta_hip_stream 
     a.out_type = out_dtype;
     const OnDevice on(ctx->device);
     OBJ_HIP(on.status(), action);
-    return launch_i8(resolve_stream(ctx, stream), a, action);
+    return launch_i8(ctx, resolve_stream(ctx, stream), a, action);
     OBJ_GUARD_END
 }
 

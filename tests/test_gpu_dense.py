@@ -282,6 +282,42 @@ def test_product_of_many_rows_on_another_stream(backend, dense, n, rows, cols):
     check_product(backend, dense, n, rows, cols, "bf16", stream=backend.stream(1))
 
 
+@pytest.mark.parametrize("cols", [15, 16, 17, 35, 130])
+@pytest.mark.parametrize("skews,pads", [((0, 0, 0), (0, 0, 0)), ((3, 0, 0), (1, 0, 0)), ((0, 2, 1), (13, 30, 1))])
+def test_product_of_many_rows_that_begin_anywhere(backend, dense, cols, skews, pads):
+    """Past some size such rows are copied to whole chunks first."""
+    check_product(backend, dense, 1700, 1650, cols, "f32", skews=skews, pads=pads)
+
+
+@pytest.mark.parametrize("n,rows,cols", [(1700, 1650, 37), (1700, 1650, 48), (5, 40, 130)])
+def test_product_captured_without_a_call_ahead(n, rows, cols):
+    """On a stream of its own that has no workspace: such rows are then read where they lie."""
+    import ctypes as C
+    from objeta_amd import HipBackend
+    from objeta_amd.api import check as ok
+    with HipBackend(0, 1) as be:
+        rng = np.random.default_rng(21)
+        a, w = (rng.integers(-128, 128, (m, cols)).astype(np.int8) for m in (n, rows))
+        sa, sw = (np.exp(rng.standard_normal(m)).astype(np.float32) for m in (n, rows))
+        d = [be.to_device(x) for x in (a, sa, w, sw)]
+        out = be.alloc(4 * n * rows)
+        st, g = be.stream(0), C.c_void_p()
+        ok(be.L.objeta_hip_graph_begin_capture(be.ctx, st))
+        DenseBackend(be).i8_product_device(n, rows, cols, d[0], d[1], d[2], d[3], out)
+        ok(be.L.objeta_hip_graph_end_capture(be.ctx, st, C.byref(g)))
+        want = product(a, sa, w, sw)
+        for _ in range(3):
+            ok(be.L.objeta_hip_zero_device(be.ctx, st, out.addr(), out.nbytes))
+            ok(be.L.objeta_hip_graph_launch(be.ctx, g, st))
+            be.synchronize()
+            assert np.array_equal(out.download(np.float32, n * rows).reshape(n, rows), want)
+        DenseBackend(be).i8_product_device(n, rows, cols, d[0], d[1], d[2], d[3], out)
+        be.synchronize()
+        assert np.array_equal(out.download(np.float32, n * rows).reshape(n, rows), want)
+        ok(be.L.objeta_hip_graph_destroy(be.ctx, g))
+        del d, out
+
+
 def test_product_results_do_not_depend_on_the_batch(backend, dense):
     """A token's row is the same bits alone and in batches of any size."""
     rng, rows, cols = np.random.default_rng(11), 200, 640
