@@ -5,9 +5,9 @@
 // far, in units of ln 2), s = sum 2^(z - R) and t = sum 2^(z - R) (z - R), and moves both when R grows:
 // with d = R - R', s' = 2^d s and t' = 2^d (t + d s).
 //
-// The best N: a thread also keeps the largest x of each stretch it read (up to 16). The N-th largest
-// of the threads' maxima bounds the N-th best from below, so only the few stretches that reach it are
-// read again, and what reaches it there is ranked. A value's key is its bits in their order above the
+// The best N: a thread also keeps the largest x of each stretch it read (up to 8). The N-th largest of 64
+// maxima of four threads each bounds the N-th best from below, so only the few stretches that reach it
+// are read again, and what reaches it there is ranked. A value's key is its bits in their order above the
 // complement of its index: equal values go by the lowest index. Where too many values reach the bound
 // (ties, all of the best in few threads), the N-th value is found bit by bit over the row instead.
 //
@@ -19,8 +19,8 @@ namespace objeta {
 namespace dev {
 
 constexpr uint32_t kLpThreads = 256;
-constexpr uint32_t kLpVecs = 4;      // 16-byte loads of a thread in flight
-constexpr uint32_t kLpStretches = 16;
+constexpr uint32_t kLpVecs = 2;      // 16-byte loads of a turn; the next turn's are in flight
+constexpr uint32_t kLpStretches = 8;  // (with 16, LDS held five workgroups a CU in place of eight)
 constexpr uint32_t kLpMostTop = 32;
 constexpr uint32_t kLpMostCandidates = 1024;  // no less than kLpMostTop^2, for the join
 // References lie between -2^24 and 2^24, where rounding one moves its largest term by a factor of two
@@ -103,47 +103,72 @@ struct LpSums {
         s *= f;
         ref = to;
     }
-    __device__ __forceinline__ void join(LpSums o) {
-        const float to = __builtin_fmaxf(ref, o.ref);
-        move(to);
-        o.move(to);
+    // Of references moved to one another's largest.
+    __device__ __forceinline__ void add(LpSums o) {
         m = __builtin_fmaxf(m, o.m);
         s += o.s;
         t += o.t;
-    }
-    __device__ __forceinline__ LpSums from(int off) const {
-        return LpSums{__shfl_xor(m, off, 64), __shfl_xor(ref, off, 64), __shfl_xor(s, off, 64), __shfl_xor(t, off, 64)};
     }
 };
 
 struct LpShared {
     LpSums sums[kLpThreads / 64];
     uint32_t max[kLpThreads];
-    uint64_t keys[kLpMostCandidates];
+    uint64_t keys[kLpMostCandidates + 8];
     uint64_t best[kLpMostTop];
     uint32_t hist[256];
-    uint32_t count, bound, digit, wave[kLpThreads / 64];
+    uint32_t count, bound, digit, hits, wave[kLpThreads / 64];
 };
+constexpr uint32_t kLpMostHits = 512;
 
-__device__ __forceinline__ LpSums lp_join_all(LpSums v, LpShared& sh) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v.join(v.from(off));
-    if ((threadIdx.x & 63) == 0) sh.sums[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = sh.sums[0];
-    for (uint32_t i = 1; i < kLpThreads / 64; ++i) v.join(sh.sums[i]);
-    __syncthreads();
-    return v;
+// A row's given token that falls to this thread, read ahead of the rest.
+struct LpGiven {
+    int32_t token;
+    float x;
+};
+template <int TYPE>
+__device__ __forceinline__ LpGiven lp_given(const LpArgs& a, uint64_t r, uint32_t g) {
+    LpGiven n{-1, 0.0f};
+    if (g < a.n_given) {
+        n.token = a.tokens[r * a.n_given + g];
+        if (static_cast<uint32_t>(n.token) < a.vocab)
+            n.x = lp_at<TYPE>(static_cast<const char*>(a.x) + r * a.stride * (16 / LpElem<TYPE>::kPer), n.token);
+    }
+    return n;
 }
 
-// sh.keys[0 .. n) to sh.best, the n_top largest in order, 0 behind the last; keys differ.
+__device__ __forceinline__ LpSums lp_join_all(LpSums v, LpShared& sh) {
+    v.move(max_of_wave(v.ref));
+    v = LpSums{max_of_wave(v.m), v.ref, sum_of_wave(v.s), sum_of_wave(v.t)};
+    if ((threadIdx.x & 63) == 0) sh.sums[threadIdx.x >> 6] = v;
+    __syncthreads();
+    LpSums w[kLpThreads / 64];
+    float to = v.ref;
+#pragma unroll
+    for (uint32_t i = 0; i < kLpThreads / 64; ++i) w[i] = sh.sums[i], to = __builtin_fmaxf(to, w[i].ref);
+#pragma unroll
+    for (uint32_t i = 0; i < kLpThreads / 64; ++i) w[i].move(to);
+#pragma unroll
+    for (uint32_t i = 1; i < kLpThreads / 64; ++i) w[0].add(w[i]);
+    __syncthreads();
+    return w[0];
+}
+
+// sh.keys[0 .. n) to sh.best, the n_top largest in order, 0 behind the last; keys differ (but for zeros).
 __device__ __forceinline__ void lp_rank(LpShared& sh, uint32_t n, uint32_t n_top) {
     if (threadIdx.x < kLpMostTop) sh.best[threadIdx.x] = 0;
+    if (threadIdx.x < 8) sh.keys[n + threadIdx.x] = 0;  // whole turns of eight
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < n; i += kLpThreads) {
         const uint64_t k = sh.keys[i];
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < n && rank < n_top; ++j) rank += sh.keys[j] > k;
+        for (uint32_t j = 0; j < n; j += 8) {
+            uint64_t o[8];
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u) o[u] = sh.keys[j + u];
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u) rank += o[u] > k;
+        }
         if (rank < n_top) sh.best[rank] = k;
     }
     __syncthreads();
@@ -210,7 +235,7 @@ __device__ void lp_by_digits(const void* row, uint32_t lo, uint32_t hi, uint32_t
 
 // What a row's sums and best come to.
 template <int TYPE>
-__device__ void lp_finish(const LpArgs& a, uint64_t r, LpSums v, LpShared& sh) {
+__device__ void lp_finish(const LpArgs& a, uint64_t r, LpSums v, LpGiven first, LpShared& sh) {
     const void* row = static_cast<const char*>(a.x) + r * a.stride * (16 / LpElem<TYPE>::kPer);
     const uint32_t tid = threadIdx.x;
     const bool none = v.m == -__builtin_inff() && v.s == v.s;  // (the sum is NaN where the row holds one)
@@ -235,18 +260,17 @@ __device__ void lp_finish(const LpArgs& a, uint64_t r, LpSums v, LpShared& sh) {
         if (a.lse) a.lse[r] = none ? -__builtin_inff() : __builtin_fmaf(v.m, a.scale, more);
         if (a.entropy) a.entropy[r] = none ? 0.0f : -not_above_0((v.t / v.s - log_s) * kLn2);
     }
-    if (a.lp)
-        for (uint32_t g = tid; g < a.n_given; g += kLpThreads) {
-            const int32_t token = a.tokens[r * a.n_given + g];
-            float p = 0.0f;
-            if (static_cast<uint32_t>(token) < a.vocab) {
-                p = log_prob(lp_at<TYPE>(row, token));
-            } else if (token != -1) {
-                p = __builtin_nanf("");
-                atomicOr(a.err, kErrIndex);
-            }
-            a.lp[r * a.n_given + g] = p;
+    for (uint32_t g = tid; g < a.n_given; g += kLpThreads) {
+        if (g != tid) first = lp_given<TYPE>(a, r, g);
+        float p = 0.0f;
+        if (static_cast<uint32_t>(first.token) < a.vocab) {
+            p = log_prob(first.x);
+        } else if (first.token != -1) {
+            p = __builtin_nanf("");
+            atomicOr(a.err, kErrIndex);
         }
+        a.lp[r * a.n_given + g] = p;
+    }
     if (a.n_top) {
         // sh.best holds the values above -infinity; the others by their indices
         if (sh.best[a.n_top - 1] == 0) {
@@ -271,94 +295,122 @@ __device__ void lp_finish(const LpArgs& a, uint64_t r, LpSums v, LpShared& sh) {
 }
 
 template <int TYPE, bool TOP, bool ENTROPY>
-__global__ __launch_bounds__(kLpThreads) void lp_part_kernel(LpArgs a) {
+__global__ __launch_bounds__(kLpThreads, 8) void lp_part_kernel(LpArgs a) {
     constexpr uint32_t kPer = LpElem<TYPE>::kPer, kStep = kLpThreads * kPer, kTurn = kLpVecs * kStep;
     __shared__ LpShared sh;
     __shared__ float stretch[TOP ? kLpStretches : 1][kLpThreads];
+    __shared__ uint16_t hit[TOP ? kLpMostHits : 1];
     const uint64_t r = a.first + blockIdx.x;
     const uint32_t part = blockIdx.y, tid = threadIdx.x;
     const uint32_t lo = part * a.part_size, hi = a.vocab - lo < a.part_size ? a.vocab : lo + a.part_size;
     const void* row = static_cast<const char*>(a.x) + r * a.stride * (16 / kPer);
     const uint32_t turns = (hi - lo + kTurn - 1) / kTurn, per = (turns + kLpStretches - 1) / kLpStretches;
+    const uint32_t whole = (hi - lo) / kTurn;  // turns without an end inside
 
+    const LpGiven given = a.parts == 1 ? lp_given<TYPE>(a, r, tid) : LpGiven{-1, 0.0f};
     const float ninf = -__builtin_inff();
     LpSums v{ninf, -kLpFar, 0.0f, 0.0f};
     float longest = ninf;
+    uint32_t left = per, g = 0;  // turns until the stretch ends; its index
     reg_u32x4 next[kLpVecs];
+    const char* mine_at = static_cast<const char*>(row) + (static_cast<uint64_t>(lo) + tid * kPer) * (16 / kPer);
+    auto load = [&](uint32_t turn) {
+        if (turn < whole) {
 #pragma unroll
-    for (uint32_t u = 0; u < kLpVecs; ++u) next[u] = lp_load<TYPE>(row, lo + u * kStep + tid * kPer, hi);
+            for (uint32_t u = 0; u < kLpVecs; ++u)
+                next[u] = *reinterpret_cast<const any_u32x4*>(mine_at + (static_cast<uint64_t>(turn) * kLpVecs + u) * kLpThreads * 16);
+        } else if (turn < turns) {
+#pragma unroll
+            for (uint32_t u = 0; u < kLpVecs; ++u) next[u] = lp_load<TYPE>(row, lo + turn * kTurn + u * kStep + tid * kPer, hi);
+        }
+    };
+    load(0);
     for (uint32_t turn = 0; turn < turns; ++turn) {
         float x[kLpVecs][kPer];
 #pragma unroll
         for (uint32_t u = 0; u < kLpVecs; ++u) lp_floats<TYPE>(next[u], x[u]);
-        if (turn + 1 < turns) {
-#pragma unroll
-            for (uint32_t u = 0; u < kLpVecs; ++u) next[u] = lp_load<TYPE>(row, lo + (turn + 1) * kTurn + u * kStep + tid * kPer, hi);
-        }
+        load(turn + 1);
         float m = ninf;
 #pragma unroll
         for (uint32_t u = 0; u < kLpVecs; ++u)
 #pragma unroll
             for (uint32_t i = 0; i < kPer; ++i) m = __builtin_fmaxf(m, x[u][i]);
-        longest = __builtin_fmaxf(longest, m);
-        if (TOP && (turn % per == per - 1 || turn + 1 == turns)) {
-            stretch[turn / per][tid] = longest;
-            longest = ninf;
+        if constexpr (TOP) {
+            longest = __builtin_fmaxf(longest, m);
+            if (--left == 0 || turn + 1 == turns) {
+                stretch[g++][tid] = longest;
+                longest = ninf;
+                left = per;
+            }
         }
         if (m > v.m) {
             v.m = m;
             v.move(__builtin_fmaxf(m * a.c, -kLpFar));
         }
+        float s2 = 0.0f, t2 = 0.0f;  // every other one apart: shorter chains
 #pragma unroll
         for (uint32_t u = 0; u < kLpVecs; ++u)
 #pragma unroll
             for (uint32_t i = 0; i < kPer; ++i) {
                 const float d = __builtin_fmaf(x[u][i], a.c, -v.ref), e = __builtin_amdgcn_exp2f(d);
-                v.s += e;
-                if (ENTROPY) v.t = __builtin_fmaf(e, __builtin_fmaxf(d, -200.0f), v.t);
+                (i & 1 ? s2 : v.s) += e;
+                if (ENTROPY) (i & 1 ? t2 : v.t) = __builtin_fmaf(e, __builtin_fmaxf(d, -200.0f), i & 1 ? t2 : v.t);
             }
+        v.s += s2;
+        v.t += t2;
     }
     const float mine = v.m;
     v = lp_join_all(v, sh);
 
     if constexpr (TOP) {
-        // The n_top-th largest of the threads' maxima.
+        // The n_top-th largest of the maxima of four threads, lane by lane over the waves.
         const uint32_t key = ordered(mine);
         sh.max[tid] = key;
-        if (tid == 0) sh.count = 0;
+        if (tid == 0) sh.count = sh.hits = 0;
         __syncthreads();
-        uint32_t rank = 0;
-        for (uint32_t i = 0; i < kLpThreads; ++i) rank += sh.max[i] > key || (sh.max[i] == key && i < tid);
-        if (rank == a.n_top - 1) sh.bound = key;
+        if (tid < 64) {
+            uint32_t most = key;
+#pragma unroll
+            for (uint32_t i = 64; i < kLpThreads; i += 64) most = sh.max[tid + i] > most ? sh.max[tid + i] : most;
+            uint32_t rank = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 64; ++i) {
+                const uint32_t o = __builtin_amdgcn_readlane(most, i);
+                rank += o > most || (o == most && i < tid);
+            }
+            if (rank == a.n_top - 1) sh.bound = most > kOrderedInf ? most : kOrderedInf + 1;
+        }
         __syncthreads();
-        uint32_t bound = sh.bound;
-        if (bound <= kOrderedInf) bound = kOrderedInf + 1;
-        if (key >= bound) {
-            for (uint32_t g = 0; g * per < turns; ++g) {
-                if (ordered(stretch[g][tid]) < bound) continue;
-                const uint32_t end = (g + 1) * per < turns ? (g + 1) * per : turns;
-                for (uint32_t turn = g * per; turn < end; ++turn)
+        const uint32_t bound = sh.bound;
+        if (key >= bound)
+            for (uint32_t j = 0; j < g; ++j)
+                if (ordered(stretch[j][tid]) >= bound) {
+                    const uint32_t place = atomicAdd(&sh.hits, 1u);
+                    if (place < kLpMostHits) hit[place] = static_cast<uint16_t>(tid * kLpStretches + j);
+                }
+        __syncthreads();
+        // Every thread takes 16 bytes of a stretch that was hit.
+        const uint32_t each = per * kLpVecs, items = sh.hits <= kLpMostHits ? sh.hits * each : 0;
+        for (uint32_t i = tid; i < items; i += kLpThreads) {
+            const uint32_t h = hit[i / each], in = i % each, turn = h % kLpStretches * per + in / kLpVecs;
+            const uint32_t from = lo + turn * kTurn + in % kLpVecs * kStep + h / kLpStretches * kPer;
+            if (turn >= turns) continue;
+            float x[kPer];
+            lp_floats<TYPE>(lp_load<TYPE>(row, from, hi), x);
 #pragma unroll
-                    for (uint32_t u = 0; u < kLpVecs; ++u) {
-                        const uint32_t at = lo + turn * kTurn + u * kStep + tid * kPer;
-                        float x[kPer];
-                        lp_floats<TYPE>(lp_load<TYPE>(row, at, hi), x);
-#pragma unroll
-                        for (uint32_t i = 0; i < kPer; ++i) {
-                            const uint32_t o = ordered(x[i]);
-                            if (o < bound) continue;
-                            const uint32_t place = atomicAdd(&sh.count, 1u);
-                            if (place < kLpMostCandidates) sh.keys[place] = lp_key(o, at + i);
-                        }
-                    }
+            for (uint32_t u = 0; u < kPer; ++u) {
+                const uint32_t o = ordered(x[u]);
+                if (o < bound) continue;
+                const uint32_t place = atomicAdd(&sh.count, 1u);
+                if (place < kLpMostCandidates) sh.keys[place] = lp_key(o, from + u);
             }
         }
         __syncthreads();
-        if (sh.count > kLpMostCandidates) lp_by_digits<TYPE>(row, lo, hi, a.n_top, sh);
+        if (sh.count > kLpMostCandidates || sh.hits > kLpMostHits) lp_by_digits<TYPE>(row, lo, hi, a.n_top, sh);
         lp_rank(sh, sh.count, a.n_top);
     }
     if (a.parts == 1) {
-        lp_finish<TYPE>(a, r, v, sh);
+        lp_finish<TYPE>(a, r, v, given, sh);
         return;
     }
     const uint64_t at = r * a.parts + part;
@@ -371,6 +423,7 @@ __global__ __launch_bounds__(kLpThreads) void lp_join_kernel(LpArgs a) {
     __shared__ LpShared sh;
     const uint64_t r = a.first + blockIdx.x;
     const uint32_t tid = threadIdx.x;
+    const LpGiven given = lp_given<TYPE>(a, r, tid);
     LpSums v{-__builtin_inff(), -kLpFar, 0.0f, 0.0f};
     if (tid < a.parts) {
         const float4 p = a.stats[r * a.parts + tid];
@@ -380,22 +433,28 @@ __global__ __launch_bounds__(kLpThreads) void lp_join_kernel(LpArgs a) {
     if (a.n_top) {
         // A part's first key is its best; with n_top parts or more the n_top-th of these bounds the rest.
         const uint64_t* keys = a.keys + r * a.parts * a.n_top;
+        const uint32_t all = a.parts * a.n_top;
+        constexpr uint32_t kAhead = 4;
+        uint64_t k[kAhead];  // read beside the first ones
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u) k[u] = tid + u * kLpThreads < all ? keys[tid + u * kLpThreads] : 0;
         if (tid < a.parts) sh.keys[tid] = keys[static_cast<uint64_t>(tid) * a.n_top];
         __syncthreads();
         lp_rank(sh, a.parts, a.n_top);
         const uint64_t bound = sh.best[a.n_top - 1];
         if (tid == 0) sh.count = 0;
         __syncthreads();
-        if (tid < a.parts)
-            for (uint32_t i = 0; i < a.n_top; ++i) {
-                const uint64_t k = keys[static_cast<uint64_t>(tid) * a.n_top + i];
-                if (k == 0 || k < bound) break;
-                sh.keys[atomicAdd(&sh.count, 1u)] = k;  // of at most n_top parts n_top each
-            }
+        for (uint32_t i = tid, n = 0; i < all; i += kLpThreads, ++n) {
+            uint64_t o = 0;
+#pragma unroll
+            for (uint32_t u = 0; u < kAhead; ++u) o = n == u ? k[u] : o;
+            if (n >= kAhead) o = keys[i];
+            if (o != 0 && o >= bound) sh.keys[atomicAdd(&sh.count, 1u)] = o;  // of at most n_top parts n_top each
+        }
         __syncthreads();
         lp_rank(sh, sh.count, a.n_top);
     }
-    lp_finish<TYPE>(a, r, v, sh);
+    lp_finish<TYPE>(a, r, v, given, sh);
 }
 
 }  // namespace dev

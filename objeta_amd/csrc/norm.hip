@@ -115,8 +115,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rows_kernel(Nor
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum = __builtin_fma(static_cast<double>(y[v][i]), static_cast<double>(y[v][i]), sum);
         }
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        sum = sum_of_wave(sum);
         if (WAVES > 1) {
             if (lane == 0) sh_sum[wave] = sum;
             __syncthreads();
@@ -147,11 +146,7 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rows_kernel(Nor
                 const uint32_t m = static_cast<uint32_t>(i) < left[v] ? __float_as_uint(y[v][i]) & 0x7FFFFFFFu : 0u;
                 most = m > most ? m : most;
             }
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) {
-            const uint32_t o = __shfl_xor(most, off, 64);
-            most = o > most ? o : most;
-        }
+        most = max_of_wave(most);
         if (WAVES > 1) {
             if (lane == 0) sh_max[wave] = __uint_as_float(most);
             __syncthreads();
