@@ -18,11 +18,13 @@
 namespace objeta {
 namespace dev {
 
-constexpr uint32_t kLpThreads = 256;
+constexpr uint32_t kLpJoin = 256;    // threads that join a row's parts; as many parts at most
+constexpr uint32_t kLpBlocks = 64;  // of a part
 constexpr uint32_t kLpVecs = 2;      // 16-byte loads of a turn; the next turn's are in flight
 constexpr uint32_t kLpStretches = 8;  // (with 16, LDS held five workgroups a CU in place of eight)
 constexpr uint32_t kLpMostTop = 32;
-constexpr uint32_t kLpMostCandidates = 1024;  // no less than kLpMostTop^2, for the join
+constexpr uint32_t kLpMostCandidates = 1024;
+constexpr uint32_t kLpMostHits = 512;
 // References lie between -2^24 and 2^24, where rounding one moves its largest term by a factor of two
 // at most. Threads whose values are all lower add nothing to a row within; a row whose largest is
 // outside is summed a second time about that value itself.
@@ -37,8 +39,8 @@ struct LpArgs {
     const int32_t* tokens;
     float *lp, *lse, *entropy, *top;
     int32_t* ids;
-    float4* stats;   // [rows][parts]: m, R, s, t
-    uint64_t* keys;  // [rows][parts][n_top], the best first, 0 behind the last
+    float4* stats;  // [rows][parts]: m, R, s, t
+    float* blocks;  // [rows][parts][kLpBlocks]: the largest of what four neighbouring threads read
     uint32_t* err;
 };
 
@@ -103,63 +105,55 @@ struct LpSums {
         s *= f;
         ref = to;
     }
-    // Of references moved to one another's largest.
-    __device__ __forceinline__ void add(LpSums o) {
-        m = __builtin_fmaxf(m, o.m);
-        s += o.s;
-        t += o.t;
-    }
 };
 
+template <int THREADS>
 struct LpShared {
-    LpSums sums[kLpThreads / 64];
-    uint32_t max[kLpThreads];
+    LpSums sums[THREADS / 64];
+    uint32_t max[THREADS];
     uint64_t keys[kLpMostCandidates + 8];
     uint64_t best[kLpMostTop];
+    uint16_t hit[kLpMostHits];
     uint32_t hist[256];
-    uint32_t count, bound, digit, hits, wave[kLpThreads / 64];
+    uint32_t count, bound, digit, hits, wave[THREADS / 64];
 };
-constexpr uint32_t kLpMostHits = 512;
 
 // A row's given token that falls to this thread, read ahead of the rest.
 struct LpGiven {
     int32_t token;
     float x;
 };
+__device__ __forceinline__ int32_t lp_token(const LpArgs& a, uint64_t r, uint32_t g) { return g < a.n_given ? a.tokens[r * a.n_given + g] : -1; }
 template <int TYPE>
-__device__ __forceinline__ LpGiven lp_given(const LpArgs& a, uint64_t r, uint32_t g) {
-    LpGiven n{-1, 0.0f};
-    if (g < a.n_given) {
-        n.token = a.tokens[r * a.n_given + g];
-        if (static_cast<uint32_t>(n.token) < a.vocab)
-            n.x = lp_at<TYPE>(static_cast<const char*>(a.x) + r * a.stride * (16 / LpElem<TYPE>::kPer), n.token);
-    }
+__device__ __forceinline__ LpGiven lp_given(const LpArgs& a, uint64_t r, int32_t token) {
+    LpGiven n{token, 0.0f};
+    if (static_cast<uint32_t>(token) < a.vocab) n.x = lp_at<TYPE>(static_cast<const char*>(a.x) + r * a.stride * (16 / LpElem<TYPE>::kPer), token);
     return n;
 }
 
-__device__ __forceinline__ LpSums lp_join_all(LpSums v, LpShared& sh) {
-    v.move(max_of_wave(v.ref));
-    v = LpSums{max_of_wave(v.m), v.ref, sum_of_wave(v.s), sum_of_wave(v.t)};
-    if ((threadIdx.x & 63) == 0) sh.sums[threadIdx.x >> 6] = v;
+template <int THREADS>
+__device__ __forceinline__ LpSums lp_join_all(LpSums v, LpShared<THREADS>& sh) {
+    auto over_wave = [](LpSums u) {
+        u.move(max_of_wave(u.ref));
+        return LpSums{max_of_wave(u.m), u.ref, sum_of_wave(u.s), sum_of_wave(u.t)};
+    };
+    v = over_wave(v);
+    const uint32_t lane = threadIdx.x & 63;
+    if (lane == 0) sh.sums[threadIdx.x >> 6] = v;
     __syncthreads();
-    LpSums w[kLpThreads / 64];
-    float to = v.ref;
-#pragma unroll
-    for (uint32_t i = 0; i < kLpThreads / 64; ++i) w[i] = sh.sums[i], to = __builtin_fmaxf(to, w[i].ref);
-#pragma unroll
-    for (uint32_t i = 0; i < kLpThreads / 64; ++i) w[i].move(to);
-#pragma unroll
-    for (uint32_t i = 1; i < kLpThreads / 64; ++i) w[0].add(w[i]);
+    v = lane < THREADS / 64 ? sh.sums[lane] : LpSums{-__builtin_inff(), -kLpFar, 0.0f, 0.0f};
+    v = over_wave(v);
     __syncthreads();
-    return w[0];
+    return v;
 }
 
 // sh.keys[0 .. n) to sh.best, the n_top largest in order, 0 behind the last; keys differ (but for zeros).
-__device__ __forceinline__ void lp_rank(LpShared& sh, uint32_t n, uint32_t n_top) {
+template <int THREADS>
+__device__ __forceinline__ void lp_rank(LpShared<THREADS>& sh, uint32_t n, uint32_t n_top) {
     if (threadIdx.x < kLpMostTop) sh.best[threadIdx.x] = 0;
     if (threadIdx.x < 8) sh.keys[n + threadIdx.x] = 0;  // whole turns of eight
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += kLpThreads) {
+    for (uint32_t i = threadIdx.x; i < n; i += THREADS) {
         const uint64_t k = sh.keys[i];
         uint32_t rank = 0;
         for (uint32_t j = 0; j < n; j += 8) {
@@ -180,10 +174,10 @@ __device__ __forceinline__ uint64_t lp_key(uint32_t value, uint32_t index) {
 
 // Appends to sh.keys the elements of [lo, hi) whose ordered value is `value`, the lowest indices
 // first, until there are `want` keys.
-template <int TYPE>
-__device__ void lp_fill(const void* row, uint32_t lo, uint32_t hi, uint32_t value, uint32_t want, LpShared& sh) {
+template <int TYPE, int THREADS>
+__device__ void lp_fill(const void* row, uint32_t lo, uint32_t hi, uint32_t value, uint32_t want, LpShared<THREADS>& sh) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (uint32_t i = lo; i < hi; i += kLpThreads) {
+    for (uint32_t i = lo; i < hi; i += THREADS) {
         const uint32_t have = sh.count;
         if (have >= want) break;
         const uint32_t at = i + threadIdx.x;
@@ -192,7 +186,7 @@ __device__ void lp_fill(const void* row, uint32_t lo, uint32_t hi, uint32_t valu
         if (lane == 0) sh.wave[wave] = __popcll(hits);
         __syncthreads();
         uint32_t place = have + __popcll(hits & ((uint64_t(1) << lane) - 1)), all = have;
-        for (uint32_t w = 0; w < kLpThreads / 64; ++w) {
+        for (uint32_t w = 0; w < THREADS / 64; ++w) {
             if (w < wave) place += sh.wave[w];
             all += sh.wave[w];
         }
@@ -204,20 +198,22 @@ __device__ void lp_fill(const void* row, uint32_t lo, uint32_t hi, uint32_t valu
 }
 
 // The n_top best above -infinity of [lo, hi) by the digits of their values; there are more than n_top.
-template <int TYPE>
-__device__ void lp_by_digits(const void* row, uint32_t lo, uint32_t hi, uint32_t n_top, LpShared& sh) {
+template <int TYPE, int THREADS>
+__device__ void lp_by_digits(const void* row, uint32_t lo, uint32_t hi, uint32_t n_top, LpShared<THREADS>& sh) {
     uint32_t prefix = 0, want = n_top;  // values whose upper digits are the prefix's: `want` of them are among the best
     for (int shift = 24; shift >= 0; shift -= 8) {
-        sh.hist[threadIdx.x] = 0;
+        if (threadIdx.x < 256) sh.hist[threadIdx.x] = 0;
         __syncthreads();
-        for (uint32_t i = lo + threadIdx.x; i < hi; i += kLpThreads) {
+        for (uint32_t i = lo + threadIdx.x; i < hi; i += THREADS) {
             const uint32_t o = ordered(lp_at<TYPE>(row, i));
             if (o > kOrderedInf && (shift == 24 || o >> (shift + 8) == prefix >> (shift + 8))) atomicAdd(&sh.hist[o >> shift & 255], 1u);
         }
         __syncthreads();
-        uint32_t above = 0;
-        for (uint32_t d = threadIdx.x + 1; d < 256; ++d) above += sh.hist[d];
-        if (above < want && above + sh.hist[threadIdx.x] >= want) sh.digit = threadIdx.x, sh.bound = want - above;
+        if (threadIdx.x < 256) {
+            uint32_t above = 0;
+            for (uint32_t d = threadIdx.x + 1; d < 256; ++d) above += sh.hist[d];
+            if (above < want && above + sh.hist[threadIdx.x] >= want) sh.digit = threadIdx.x, sh.bound = want - above;
+        }
         __syncthreads();
         prefix |= sh.digit << shift;
         want = sh.bound;
@@ -225,7 +221,7 @@ __device__ void lp_by_digits(const void* row, uint32_t lo, uint32_t hi, uint32_t
     }
     if (threadIdx.x == 0) sh.count = 0;
     __syncthreads();
-    for (uint32_t i = lo + threadIdx.x; i < hi; i += kLpThreads) {
+    for (uint32_t i = lo + threadIdx.x; i < hi; i += THREADS) {
         const uint32_t o = ordered(lp_at<TYPE>(row, i));
         if (o > prefix) sh.keys[atomicAdd(&sh.count, 1u)] = lp_key(o, i);  // n_top - want of them
     }
@@ -233,16 +229,58 @@ __device__ void lp_by_digits(const void* row, uint32_t lo, uint32_t hi, uint32_t
     lp_fill<TYPE>(row, lo, hi, prefix, n_top, sh);
 }
 
+// Bounds the n_top-th best from below by the n_top-th largest of 64 maxima of `mine`, lane by lane over
+// the waves; above -infinity. Clears the counts.
+template <int THREADS>
+__device__ __forceinline__ uint32_t lp_bound(uint32_t mine, uint32_t n_top, LpShared<THREADS>& sh) {
+    const uint32_t tid = threadIdx.x;
+    sh.max[tid] = mine;
+    if (tid == 0) sh.count = sh.hits = 0;
+    __syncthreads();
+    if (tid < 64) {
+        uint32_t most = mine;
+#pragma unroll
+        for (uint32_t i = 64; i < THREADS; i += 64) most = larger(most, sh.max[tid + i]);
+        most = (most & ~63u) | tid;  // all different, and none above what it was but by those bits
+        uint32_t rank = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 64; ++i) rank += lane_of(most, i) > most;
+        if (rank == n_top - 1) sh.bound = larger(most & ~63u, kOrderedInf + 1);
+    }
+    __syncthreads();
+    return sh.bound;
+}
+
+template <int THREADS>
+__device__ __forceinline__ void lp_hit(uint32_t what, LpShared<THREADS>& sh) {
+    const uint32_t place = atomicAdd(&sh.hits, 1u);
+    if (place < kLpMostHits) sh.hit[place] = static_cast<uint16_t>(what);
+}
+
+// Keys of the values of 16 bytes that reach the bound.
+template <int TYPE, int THREADS>
+__device__ __forceinline__ void lp_search(const void* row, uint32_t from, uint32_t hi, uint32_t bound, LpShared<THREADS>& sh) {
+    float x[LpElem<TYPE>::kPer];
+    lp_floats<TYPE>(lp_load<TYPE>(row, from, hi), x);
+#pragma unroll
+    for (uint32_t u = 0; u < LpElem<TYPE>::kPer; ++u) {
+        const uint32_t o = ordered(x[u]);
+        if (o < bound) continue;
+        const uint32_t place = atomicAdd(&sh.count, 1u);
+        if (place < kLpMostCandidates) sh.keys[place] = lp_key(o, from + u);
+    }
+}
+
 // What a row's sums and best come to.
-template <int TYPE>
-__device__ void lp_finish(const LpArgs& a, uint64_t r, LpSums v, LpGiven first, LpShared& sh) {
+template <int TYPE, int THREADS>
+__device__ void lp_finish(const LpArgs& a, uint64_t r, LpSums v, LpGiven first, LpShared<THREADS>& sh) {
     const void* row = static_cast<const char*>(a.x) + r * a.stride * (16 / LpElem<TYPE>::kPer);
     const uint32_t tid = threadIdx.x;
     const bool none = v.m == -__builtin_inff() && v.s == v.s;  // (the sum is NaN where the row holds one)
     const bool again = v.m != -__builtin_inff() && !(v.ref > -kLpFar && v.ref < kLpFar);
     if (again) {
         LpSums u{v.m, 0.0f, 0.0f, 0.0f};
-        for (uint32_t i = tid; i < a.vocab; i += kLpThreads) {
+        for (uint32_t i = tid; i < a.vocab; i += THREADS) {
             const float d = (lp_at<TYPE>(row, i) - v.m) * a.c, e = __builtin_amdgcn_exp2f(d);
             u.s += e;
             u.t = __builtin_fmaf(e, __builtin_fmaxf(d, -200.0f), u.t);
@@ -260,8 +298,8 @@ __device__ void lp_finish(const LpArgs& a, uint64_t r, LpSums v, LpGiven first, 
         if (a.lse) a.lse[r] = none ? -__builtin_inff() : __builtin_fmaf(v.m, a.scale, more);
         if (a.entropy) a.entropy[r] = none ? 0.0f : -not_above_0((v.t / v.s - log_s) * kLn2);
     }
-    for (uint32_t g = tid; g < a.n_given; g += kLpThreads) {
-        if (g != tid) first = lp_given<TYPE>(a, r, g);
+    for (uint32_t g = tid; g < a.n_given; g += THREADS) {
+        if (g != tid) first = lp_given<TYPE>(a, r, lp_token(a, r, g));
         float p = 0.0f;
         if (static_cast<uint32_t>(first.token) < a.vocab) {
             p = log_prob(first.x);
@@ -294,12 +332,13 @@ __device__ void lp_finish(const LpArgs& a, uint64_t r, LpSums v, LpGiven first, 
     }
 }
 
-template <int TYPE, bool TOP, bool ENTROPY>
-__global__ __launch_bounds__(kLpThreads, 8) void lp_part_kernel(LpArgs a) {
-    constexpr uint32_t kPer = LpElem<TYPE>::kPer, kStep = kLpThreads * kPer, kTurn = kLpVecs * kStep;
-    __shared__ LpShared sh;
-    __shared__ float stretch[TOP ? kLpStretches : 1][kLpThreads];
-    __shared__ uint16_t hit[TOP ? kLpMostHits : 1];
+enum : int { kTopNone = 0, kTopHere = 1, kTopJoin = 2 };  // who finds the best: nobody, this workgroup, the join
+
+template <int TYPE, int TOP, bool ENTROPY, int THREADS>
+__global__ __launch_bounds__(THREADS, THREADS == 256 ? 8 : 4) void lp_part_kernel(LpArgs a) {
+    constexpr uint32_t kPer = LpElem<TYPE>::kPer, kStep = THREADS * kPer, kTurn = kLpVecs * kStep;
+    __shared__ LpShared<THREADS> sh;
+    __shared__ float stretch[TOP == kTopHere ? kLpStretches : 1][THREADS];
     const uint64_t r = a.first + blockIdx.x;
     const uint32_t part = blockIdx.y, tid = threadIdx.x;
     const uint32_t lo = part * a.part_size, hi = a.vocab - lo < a.part_size ? a.vocab : lo + a.part_size;
@@ -307,7 +346,7 @@ __global__ __launch_bounds__(kLpThreads, 8) void lp_part_kernel(LpArgs a) {
     const uint32_t turns = (hi - lo + kTurn - 1) / kTurn, per = (turns + kLpStretches - 1) / kLpStretches;
     const uint32_t whole = (hi - lo) / kTurn;  // turns without an end inside
 
-    const LpGiven given = a.parts == 1 ? lp_given<TYPE>(a, r, tid) : LpGiven{-1, 0.0f};
+    const int32_t token = a.parts == 1 ? lp_token(a, r, tid) : -1;
     const float ninf = -__builtin_inff();
     LpSums v{ninf, -kLpFar, 0.0f, 0.0f};
     float longest = ninf;
@@ -318,13 +357,14 @@ __global__ __launch_bounds__(kLpThreads, 8) void lp_part_kernel(LpArgs a) {
         if (turn < whole) {
 #pragma unroll
             for (uint32_t u = 0; u < kLpVecs; ++u)
-                next[u] = *reinterpret_cast<const any_u32x4*>(mine_at + (static_cast<uint64_t>(turn) * kLpVecs + u) * kLpThreads * 16);
+                next[u] = *reinterpret_cast<const any_u32x4*>(mine_at + (static_cast<uint64_t>(turn) * kLpVecs + u) * THREADS * 16);
         } else if (turn < turns) {
 #pragma unroll
             for (uint32_t u = 0; u < kLpVecs; ++u) next[u] = lp_load<TYPE>(row, lo + turn * kTurn + u * kStep + tid * kPer, hi);
         }
     };
     load(0);
+    const LpGiven given = lp_given<TYPE>(a, r, token);
     for (uint32_t turn = 0; turn < turns; ++turn) {
         float x[kLpVecs][kPer];
 #pragma unroll
@@ -335,7 +375,7 @@ __global__ __launch_bounds__(kLpThreads, 8) void lp_part_kernel(LpArgs a) {
         for (uint32_t u = 0; u < kLpVecs; ++u)
 #pragma unroll
             for (uint32_t i = 0; i < kPer; ++i) m = __builtin_fmaxf(m, x[u][i]);
-        if constexpr (TOP) {
+        if constexpr (TOP == kTopHere) {
             longest = __builtin_fmaxf(longest, m);
             if (--left == 0 || turn + 1 == turns) {
                 stretch[g++][tid] = longest;
@@ -362,48 +402,17 @@ __global__ __launch_bounds__(kLpThreads, 8) void lp_part_kernel(LpArgs a) {
     const float mine = v.m;
     v = lp_join_all(v, sh);
 
-    if constexpr (TOP) {
-        // The n_top-th largest of the maxima of four threads, lane by lane over the waves.
-        const uint32_t key = ordered(mine);
-        sh.max[tid] = key;
-        if (tid == 0) sh.count = sh.hits = 0;
-        __syncthreads();
-        if (tid < 64) {
-            uint32_t most = key;
-#pragma unroll
-            for (uint32_t i = 64; i < kLpThreads; i += 64) most = sh.max[tid + i] > most ? sh.max[tid + i] : most;
-            uint32_t rank = 0;
-#pragma unroll
-            for (uint32_t i = 0; i < 64; ++i) {
-                const uint32_t o = __builtin_amdgcn_readlane(most, i);
-                rank += o > most || (o == most && i < tid);
-            }
-            if (rank == a.n_top - 1) sh.bound = most > kOrderedInf ? most : kOrderedInf + 1;
-        }
-        __syncthreads();
-        const uint32_t bound = sh.bound;
+    if constexpr (TOP == kTopHere) {
+        const uint32_t key = ordered(mine), bound = lp_bound(key, a.n_top, sh);
         if (key >= bound)
             for (uint32_t j = 0; j < g; ++j)
-                if (ordered(stretch[j][tid]) >= bound) {
-                    const uint32_t place = atomicAdd(&sh.hits, 1u);
-                    if (place < kLpMostHits) hit[place] = static_cast<uint16_t>(tid * kLpStretches + j);
-                }
+                if (ordered(stretch[j][tid]) >= bound) lp_hit(tid * kLpStretches + j, sh);
         __syncthreads();
         // Every thread takes 16 bytes of a stretch that was hit.
         const uint32_t each = per * kLpVecs, items = sh.hits <= kLpMostHits ? sh.hits * each : 0;
-        for (uint32_t i = tid; i < items; i += kLpThreads) {
-            const uint32_t h = hit[i / each], in = i % each, turn = h % kLpStretches * per + in / kLpVecs;
-            const uint32_t from = lo + turn * kTurn + in % kLpVecs * kStep + h / kLpStretches * kPer;
-            if (turn >= turns) continue;
-            float x[kPer];
-            lp_floats<TYPE>(lp_load<TYPE>(row, from, hi), x);
-#pragma unroll
-            for (uint32_t u = 0; u < kPer; ++u) {
-                const uint32_t o = ordered(x[u]);
-                if (o < bound) continue;
-                const uint32_t place = atomicAdd(&sh.count, 1u);
-                if (place < kLpMostCandidates) sh.keys[place] = lp_key(o, from + u);
-            }
+        for (uint32_t i = tid; i < items; i += THREADS) {
+            const uint32_t h = sh.hit[i / each], in = i % each, turn = h % kLpStretches * per + in / kLpVecs;
+            if (turn < turns) lp_search<TYPE>(row, lo + turn * kTurn + in % kLpVecs * kStep + h / kLpStretches * kPer, hi, bound, sh);
         }
         __syncthreads();
         if (sh.count > kLpMostCandidates || sh.hits > kLpMostHits) lp_by_digits<TYPE>(row, lo, hi, a.n_top, sh);
@@ -415,43 +424,65 @@ __global__ __launch_bounds__(kLpThreads, 8) void lp_part_kernel(LpArgs a) {
     }
     const uint64_t at = r * a.parts + part;
     if (tid == 0) a.stats[at] = make_float4(v.m, v.ref, v.s, v.t);
-    if (TOP && tid < a.n_top) a.keys[at * a.n_top + tid] = sh.best[tid];
+    if constexpr (TOP == kTopJoin) {
+        static_assert(THREADS == 4 * kLpBlocks, "four threads a block");
+        const float m = larger(mine, max_moved<0xB1>(mine));  // of pairs, then of fours
+        const float m4 = larger(m, max_moved<0x4E>(m));
+        if ((tid & 3) == 0) a.blocks[at * kLpBlocks + tid / 4] = m4;
+    }
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(kLpThreads) void lp_join_kernel(LpArgs a) {
-    __shared__ LpShared sh;
+__global__ __launch_bounds__(kLpJoin) void lp_join_kernel(LpArgs a) {
+    __shared__ LpShared<kLpJoin> sh;
     const uint64_t r = a.first + blockIdx.x;
     const uint32_t tid = threadIdx.x;
-    const LpGiven given = lp_given<TYPE>(a, r, tid);
-    LpSums v{-__builtin_inff(), -kLpFar, 0.0f, 0.0f};
-    if (tid < a.parts) {
-        const float4 p = a.stats[r * a.parts + tid];
-        v = LpSums{p.x, p.y, p.z, p.w};
+    const int32_t token = lp_token(a, r, tid);
+    float4 sums = make_float4(-__builtin_inff(), -kLpFar, 0.0f, 0.0f);
+    if (tid < a.parts) sums = a.stats[r * a.parts + tid];
+    constexpr uint32_t kKept = 20;  // maxima of a thread, read beside the sums
+    float kept[kKept], mine = -__builtin_inff();
+    if (a.n_top) {
+        const uint32_t all = a.parts * kLpBlocks;
+#pragma unroll
+        for (uint32_t u = 0; u < kKept; ++u) {
+            const uint32_t i = tid + u * kLpJoin;
+            kept[u] = i < all ? a.blocks[r * all + i] : -__builtin_inff();
+        }
     }
+    const LpGiven given = lp_given<TYPE>(a, r, token);
+    LpSums v{sums.x, sums.y, sums.z, sums.w};
     v = lp_join_all(v, sh);
     if (a.n_top) {
-        // A part's first key is its best; with n_top parts or more the n_top-th of these bounds the rest.
-        const uint64_t* keys = a.keys + r * a.parts * a.n_top;
-        const uint32_t all = a.parts * a.n_top;
-        constexpr uint32_t kAhead = 4;
-        uint64_t k[kAhead];  // read beside the first ones
+        constexpr uint32_t kPer = LpElem<TYPE>::kPer, kStep = 4 * kLpBlocks * kPer, kTurn = kLpVecs * kStep;
+        const void* row = static_cast<const char*>(a.x) + r * a.stride * (16 / kPer);
+        const float* blocks = a.blocks + r * a.parts * kLpBlocks;
+        const uint32_t all = a.parts * kLpBlocks, turns = a.part_size / kTurn, each = turns * kLpVecs * 4;
 #pragma unroll
-        for (uint32_t u = 0; u < kAhead; ++u) k[u] = tid + u * kLpThreads < all ? keys[tid + u * kLpThreads] : 0;
-        if (tid < a.parts) sh.keys[tid] = keys[static_cast<uint64_t>(tid) * a.n_top];
-        __syncthreads();
-        lp_rank(sh, a.parts, a.n_top);
-        const uint64_t bound = sh.best[a.n_top - 1];
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        for (uint32_t i = tid, n = 0; i < all; i += kLpThreads, ++n) {
-            uint64_t o = 0;
+        for (uint32_t u = 0; u < kKept; ++u) mine = larger(mine, kept[u]);
+        uint32_t bound;
+        if (all <= kKept * kLpJoin) {
+            const uint32_t key = ordered(mine);
+            bound = lp_bound(key, a.n_top, sh);
+            if (key >= bound)
 #pragma unroll
-            for (uint32_t u = 0; u < kAhead; ++u) o = n == u ? k[u] : o;
-            if (n >= kAhead) o = keys[i];
-            if (o != 0 && o >= bound) sh.keys[atomicAdd(&sh.count, 1u)] = o;  // of at most n_top parts n_top each
+                for (uint32_t u = 0; u < kKept; ++u)
+                    if (ordered(kept[u]) >= bound) lp_hit(tid + u * kLpJoin, sh);
+        } else {
+            for (uint32_t i = tid + kKept * kLpJoin; i < all; i += kLpJoin) mine = larger(mine, blocks[i]);
+            bound = lp_bound(ordered(mine), a.n_top, sh);
+            for (uint32_t i = tid; i < all; i += kLpJoin)
+                if (ordered(blocks[i]) >= bound) lp_hit(i, sh);
         }
         __syncthreads();
+        const uint32_t items = sh.hits <= kLpMostHits ? sh.hits * each : 0;
+        for (uint32_t i = tid; i < items; i += kLpJoin) {
+            const uint32_t h = sh.hit[i / each], in = i % each, vec = in / 4;
+            const uint32_t from = h / kLpBlocks * a.part_size + vec * kStep + (h % kLpBlocks * 4 + in % 4) * kPer;
+            if (from < a.vocab) lp_search<TYPE>(row, from, a.vocab, bound, sh);
+        }
+        __syncthreads();
+        if (sh.count > kLpMostCandidates || sh.hits > kLpMostHits) lp_by_digits<TYPE>(row, 0, a.vocab, a.n_top, sh);
         lp_rank(sh, sh.count, a.n_top);
     }
     lp_finish<TYPE>(a, r, v, given, sh);
@@ -463,22 +494,33 @@ using namespace dev;
 
 namespace {
 
+template <int TYPE, int TOP, int THREADS>
+void launch_part(hipStream_t s, dim3 grid, const LpArgs& a) {
+    if (a.entropy) hipLaunchKernelGGL((lp_part_kernel<TYPE, TOP, true, THREADS>), grid, dim3(THREADS), 0, s, a);
+    else hipLaunchKernelGGL((lp_part_kernel<TYPE, TOP, false, THREADS>), grid, dim3(THREADS), 0, s, a);
+}
 template <int TYPE>
-void launch_parts(hipStream_t s, dim3 grid, const LpArgs& a) {
-    if (a.n_top && a.entropy) hipLaunchKernelGGL((lp_part_kernel<TYPE, true, true>), grid, dim3(kLpThreads), 0, s, a);
-    else if (a.n_top) hipLaunchKernelGGL((lp_part_kernel<TYPE, true, false>), grid, dim3(kLpThreads), 0, s, a);
-    else if (a.entropy) hipLaunchKernelGGL((lp_part_kernel<TYPE, false, true>), grid, dim3(kLpThreads), 0, s, a);
-    else hipLaunchKernelGGL((lp_part_kernel<TYPE, false, false>), grid, dim3(kLpThreads), 0, s, a);
-    if (a.parts > 1) hipLaunchKernelGGL((lp_join_kernel<TYPE>), dim3(grid.x), dim3(kLpThreads), 0, s, a);
+void launch_typed(hipStream_t s, dim3 grid, uint32_t threads, const LpArgs& a) {
+    if (a.parts > 1) {
+        if (a.n_top) launch_part<TYPE, kTopJoin, 256>(s, grid, a);
+        else launch_part<TYPE, kTopNone, 256>(s, grid, a);
+        hipLaunchKernelGGL((lp_join_kernel<TYPE>), dim3(grid.x), dim3(kLpJoin), 0, s, a);
+    } else if (threads == 256) {
+        if (a.n_top) launch_part<TYPE, kTopHere, 256>(s, grid, a);
+        else launch_part<TYPE, kTopNone, 256>(s, grid, a);
+    } else {
+        if (a.n_top) launch_part<TYPE, kTopHere, 1024>(s, grid, a);
+        else launch_part<TYPE, kTopNone, 1024>(s, grid, a);
+    }
 }
 
-int32_t launch_lp(hipStream_t s, int32_t type, LpArgs a, const char* action) {
-    for (a.first = 0; a.first < a.n_rows; a.first += kMostGroups) {
+int32_t launch_lp(hipStream_t s, int32_t type, uint32_t threads, LpArgs a, const char* action) {
+    for (a.first = 0; a.first < a.n_rows; a.first += kMostGroups / 4) {
         const uint64_t n = a.n_rows - a.first;
-        const dim3 grid(static_cast<uint32_t>(n < kMostGroups ? n : kMostGroups), a.parts);
-        if (type == kDtF32) launch_parts<kDtF32>(s, grid, a);
-        else if (type == kDtF16) launch_parts<kDtF16>(s, grid, a);
-        else launch_parts<kDtBF16>(s, grid, a);
+        const dim3 grid(static_cast<uint32_t>(n < kMostGroups / 4 ? n : kMostGroups / 4), a.parts);
+        if (type == kDtF32) launch_typed<kDtF32>(s, grid, threads, a);
+        else if (type == kDtF16) launch_typed<kDtF16>(s, grid, threads, a);
+        else launch_typed<kDtBF16>(s, grid, threads, a);
         OBJ_HIP(hipGetLastError(), action);
     }
     return 0;
@@ -536,21 +578,27 @@ int32_t objeta_hip_log_probs_device(objeta_hip_context* ctx, objeta_hip_stream s
     a.scale = scale, a.c = static_cast<float>(scale * 1.4426950408889634074);
     a.tokens = d_tokens, a.lp = d_token_log_probs, a.lse = d_lse, a.entropy = d_entropy, a.ids = d_top_ids, a.top = d_top_log_probs;
     a.err = ctx->err_word;
-    const uint32_t turn = kLpThreads * kLpVecs * (dtype == kDtF32 ? 4 : 8);
-    const uint64_t most = (vocab + turn - 1) / turn, want = 1024 / n_rows;
+    // One workgroup a row where rows fill the card or are short (of 1024 threads while there is a CU for
+    // each), otherwise rows are cut and joined. us, 1024 threads / cut: 1 row of 32000 floats 8.3 / 10.5,
+    // of 151936 18.3 / 10.8; 64 rows of 50000 in 16 bits 12.0 / 12.9, of 151936 19.8 / 17.5; 200 rows of 151936
+    // 20.5 / 24.1. 256 threads / cut: 300 rows of 32000 in 16 bits 14.6 / 16.1, of 151936 42 / 30.
+    const uint64_t row_bytes = vocab * es;
+    const bool large = n_rows <= 256 && (row_bytes <= 200000 || n_rows >= 128);
+    const uint32_t threads = large ? 1024 : 256, turn = threads * kLpVecs * (dtype == kDtF32 ? 4 : 8);
+    const uint64_t most = (vocab + turn - 1) / turn, want = large || row_bytes <= 100000 ? 1 : 1024 / n_rows;
     uint64_t parts = want < 1 ? 1 : (want < most ? want : most);
-    if (parts > kLpThreads) parts = kLpThreads;
+    if (parts > kLpJoin) parts = kLpJoin;
     const uint64_t size = ((vocab + parts - 1) / parts + turn - 1) / turn * turn;
     a.part_size = static_cast<uint32_t>(size);
     a.parts = static_cast<uint32_t>((vocab + size - 1) / size);
     if (a.parts > 1) {
         void* ws = nullptr;
         const size_t n = static_cast<size_t>(n_rows) * a.parts;
-        OBJ_TRY(ensure_workspace(ctx, s, kWsLogProbs, n * (sizeof(float4) + 8 * n_top), &ws));
+        OBJ_TRY(ensure_workspace(ctx, s, kWsLogProbs, n * (sizeof(float4) + (n_top ? 4 * kLpBlocks : 0)), &ws));
         a.stats = static_cast<float4*>(ws);
-        a.keys = reinterpret_cast<uint64_t*>(a.stats + n);
+        a.blocks = reinterpret_cast<float*>(a.stats + n);
     }
-    return launch_lp(s, dtype, a, action);
+    return launch_lp(s, dtype, threads, a, action);
     OBJ_GUARD_END
 }
 
