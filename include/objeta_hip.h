@@ -1011,7 +1011,7 @@ int32_t objeta_hip_kv_free_device(objeta_hip_context* ctx, objeta_hip_stream str
  *   leaves them. */
 enum { OBJETA_HIP_CODES_NONE = 0, OBJETA_HIP_CODES_INT8 = 1, OBJETA_HIP_CODES_FP8 = 2 };
 
-/* The RMS norm of n_tokens rows of `hidden` elements (1 .. 65536) with the residual's addition:
+/* The RMS norm of n_tokens rows of `hidden` elements (1 .. 32768) with the residual's addition:
  *   h = x + residual                                   (float; d_residual NULL: h = x)
  *   y_i = h_i (weight_i + weight_offset) / sqrt(sum_j h_j^2 / hidden + eps)
  * d_residual_out (nullable) receives h rounded to residual_dtype, and it is this that is normed;

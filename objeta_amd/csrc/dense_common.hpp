@@ -162,6 +162,14 @@ template <class T> __device__ __forceinline__ T max_of_wave(T v) {
     return larger(larger(lane_of(v, 15), lane_of(v, 31)), larger(lane_of(v, 47), lane_of(v, 63)));
 }
 
+// A value of the lane that a turn of the row of 16 lanes brings here.
+template <int CTRL> __device__ __forceinline__ uint32_t turned(uint32_t v) { return moved_or_same<CTRL>(v); }
+template <int CTRL> __device__ __forceinline__ float turned(float v) { return __uint_as_float(moved_or_same<CTRL>(__float_as_uint(v))); }
+template <int CTRL> __device__ __forceinline__ double turned(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(moved_or_same<CTRL>(static_cast<uint32_t>(u >> 32))) << 32 | moved_or_same<CTRL>(static_cast<uint32_t>(u)));
+}
+
 }  // namespace dev
 #endif
 

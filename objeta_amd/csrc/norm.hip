@@ -49,7 +49,7 @@ struct NormArgs {
     uint32_t width;
     int32_t x_type, r_type, w_type, y_type;
     float offset;
-    double eps;
+    double eps, inv_width;
 };
 enum : int { kCodesNone = 0, kCodesInt8 = 1, kCodesFp8 = 2 };
 
@@ -65,73 +65,112 @@ __device__ __forceinline__ float whole_quotient(float x, float s, float inv) {
     return n;
 }
 
+// 1 / sqrt(m), to an error of some 2^-52: the hardware's estimate (to 2^-23 at least) and two steps
+// y + y (e / 2 + 3/8 e^2), e = 1 - m y^2, each of which leaves 5/16 e^3.
+__device__ __forceinline__ double inverse_root(double m) {
+    double y = __builtin_amdgcn_rsq(m);
+    if (!(m > 0.0 && m < __builtin_inf())) return y;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const double e = __builtin_fma(-m * y, y, 1.0);
+        y = __builtin_fma(y * e, __builtin_fma(e, 0.375, 0.5), y);
+    }
+    return y;
+}
+
+// A row's total, in every lane: within 16 lanes (WAVES 0) by turning them, over a wave, or over the
+// waves of a workgroup.
+template <int WAVES, class T, class Op, class Wave>
+__device__ __forceinline__ T over_row(T v, Op op, Wave wave, T none, T* shared) {
+    if constexpr (WAVES == 0) {
+        v = op(v, turned<0x128>(v));
+        v = op(v, turned<0x124>(v));
+        v = op(v, turned<0x122>(v));
+        return op(v, turned<0x121>(v));
+    } else {
+        v = wave(v);
+        if constexpr (WAVES > 1) {
+            const uint32_t lane = threadIdx.x & 63;
+            if (lane == 0) shared[threadIdx.x >> 6] = v;
+            __syncthreads();
+            v = wave(lane < WAVES ? shared[lane] : none);
+        }
+        return v;
+    }
+}
+
 template <int WAVES, int VECS, bool NORM, int CODES>
-__global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rows_kernel(NormArgs a) {
-    constexpr uint32_t kLanes = 64 * WAVES;
-    constexpr uint32_t kRows = WAVES == 1 ? 4 : 1;  // rows of a workgroup
-    __shared__ double sh_sum[WAVES];
-    __shared__ float sh_max[WAVES];
-    const uint32_t slot = threadIdx.x % kLanes, wave = slot / 64, lane = threadIdx.x & 63;
-    const uint64_t row = a.first + static_cast<uint64_t>(blockIdx.x) * kRows + (WAVES == 1 ? threadIdx.x / 64 : 0);
-    if (row >= a.n_rows) return;  // whole waves; with several waves a row, whole workgroups
+__global__ __launch_bounds__(WAVES <= 1 ? 256 : 64 * WAVES, VECS >= 3 ? 4 : 1) void rows_kernel(NormArgs a) {
+    constexpr uint32_t kLanes = WAVES == 0 ? 16 : 64 * WAVES;
+    constexpr uint32_t kRows = WAVES <= 1 ? 256 / kLanes : 1;  // rows of a workgroup
+    // All of a row and its weights asked for at once; with more vectors registers do not hold them.
+    constexpr bool kEarly = VECS <= (WAVES <= 8 ? 4 : 2);
+    __shared__ double sh_sum[WAVES > 1 ? WAVES : 1];
+    __shared__ uint32_t sh_max[WAVES > 1 ? WAVES : 1];
+    const uint32_t slot = threadIdx.x % kLanes;
+    const uint64_t row = a.first + static_cast<uint64_t>(blockIdx.x) * kRows + (kRows > 1 ? threadIdx.x / kLanes : 0);
+    if (row >= a.n_rows) return;  // a row's lanes together
 
     uint32_t left[VECS];  // elements of each vector that are there
     Raw8 rx[VECS], rr[VECS], rw[VECS];
+    float y[VECS][8];
+    auto place = [&](int v) { return 8 * (slot + v * kLanes); };
+    auto load_x = [&](int v) { rx[v] = left[v] ? load_raw8(a.x_type, a.x, row * a.x_stride + place(v), left[v]) : Raw8{}; };
+    auto load_r = [&](int v) { rr[v] = a.r && left[v] ? load_raw8(a.r_type, a.r, row * a.r_stride + place(v), left[v]) : Raw8{}; };
+    auto load_w = [&](int v) { rw[v] = left[v] ? load_raw8(a.w_type, a.w, place(v), left[v]) : Raw8{}; };
+    auto add = [&](int v) {
+        to_floats(a.x_type, rx[v], y[v]);
+        if (NORM && a.r) {
+            float r[8];
+            to_floats(a.r_type, rr[v], r);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[v][i] += r[i];
+        }
+    };
 #pragma unroll
     for (int v = 0; v < VECS; ++v) {
-        const uint32_t at = 8 * (slot + v * kLanes);
-        left[v] = at < a.width ? (a.width - at < 8 ? a.width - at : 8) : 0;
-        if (left[v]) rx[v] = load_raw8(a.x_type, a.x, row * a.x_stride + at, left[v]);
-        else rx[v] = Raw8{};
-    }
-    if (NORM) {
-#pragma unroll
-        for (int v = 0; v < VECS; ++v) {
-            const uint32_t at = 8 * (slot + v * kLanes);
-            rr[v] = rw[v] = Raw8{};
-            if (a.r && left[v]) rr[v] = load_raw8(a.r_type, a.r, row * a.r_stride + at, left[v]);
-            if (left[v]) rw[v] = load_raw8(a.w_type, a.w, at, left[v]);
+        left[v] = place(v) < a.width ? (a.width - place(v) < 8 ? a.width - place(v) : 8) : 0;
+        load_x(v);
+        if constexpr (!kEarly) {
+            if (NORM) load_r(v);
+            add(v);
         }
     }
-
-    float y[VECS][8];
+    if constexpr (kEarly) {
+        if constexpr (NORM) {
 #pragma unroll
-    for (int v = 0; v < VECS; ++v) to_floats(a.x_type, rx[v], y[v]);
+            for (int v = 0; v < VECS; ++v) load_r(v);
+#pragma unroll
+            for (int v = 0; v < VECS; ++v) load_w(v);
+        }
+#pragma unroll
+        for (int v = 0; v < VECS; ++v) add(v);
+    }
+
     if constexpr (NORM) {
         double sum = 0.0;
 #pragma unroll
         for (int v = 0; v < VECS; ++v) {
-            if (a.r) {
-                float r[8];
-                to_floats(a.r_type, rr[v], r);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[v][i] += r[i];
-            }
             if (a.h) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) y[v][i] = rounded_to(a.r_type, y[v][i]);
-                if (left[v]) store_floats(a.r_type, a.h, row * a.h_stride + 8 * (slot + v * kLanes), left[v], y[v]);
+                if (left[v]) store_floats(a.r_type, a.h, row * a.h_stride + place(v), left[v], y[v]);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) sum = __builtin_fma(static_cast<double>(y[v][i]), static_cast<double>(y[v][i]), sum);
         }
-        sum = sum_of_wave(sum);
-        if (WAVES > 1) {
-            if (lane == 0) sh_sum[wave] = sum;
-            __syncthreads();
-            sum = 0.0;
-            for (int i = 0; i < WAVES; ++i) sum += sh_sum[i];
-        }
-        const double inv = 1.0 / sqrt(sum / a.width + a.eps);
+        sum = over_row<WAVES>(sum, [](double p, double q) { return p + q; }, [](double p) { return sum_of_wave(p); }, 0.0, sh_sum);
+        const double inv = inverse_root(sum * a.inv_width + a.eps);
 #pragma unroll
         for (int v = 0; v < VECS; ++v) {
             float w[8];
+            if (!kEarly) load_w(v);
             to_floats(a.w_type, rw[v], w);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 y[v][i] = static_cast<float>(static_cast<double>(y[v][i]) * inv *
                                              (static_cast<double>(w[i]) + static_cast<double>(a.offset)));
-            if (a.y && left[v]) store_floats(a.y_type, a.y, row * a.y_stride + 8 * (slot + v * kLanes), left[v], y[v]);
+            if (a.y && left[v]) store_floats(a.y_type, a.y, row * a.y_stride + place(v), left[v], y[v]);
         }
     }
 
@@ -146,33 +185,39 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rows_kernel(Nor
                 const uint32_t m = static_cast<uint32_t>(i) < left[v] ? __float_as_uint(y[v][i]) & 0x7FFFFFFFu : 0u;
                 most = m > most ? m : most;
             }
-        most = max_of_wave(most);
-        if (WAVES > 1) {
-            if (lane == 0) sh_max[wave] = __uint_as_float(most);
-            __syncthreads();
-            for (int i = 0; i < WAVES; ++i) {
-                const uint32_t o = __float_as_uint(sh_max[i]);
-                most = o > most ? o : most;
-            }
-        }
+        most = over_row<WAVES>(most, [](uint32_t p, uint32_t q) { return larger(p, q); }, [](uint32_t p) { return max_of_wave(p); }, 0u, sh_max);
         const bool finite = most < 0x7F800000u;
         float s = finite ? __uint_as_float(most) / 127.0f : __builtin_nanf("");
         if (slot == 0) static_cast<float*>(a.scales)[row] = s;
         // Where s or its reciprocal would be no normal number, both sides are taken 2^64 times.
-        const float up = s < 1e-30f ? 18446744073709551616.0f : 1.0f;
+        const bool tiny = s < 1e-30f, zero = !finite || s == 0.0f;
+        const float up = tiny ? 18446744073709551616.0f : 1.0f, inv = 1.0f / (s * up);
         s *= up;
-        const bool zero = !finite || s == 0.0f;
-        const float inv = 1.0f / s;
 #pragma unroll
         for (int v = 0; v < VECS; ++v) {
-            uint32_t c[2] = {0, 0};
+            // x inv + 1.5 2^23 has the nearest whole number in its last byte. The product is off by less than
+            // 127 2^-24; where it comes nearer to a half than that, the quotients are taken exactly.
+            constexpr float kWhole = 12582912.0f;
+            uint32_t t[8];
+            float far = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                float n = zero ? 0.0f : whole_quotient(y[v][i] * up, s, inv);
-                n = __builtin_fminf(__builtin_fmaxf(n, -127.0f), 127.0f);
-                c[i / 4] |= (static_cast<uint32_t>(static_cast<int32_t>(n)) & 0xFFu) << (8 * (i % 4));
+                const float n = __builtin_fmaf(y[v][i], inv, kWhole);
+                t[i] = __float_as_uint(n);
+                far = __builtin_fmaxf(far, __builtin_fabsf(__builtin_fmaf(y[v][i], inv, kWhole - n)));
             }
-            uint8_t* to = static_cast<uint8_t*>(a.codes) + row * a.code_stride + 8 * (slot + v * kLanes);
+            if (tiny || far > 0.49999f) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float n = __builtin_fminf(__builtin_fmaxf(whole_quotient(y[v][i] * up, s, inv), -127.0f), 127.0f);
+                    t[i] = __float_as_uint(n + kWhole);
+                }
+            }
+            uint32_t c[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                c[i] = zero ? 0 : __builtin_amdgcn_perm(t[4 * i + 1], t[4 * i], 0x0C0C0400u) | __builtin_amdgcn_perm(t[4 * i + 3], t[4 * i + 2], 0x04000C0Cu);
+            uint8_t* to = static_cast<uint8_t*>(a.codes) + row * a.code_stride + place(v);
             if (left[v] == 8) {
                 *reinterpret_cast<any_u32x2*>(to) = any_u32x2{c[0], c[1]};
             } else {
@@ -193,19 +238,15 @@ __global__ __launch_bounds__(WAVES == 1 ? 256 : 64 * WAVES) void rows_kernel(Nor
                 const float x = __builtin_fabsf(y[v][i]);
                 if (left[v] && x > m) m = x;
             }
-#pragma unroll
-            for (int off = 8; off > 0; off >>= 1) {
-                const float o = __shfl_xor(m, off, 64);
-                m = o > m ? o : m;
-            }
+            m = over_row<0>(m, [](float p, float q) { return larger(p, q); }, 0, 0.0f, static_cast<float*>(nullptr));
             if (!left[v]) continue;
             const rules::Fp8ActScale sc = rules::fp8_act_scale(m);
             uint32_t c[2] = {0, 0};
 #pragma unroll
             for (int i = 0; i < 8; ++i) c[i / 4] |= static_cast<uint32_t>(rules::fp8_act_code(y[v][i], sc.inv)) << (8 * (i % 4));
-            const uint32_t at = 8 * (slot + v * kLanes);
+            const uint32_t at = place(v);
             *reinterpret_cast<any_u32x2*>(static_cast<uint8_t*>(a.codes) + row * a.code_stride + at) = any_u32x2{c[0], c[1]};
-            if ((lane & 15) == 0) static_cast<uint8_t*>(a.scales)[row * (a.width / 128) + at / 128] = sc.raw;
+            if ((slot & 15) == 0) static_cast<uint8_t*>(a.scales)[row * (a.width / 128) + at / 128] = sc.raw;
         }
     }
 }
@@ -217,11 +258,12 @@ using namespace dev;
 namespace {
 
 constexpr uint64_t kMaxWidth = 65536;             // a row in the registers of 16 waves, eight vectors a thread
+constexpr uint64_t kMaxHidden = 32768;            // four, whose sums and weights take registers too
 constexpr uint64_t kGroups = kMostGroups / 4;     // of a launch: they have up to 1024 threads
 
 template <int WAVES, int VECS, bool NORM>
 void launch_shape(hipStream_t s, uint32_t groups, int codes, const NormArgs& a) {
-    const dim3 block(WAVES == 1 ? 256 : 64 * WAVES);
+    const dim3 block(WAVES <= 1 ? 256 : 64 * WAVES);
     if (codes == kCodesInt8) hipLaunchKernelGGL((rows_kernel<WAVES, VECS, NORM, kCodesInt8>), dim3(groups), block, 0, s, a);
     else if constexpr (NORM) {
         if (codes == kCodesFp8) hipLaunchKernelGGL((rows_kernel<WAVES, VECS, NORM, kCodesFp8>), dim3(groups), block, 0, s, a);
@@ -229,22 +271,30 @@ void launch_shape(hipStream_t s, uint32_t groups, int codes, const NormArgs& a) 
     }
 }
 
-// As many waves as leave a thread one or two vectors.
+// Waves of a row and vectors of a thread. A vector that a row does not fill costs what a full one does,
+// so that the smallest shape that holds a row is taken; of rows enough to fill the card those with few
+// waves, which wait for one another less (8192 rows of 6144: four waves of three vectors 85 us, sixteen of
+// one 105), of fewer rows those with most (32 rows of 4096: eight waves of one 6.2 us, four of two 7.1).
 template <bool NORM>
 int32_t launch_rows(hipStream_t s, int codes, NormArgs a, const char* action) {
     const uint32_t vectors = (a.width + 7) / 8;
-    const uint64_t rows = vectors <= 128 ? 4 : 1;  // of a workgroup
+    const bool many = a.n_rows >= 1024;
+    const uint64_t rows = vectors <= 32 ? 16 : vectors <= (many ? 128u : 64u) ? 4 : 1;  // of a workgroup
     for (a.first = 0; a.first < a.n_rows; a.first += kGroups * rows) {
         const uint64_t n = (a.n_rows - a.first + rows - 1) / rows;
-        const uint32_t groups = static_cast<uint32_t>(n < kGroups ? n : kGroups);
-        if (vectors <= 64) launch_shape<1, 1, NORM>(s, groups, codes, a);
-        else if (vectors <= 128) launch_shape<1, 2, NORM>(s, groups, codes, a);
-        else if (vectors <= 256) launch_shape<4, 1, NORM>(s, groups, codes, a);
-        else if (vectors <= 512) launch_shape<4, 2, NORM>(s, groups, codes, a);
-        else if (vectors <= 1024) launch_shape<16, 1, NORM>(s, groups, codes, a);
-        else if (vectors <= 2048) launch_shape<16, 2, NORM>(s, groups, codes, a);
-        else if (vectors <= 4096) launch_shape<16, 4, NORM>(s, groups, codes, a);
-        else launch_shape<16, 8, NORM>(s, groups, codes, a);
+        const uint32_t g = static_cast<uint32_t>(n < kGroups ? n : kGroups);
+        if (vectors <= 16) launch_shape<0, 1, NORM>(s, g, codes, a);
+        else if (vectors <= 32) launch_shape<0, 2, NORM>(s, g, codes, a);
+        else if (vectors <= 64) launch_shape<1, 1, NORM>(s, g, codes, a);
+        else if (vectors <= 128) many ? launch_shape<1, 2, NORM>(s, g, codes, a) : launch_shape<2, 1, NORM>(s, g, codes, a);
+        else if (vectors <= 256) launch_shape<4, 1, NORM>(s, g, codes, a);
+        else if (vectors <= 512) many ? launch_shape<4, 2, NORM>(s, g, codes, a) : launch_shape<8, 1, NORM>(s, g, codes, a);
+        else if (vectors <= 768 && many) launch_shape<4, 3, NORM>(s, g, codes, a);
+        else if (vectors <= 1024) many ? launch_shape<8, 2, NORM>(s, g, codes, a) : launch_shape<16, 1, NORM>(s, g, codes, a);
+        else if (vectors <= 1536 && many) launch_shape<8, 3, NORM>(s, g, codes, a);
+        else if (vectors <= 2048) many ? launch_shape<8, 4, NORM>(s, g, codes, a) : launch_shape<16, 2, NORM>(s, g, codes, a);
+        else if (vectors <= 4096) launch_shape<16, 4, NORM>(s, g, codes, a);
+        else if constexpr (!NORM) launch_shape<16, 8, NORM>(s, g, codes, a);
         OBJ_HIP(hipGetLastError(), action);
     }
     return 0;
@@ -267,8 +317,8 @@ int32_t objeta_hip_rms_norm_device(objeta_hip_context* ctx, objeta_hip_stream st
     OBJ_GUARD_BEGIN
     const char* action = "rms_norm_device";
     OBJ_TRY(check_ctx(ctx, action));
-    if (hidden == 0 || hidden > kMaxWidth)
-        OBJ_FAIL(kInvalidInput, action, strf("hidden %llu must be 1 to 65536", (unsigned long long)hidden));
+    if (hidden == 0 || hidden > kMaxHidden)
+        OBJ_FAIL(kInvalidInput, action, strf("hidden %llu must be 1 to 32768", (unsigned long long)hidden));
     if (!dtype_ok(dtype) || !dtype_ok(weight_dtype)) OBJ_FAIL(kInvalidInput, action, "dtype must be F32, F16 or BF16");
     if ((d_residual || d_residual_out) && !dtype_ok(residual_dtype))
         OBJ_FAIL(kInvalidInput, action, "residual dtype must be F32, F16 or BF16");
@@ -317,7 +367,7 @@ int32_t objeta_hip_rms_norm_device(objeta_hip_context* ctx, objeta_hip_stream st
     a.code_stride = codes_stride;
     a.n_rows = n, a.width = static_cast<uint32_t>(hidden);
     a.x_type = dtype, a.r_type = residual_dtype, a.w_type = weight_dtype, a.y_type = out_dtype;
-    a.offset = weight_offset, a.eps = eps;
+    a.offset = weight_offset, a.eps = eps, a.inv_width = 1.0 / static_cast<double>(hidden);
     const OnDevice on(ctx->device);
     OBJ_HIP(on.status(), action);
     return launch_rows<true>(resolve_stream(ctx, stream), codes, a, action);

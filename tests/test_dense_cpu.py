@@ -36,7 +36,7 @@ def call_norm(lib, ctx, **kw):
 
 
 @pytest.mark.parametrize("kw,text", [
-    ({"hidden": 0}, "hidden"), ({"hidden": 65537}, "hidden"), ({"dtype": 3}, "dtype"), ({"wt": 9}, "dtype"), ({"rt": 3}, "residual dtype"),
+    ({"hidden": 0}, "hidden"), ({"hidden": 32769}, "hidden"), ({"dtype": 3}, "dtype"), ({"wt": 9}, "dtype"), ({"rt": 3}, "residual dtype"),
     ({"ot": -1}, "out dtype"), ({"codes": 3}, "unknown codes"), ({"codes": -1}, "unknown codes"), ({"codes": 2, "hidden": 200}, "multiple of 128"),
     ({"eps": -1e-9}, "eps"), ({"eps": float("nan")}, "eps"), ({"eps": float("inf")}, "eps"), ({"offset": float("nan")}, "offset"),
     ({"n": 1 << 31}, "too many tokens"), ({"o": None, "ro": None, "codes": 0}, "no output"), ({"x": None}, "x is NULL"),

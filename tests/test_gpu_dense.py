@@ -93,7 +93,7 @@ def run_norm(be, dense, hidden, n, t, rt=None, ot=None, codes=None, kept=False, 
 
 
 @pytest.mark.parametrize("hidden", [1, 7, 8, 9, 63, 64, 511, 512, 513, 1000, 1024, 1025, 2047, 2048, 2049, 4096, 4100, 8191, 8192, 8193,
-                                    16384, 16385, 32768, 32769, 65535, 65536])
+                                    16384, 16385, 32767, 32768])
 @pytest.mark.parametrize("n", [1, 5])
 def test_norm_widths(backend, dense, hidden, n):
     run_norm(backend, dense, hidden, n, "bf16", "f32", "f32", "i8", kept=True)
