@@ -243,7 +243,7 @@ __global__ __launch_bounds__(WAVES <= 1 ? 256 : 64 * WAVES, VECS >= 3 ? 4 : 1) v
             const rules::Fp8ActScale sc = rules::fp8_act_scale(m);
             uint32_t c[2] = {0, 0};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) c[i / 4] |= static_cast<uint32_t>(rules::fp8_act_code(y[v][i], sc.inv)) << (8 * (i % 4));
+            for (int i = 0; i < 8; ++i) c[i / 4] |= static_cast<uint32_t>(rules::fp8_act_code_short(y[v][i], sc.inv)) << (8 * (i % 4));
             const uint32_t at = place(v);
             *reinterpret_cast<any_u32x2*>(static_cast<uint8_t*>(a.codes) + row * a.code_stride + at) = any_u32x2{c[0], c[1]};
             if ((slot & 15) == 0) static_cast<uint8_t*>(a.scales)[row * (a.width / 128) + at / 128] = sc.raw;

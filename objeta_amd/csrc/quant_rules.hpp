@@ -325,6 +325,18 @@ OBJ_HD uint8_t fp8_act_code(float x, float inv) {
     return f32_to_f8e4m3_exact(v);
 }
 
+// fp8_act_code without branches, for a NaN or infinity too. Above the zeros and below 448 a code is
+// the magnitude's exponent and three mantissa bits, biased by 120 in place of 127 - 7: rounding half
+// up carries from the one into the other.
+OBJ_HD uint8_t fp8_act_code_short(float x, float inv) {
+    const float v = x * inv, a = __builtin_fabsf(v);
+    const int32_t full = static_cast<int32_t>((f2u(a) + (1u << 19)) >> 20) - (120 << 3);
+    int32_t code = full < 0x77 ? full : 0x77;
+    code = a >= 448.0f ? 0x7E : code;
+    code = a < 0.0078125f ? 0 : code;
+    return static_cast<uint8_t>(code | (v < 0.0f ? 0x80 : 0));
+}
+
 // Counter-based synthetic generator: element i of stream `seed` is
 // sigma * z with z an Irwin-Hall(12) draw from four splitmix64 words (3 x 21-bit
 // fields each). The integer sum is exact and its centred value stays below 2^24,
