@@ -23,6 +23,7 @@ struct I8Args {
     uint64_t a_stride, w_stride, out_stride;
     uint32_t n_tokens, rows, cols;
     int32_t out_type;
+    bool once;  // channels' codes are not kept in the caches
 };
 
 typedef uint32_t word_u32x4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -161,6 +162,8 @@ __global__ __launch_bounds__(64 * WAVES) void i8_stream_kernel(I8Args a) {
     }
 }
 
+constexpr int kOnce = 2;  // a buffer load that asks the caches not to keep its lines
+
 // More tokens: a workgroup computes 32 TC WC channels by 32 TT WT tokens, 128 KG columns a step; each
 // of KG groups of WC WT waves takes 128 of these, and the groups' sums are added at the end. A group's
 // columns lie twice in LDS, rows of 128 bytes whose 16-byte chunks are exchanged by the row (chunk c of
@@ -216,6 +219,17 @@ __global__ __launch_bounds__(64 * WC * WT * KG, 2) void i8_tile_kernel(I8Args a,
     const uint32_t last = a.cols < 16 ? 0 : a.cols - 16;
     auto load = [&](Stage& v, uint32_t step, uint32_t j0, uint32_t j1) {
         const uint32_t k = 128 * (step * KG + kg) + 16 * chunk;
+        if constexpr (WHOLE && kC * kT <= 8192) {  // (larger tiles have no registers for it)
+            if (a.once) {
+#pragma unroll
+                for (uint32_t j = j0; j < j1; ++j) {
+                    const int at = k < a.cols ? static_cast<int>(from[j] + k) : -1;
+                    v[j] = __builtin_bit_cast(i32x4, j < kLoadsC ? __builtin_amdgcn_raw_buffer_load_b128(rs_c, at, 0, kOnce)
+                                                                 : __builtin_amdgcn_raw_buffer_load_b128(rs_t, at, 0, 0));
+                }
+                return;
+            }
+        }
 #pragma unroll
         for (uint32_t j = j0; j < j1; ++j) {
             if constexpr (WHOLE) {  // columns past the last are out of the buffer's range: zeros
@@ -499,6 +513,9 @@ int32_t straighten(objeta_hip_context* ctx, hipStream_t s, I8Args& a, const char
 int32_t launch_i8(objeta_hip_context* ctx, hipStream_t s, I8Args a, const char* action) {
     if (!whole_chunks(a)) OBJ_TRY(straighten(ctx, s, a, action));
     const bool whole = whole_chunks(a);
+    // Codes of channels past what the last-level cache keeps from one layer's turn to the next: 64 tokens of
+    // 4096 to 14336 17.6 and 15.9 us; of 2048 to 5120 (which it keeps) 7.6 and 8.7.
+    a.once = static_cast<uint64_t>(a.rows) * a.cols >= (uint64_t(32) << 20) && a.n_tokens <= 256;
     const bool near = a.a_stride < (1u << 22) && a.w_stride < (1u << 22);  // a tile's rows within a buffer's 32-bit range
     if (a.n_tokens <= 16 || !near || a.cols < 16) {
         // 16 channels a workgroup where these are few, 32 otherwise, whose tokens' codes are read half as
