@@ -78,87 +78,75 @@ __device__ __forceinline__ void store_one(int32_t type, void* out, uint64_t at, 
     else static_cast<uint16_t*>(out)[at] = static_cast<uint16_t>(bits_of(type, x));
 }
 
-// Few tokens: a workgroup takes 16 NC channels and 16 NT tokens, its waves share the columns. The
+// Few tokens: a workgroup takes 16 channels and 16 tokens, its eight waves share the columns. The
 // matrix instruction's operands are sixteen codes of a channel (lane % 16) and of a token, columns
-// 16 (lane / 16) on; channels' codes come straight from memory, each once, U loads ahead.
-template <int WAVES, int NC, int NT, int U, bool WHOLE>
-__global__ __launch_bounds__(64 * WAVES) void i8_stream_kernel(I8Args a) {
-    __shared__ i32x4 part[WAVES][NC * NT][64];
+// 16 (lane / 16) on; channels' codes come straight from memory, each once, four loads ahead. (One token:
+// 4096 of 14336 columns 12.9 us, 4.6 TB/s; 151936 of 4096 103 us, 6.0 TB/s. Loads past the caches
+// changed nothing here. 32 channels a workgroup read tokens' codes half as often, but 4096 channels
+// are then 128 workgroups: 18 us; the 151936 take 111.)
+constexpr int kStreamWaves = 8, kStreamAhead = 4;
+template <bool WHOLE>
+__global__ __launch_bounds__(64 * kStreamWaves) void i8_stream_kernel(I8Args a) {
+    __shared__ i32x4 part[kStreamWaves][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t r0 = 16 * NC * blockIdx.x, t0 = 16 * NT * blockIdx.y;
-    constexpr int kRows = NC + NT;
-    const int8_t* row[kRows];  // channels, then tokens (the last one again past it)
-#pragma unroll
-    for (int n = 0; n < kRows; ++n) {
-        const uint32_t i = (n < NC ? r0 + 16 * n : t0 + 16 * (n - NC)) + (lane & 15), all = n < NC ? a.rows : a.n_tokens;
-        row[n] = (n < NC ? a.w : a.a) + (i < all ? i : all - 1) * (n < NC ? a.w_stride : a.a_stride);
-    }
+    const uint32_t r0 = 16 * blockIdx.x, t0 = 16 * blockIdx.y, r = r0 + (lane & 15), t = t0 + (lane & 15);
+    // (past the last channel and token: these again)
+    const int8_t* const row[2] = {a.w + (r < a.rows ? r : a.rows - 1) * a.w_stride, a.a + (t < a.n_tokens ? t : a.n_tokens - 1) * a.a_stride};
     typedef typename std::conditional<WHOLE, i32x4, Raw16>::type Raw;
-    Raw next[U][kRows];
-    auto load = [&](uint32_t k) {
+    typedef Raw Stage[kStreamAhead][2];
+    auto load = [&](Stage& v, uint32_t k) {
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < kStreamAhead; ++u)
 #pragma unroll
-            for (int n = 0; n < kRows; ++n) {
+            for (int n = 0; n < 2; ++n) {
                 const uint32_t at = k + 64 * u + 16 * (lane >> 4);
                 if constexpr (WHOLE) {
-                    next[u][n] = load16(row[n] + (at < a.cols ? at : 0));
+                    v[u][n] = load16(row[n] + (at < a.cols ? at : 0));
                 } else if (a.cols >= 16) {
                     const uint64_t p = reinterpret_cast<uint64_t>(row[n]);
-                    next[u][n] = load_raw16(reinterpret_cast<const int8_t*>(p & ~uint64_t(3)), static_cast<uint32_t>(p & 3) + read_at(at, a.cols));
+                    v[u][n] = load_raw16(reinterpret_cast<const int8_t*>(p & ~uint64_t(3)), static_cast<uint32_t>(p & 3) + read_at(at, a.cols));
                 } else {
-                    next[u][n] = Raw16{load_few(row[n], at, a.cols), 0};
+                    v[u][n] = Raw16{load_few(row[n], at, a.cols), 0};
                 }
             }
     };
     // past the last column: channels' codes 0, tokens' any
-    auto codes = [&](const Raw& r, int n, uint32_t k, uint32_t at) {
+    auto codes = [&](const Raw& v, int n, uint32_t k, uint32_t at) {
         if constexpr (WHOLE) {
-            return n < NC && at >= a.cols ? i32x4{0, 0, 0, 0} : r;
+            return n == 0 && at >= a.cols ? i32x4{0, 0, 0, 0} : v;
         } else {
-            if (a.cols < 16) return r.v;
+            if (a.cols < 16) return v.v;
             const uint32_t from = read_at(at, a.cols);
-            const i32x4 v = straight(r, static_cast<uint32_t>(reinterpret_cast<uint64_t>(row[n])) + from);
-            return k + 64 <= a.cols ? v : moved(v, at - from);
+            const i32x4 x = straight(v, static_cast<uint32_t>(reinterpret_cast<uint64_t>(row[n])) + from);
+            return k + 64 <= a.cols ? x : moved(x, at - from);
         }
     };
-    i32x4 sum[NC][NT] = {};
-    constexpr uint32_t kStep = 64 * U * WAVES;
-    load(64 * U * wave);
-    for (uint32_t k = 64 * U * wave; k < a.cols; k += kStep) {
-        Raw now[U][kRows];
+    i32x4 sum = {};
+    constexpr uint32_t kEach = 64 * kStreamAhead, kStep = kEach * kStreamWaves;
+    Stage next;
+    load(next, kEach * wave);
+    for (uint32_t k = kEach * wave; k < a.cols; k += kStep) {
+        Stage now;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < kStreamAhead; ++u) now[u][0] = next[u][0], now[u][1] = next[u][1];
+        if (k + kStep < a.cols) load(next, k + kStep);
 #pragma unroll
-            for (int n = 0; n < kRows; ++n) now[u][n] = next[u][n];
-        if (k + kStep < a.cols) load(k + kStep);
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            i32x4 v[kRows];
-#pragma unroll
-            for (int n = 0; n < kRows; ++n) v[n] = codes(now[u][n], n, k + 64 * u, k + 64 * u + 16 * (lane >> 4));
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int n = 0; n < NT; ++n) sum[c][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[c], v[NC + n], sum[c][n], 0, 0, 0);
+        for (int u = 0; u < kStreamAhead; ++u) {
+            const uint32_t at = k + 64 * u + 16 * (lane >> 4);
+            sum = __builtin_amdgcn_mfma_i32_16x16x64_i8(codes(now[u][0], 0, k + 64 * u, at), codes(now[u][1], 1, k + 64 * u, at), sum, 0, 0, 0);
         }
     }
-#pragma unroll
-    for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int n = 0; n < NT; ++n) part[wave][c * NT + n][lane] = sum[c][n];
+    part[wave][lane] = sum;
     __syncthreads();
-    for (uint32_t i = wave; i < NC * NT; i += WAVES) {
-        i32x4 s = part[0][i][lane];
-        for (int v = 1; v < WAVES; ++v) s += part[v][i][lane];
-        const uint32_t t = t0 + 16 * (i % NT) + (lane & 15);
-        if (t >= a.n_tokens) continue;
-        const float sa = a.sa[t];
+    if (wave || t >= a.n_tokens) return;
+    i32x4 s = part[0][lane];
 #pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t c = r0 + 16 * (i / NT) + 4 * (lane >> 4) + j;
-            if (c < a.rows) store_one(a.out_type, a.out, t * a.out_stride + c, scaled(s[j], sa, a.sw[c], a.bias, a.bias ? a.bias[c] : 0.0f));
-        }
+    for (int v = 1; v < kStreamWaves; ++v) s += part[v][lane];
+    const float sa = a.sa[t];
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t c = r0 + 4 * (lane >> 4) + j;
+        if (c < a.rows) store_one(a.out_type, a.out, t * a.out_stride + c, scaled(s[j], sa, a.sw[c], a.bias, a.bias ? a.bias[c] : 0.0f));
     }
 }
 
@@ -428,11 +416,10 @@ namespace {
 
 constexpr uint64_t kMaxCols = 131071;  // sums of products of codes from -128 on stay below 2^31
 
-template <int WAVES, int NC, int NT, int U>
 void launch_stream(hipStream_t s, const I8Args& a, bool whole) {
-    const dim3 grid((a.rows + 16 * NC - 1) / (16 * NC), (a.n_tokens + 16 * NT - 1) / (16 * NT)), block(64 * WAVES);
-    if (whole) hipLaunchKernelGGL((i8_stream_kernel<WAVES, NC, NT, U, true>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((i8_stream_kernel<WAVES, NC, NT, U, false>), grid, block, 0, s, a);
+    const dim3 grid((a.rows + 15) / 16, (a.n_tokens + 15) / 16), block(64 * kStreamWaves);
+    if (whole) hipLaunchKernelGGL((i8_stream_kernel<true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((i8_stream_kernel<false>), grid, block, 0, s, a);
 }
 
 template <int WC, int WT, int TC, int TT, int KG, int AHEAD, bool WHOLE>
@@ -447,7 +434,7 @@ void launch_either(hipStream_t s, const I8Args& a, bool whole) {
     else launch_tile<WC, WT, TC, TT, KG, 1, false>(s, a);
 }
 
-// What a tile costs, in us, measured over batches of 17 to 8192 tokens and matrices of 512 to 151936
+// What a tile costs, in us, measured over batches of 5 to 8192 tokens and matrices of 512 to 151936
 // channels by 2048 to 14336 columns: `fixed` around the columns; for 128 columns `low` where a CU has one
 // workgroup and few others run, `full` a workgroup of a full card, where the products of real codes
 // draw the clock down (8192^3: 450 us, of zeros 318). `resident` workgroups share a CU.
@@ -514,14 +501,17 @@ int32_t launch_i8(objeta_hip_context* ctx, hipStream_t s, I8Args a, const char* 
     if (!whole_chunks(a)) OBJ_TRY(straighten(ctx, s, a, action));
     const bool whole = whole_chunks(a);
     // Codes of channels past what the last-level cache keeps from one layer's turn to the next: 64 tokens of
-    // 4096 to 14336 17.6 and 15.9 us; of 2048 to 5120 (which it keeps) 7.6 and 8.7.
+    // 4096 to 14336 19.1 and 17.3 us, 17 of 4096 to 32000 33.0 and 30.2; 64 of 2048 to 5120 (which it keeps)
+    // 7.6 and 8.7.
     a.once = static_cast<uint64_t>(a.rows) * a.cols >= (uint64_t(32) << 20) && a.n_tokens <= 256;
     const bool near = a.a_stride < (1u << 22) && a.w_stride < (1u << 22);  // a tile's rows within a buffer's 32-bit range
-    if (a.n_tokens <= 16 || !near || a.cols < 16) {
-        // 16 channels a workgroup where these are few, 32 otherwise, whose tokens' codes are read half as
-        // often (one token, 4096 of 14336 columns: 12.9 and 18.0 us; 151936 of 4096: 123 and 109)
-        if (a.rows <= 8192) launch_stream<8, 1, 1, 4>(s, a, whole);
-        else launch_stream<8, 2, 1, 2>(s, a, whole);
+    // Tiles load tokens' codes once for more channels, and pass large matrices by the caches: 8 tokens of
+    // 4096 to 14336 16.5 us, streamed 17.2 (3 tokens: 16.6 and 15.5), of 4096 to 151936 123 and
+    // 135, of 14336 to 4096 19.1 and 14.6 (16 tokens: 19.7 and 18.2). Rows that begin anywhere cost them
+    // more: 8 tokens of 4095 to 14336 27.9 and 27.2.
+    const uint32_t few = a.rows >= 7168 && whole ? 4 : 16;
+    if (a.n_tokens <= few || !near || a.cols < 16) {
+        launch_stream(s, a, whole);
     } else {
         switch (best_tile(a, whole)) {
             case kTile256: launch_tile<2, 4, 4, 2, 1, 1, true>(s, a); break;

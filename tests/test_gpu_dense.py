@@ -282,6 +282,13 @@ def test_product_of_many_rows_on_another_stream(backend, dense, n, rows, cols):
     check_product(backend, dense, n, rows, cols, "bf16", stream=backend.stream(1))
 
 
+@pytest.mark.parametrize("n,rows,cols", [(5, 9000, 4096), (16, 7168, 64), (4, 7200, 80), (12, 8000, 33), (100, 9000, 4096),
+                                         (100, 9000, 1001), (100, 20000, 4096), (600, 9000, 33), (1500, 9000, 512),
+                                         (1000, 4097, 4096), (600, 7200, 4700)])
+def test_product_of_every_tile(backend, dense, n, rows, cols):
+    check_product(backend, dense, n, rows, cols, "bf16" if n % 3 else "f32", pads=(0, 0, n % 2 * 5))
+
+
 @pytest.mark.parametrize("cols", [15, 16, 17, 35, 130])
 @pytest.mark.parametrize("skews,pads", [((0, 0, 0), (0, 0, 0)), ((3, 0, 0), (1, 0, 0)), ((0, 2, 1), (13, 30, 1))])
 def test_product_of_many_rows_that_begin_anywhere(backend, dense, cols, skews, pads):
