@@ -506,10 +506,9 @@ int32_t launch_i8(objeta_hip_context* ctx, hipStream_t s, I8Args a, const char* 
     a.once = static_cast<uint64_t>(a.rows) * a.cols >= (uint64_t(32) << 20) && a.n_tokens <= 256;
     const bool near = a.a_stride < (1u << 22) && a.w_stride < (1u << 22);  // a tile's rows within a buffer's 32-bit range
     // Tiles load tokens' codes once for more channels, and pass large matrices by the caches: 8 tokens of
-    // 4096 to 14336 16.5 us, streamed 17.2 (3 tokens: 16.6 and 15.5), of 4096 to 151936 123 and
-    // 135, of 14336 to 4096 19.1 and 14.6 (16 tokens: 19.7 and 18.2). Rows that begin anywhere cost them
-    // more: 8 tokens of 4095 to 14336 27.9 and 27.2.
-    const uint32_t few = a.rows >= 7168 && whole ? 4 : 16;
+    // 4096 to 14336 14.4 us, streamed 16.7 (one: 14.5 and 14.6), of 4096 to 151936 106 and 128 (one: 103 and
+    // 102), of 4095 to 14336 20.6 and 27.2, of 14336 to 4096 19.1 and 14.5 (16 tokens: 19.7 and 18.0).
+    const uint32_t few = a.rows >= 7168 ? 2 : 16;
     if (a.n_tokens <= few || !near || a.cols < 16) {
         launch_stream(s, a, whole);
     } else {
@@ -518,7 +517,13 @@ int32_t launch_i8(objeta_hip_context* ctx, hipStream_t s, I8Args a, const char* 
             case kTile128x256: launch_either<2, 4, 2, 2, 1, 2>(s, a, whole); break;
             case kTile128: launch_either<2, 2, 2, 2, 1, 2>(s, a, whole); break;
             case kTile64x128: launch_either<2, 2, 1, 2, 1, 3>(s, a, whole); break;
-            case kTile64: launch_either<2, 2, 1, 1, 1, 3>(s, a, whole); break;
+            case kTile64:
+                // Up to 32 tokens a tile half as high, two groups along the columns: 32 tokens of 4096 to 14336
+                // 16.8 -> 14.8 us, to 151936 139 -> 126, 20 of 4095 to 14336 28.7 -> 21.5; of 1024 to
+                // 32000 9.3 and 10.5.
+                if (a.n_tokens <= 32 && a.cols >= 2048) launch_either<2, 1, 1, 1, 2, 4>(s, a, whole);
+                else launch_either<2, 2, 1, 1, 1, 3>(s, a, whole);
+                break;
             case kTile32x64: launch_either<1, 2, 1, 1, 4, 2>(s, a, whole); break;
             default: launch_either<1, 1, 1, 1, 8, 3>(s, a, whole); break;
         }

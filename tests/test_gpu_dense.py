@@ -282,7 +282,7 @@ def test_product_of_many_rows_on_another_stream(backend, dense, n, rows, cols):
     check_product(backend, dense, n, rows, cols, "bf16", stream=backend.stream(1))
 
 
-@pytest.mark.parametrize("n,rows,cols", [(5, 9000, 4096), (16, 7168, 64), (4, 7200, 80), (12, 8000, 33), (100, 9000, 4096),
+@pytest.mark.parametrize("n,rows,cols", [(5, 9000, 4096), (16, 7168, 64), (4, 7200, 80), (12, 8000, 33), (100, 9000, 4096), (32, 9000, 2048), (20, 9000, 4095),
                                          (100, 9000, 1001), (100, 20000, 4096), (600, 9000, 33), (1500, 9000, 512),
                                          (1000, 4097, 4096), (600, 7200, 4700)])
 def test_product_of_every_tile(backend, dense, n, rows, cols):
