@@ -11,8 +11,8 @@
 // complement of its index: equal values go by the lowest index. Where too many values reach the bound
 // (ties, all of the best in few threads), the N-th value is found bit by bit over the row instead.
 //
-// Bound: rows that are many by HBM and the instructions of an element, some ten, alike (2048 rows of
-// 151936 bf16 with the best five 117 us, 5.3 TB/s); few rows are cut over workgroups, whose parts a
+// Bound: rows that are many by HBM, 16-bit ones by the instructions of an element, some ten, too (2048 rows of
+// 151936 floats with the best five 194 us, 6.4 TB/s; bf16 105, 5.9 TB/s); few rows are cut over workgroups, whose parts a
 // second launch joins (one row of 151936 floats with the best twenty 9.8 us, two launches).
 #include "dense_common.hpp"
 #include "kernels.hpp"
@@ -336,7 +336,8 @@ __device__ void lp_finish(const LpArgs& a, uint64_t r, LpSums v, LpGiven first, 
 
 enum : int { kTopNone = 0, kTopHere = 1, kTopJoin = 2 };  // who finds the best: nobody, this workgroup, the join
 
-template <int TYPE, int TOP, bool ENTROPY, int THREADS>
+// ONCE: logits are not kept in the caches.
+template <int TYPE, int TOP, bool ENTROPY, bool ONCE, int THREADS>
 __global__ __launch_bounds__(THREADS, THREADS == 256 ? 8 : 4) void lp_part_kernel(LpArgs a) {
     constexpr uint32_t kPer = LpElem<TYPE>::kPer, kStep = THREADS * kPer, kTurn = kLpVecs * kStep;
     __shared__ LpShared<THREADS> sh;
@@ -357,9 +358,9 @@ __global__ __launch_bounds__(THREADS, THREADS == 256 ? 8 : 4) void lp_part_kerne
     const char* mine_at = static_cast<const char*>(row) + (static_cast<uint64_t>(lo) + tid * kPer) * (16 / kPer);
     auto load = [&](uint32_t turn) {
         if (turn < whole) {
+            const any_u32x4* at = reinterpret_cast<const any_u32x4*>(mine_at + static_cast<uint64_t>(turn) * kLpVecs * THREADS * 16);
 #pragma unroll
-            for (uint32_t u = 0; u < kLpVecs; ++u)
-                next[u] = *reinterpret_cast<const any_u32x4*>(mine_at + (static_cast<uint64_t>(turn) * kLpVecs + u) * THREADS * 16);
+            for (uint32_t u = 0; u < kLpVecs; ++u) next[u] = ONCE ? __builtin_nontemporal_load(at + u * THREADS) : at[u * THREADS];
         } else if (turn < turns) {
 #pragma unroll
             for (uint32_t u = 0; u < kLpVecs; ++u) next[u] = lp_load<TYPE>(row, lo + turn * kTurn + u * kStep + tid * kPer, hi);
@@ -497,32 +498,34 @@ using namespace dev;
 namespace {
 
 template <int TYPE, int TOP, int THREADS>
-void launch_part(hipStream_t s, dim3 grid, const LpArgs& a) {
-    if (a.entropy) hipLaunchKernelGGL((lp_part_kernel<TYPE, TOP, true, THREADS>), grid, dim3(THREADS), 0, s, a);
-    else hipLaunchKernelGGL((lp_part_kernel<TYPE, TOP, false, THREADS>), grid, dim3(THREADS), 0, s, a);
+void launch_part(hipStream_t s, dim3 grid, bool once, const LpArgs& a) {
+    if (a.entropy && once) hipLaunchKernelGGL((lp_part_kernel<TYPE, TOP, true, true, THREADS>), grid, dim3(THREADS), 0, s, a);
+    else if (a.entropy) hipLaunchKernelGGL((lp_part_kernel<TYPE, TOP, true, false, THREADS>), grid, dim3(THREADS), 0, s, a);
+    else if (once) hipLaunchKernelGGL((lp_part_kernel<TYPE, TOP, false, true, THREADS>), grid, dim3(THREADS), 0, s, a);
+    else hipLaunchKernelGGL((lp_part_kernel<TYPE, TOP, false, false, THREADS>), grid, dim3(THREADS), 0, s, a);
 }
 template <int TYPE>
-void launch_typed(hipStream_t s, dim3 grid, uint32_t threads, const LpArgs& a) {
+void launch_typed(hipStream_t s, dim3 grid, uint32_t threads, bool once, const LpArgs& a) {
     if (a.parts > 1) {
-        if (a.n_top) launch_part<TYPE, kTopJoin, 256>(s, grid, a);
-        else launch_part<TYPE, kTopNone, 256>(s, grid, a);
+        if (a.n_top) launch_part<TYPE, kTopJoin, 256>(s, grid, once, a);
+        else launch_part<TYPE, kTopNone, 256>(s, grid, once, a);
         hipLaunchKernelGGL((lp_join_kernel<TYPE>), dim3(grid.x), dim3(kLpJoin), 0, s, a);
     } else if (threads == 256) {
-        if (a.n_top) launch_part<TYPE, kTopHere, 256>(s, grid, a);
-        else launch_part<TYPE, kTopNone, 256>(s, grid, a);
+        if (a.n_top) launch_part<TYPE, kTopHere, 256>(s, grid, once, a);
+        else launch_part<TYPE, kTopNone, 256>(s, grid, once, a);
     } else {
-        if (a.n_top) launch_part<TYPE, kTopHere, 1024>(s, grid, a);
-        else launch_part<TYPE, kTopNone, 1024>(s, grid, a);
+        if (a.n_top) launch_part<TYPE, kTopHere, 1024>(s, grid, once, a);
+        else launch_part<TYPE, kTopNone, 1024>(s, grid, once, a);
     }
 }
 
-int32_t launch_lp(hipStream_t s, int32_t type, uint32_t threads, LpArgs a, const char* action) {
+int32_t launch_lp(hipStream_t s, int32_t type, uint32_t threads, bool once, LpArgs a, const char* action) {
     for (a.first = 0; a.first < a.n_rows; a.first += kMostGroups / 4) {
         const uint64_t n = a.n_rows - a.first;
         const dim3 grid(static_cast<uint32_t>(n < kMostGroups / 4 ? n : kMostGroups / 4), a.parts);
-        if (type == kDtF32) launch_typed<kDtF32>(s, grid, threads, a);
-        else if (type == kDtF16) launch_typed<kDtF16>(s, grid, threads, a);
-        else launch_typed<kDtBF16>(s, grid, threads, a);
+        if (type == kDtF32) launch_typed<kDtF32>(s, grid, threads, once, a);
+        else if (type == kDtF16) launch_typed<kDtF16>(s, grid, threads, once, a);
+        else launch_typed<kDtBF16>(s, grid, threads, once, a);
         OBJ_HIP(hipGetLastError(), action);
     }
     return 0;
@@ -585,6 +588,9 @@ int32_t objeta_hip_log_probs_device(objeta_hip_context* ctx, objeta_hip_stream s
     // of 151936 18.3 / 10.8; 64 rows of 50000 in 16 bits 12.0 / 12.9, of 151936 19.8 / 17.5; 200 rows of 151936
     // 20.5 / 24.1. 256 threads / cut: 300 rows of 32000 in 16 bits 14.6 / 16.1, of 151936 42 / 30.
     const uint64_t row_bytes = vocab * es;
+    // Logits of 64 MiB and more (held / not kept, us: 2048 rows of 151936 bf16 117 / 105, floats 219 / 194, 8192
+    // of 32000 bf16 104 / 94; 64 rows of 151936, 19 MB, 16.4 / 17.6).
+    const bool once = n_rows * row_bytes >= (uint64_t(64) << 20);
     const bool large = n_rows <= 256 && (row_bytes <= 200000 || n_rows >= 128);
     const uint32_t threads = large ? 1024 : 256, turn = threads * kLpVecs * (dtype == kDtF32 ? 4 : 8);
     const uint64_t most = (vocab + turn - 1) / turn, want = large || row_bytes <= 100000 ? 1 : 1024 / n_rows;
@@ -600,7 +606,7 @@ int32_t objeta_hip_log_probs_device(objeta_hip_context* ctx, objeta_hip_stream s
         a.stats = static_cast<float4*>(ws);
         a.blocks = reinterpret_cast<float*>(a.stats + n);
     }
-    return launch_lp(s, dtype, threads, a, action);
+    return launch_lp(s, dtype, threads, once, a, action);
     OBJ_GUARD_END
 }
 
