@@ -69,6 +69,15 @@ __device__ __forceinline__ Raw8 load_raw8(int32_t type, const void* base, uint64
     if (n < 8) return load_some(p, n);
     return Raw8{*reinterpret_cast<const any_u32x4*>(p), reg_u32x4{0, 0, 0, 0}};
 }
+// The same of rows that the caches need not keep.
+__device__ __forceinline__ Raw8 load_raw8_once(int32_t type, const void* base, uint64_t at, uint32_t n) {
+    if (n < 8) return load_raw8(type, base, at, n);
+    if (type == kDtF32) {
+        const any_u32x4* p = reinterpret_cast<const any_u32x4*>(static_cast<const uint32_t*>(base) + at);
+        return Raw8{__builtin_nontemporal_load(p), __builtin_nontemporal_load(p + 1)};
+    }
+    return Raw8{__builtin_nontemporal_load(reinterpret_cast<const any_u32x4*>(static_cast<const uint16_t*>(base) + at)), reg_u32x4{0, 0, 0, 0}};
+}
 __device__ __forceinline__ void to_floats(int32_t type, const Raw8& r, float (&x)[8]) {
     if (type == kDtF32) {
 #pragma unroll

@@ -12,7 +12,7 @@
 //
 // A row's elements stay in the registers of WAVES waves, eight of each vector in a thread, from
 // the one read to the one write. Bound: HBM (8192 rows of 4096 in bf16, the residual in float, to int8
-// 69 us, 5.35 TB/s; 14336 rows of 4096 floats quantized 53.7 us, 5.5 TB/s, where a copy reaches 5.1), or the
+// 69 us, 5.35 TB/s; 14336 rows of 4096 floats quantized 49.9 us, 5.9 TB/s, where a copy reaches 5.1), or the
 // latency of one row (one of 2048: 5.6 us a call).
 #include "dense_common.hpp"
 #include "kernels.hpp"
@@ -101,7 +101,8 @@ __device__ __forceinline__ T over_row(T v, Op op, Wave wave, T none, T* shared) 
     }
 }
 
-template <int WAVES, int VECS, bool NORM, int CODES>
+// ONCE: what is read and the codes are not kept in the caches.
+template <int WAVES, int VECS, bool NORM, int CODES, bool ONCE>
 __global__ __launch_bounds__(WAVES <= 1 ? 256 : 64 * WAVES, VECS >= 3 ? 4 : 1) void rows_kernel(NormArgs a) {
     constexpr uint32_t kLanes = WAVES == 0 ? 16 : 64 * WAVES;
     constexpr uint32_t kRows = WAVES <= 1 ? 256 / kLanes : 1;  // rows of a workgroup
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(WAVES <= 1 ? 256 : 64 * WAVES, VECS >= 3 ? 4 : 1) v
     Raw8 rx[VECS], rr[VECS], rw[VECS];
     float y[VECS][8];
     auto place = [&](int v) { return 8 * (slot + v * kLanes); };
-    auto load_x = [&](int v) { rx[v] = left[v] ? load_raw8(a.x_type, a.x, row * a.x_stride + place(v), left[v]) : Raw8{}; };
+    auto load_x = [&](int v) { rx[v] = !left[v] ? Raw8{} : ONCE ? load_raw8_once(a.x_type, a.x, row * a.x_stride + place(v), left[v]) : load_raw8(a.x_type, a.x, row * a.x_stride + place(v), left[v]); };
     auto load_r = [&](int v) { rr[v] = a.r && left[v] ? load_raw8(a.r_type, a.r, row * a.r_stride + place(v), left[v]) : Raw8{}; };
     auto load_w = [&](int v) { rw[v] = left[v] ? load_raw8(a.w_type, a.w, place(v), left[v]) : Raw8{}; };
     auto add = [&](int v) {
@@ -221,7 +222,8 @@ __global__ __launch_bounds__(WAVES <= 1 ? 256 : 64 * WAVES, VECS >= 3 ? 4 : 1) v
                 c[i] = zero ? 0 : __builtin_amdgcn_perm(t[4 * i + 1], t[4 * i], 0x0C0C0400u) | __builtin_amdgcn_perm(t[4 * i + 3], t[4 * i + 2], 0x04000C0Cu);
             uint8_t* to = static_cast<uint8_t*>(a.codes) + row * a.code_stride + place(v);
             if (left[v] == 8) {
-                *reinterpret_cast<any_u32x2*>(to) = any_u32x2{c[0], c[1]};
+                if (ONCE) __builtin_nontemporal_store(any_u32x2{c[0], c[1]}, reinterpret_cast<any_u32x2*>(to));
+                else *reinterpret_cast<any_u32x2*>(to) = any_u32x2{c[0], c[1]};
             } else {
 #pragma unroll
                 for (uint32_t i = 0; i < 8; ++i)
@@ -263,14 +265,22 @@ constexpr uint64_t kMaxWidth = 65536;             // a row in the registers of 1
 constexpr uint64_t kMaxHidden = 32768;            // four, whose sums and weights take registers too
 constexpr uint64_t kGroups = kMostGroups / 4;     // of a launch: they have up to 1024 threads
 
+// Matrices of 64 MiB and more quantized past the caches, held / not, us: 14336 rows of 4096 floats 53.8 / 49.9, in
+// bf16 37.3 / 35.3; 4096 of 14336 floats 57.9 / 51.6; beyond 16384 elements a row 2000 of 18432 43.7 / 45.8. A
+// norm's codes are read by the next product, and its float rows took longer so (16384 of 1536 39.7 / 42.5).
+bool quantized_once(const NormArgs& a) {
+    return a.width <= 16384 && a.n_rows * a.width * (a.x_type == kDtF32 ? 4 : 2) >= (uint64_t(64) << 20);
+}
+
 template <int WAVES, int VECS, bool NORM>
 void launch_shape(hipStream_t s, uint32_t groups, int codes, const NormArgs& a) {
     const dim3 block(WAVES <= 1 ? 256 : 64 * WAVES);
-    if (codes == kCodesInt8) hipLaunchKernelGGL((rows_kernel<WAVES, VECS, NORM, kCodesInt8>), dim3(groups), block, 0, s, a);
-    else if constexpr (NORM) {
-        if (codes == kCodesFp8) hipLaunchKernelGGL((rows_kernel<WAVES, VECS, NORM, kCodesFp8>), dim3(groups), block, 0, s, a);
-        else hipLaunchKernelGGL((rows_kernel<WAVES, VECS, NORM, kCodesNone>), dim3(groups), block, 0, s, a);
-    }
+    if constexpr (!NORM) {
+        if (WAVES * VECS <= 32 && quantized_once(a)) hipLaunchKernelGGL((rows_kernel<WAVES, VECS, NORM, kCodesInt8, WAVES * VECS <= 32>), dim3(groups), block, 0, s, a);
+        else hipLaunchKernelGGL((rows_kernel<WAVES, VECS, NORM, kCodesInt8, false>), dim3(groups), block, 0, s, a);
+    } else if (codes == kCodesInt8) hipLaunchKernelGGL((rows_kernel<WAVES, VECS, NORM, kCodesInt8, false>), dim3(groups), block, 0, s, a);
+    else if (codes == kCodesFp8) hipLaunchKernelGGL((rows_kernel<WAVES, VECS, NORM, kCodesFp8, false>), dim3(groups), block, 0, s, a);
+    else hipLaunchKernelGGL((rows_kernel<WAVES, VECS, NORM, kCodesNone, false>), dim3(groups), block, 0, s, a);
 }
 
 // Waves of a row and vectors of a thread. A vector that a row does not fill costs what a full one does,

@@ -238,6 +238,13 @@ def test_quantize_many_rows(backend, dense):
     check_quantize(backend, dense, np.random.default_rng(9).standard_normal((9001, 72)), "f16")
 
 
+@pytest.mark.parametrize("t,n,cols,pad,skew", [("f32", 4100, 4096, 0, 0), ("f16", 33000, 1025, 3, 1), ("bf16", 280000, 120, 0, 0),
+                                               ("f32", 1025, 16384, 4, 0)])
+def test_quantize_large_matrices(backend, dense, t, n, cols, pad, skew):
+    x = np.random.default_rng(cols).standard_normal((n, cols), dtype=np.float32)
+    check_quantize(backend, dense, x, t, pad=pad, skew=skew)
+
+
 # ----------------------------------------------------------------------- product
 def check_product(be, dense, n, rows, cols, ot="f32", bias=True, skews=(0, 0, 0), pads=(0, 0, 0), extreme=False, seed=0, stream=None):
     rng = np.random.default_rng(seed + 31 * n + rows + cols)
@@ -401,6 +408,11 @@ def test_log_probs_of_the_best(backend, dense, n_top, n, vocab):
     rng = np.random.default_rng(n_top)
     check_log_probs(backend, dense, rng.standard_normal((n, vocab)) * 2.5, "bf16" if n > 1 else "f32", n_top, given(rng, n, vocab, 1),
                     entropy=n_top != 5, lse=n_top != 2)
+
+
+@pytest.mark.parametrize("t,n,vocab,n_top", [("f32", 130, 130001, 3), ("f32", 300, 60000, 7), ("f16", 1300, 26003, 0), ("bf16", 1100, 31000, 5)])
+def test_log_probs_of_large_batches(backend, dense, t, n, vocab, n_top):
+    check_log_probs(backend, dense, np.random.default_rng(n).standard_normal((n, vocab), dtype=np.float32) * 3, t, n_top=n_top)
 
 
 @pytest.mark.parametrize("scale", [0.01, 0.7, 5.0])
