@@ -7,7 +7,7 @@
 //
 // Bound: up to some 100 tokens by the channels' codes from HBM (one token of 4096 columns to 151936
 // channels 102 us, 6.1 TB/s; 32 tokens 124, 5.2 TB/s), beyond by the matrix cores, whose clock real codes draw down
-// (4099 tokens of 4096 to 14336 232 to 236 us, 2.05 POP/s); small products by a workgroup's chain of loads,
+// (4099 tokens of 4096 to 14336 228 to 236 us, 2.04 to 2.11 POP/s); small products by a workgroup's chain of loads,
 // products and their join.
 #include "dense_common.hpp"
 #include "kernels.hpp"
