@@ -1,0 +1,40 @@
+"""The host side of the 8-bit product and the log probabilities over a runtime that stands in for the
+device: which launches a call makes, what memory it takes, and that it does without where it can."""
+import os
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+LIB = os.path.join(ROOT, "objeta_amd", "lib")
+STRAIGHTEN = (2048, 1, 256)
+
+
+@pytest.fixture(scope="module")
+def check(tmp_path_factory):
+    exe = str(tmp_path_factory.mktemp("dense_host") / "check")
+    subprocess.run(["g++", "-O1", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I" + os.path.join(ROOT, "objeta_amd", "csrc"),
+                    os.path.join(ROOT, "tests", "native", "dense_host_check.cpp"), "-o", exe, "-rdynamic", "-L" + LIB, "-lobjeta_hip",
+                    "-L/opt/rocm/lib", "-lamdhip64", "-Wl,-rpath," + LIB, "-Wl,-rpath,/opt/rocm/lib"], check=True)
+
+    def run(*commands):
+        """Calls as (status, launches), and the sizes of the allocations."""
+        out = subprocess.run([exe, *commands], capture_output=True, text=True, check=True, timeout=120).stdout.splitlines()
+        calls = []
+        for line in out[:-1]:
+            status, *launches = line.split()
+            calls.append((int(status), [tuple(map(int, x.split(","))) for x in launches]))
+        return calls, [int(x) for x in out[-1].split()[1:]]
+    return run
+
+
+def test_product_without_memory_for_copies_reads_rows_where_they_lie(check):
+    """Rows that begin anywhere are copied where there is room; without any the call computes the same
+    from where they lie, as a captured one does."""
+    (copied,), _ = check("product:1700,1650,37")
+    assert copied[0] == 0 and copied[1][:2] == [STRAIGHTEN, STRAIGHTEN] and len(copied[1]) == 3
+    (captured,), _ = check("capture:1", "product:1700,1650,37")
+    assert captured[0] == 0 and len(captured[1]) == 1 and STRAIGHTEN not in captured[1]
+    for room in (0, 16384, 100000):
+        (short, again), _ = check(f"memory:{room}", "product:1700,1650,37", "product:1700,1650,37")
+        assert short == captured and again == captured
