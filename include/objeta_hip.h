@@ -1002,10 +1002,11 @@ int32_t objeta_hip_kv_free_device(objeta_hip_context* ctx, objeta_hip_stream str
  * time. Calls may be captured. Norms and quantized rows need no workspace. Log probabilities of few
  * long rows keep their parts in the stream's workspace: made by an eager call of the same sizes;
  * captured without one such a call is refused (Unsupported). The product keeps copies of rows that
- * do not begin at multiples of 16 bytes there where tokens and channels are both many (at most 1
- * GiB; captured without one, or where there is no memory for it, it reads them where they lie).
- * Graphs captured on one stream share that stream's workspace: their replays are ordered one after
- * the other. */
+ * do not begin at multiples of 16 bytes there where tokens and channels are both many: at most 1
+ * GiB a stream, and below another GiB in regions that it outgrew, which stay until the context is
+ * destroyed; captured without one, or where there is no memory for it, it reads them where they
+ * lie. Graphs captured on one stream share that stream's workspace: their replays, and calls on that
+ * stream, are ordered one after the other. */
 
 /* 8-bit codes of a row y of floats.
  * INT8: s = max |y| / 127 (a float; one a row), code = y / s rounded to the nearest, halves to even,

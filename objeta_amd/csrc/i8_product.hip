@@ -491,10 +491,14 @@ constexpr uint64_t kMostStraight = uint64_t(1) << 30;
 int32_t straighten(objeta_hip_context* ctx, hipStream_t s, I8Args& a, const char* action) {
     const uint64_t pitch = (static_cast<uint64_t>(a.cols) + 15) / 16 * 16, n = a.n_tokens, r = a.rows;
     if (n * r < 800 * (n + r) || a.cols < 16 || (n + r) * pitch > kMostStraight) return 0;
+    // Powers of two, so that the workspace stays within the largest copies and the regions that it
+    // outgrew (kept for graphs that use them) come to less than it together.
+    uint64_t bytes = uint64_t(1) << 20;
+    while (bytes < (n + r) * pitch) bytes *= 2;
     // Captured without a workspace, or with no memory for one: read as they are.
-    if (!workspace_ready(ctx, s, kWsCodes, (n + r) * pitch)) return 0;
+    if (!workspace_ready(ctx, s, kWsCodes, bytes)) return 0;
     void* ws = nullptr;
-    if (ensure_workspace(ctx, s, kWsCodes, (n + r) * pitch, &ws) != 0) return 0;
+    if (ensure_workspace(ctx, s, kWsCodes, bytes, &ws) != 0) return 0;
     int8_t* to = static_cast<int8_t*>(ws);
     hipLaunchKernelGGL(i8_straighten_kernel, dim3(2048), dim3(256), 0, s, a.a, a.a_stride, a.n_tokens, a.cols, to);
     hipLaunchKernelGGL(i8_straighten_kernel, dim3(2048), dim3(256), 0, s, a.w, a.w_stride, a.rows, a.cols, to + n * pitch);

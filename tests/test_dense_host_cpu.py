@@ -38,3 +38,18 @@ def test_product_without_memory_for_copies_reads_rows_where_they_lie(check):
     for room in (0, 16384, 100000):
         (short, again), _ = check(f"memory:{room}", "product:1700,1650,37", "product:1700,1650,37")
         assert short == captured and again == captured
+
+
+def test_product_copies_stay_within_their_bounds(check):
+    """Calls that climb in odd sizes: no region past 1 GiB, those it replaced together below another."""
+    sizes, cols = [], 33
+    while cols < 131071:
+        sizes.append((2000, 2000, cols))
+        cols = cols * 5 // 4 + 1 | 1
+    sizes += [(2000 + 100 * i, 2000, 131071) for i in range(40)] + [(8190, 8192, 65535), (8192, 8192, 65535), (8192, 8192, 65535)]
+    calls, regions = check(*(f"product:{n},{r},{k}" for n, r, k in sizes))
+    for (n, r, k), (status, launches) in zip(sizes, calls):
+        fits = (n + r) * ((k + 15) // 16 * 16) <= 1 << 30
+        assert status == 0 and len(launches) == (3 if fits else 1), (n, r, k, launches)
+    copies = regions[1:]  # (the first is the stream's own counters)
+    assert max(copies) == copies[-1] <= 1 << 30 and sum(copies[:-1]) < 1 << 30, copies
