@@ -439,18 +439,22 @@ void launch_either(hipStream_t s, const I8Args& a, bool whole) {
     else launch_tile<WC, WT, TC, TT, KG, 1, false>(s, a);
 }
 
-// What a tile costs, in us, measured over batches of 5 to 8192 tokens and matrices of 512 to 151936
-// channels by 2048 to 14336 columns: `fixed` around the columns; for 128 columns `low` where a CU has one
+// What a tile costs, in us, measured over batches of 5 to 8192 tokens and matrices of 512 to 160000
+// channels by 64 to 14336 columns: `fixed` around the columns; for 128 columns `low` where a CU has one
 // workgroup and few others run, `full` a workgroup of a full card, where the products of real codes
-// draw the clock down (8192^3: 450 us, of zeros 318). `resident` workgroups share a CU.
+// draw the clock down (8192^3: 450 us, of zeros 318). `resident` workgroups share a CU (two of four waves:
+// they take 172 to 246 registers; eight waves have it to themselves), and `again` is what each further round of them
+// adds, whose loads begin beside the last one's products (300 tokens of 4096 to 14336: five 64 x 64 tiles a CU 49.0 us,
+// 128 x 256 38.5; 8192 of 1024 to 28672: 28 of 128 x 128 390, 14 of 256 x 256 345).
 struct TileCost {
     uint32_t channels, tokens, resident;
-    double fixed, low, full;
+    double fixed, again, low, full;
 };
 enum : int { kTile256, kTile128x256, kTile128, kTile64x128, kTile64, kTile32x64, kTile32, kTiles };
 constexpr TileCost kTileCosts[kTiles] = {
-    {256, 256, 1, 6.7, 1.03, 1.70}, {128, 256, 1, 5.1, 0.85, 1.15}, {128, 128, 2, 3.7, 0.65, 0.60}, {64, 128, 3, 3.9, 0.42, 0.39},
-    {64, 64, 4, 3.6, 0.30, 0.23},   {32, 64, 1, 4.2, 0.21, 0.22},   {32, 32, 1, 4.9, 0.15, 0.16},
+    {256, 256, 1, 6.7, 6.7, 1.03, 1.70}, {128, 256, 1, 5.1, 5.1, 0.85, 1.15}, {128, 128, 2, 3.7, 2.6, 0.65, 0.60},
+    {64, 128, 2, 3.9, 2.6, 0.42, 0.39},  {64, 64, 2, 3.6, 1.6, 0.30, 0.23},   {32, 64, 1, 4.2, 4.2, 0.21, 0.22},
+    {32, 32, 1, 4.9, 4.9, 0.15, 0.16},
 };
 
 // The tile that would take the least time: large ones do the most products for what they load, but
@@ -466,13 +470,13 @@ int best_tile(const I8Args& a, bool whole) {
         const TileCost& c = kTileCosts[i];
         const double tiles = static_cast<double>((a.rows + c.channels - 1) / c.channels) * ((a.n_tokens + c.tokens - 1) / c.tokens);
         const double each = ceil(tiles / 256);  // of the CU with most
-        double us;
+        const double rounds = ceil(each / c.resident);
+        double us = c.fixed + (rounds - 1) * c.again;
         if (c.resident > 1) {
-            const double step = each * c.full > c.low ? each * c.full : c.low;
-            us = c.fixed + steps * step;
+            us += steps * (each * c.full > c.low ? each * c.full : c.low);
         } else {
             const double busy = tiles < 256 ? tiles / 256 : 1;
-            us = each * (c.fixed + steps * (c.low + (c.full - c.low) * busy));
+            us += steps * each * (c.low + (c.full - c.low) * busy);
         }
         if (i == first || us < least) best = i, least = us;
     }
