@@ -294,7 +294,11 @@ __device__ void lp_finish(const LpArgs& a, uint64_t r, LpSums v, LpGiven first, 
     const float more = (again ? log_s : log_s + __builtin_fmaf(-v.m, a.c, v.ref)) * kLn2;  // ln sum exp(z - m)
     auto not_above_0 = [](float p) { return p > 0.0f ? 0.0f : p; };  // NaN stays
     auto log_prob = [&](float x) {
-        return none ? -__builtin_inff() : not_above_0(__builtin_fmaf(x - v.m, a.scale, -more));
+        if (none) return -__builtin_inff();
+        const float d = x - v.m;
+        // (logits so far apart that a float does not hold their difference: it may hold the scaled one)
+        const float z = d == -__builtin_inff() ? __builtin_fmaf(x, a.scale, -v.m * a.scale) - more : __builtin_fmaf(d, a.scale, -more);
+        return not_above_0(z);
     };
     if (tid == 0) {
         if (a.lse) a.lse[r] = none ? -__builtin_inff() : __builtin_fmaf(v.m, a.scale, more);
