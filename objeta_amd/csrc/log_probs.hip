@@ -5,9 +5,10 @@
 // far, in units of ln 2), s = sum 2^(z - R) and t = sum 2^(z - R) (z - R), and moves both when R grows:
 // with d = R - R', s' = 2^d s and t' = 2^d (t + d s).
 //
-// The best N: a thread also keeps the largest x of each stretch it read (up to 8). The N-th largest of 64
-// maxima of four threads each bounds the N-th best from below, so only the few stretches that reach it
-// are read again, and what reaches it there is ranked. A value's key is its bits in their order above the
+// The best N: a thread also keeps the largest x of each stretch it read (up to 8; of a cut row four threads
+// keep one for their part). The N-th largest of 64 maxima, each of every 64th thread's values (in the join every
+// 64th block's), bounds the N-th best from below, so only the few stretches that reach it are read again, and
+// what reaches it there is ranked. A value's key is its bits in their order above the
 // complement of its index: equal values go by the lowest index. Where too many values reach the bound
 // (ties, all of the best in few threads), the N-th value is found bit by bit over the row instead.
 //
@@ -22,6 +23,8 @@ namespace dev {
 
 constexpr uint32_t kLpJoin = 256;    // threads that join a row's parts; as many parts at most
 constexpr uint32_t kLpBlocks = 64;  // of a part
+constexpr uint32_t kLpKept = 20;    // blocks' largest that a thread of the join holds
+constexpr uint32_t kLpMostParts = kLpKept * kLpJoin / kLpBlocks;  // of a row whose best are asked for
 constexpr uint32_t kLpVecs = 2;      // 16-byte loads of a turn; the next turn's are in flight
 constexpr uint32_t kLpStretches = 8;  // (with 16, LDS held five workgroups a CU in place of eight)
 constexpr uint32_t kLpMostTop = 32;
@@ -447,12 +450,11 @@ __global__ __launch_bounds__(kLpJoin) void lp_join_kernel(LpArgs a) {
     const int32_t token = lp_token(a, r, tid);
     float4 sums = make_float4(-__builtin_inff(), -kLpFar, 0.0f, 0.0f);
     if (tid < a.parts) sums = a.stats[r * a.parts + tid];
-    constexpr uint32_t kKept = 20;  // maxima of a thread, read beside the sums
-    float kept[kKept], mine = -__builtin_inff();
+    float kept[kLpKept], mine = -__builtin_inff();  // read beside the sums
     if (a.n_top) {
         const uint32_t all = a.parts * kLpBlocks;
 #pragma unroll
-        for (uint32_t u = 0; u < kKept; ++u) {
+        for (uint32_t u = 0; u < kLpKept; ++u) {
             const uint32_t i = tid + u * kLpJoin;
             kept[u] = i < all ? a.blocks[r * all + i] : -__builtin_inff();
         }
@@ -463,24 +465,14 @@ __global__ __launch_bounds__(kLpJoin) void lp_join_kernel(LpArgs a) {
     if (a.n_top) {
         constexpr uint32_t kPer = LpElem<TYPE>::kPer, kStep = 4 * kLpBlocks * kPer, kTurn = kLpVecs * kStep;
         const void* row = static_cast<const char*>(a.x) + r * a.stride * (16 / kPer);
-        const float* blocks = a.blocks + r * a.parts * kLpBlocks;
-        const uint32_t all = a.parts * kLpBlocks, turns = a.part_size / kTurn, each = turns * kLpVecs * 4;
+        const uint32_t turns = a.part_size / kTurn, each = turns * kLpVecs * 4;
 #pragma unroll
-        for (uint32_t u = 0; u < kKept; ++u) mine = larger(mine, kept[u]);
-        uint32_t bound;
-        if (all <= kKept * kLpJoin) {
-            const uint32_t key = ordered(mine);
-            bound = lp_bound(key, a.n_top, sh);
-            if (key >= bound)
+        for (uint32_t u = 0; u < kLpKept; ++u) mine = larger(mine, kept[u]);
+        const uint32_t key = ordered(mine), bound = lp_bound(key, a.n_top, sh);
+        if (key >= bound)
 #pragma unroll
-                for (uint32_t u = 0; u < kKept; ++u)
-                    if (ordered(kept[u]) >= bound) lp_hit(tid + u * kLpJoin, sh);
-        } else {
-            for (uint32_t i = tid + kKept * kLpJoin; i < all; i += kLpJoin) mine = larger(mine, blocks[i]);
-            bound = lp_bound(ordered(mine), a.n_top, sh);
-            for (uint32_t i = tid; i < all; i += kLpJoin)
-                if (ordered(blocks[i]) >= bound) lp_hit(i, sh);
-        }
+            for (uint32_t u = 0; u < kLpKept; ++u)
+                if (ordered(kept[u]) >= bound) lp_hit(tid + u * kLpJoin, sh);
         __syncthreads();
         const uint32_t items = sh.hits <= kLpMostHits ? sh.hits * each : 0;
         for (uint32_t i = tid; i < items; i += kLpJoin) {
@@ -599,7 +591,12 @@ int32_t objeta_hip_log_probs_device(objeta_hip_context* ctx, objeta_hip_stream s
     const uint32_t threads = large ? 1024 : 256, turn = threads * kLpVecs * (dtype == kDtF32 ? 4 : 8);
     const uint64_t most = (vocab + turn - 1) / turn, want = large || row_bytes <= 100000 ? 1 : 1024 / n_rows;
     uint64_t parts = want < 1 ? 1 : (want < most ? want : most);
-    if (parts > kLpJoin) parts = kLpJoin;
+    // The join holds the largest of as many parts as it has registers for, since reading them a second time costs
+    // more than longer parts up to some 8 million logits: one row with the best twenty in 80 parts / up to 256, us:
+    // 200000 floats 11.0 / 13.3, 262144 11.3 / 16.7, a million 15.5 / 29.6, 4 million 23 / 33, 16 million 67 / 49. (With
+    // 32 or 64 held in place of 20 a row of 151936 takes 11.3 or 14.5 for 10.6, shorter ones the same.)
+    const uint64_t most_parts = n_top ? kLpMostParts : kLpJoin;
+    if (parts > most_parts) parts = most_parts;
     const uint64_t size = ((vocab + parts - 1) / parts + turn - 1) / turn * turn;
     a.part_size = static_cast<uint32_t>(size);
     a.parts = static_cast<uint32_t>((vocab + size - 1) / size);

@@ -66,3 +66,16 @@ def test_tiles_are_charged_for_every_round(check, n, rows, cols, groups, threads
     round of workgroups that the card takes in turn."""
     ((status, launches),), _ = check(f"product:{n},{rows},{cols}")
     assert status == 0 and launches == [((groups + 7) // 8 * 8, 1, threads)]
+
+
+@pytest.mark.parametrize("rows,vocab,dtype", [(1, 151936, 0), (1, 200000, 0), (1, 262144, 0), (4, 262144, 0), (1, 1000000, 0), (1, 524288, 2),
+                                              (3, 2000000, 2), (1, (1 << 31) - (1 << 16), 1)])
+def test_the_join_holds_every_part_of_a_row(check, rows, vocab, dtype):
+    """The best of a cut row are found from the largest value of each 64th of its parts, twenty held by each of
+    256 threads; rows of which only sums are asked are cut as far as the join has threads."""
+    (best, sums), _ = check(f"logprobs:{rows},{vocab},{dtype},20", f"logprobs:{rows},{vocab},{dtype},0")
+    for (status, launches), most in ((best, 80), (sums, 256)):
+        assert status == 0 and len(launches) == 2
+        (n, parts, threads), join = launches
+        assert n == rows and 1 < parts <= most and threads == 256 and join == (rows, 1, 256)
+    assert sums[1][0][1] >= best[1][0][1]

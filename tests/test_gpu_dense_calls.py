@@ -21,3 +21,12 @@ def test_log_probs_of_logits_whose_difference_is_past_a_float(backend, dense, t,
     x[0, 7] = far
     x[1, 1::2] = far
     check_log_probs(backend, dense, x, t, 5, np.array([[7, 0, 8]] * 2), scale)
+
+
+@pytest.mark.parametrize("t,vocab", [("f32", 163841), ("f32", 262144), ("f32", 1000003), ("bf16", 700001)])
+@pytest.mark.parametrize("n_top", [0, 20])
+def test_log_probs_of_long_hard_rows(backend, dense, t, vocab, n_top):
+    """Rows cut into as many parts as their join takes: masks, ties, NaN, the best in few places."""
+    x = hard_rows(vocab, LOWEST[t])
+    for rows in (range(7, 8), range(0, 4), range(4, 7), range(8, 12), range(12, 18)):
+        check_log_probs(backend, dense, x[rows], t, n_top, given(np.random.default_rng(14), len(rows), vocab, 2))
