@@ -1026,7 +1026,8 @@ enum { OBJETA_HIP_CODES_NONE = 0, OBJETA_HIP_CODES_INT8 = 1, OBJETA_HIP_CODES_FP
  * [n_tokens][hidden] bytes (codes_stride) and d_scales (INT8 float [n_tokens], FP8 bytes
  * [n_tokens][hidden / 128], hidden a multiple of 128) of y rounded to float; they do not
  * depend on out_dtype. One output at least is given. y is computed in 64 bits and rounded
- * once (16-bit types: from its float). eps >= 0; with eps 0 a row of zeros gives NaN. */
+ * once (16-bit types: from its float). eps from 0 to below 1e300 (with 0 a row of zeros gives NaN),
+ * |weight_offset| < 1e30, n_tokens < 2^31. */
 int32_t objeta_hip_rms_norm_device(objeta_hip_context* ctx, objeta_hip_stream stream, uint64_t n_tokens, uint64_t hidden,
                                    int32_t dtype, const void* d_x, uint64_t x_stride, int32_t weight_dtype,
                                    const void* d_weight, float weight_offset, double eps, int32_t residual_dtype,
@@ -1035,7 +1036,7 @@ int32_t objeta_hip_rms_norm_device(objeta_hip_context* ctx, objeta_hip_stream st
                                    int32_t codes, void* d_codes, uint64_t codes_stride, void* d_scales);
 
 /* Rows of a matrix (a weight's channels, tokens) to int8 codes with a scale a row: INT8 above.
- * x [n_rows][cols] of `dtype`, cols 1 .. 65536. */
+ * x [n_rows][cols] of `dtype`, cols 1 .. 65536, n_rows < 2^31. */
 int32_t objeta_hip_quantize_rows_i8_device(objeta_hip_context* ctx, objeta_hip_stream stream, uint64_t n_rows, uint64_t cols,
                                            int32_t dtype, const void* d_x, uint64_t x_stride, int8_t* d_codes,
                                            uint64_t codes_stride, float* d_scales);
@@ -1062,7 +1063,9 @@ int32_t objeta_hip_i8_product_device(objeta_hip_context* ctx, objeta_hip_stream 
  *     index, and their ln p
  * Logits of -infinity have ln p -inf; a row of nothing else lse -inf and entropy 0. A row that
  * holds NaN or +infinity has NaN for lse, entropy and every ln p; NaN ranks below -infinity.
- * scale > 0 (1 / temperature). Sums are held in float, references in units of ln 2. */
+ * 0 < scale < 1e30 (1 / temperature); vocab 1 .. 2^31 - 2^16, n_rows < 2^31, n_given at most 1024.
+ * Sums are held in float, references in units of ln 2: ln p of a nearly sure token is right to some
+ * 2^-24, and may be 0. */
 int32_t objeta_hip_log_probs_device(objeta_hip_context* ctx, objeta_hip_stream stream, uint64_t n_rows, uint64_t vocab,
                                     int32_t dtype, const void* d_logits, uint64_t stride, float scale, const int32_t* d_tokens,
                                     uint64_t n_given, float* d_token_log_probs, float* d_lse, float* d_entropy, uint64_t n_top,

@@ -130,3 +130,24 @@ def test_fp8_codes_of_the_norm_through_the_official_product(backend, dense, n, h
     q, s, got = codes.get(), scales.get(), y.get()
     for i in range(n):
         assert_gemv_close(got[i], ref(q[i], s[i], w, ws, rows, hidden))
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hidden", [128, 2048, 20480])
+def test_fp8_codes_of_rows_that_are_not_numbers(backend, dense, t, hidden):
+    """Zeros over eps 0, infinities and NaN: the bytes that the activation quantizer gives the float norm."""
+    x = np.random.default_rng(51).standard_normal((6, hidden))
+    x[0] = 0
+    x[1, hidden // 2] = np.inf
+    x[2, 3] = np.nan
+    x[3, 100] = -np.inf
+    x[4] = np.inf
+    dx, dw = Rows(backend, to_type(x, t), t), Rows(backend, to_type(np.ones((1, hidden)), t), t)
+    dy = blank(backend, 6, hidden, "f32")
+    out = [(blank(backend, 6, hidden, None, dtype=np.uint8), blank(backend, 6, hidden // 128, None, dtype=np.uint8)) for _ in range(2)]
+    dense.rms_norm_device(6, hidden, t, dx.ptr, dw.ptr, eps=0.0, d_out=dy.ptr, out_dtype="f32", codes="fp8", d_codes=out[0][0].ptr,
+                          d_scales=out[0][1].ptr)
+    QuantBackend(backend).act_quant_device(None, dy.ptr, 6, hidden, out[1][0].ptr, out[1][1].ptr)
+    backend.synchronize()
+    assert np.isnan(dy.get()[0]).all()
+    assert np.array_equal(out[0][0].get(), out[1][0].get()) and np.array_equal(out[0][1].get(), out[1][1].get())
