@@ -443,19 +443,20 @@ void launch_either(hipStream_t s, const I8Args& a, bool whole) {
 // What a tile costs, in us, measured over batches of 5 to 8192 tokens and matrices of 512 to 160000
 // channels by 64 to 14336 columns: `fixed` around the columns; for 128 columns `low` where a CU has one
 // workgroup and few others run, `full` a workgroup of a full card, where the products of real codes
-// draw the clock down (8192^3: 450 us, of zeros 318). `resident` workgroups share a CU (two of four waves:
-// they take 172 to 246 registers; eight waves have it to themselves), and `again` is what each further round of them
-// adds, whose loads begin beside the last one's products (300 tokens of 4096 to 14336: five 64 x 64 tiles a CU 49.0 us,
-// 128 x 256 38.5; 8192 of 1024 to 28672: 28 of 128 x 128 390, 14 of 256 x 256 345).
+// draw the clock down (8192^3: 450 us, of zeros 318). `resident` workgroups share a CU, as far as registers go and, of
+// rows that begin anywhere (fewer loads ahead, 90 to 178 registers for 172 to 246), LDS; eight waves have it to
+// themselves. `again` is what each further round of them adds, whose loads begin beside the last one's products (300
+// tokens of 4096 to 14336: five 64 x 64 tiles a CU 49.0 us, 128 x 256 38.5; 8192 of 1024 to 28672: 28 of 128 x 128 390,
+// 14 of 256 x 256 345; 15 of 328 to 52105, anywhere: four of 64 x 64 9.9, two of 128 x 128 11.5).
 struct TileCost {
-    uint32_t channels, tokens, resident;
+    uint32_t channels, tokens, resident, resident_anywhere;
     double fixed, again, low, full;
 };
 enum : int { kTile256, kTile128x256, kTile128, kTile64x128, kTile64, kTile32x64, kTile32, kTiles };
 constexpr TileCost kTileCosts[kTiles] = {
-    {256, 256, 1, 6.7, 6.7, 1.03, 1.70}, {128, 256, 1, 5.1, 5.1, 0.85, 1.15}, {128, 128, 2, 3.7, 2.6, 0.65, 0.60},
-    {64, 128, 2, 3.9, 2.6, 0.42, 0.39},  {64, 64, 2, 3.6, 1.6, 0.30, 0.23},   {32, 64, 1, 4.2, 4.2, 0.21, 0.22},
-    {32, 32, 1, 4.9, 4.9, 0.15, 0.16},
+    {256, 256, 1, 1, 6.7, 6.7, 1.03, 1.70}, {128, 256, 1, 1, 5.1, 5.1, 0.85, 1.15}, {128, 128, 2, 2, 3.7, 2.6, 0.65, 0.60},
+    {64, 128, 2, 3, 3.9, 2.6, 0.42, 0.39},  {64, 64, 2, 4, 3.6, 1.6, 0.30, 0.23},   {32, 64, 1, 1, 4.2, 4.2, 0.21, 0.22},
+    {32, 32, 1, 1, 4.9, 4.9, 0.15, 0.16},
 };
 
 // The tile that would take the least time: large ones do the most products for what they load, but
@@ -471,7 +472,7 @@ int best_tile(const I8Args& a, bool whole) {
         const TileCost& c = kTileCosts[i];
         const double tiles = static_cast<double>((a.rows + c.channels - 1) / c.channels) * ((a.n_tokens + c.tokens - 1) / c.tokens);
         const double each = ceil(tiles / 256);  // of the CU with most
-        const double rounds = ceil(each / c.resident);
+        const double rounds = ceil(each / (whole ? c.resident : c.resident_anywhere));
         double us = c.fixed + (rounds - 1) * c.again;
         if (c.resident > 1) {
             us += steps * (each * c.full > c.low ? each * c.full : c.low);

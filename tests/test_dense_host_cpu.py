@@ -59,6 +59,7 @@ def test_product_copies_stay_within_their_bounds(check):
     (300, 14336, 4096, 112 * 2, 512),  # 128 x 256; 64 x 64 would be five tiles a CU in three rounds
     (8192, 28672, 1024, 112 * 32, 512),  # 256 x 256; 128 x 128 28 a CU in fourteen
     (2048, 32000, 256, 125 * 8, 512), (700, 32000, 5120, 125 * 3, 512), (20, 65536, 512, 512, 256),
+    (15, 52105, 328, 815, 256),  # 64 x 64 of rows that begin anywhere: four share a CU
     (200, 160000, 256, 1250 * 2, 256),  # 128 x 128: 256 tokens a tile would be a fifth empty
     (512, 4096, 4096, 64 * 4, 256), (64, 14336, 4096, 224, 256), (64, 4096, 14336, 128 * 2, 512)])
 def test_tiles_are_charged_for_every_round(check, n, rows, cols, groups, threads):
